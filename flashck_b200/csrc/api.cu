@@ -270,6 +270,49 @@ int FmhaFwdBias(void* q, void* k, void* v, void* bias, void* o, int64_t* q_seq_s
     return run_fwd(p, (cudaStream_t)stream);
 }
 
+int FmhaBwd(void* dout, void* q, void* k, void* v, void* bias, void* o, void* lse, void* dlse, void* dq, void* dk, void* dv_out,
+            void* dbias, void* delta, int64_t* q_seq_start, int64_t* k_seq_start, int64_t batch, int64_t q_seq_len,
+            int64_t kv_seq_len, int64_t hq, int64_t hkv, int64_t d, int64_t dv, int64_t q_max_seq_len, int64_t kv_max_seq_len,
+            float scale, int64_t window_left, int64_t window_right, uint32_t mask_type, void* stream, int dtype, int bias_enum,
+            int bias_rank_info, float logits_soft_cap) {
+    int rc = check_common("FmhaBwd", dtype, hq, hkv, d, dv, nullptr);
+    if (rc) return rc;
+    FCK_REQUIRE(d == dv && (d == 64 || d == 128), FLASHCK_ERR_UNSUPPORTED,
+                "FmhaBwd: hdim_q == hdim_v in {64,128} required (got %lld/%lld)", (long long)d, (long long)dv);
+    FCK_REQUIRE(bias_enum >= 0 && bias_enum <= 2, FLASHCK_ERR_INVALID_ARGUMENT,
+                "FmhaBwd: bias_enum must be 0 (none), 1 (elementwise) or 2 (alibi), got %d", bias_enum);
+    FCK_REQUIRE(bias_enum == 0 || bias != nullptr, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaBwd: bias_enum %d without a bias buffer", bias_enum);
+    FCK_REQUIRE(bias_rank_info >= 0 && bias_rank_info <= (bias_enum == 2 || q_seq_start ? 1 : 2), FLASHCK_ERR_INVALID_ARGUMENT,
+                "FmhaBwd: bias_rank_info %d out of range for bias_enum %d", bias_rank_info, bias_enum);
+    FCK_REQUIRE(dbias == nullptr || bias_enum == 1, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaBwd: dbias goes with an elementwise bias");
+    FCK_REQUIRE(logits_soft_cap >= 0.f, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaBwd: logits_soft_cap must be >= 0");
+    FCK_REQUIRE(batch >= 0 && q_seq_len >= 0 && kv_seq_len >= 0 && q_max_seq_len >= 0 && kv_max_seq_len >= 0,
+                FLASHCK_ERR_INVALID_ARGUMENT, "FmhaBwd: negative size");
+    FCK_REQUIRE(mask_type <= 3, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaBwd: mask_type must be 0..3");
+    FCK_REQUIRE((q_seq_start == nullptr) == (k_seq_start == nullptr), FLASHCK_ERR_INVALID_ARGUMENT,
+                "FmhaBwd: group mode needs both seqstart arrays");
+    const int64_t rows_q = q_seq_start ? q_seq_len : batch * q_seq_len, rows_k = q_seq_start ? kv_seq_len : batch * kv_seq_len;
+    FCK_REQUIRE(batch < (1ll << 31) && rows_q < (1ll << 31) && rows_k < (1ll << 31), FLASHCK_ERR_UNSUPPORTED,
+                "FmhaBwd: %lld query rows and %lld key rows (fewer than 2^31 of each)", (long long)rows_q, (long long)rows_k);
+    FCK_REQUIRE((rows_q == 0 || (dout && q && o && lse && dq && delta)) && (rows_k == 0 || (k && v && dk && dv_out)),
+                FLASHCK_ERR_INVALID_ARGUMENT, "FmhaBwd: null pointer argument");
+    const uintptr_t bits = (uintptr_t)dout | (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o | (uintptr_t)dq | (uintptr_t)dk |
+                           (uintptr_t)dv_out;
+    FCK_REQUIRE((bits & 15) == 0, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaBwd: the tensors must start on 16-byte boundaries");
+    if (batch == 0 || (rows_q == 0 && rows_k == 0)) return FLASHCK_OK;
+    BwdParams p{};
+    p.dout = dout; p.q = q; p.k = k; p.v = v; p.o = o; p.lse = (const float*)lse; p.dlse = (const float*)dlse;
+    p.dq = dq; p.dk = dk; p.dv = dv_out; p.dbias = dbias; p.delta = (float*)delta;
+    p.seqstart_q = q_seq_start; p.seqstart_k = k_seq_start;
+    p.batch = batch; p.seqlen_q = q_seq_len; p.seqlen_k = kv_seq_len; p.hq = hq; p.hkv = hkv; p.d = d;
+    p.max_seqlen_q = q_seq_start && q_max_seq_len > 0 && q_max_seq_len < q_seq_len ? q_max_seq_len : q_seq_len;
+    p.max_seqlen_k = q_seq_start && kv_max_seq_len > 0 && kv_max_seq_len < kv_seq_len ? kv_max_seq_len : kv_seq_len;
+    p.scale = resolve_scale(scale, d);
+    p.mask_type = (int)mask_type; p.wl = window_left; p.wr = window_right; p.dtype = dtype;
+    p.bias = bias_enum ? bias : nullptr; p.bias_type = bias_enum; p.bias_rank = bias_rank_info; p.logits_soft_cap = logits_soft_cap;
+    return launch_bwd_generic(p, (cudaStream_t)stream);
+}
+
 static int batch_prefill_impl(void* q, void* k, void* v, const float* slopes, int slope_rank, void* o, int64_t* q_seq_start,
                               void* kv_indptr, void* kv_page_indices, void* kv_last_page_len, int64_t batch,
                               int64_t q_seq_len, int64_t hq, int64_t hkv, int64_t d, int64_t dv, int64_t q_max_seq_len,

@@ -117,4 +117,31 @@ int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream);
 int fwd_set_param(const char* key, int64_t value);
 int fwd_get_param(const char* key, int64_t* value);
 
+// ---- backward of the forward (fmha_bwd_generic.cu) ----------------------------------------------------------
+struct BwdParams {
+    const void* dout;
+    const void* q;
+    const void* k;
+    const void* v;
+    const void* o;
+    const float* lse;   // of the forward: [b,hq,sq] or [hq,total_q]; -inf marks a row without keys
+    const float* dlse;  // gradient of the LSE in the same layout, or nullptr
+    void* dq;
+    void* dk;
+    void* dv;
+    void* dbias;        // element dtype, the bias tensor's shape, or nullptr
+    float* delta;       // workspace in the layout of the LSE
+    const int64_t* seqstart_q;
+    const int64_t* seqstart_k;
+    int64_t batch, seqlen_q, seqlen_k, hq, hkv, d, max_seqlen_q, max_seqlen_k;  // group mode: seqlen_q / seqlen_k are totals
+    float scale;
+    int mask_type;
+    int64_t wl, wr;
+    int dtype;
+    const void* bias;   // as in FwdParams
+    int bias_type, bias_rank;
+    float logits_soft_cap;
+};
+int launch_bwd_generic(const BwdParams& p, cudaStream_t stream);
+
 }  // namespace fck

@@ -71,16 +71,19 @@ class FlashAttention(torch.nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: Optional[torch.Tensor] = None,
                 cu_seqlens_k: Optional[torch.Tensor] = None, max_seqlen_q: int = 0, max_seqlen_k: int = 0,
                 return_lse: bool = False):
-        """Dense (4-D inputs) or variable-length (3-D packed inputs + ``cu_seqlens``) attention."""
+        """Dense (4-D inputs) or variable-length (3-D packed inputs + ``cu_seqlens``) attention, differentiable in q, k and v."""
         self._check_heads(q, k)
+        # (a call whose gradient nobody asks for runs the plain forward: no LSE is kept)
+        wanted = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)
+        dense, packed = ("autograd", "autograd_var_len") if wanted else ("forward", "forward_var_len")
         kw = dict(scale=self.scale, causal=self.causal, window_size=self.window_size, return_lse=return_lse)
         if q.dim() == 4:
             if cu_seqlens_q is not None or cu_seqlens_k is not None:
                 raise ValueError("cu_seqlens go with packed [total, heads, hdim] inputs")
-            return self._fn("forward")(q, k, v, **kw)
+            return self._fn(dense)(q, k, v, **kw)
         if cu_seqlens_q is None or cu_seqlens_k is None:
             raise ValueError("packed inputs need cu_seqlens_q and cu_seqlens_k")
-        return self._fn("forward_var_len")(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, **kw)
+        return self._fn(packed)(q, k, v, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, **kw)
 
     def forward_paged(self, q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
                       seqlen_k: torch.Tensor, cu_seqlens_q: Optional[torch.Tensor] = None, max_seqlen_q: int = 0,

@@ -125,6 +125,26 @@ FLASHCK_API int FmhaFwdFp8(void* q_buf_ptr, void* k_buf_ptr, void* v_buf_ptr, vo
                void* lse_ptr, int dtype, int o_dtype);
 
 /*
+ * FmhaBwd -- gradients of FmhaFwd / FmhaFwdBias on contiguous K/V, from dO and the forward's O and LSE (the reference is
+ * forward only and has no counterpart; the argument list follows FmhaFwdBias).  hdim 64 or 128, dtype 3 or 4.
+ *   do, o [.., hq, dv], lse fp32 (required, the forward's), dlse fp32 or NULL: gradient of the LSE, in the LSE's layout;
+ *   dq, dk, dv: gradients in the shapes and type of q, k, v, overwritten (dk and dv summed over the heads of a group).  Group
+ *      mode: rows in front of the first and behind the last sequence are set to zero;
+ *   dbias: NULL, or the gradient of an elementwise bias in its shape and type (bias_enum 1 only), summed over what a plane is
+ *      shared by; group mode: elements outside the sequences' blocks are left as they were;
+ *   delta: fp32 workspace with as many elements as the LSE;
+ *   q_max_seq_len, kv_max_seq_len: the longest sequences in group mode (0 = the packed totals).
+ * Data pointers must be 16-byte aligned.  Every result is summed in a fixed order: equal calls give equal bits.
+ * Rows whose mask leaves no key (LSE = -inf) contribute nothing and get dQ = 0.
+ */
+FLASHCK_API int FmhaBwd(void* do_buf_ptr, void* q_buf_ptr, void* k_buf_ptr, void* v_buf_ptr, void* bias_buf_ptr, void* o_buf_ptr,
+            void* lse_ptr, void* dlse_ptr, void* dq_buf_ptr, void* dk_buf_ptr, void* dv_buf_ptr, void* dbias_buf_ptr,
+            void* delta_ptr, int64_t* q_seq_start_ptr, int64_t* k_seq_start_ptr, int64_t batch, int64_t q_seq_len,
+            int64_t kv_seq_len, int64_t q_num_heads, int64_t kv_num_heads, int64_t qk_head_dim, int64_t v_head_dim,
+            int64_t q_max_seq_len, int64_t kv_max_seq_len, float scale, int64_t window_left, int64_t window_right,
+            uint32_t mask_type, void* stream, int dtype, int bias_enum, int bias_rank_info, float logits_soft_cap);
+
+/*
  * FmhaFwdBatchPrefill -- varlen prefill whose K/V sit behind an SGLang-style page table.
  * The reference emits this family (core/profiling/attention/fmha_fwd_batch_prefill/
  * fmha_fwd_batch_prefill_codegen.cc:93-162, problem ..._problem.h:20-99 `num_total_pages`) but its glue

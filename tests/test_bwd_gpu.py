@@ -1,0 +1,244 @@
+"""The backward pass against its formula in 64 bits, within bounds that count its roundings."""
+import pytest
+import torch
+
+from attention_reference import assert_within, forward, gradients, half_step
+from flashck_b200 import _lib, ops
+from flashck_b200.nn import FlashAttention
+
+pytestmark = pytest.mark.gpu
+NONE, CAUSAL = (0, -1, -1), (2, -1, 0)
+
+
+def _options(mask):
+    return dict(mask_type=mask[0], window_size=mask[1:])
+
+
+def _problem(b, sq, sk, hq, hkv, d, dtype, mask, seed=0, bias=None, slopes=None, cap=0.0, scale=None):
+    g = torch.Generator("cuda").manual_seed(seed)
+    q, dout = (torch.randn(b, sq, hq, d, device="cuda", generator=g).to(dtype) for _ in range(2))
+    k, v = (torch.randn(b, sk, hkv, d, device="cuda", generator=g).to(dtype) for _ in range(2))
+    o, lse = forward(q, k, v, scale or d ** -0.5, mask, bias, slopes, cap)
+    return dout, q, k, v, o.to(dtype), lse.float()
+
+
+def _check(args, mask, bias=None, slopes=None, cap=0.0, dlse=None, scale=None):
+    d = args[1].shape[-1]
+    want, bound = gradients(*args, scale or d ** -0.5, mask, bias, slopes, cap, dlse)
+    got = ops.fmha_bwd(*args, scale=scale, bias=bias, alibi_slopes=slopes, logits_soft_cap=cap, dlse=dlse, return_dbias=bias is not None,
+                       **_options(mask))
+    for n, x, w, e in zip(("dq", "dk", "dv"), got, want, bound):
+        assert_within(n, x, w, e)
+    if bias is not None:
+        w, e = want[3], bound[3]
+        axes = [a for a in (0, 1) if bias.shape[a] == 1]
+        if axes:
+            w, e = w.sum(axes, keepdim=True), e.sum(axes, keepdim=True)
+        assert_within("dbias", got[3], w, e + half_step(bias.dtype) * w.abs() + 2.0 ** -25)
+    return got
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sq,sk,mask", [
+    (1, 1, NONE), (1, 300, CAUSAL), (64, 64, CAUSAL), (128, 128, NONE), (129, 129, CAUSAL), (257, 1000, CAUSAL), (300, 5, NONE),
+    (200, 100, CAUSAL),                          # rows that see nothing
+    (333, 333, (2, 17, 0)), (500, 500, (1, 64, 32)), (260, 700, (3, 5, 300)), (300, 40, (1, 20, 0)),
+    (640, 640, (2, 0, 0)), (384, 512, (2, -1, 100)),
+])
+def test_dense(dtype, d, sq, sk, mask, device_ok):
+    _check(_problem(2, sq, sk, 4, 2, d, dtype, mask), mask)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv", [(1, 1), (8, 1), (12, 4), (7, 7), (6, 2)])
+def test_head_groups(d, hq, hkv, device_ok):
+    _check(_problem(3, 200, 200, hq, hkv, d, torch.bfloat16, CAUSAL), CAUSAL)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("mask", [NONE, CAUSAL, (2, 50, 0)])
+@pytest.mark.parametrize("slopes_rank", [None, 1, 2])
+@pytest.mark.parametrize("cap", [0.0, 5.0])
+def test_alibi_and_soft_cap(d, mask, slopes_rank, cap, device_ok):
+    slopes = None if slopes_rank is None else torch.rand(1 if slopes_rank == 1 else 2, 4, device="cuda") * 0.2
+    _check(_problem(2, 190, 270, 4, 2, d, torch.bfloat16, mask, slopes=slopes, cap=cap), mask, slopes=slopes, cap=cap)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("planes", [(1, 1), (1, 4), (3, 4)])
+@pytest.mark.parametrize("sq,sk,mask", [(70, 131, NONE), (130, 130, CAUSAL)])
+def test_bias_and_its_gradient(d, planes, sq, sk, mask, device_ok):
+    bias = torch.randn(*planes, sq, sk, device="cuda", dtype=torch.float16)
+    _check(_problem(3, sq, sk, 4, 2, d, torch.float16, mask, bias=bias, cap=20.0), mask, bias=bias, cap=20.0)
+
+
+def test_scale_and_gradient_of_the_lse(device_ok):
+    args = _problem(2, 150, 150, 4, 2, 128, torch.bfloat16, CAUSAL, scale=0.3)
+    _check(args, CAUSAL, dlse=torch.randn(2, 4, 150, device="cuda"), scale=0.3)
+
+
+LENGTHS = [([1, 0, 130, 64, 257], [1, 0, 130, 64, 257]), ([5, 128, 3], [300, 128, 0]), ([200], [200]), ([0, 0], [7, 9])]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("mask", [NONE, CAUSAL, (2, 40, 0)])
+@pytest.mark.parametrize("lens", LENGTHS)
+@pytest.mark.parametrize("pad", [0, 37])
+def test_packed(d, mask, lens, pad, device_ok):
+    """Sequences of unequal lengths, with rows in front of the first and behind the last one that hold NaN."""
+    nq, nk = lens
+    hq, hkv, dtype = 4, 2, torch.bfloat16
+    starts = [torch.tensor([0] + n).cumsum(0).cuda() + pad for n in lens]
+    total = [sum(n) + 2 * pad for n in lens]
+    nan = lambda rows, h: torch.full((rows, h, d), float("nan"), device="cuda", dtype=dtype)  # noqa: E731
+    q, k, v, dout, o = nan(total[0], hq), nan(total[1], hkv), nan(total[1], hkv), nan(total[0], hq), nan(total[0], hq)
+    lse = torch.full((hq, total[0]), float("nan"), device="cuda")
+    want = []
+    for n, (a, c) in enumerate(zip(nq, nk)):
+        args = _problem(1, a, c, hq, hkv, d, dtype, mask, seed=n)
+        qs, ks = slice(starts[0][n], starts[0][n + 1]), slice(starts[1][n], starts[1][n + 1])
+        for t, x, rows in ((dout, args[0], qs), (q, args[1], qs), (k, args[2], ks), (v, args[3], ks), (o, args[4], qs)):
+            t[rows] = x[0]
+        lse[:, qs] = args[5][0]
+        want.append((qs, ks, *gradients(*args, d ** -0.5, mask)))
+    for longest in ((max(nq), max(nk)), (0, 0)):
+        dq, dk, dv = ops.fmha_bwd_var_len(dout, q, k, v, o, lse, *starts, *longest, **_options(mask))
+        for qs, ks, (wq, wk, wv, _), (eq, ek, ev, _) in want:
+            assert_within("dq", dq[qs], wq[0], eq[0])
+            assert_within("dk", dk[ks], wk[0], ek[0])
+            assert_within("dv", dv[ks], wv[0], ev[0])
+        for t, s in ((dq, starts[0]), (dk, starts[1]), (dv, starts[1])):
+            assert not t[: s[0]].any() and not t[s[-1]:].any()  # rows of no sequence: zeros
+
+
+def test_packed_bias_gradient_is_zero_outside_the_blocks(device_ok):
+    nq, nk, d, hq = [40, 90], [70, 65], 64, 2
+    cu_q, cu_k = (torch.tensor([0] + n).cumsum(0).cuda() for n in (nq, nk))
+    bias = torch.randn(1, hq, sum(nq), sum(nk), device="cuda", dtype=torch.bfloat16)
+    parts = [_problem(1, a, c, hq, hq, d, torch.bfloat16, NONE, seed=n, bias=bias[:, :, cu_q[n]: cu_q[n + 1], cu_k[n]: cu_k[n + 1]])
+             for n, (a, c) in enumerate(zip(nq, nk))]
+    dout, q, k, v, o = (torch.cat([p[n][0] for p in parts]) for n in range(5))
+    lse = torch.cat([p[5][0] for p in parts], dim=1).contiguous()
+    got = ops.fmha_bwd_var_len(dout, q, k, v, o, lse, cu_q, cu_k, max(nq), max(nk), bias=bias, return_dbias=True)[3]
+    outside = torch.ones_like(got, dtype=torch.bool)
+    for n, p in enumerate(parts):
+        block = (slice(None), slice(None), slice(cu_q[n], cu_q[n + 1]), slice(cu_k[n], cu_k[n + 1]))
+        want, bound = gradients(*p, d ** -0.5, NONE, bias=bias[block])
+        assert_within("dbias", got[block], want[3], bound[3] + half_step(bias.dtype) * want[3].abs())
+        outside[block] = False
+    assert not got[outside].any()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_nan_of_another_sequence_does_not_spread(d, device_ok):
+    """Tiles reach past a sequence's end into the next one, whose rows hold NaN and infinities here."""
+    args = _problem(2, 100, 100, 2, 2, d, torch.bfloat16, NONE)
+    for t in args[:5]:
+        t[1] = float("nan")
+        t[1, ::2] = float("inf")
+    got = ops.fmha_bwd(*args)
+    want, bound = gradients(*(t[:1] for t in args), d ** -0.5, NONE)
+    for n, x, w, e in zip(("dq", "dk", "dv"), got, want, bound):
+        assert_within(n, x[:1], w, e)
+
+
+def test_equal_calls_give_equal_bits(device_ok):
+    args = _problem(2, 700, 700, 8, 2, 128, torch.bfloat16, CAUSAL)
+    first = ops.fmha_bwd(*args, causal=True)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(first, ops.fmha_bwd(*args, causal=True)))
+
+
+def test_empty_sizes(device_ok):
+    def call(b, sq, sk):
+        t = lambda n: torch.zeros(b, n, 2, 64, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+        return ops.fmha_bwd(t(sq), t(sq), t(sk), t(sk), t(sq), torch.full((b, 2, sq), -float("inf"), device="cuda"))
+    for b, sq, sk in ((0, 4, 4), (2, 0, 0), (2, 0, 5), (2, 5, 0)):
+        for x in call(b, sq, sk):
+            assert not x.any()
+
+
+def test_differences(device_ok):
+    """<gradient, direction> against the difference quotient of the exact loss, for every input at once."""
+    d, mask = 64, CAUSAL
+    dout, q, k, v, _, _ = _problem(1, 40, 60, 4, 2, d, torch.float16, mask, cap=8.0)
+    dirs = [torch.randn_like(t, dtype=torch.float64) for t in (q, k, v)]
+
+    def loss(h):
+        o, _ = forward(*(t.double() + h * x for t, x in zip((q, k, v), dirs)), d ** -0.5, mask, cap=8.0)
+        return (o * dout.double()).sum()
+
+    o, lse = forward(q, k, v, d ** -0.5, mask, cap=8.0)
+    args = (dout, q, k, v, o.half(), lse.float())
+    got = ops.fmha_bwd(*args, causal=True, logits_soft_cap=8.0)
+    _, bound = gradients(*args, d ** -0.5, mask, cap=8.0)
+    h = 1e-5
+    slope = (loss(h) - loss(-h)) / (2 * h)
+    # O enters D rounded: dq and dk move by dS = P u sum |dO O| at most
+    extra = half_step(torch.float16) * (dout.double() * o).abs().sum(-1).amax() * d ** -0.5
+    allowed = sum((e * x.abs()).sum() for e, x in zip(bound, dirs))
+    allowed = allowed + extra * (dirs[0].abs().sum() * k.double().abs().amax() + q.double().abs().amax() * dirs[1].abs().sum() * q.shape[1])
+    assert abs(sum((g.double() * x).sum() for g, x in zip(got, dirs)) - slope) <= allowed
+
+
+def test_autograd_dense_and_packed(device_ok):
+    q, k, v = (torch.randn(2, 77, h, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for h in (4, 2, 2))
+    bias = torch.randn(1, 4, 77, 77, device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    o, lse = ops.fmha_autograd(q, k, v, causal=True, return_lse=True, bias=bias)
+    plain = ops.fmha_fwd(q, k, v, causal=True, return_lse=True, bias=bias)
+    assert torch.equal(o, plain[0]) and torch.equal(lse, plain[1])
+    w, wl = torch.randn_like(o), torch.randn_like(lse)
+    ((o * w).sum() + (lse * wl).sum()).backward()
+    want = ops.fmha_bwd(w, q.detach(), k.detach(), v.detach(), o.detach(), lse.detach(), causal=True, bias=bias.detach(), dlse=wl, return_dbias=True)
+    for t, g in zip((q, k, v, bias), want):
+        assert torch.equal(t.grad, g)
+    # the LSE alone; a gradient that is expanded, not contiguous; an input that needs none
+    g = torch.autograd.grad(ops.fmha_autograd(q, k, v.detach(), return_lse=True)[1].sum(), (q, k))
+    assert all(torch.isfinite(x).all() for x in g)
+    g1 = torch.autograd.grad(ops.fmha_autograd(q, k, v).sum(), (q, k, v))
+    o, lse = ops.fmha_fwd(q, k, v, return_lse=True)
+    assert all(torch.equal(a, b) for a, b in zip(g1, ops.fmha_bwd(torch.ones_like(o), q.detach(), k.detach(), v.detach(), o, lse)))
+    cu = torch.tensor([0, 30, 77], device="cuda")
+    qp, kp, vp = (t.detach()[0].clone().requires_grad_() for t in (q, k, v))
+    ops.fmha_autograd_var_len(qp, kp, vp, cu, cu, 47, 47, causal=True).square().sum().backward()
+    assert all(torch.isfinite(t.grad).all() and t.grad.any() for t in (qp, kp, vp))
+
+
+def test_attention_module_trains(device_ok):
+    """The module inside projections: its gradients against the same layer in 64 bits."""
+    torch.manual_seed(0)
+    attn = FlashAttention(4, 64, 2, causal=True)
+    x = torch.randn(2, 50, 96, device="cuda", dtype=torch.bfloat16)
+    proj = [torch.nn.Linear(96, h * 64, bias=False, device="cuda", dtype=torch.bfloat16) for h in (4, 2, 2)]
+    q, k, v = (p(x).unflatten(-1, (-1, 64)) for p in proj)
+    out = attn(q, k, v)
+    assert out.requires_grad
+    out.square().sum().backward()
+    wide = [p.weight.detach().double().requires_grad_() for p in proj]
+    qd, kd, vd = ((x.double() @ w.T).unflatten(-1, (-1, 64)) for w in wide)
+    o, _ = forward(qd, kd, vd, 64 ** -0.5, CAUSAL)
+    o.square().sum().backward()
+    for p, w in zip(proj, wide):
+        # five roundings of at most half a step on the way (q, o, dO, dq, the product), in norm
+        assert (p.weight.grad.double() - w.grad).norm() <= 5 * half_step(torch.bfloat16) * 2 * w.grad.norm()
+    with torch.no_grad():
+        assert not attn(q, k, v).requires_grad
+
+
+def test_other_stream_and_captured(device_ok):
+    args = _problem(2, 300, 300, 4, 2, 128, torch.bfloat16, CAUSAL)
+    want = ops.fmha_bwd(*args, causal=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.fmha_bwd(*args, causal=True)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.fmha_bwd(*args, causal=True)
+    for t in args[:2]:
+        t.copy_(t.flip(1))
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(got, ops.fmha_bwd(*args, causal=True)))
