@@ -7,7 +7,7 @@ not load the library, the first operator call does -- and raises if it is missin
 """
 from . import nn, ops, utils
 from .compat import install_as_flash_ck
-from .ops import (batch_prefill, fmha_autograd, fmha_autograd_var_len, fmha_bwd, fmha_bwd_var_len, fmha_fwd, fmha_fwd_append_kv, fmha_fwd_paged_kv_prefill, fmha_fwd_splitkv,
+from .ops import (batch_prefill, fmha_autograd, fmha_autograd_var_len, fmha_bwd, fmha_bwd_var_len, fmha_fwd, fmha_fwd_append_kv, fmha_fwd_paged_kv_prefill, fmha_fwd_shared_prefix, fmha_fwd_splitkv,
                   fmha_fwd_splitkv_combine, fmha_fwd_var_len)
 from .utils import (get_available_operations, get_flag_value, is_available, print_all_flags, print_flag_info,
                     register_flashck_functions, set_flag_value)
@@ -23,6 +23,7 @@ register_flashck_functions(utils.FlashCKOperationType.FMHA.value, {
     "forward_splitkv": fmha_fwd_splitkv,
     "splitkv_combine": fmha_fwd_splitkv_combine,
     "append_kv": fmha_fwd_append_kv,
+    "forward_shared_prefix": fmha_fwd_shared_prefix,
     "backward": fmha_bwd,
     "backward_var_len": fmha_bwd_var_len,
     "autograd": fmha_autograd,
@@ -31,7 +32,7 @@ register_flashck_functions(utils.FlashCKOperationType.FMHA.value, {
 
 __all__ = [
     "ops", "nn", "utils", "install_as_flash_ck", "fmha_fwd", "fmha_fwd_var_len", "batch_prefill", "fmha_fwd_paged_kv_prefill",
-    "fmha_fwd_splitkv", "fmha_fwd_splitkv_combine", "fmha_fwd_append_kv", "fmha_bwd", "fmha_bwd_var_len", "fmha_autograd",
+    "fmha_fwd_splitkv", "fmha_fwd_splitkv_combine", "fmha_fwd_append_kv", "fmha_fwd_shared_prefix", "fmha_bwd", "fmha_bwd_var_len", "fmha_autograd",
     "fmha_autograd_var_len", "is_available",
     "get_available_operations", "get_flag_value", "set_flag_value", "print_all_flags", "print_flag_info",
 ]

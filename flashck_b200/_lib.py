@@ -41,6 +41,8 @@ SIGNATURES = {
     "FlashckPeerBufferClose": ([_P], _I),
     "FlashckPeerBufferFree": ([_P], _I),
     "FmhaFwdSplitKVStatic": ([_P] * 10 + [_I64] * 11 + [_F, _I64, _I64, _U32, _P, _I], _I),
+    "FlashckSharedPrefixWorkspace": ([_I64] * 9 + [_I, _I], _I64),
+    "FmhaFwdSharedPrefix": ([_P] * 12 + [_I64] * 14 + [_F, _I, _P, _I], _I),
     "FmhaFwdAppendKV": ([_P] * 12 + [_I64] * 9 + [_I, _I64, _I64, _P, _I], _I),
     "FlashckSetInstanceParam": ([_I, ctypes.c_char_p, _I64], _I),
     "FlashckGetInstanceParam": ([_I, ctypes.c_char_p, ctypes.POINTER(_I64)], _I),

@@ -539,6 +539,65 @@ int FmhaSplitKVCombine(void* lse_acc, void* o_acc, void* o, int64_t* q_seq_start
                                  stream, lse, dtype);
 }
 
+int64_t FlashckSharedPrefixWorkspace(int64_t prefix_len, int64_t prefix_page, int64_t paged_block_size, int64_t batch, int64_t q_seq_len,
+                                     int64_t q_max_seq_len, int64_t hq, int64_t hkv, int64_t d, int group_mode, int dtype) {
+    if (prefix_len < 0 || prefix_page < 0 || paged_block_size < 0 || batch < 0 || q_seq_len < 0 || hq <= 0 || hkv <= 0 || hq % hkv != 0 || d <= 0) {
+        set_last_error("FlashckSharedPrefixWorkspace: bad size");
+        return -1;
+    }
+    SharedPrefixParams p{};
+    int64_t somewhere = 0;  // (stands for an array: only asked whether there is one)
+    p.prefix_table = prefix_page > 0 ? (const int32_t*)&somewhere : nullptr;
+    p.block_table = paged_block_size > 0 ? (const int32_t*)&somewhere : nullptr;
+    p.seqstart_q = group_mode ? &somewhere : nullptr;
+    p.prefix_len = prefix_len; p.prefix_page = prefix_page; p.page = paged_block_size;
+    p.batch = batch; p.seqlen_q = q_seq_len; p.max_seqlen_q = group_mode && q_max_seq_len > 0 ? q_max_seq_len : q_seq_len;
+    p.hq = hq; p.hkv = hkv; p.d = d; p.dtype = dtype;
+    return shared_prefix_workspace(p);
+}
+
+int FmhaFwdSharedPrefix(void* q, void* k_prefix, void* v_prefix, void* k, void* v, void* o, void* lse, void* workspace, void* prefix_table,
+                        void* block_table, void* k_seq_len, int64_t* q_seq_start, int64_t prefix_len, int64_t prefix_page,
+                        int64_t prefix_pool_pages, int64_t paged_block_size, int64_t num_pool_pages, int64_t block_table_stride,
+                        int64_t kv_seq_len, int64_t batch, int64_t q_seq_len, int64_t q_max_seq_len, int64_t hq, int64_t hkv, int64_t d,
+                        int64_t dv, float scale, int causal, void* stream, int dtype) {
+    int rc = check_common("FmhaFwdSharedPrefix", dtype, hq, hkv, d, dv, nullptr);
+    if (rc) return rc;
+    FCK_REQUIRE(d == dv && (d == 64 || d == 128), FLASHCK_ERR_UNSUPPORTED,
+                "FmhaFwdSharedPrefix: hdim_q == hdim_v in {64,128} required (got %lld/%lld)", (long long)d, (long long)dv);
+    FCK_REQUIRE(batch >= 0 && q_seq_len >= 0 && q_max_seq_len >= 0 && prefix_len >= 0 && kv_seq_len >= 0, FLASHCK_ERR_INVALID_ARGUMENT,
+                "FmhaFwdSharedPrefix: negative size");
+    if (batch == 0 || q_seq_len == 0) return FLASHCK_OK;
+    FCK_REQUIRE(q && k && v && o && k_seq_len && workspace && (prefix_len == 0 || (k_prefix && v_prefix)), FLASHCK_ERR_INVALID_ARGUMENT,
+                "FmhaFwdSharedPrefix: null pointer argument");
+    FCK_REQUIRE(((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_prefix | (uintptr_t)v_prefix | (uintptr_t)o | (uintptr_t)workspace) & 15) == 0),
+                FLASHCK_ERR_INVALID_ARGUMENT, "FmhaFwdSharedPrefix: the tensors must start on 16-byte boundaries");
+    FCK_REQUIRE(prefix_len < (1ll << 31) - 256, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSharedPrefix: prefix_len must stay below 2^31");
+    for (int i = 0; i < 2; ++i) {  // the two caches
+        const bool paged = i ? block_table != nullptr : prefix_table != nullptr;
+        const int64_t page = i ? paged_block_size : prefix_page, pages = i ? num_pool_pages : prefix_pool_pages;
+        if (!paged || (i == 0 && prefix_len == 0)) continue;
+        FCK_REQUIRE(page > 0 && page % 16 == 0, FLASHCK_ERR_UNSUPPORTED,
+                    "FmhaFwdSharedPrefix: pages must hold a positive multiple of 16 tokens (got %lld)", (long long)page);
+        FCK_REQUIRE(pages > 0 && pages * page < (1ll << 31), FLASHCK_ERR_INVALID_ARGUMENT,
+                    "FmhaFwdSharedPrefix: %lld pages in the K/V pools (at least 1, fewer than 2^31 tokens)", (long long)pages);
+    }
+    FCK_REQUIRE(!block_table || (block_table_stride >= 0 && block_table_stride * paged_block_size < (1ll << 31)), FLASHCK_ERR_INVALID_ARGUMENT,
+                "FmhaFwdSharedPrefix: bad block_table_stride");
+    FCK_REQUIRE(block_table || batch * kv_seq_len < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSharedPrefix: the caches hold 2^31 tokens or more");
+    FCK_REQUIRE(causal == 0 || causal == 1, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaFwdSharedPrefix: causal must be 0 or 1");
+    SharedPrefixParams p{};
+    p.q = q; p.k_prefix = k_prefix; p.v_prefix = v_prefix; p.k = k; p.v = v; p.o = o; p.lse = (float*)lse; p.workspace = workspace;
+    p.prefix_table = (const int32_t*)prefix_table; p.block_table = (const int32_t*)block_table; p.seqlen_k = (const int32_t*)k_seq_len;
+    p.seqstart_q = q_seq_start;
+    p.prefix_len = prefix_len; p.prefix_page = prefix_table ? prefix_page : 0; p.prefix_pool_pages = prefix_pool_pages;
+    p.page = block_table ? paged_block_size : 0; p.pool_pages = num_pool_pages; p.bt_stride = block_table ? block_table_stride : 0;
+    p.seqlen_k_cap = block_table ? 0 : kv_seq_len;
+    p.batch = batch; p.seqlen_q = q_seq_len; p.max_seqlen_q = q_seq_start && q_max_seq_len > 0 ? q_max_seq_len : q_seq_len;
+    p.hq = hq; p.hkv = hkv; p.d = d; p.scale = resolve_scale(scale, d); p.causal = causal != 0; p.dtype = dtype;
+    return launch_shared_prefix(p, (cudaStream_t)stream);
+}
+
 int FmhaFwdAppendKV(void* q, void* k_cache, void* knew, void* v_cache, void* vnew, void* k_seq_len,
                     int64_t* q_seq_start, int64_t* knew_seq_start, void* rotary_cos, void* rotary_sin,
                     void* block_table, int64_t* cache_batch_idx, int64_t batch, int64_t q_seq_len, int64_t kv_seq_len,

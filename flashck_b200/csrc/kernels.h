@@ -64,6 +64,7 @@ struct SplitKVParams {
     // the score of query i and key j gets -slope * |i + sk - sq - j| added
     const float* alibi_slopes;
     int alibi_rank;
+    bool one_length = false;  // paged: no length array, every sequence holds seqlen_k_cap keys
 };
 int launch_splitkv_decode(const SplitKVParams& p, cudaStream_t stream);
 // instance parameters (see FlashckSetInstanceParam): "stages", "ctas_per_sm_x100" ...
@@ -143,5 +144,28 @@ struct BwdParams {
     float logits_soft_cap;
 };
 int launch_bwd_generic(const BwdParams& p, cudaStream_t stream);
+
+// ---- decode over a prefix that all sequences share (shared_prefix.cu) ------------------------------------------
+struct SharedPrefixParams {
+    const void* q;
+    const void* k_prefix;  // [prefix_len, hkv, d], or a pool behind prefix_table
+    const void* v_prefix;
+    const void* k;         // own caches: [batch, seqlen_k_cap, hkv, d], or a pool behind block_table
+    const void* v;
+    void* o;
+    float* lse;            // or nullptr
+    const int32_t* prefix_table;
+    const int32_t* block_table;  // rows bt_stride apart
+    const int32_t* seqlen_k;
+    const int64_t* seqstart_q;   // group mode or nullptr
+    void* workspace;
+    int64_t prefix_len, prefix_page, prefix_pool_pages, page, pool_pages, bt_stride, seqlen_k_cap;
+    int64_t batch, seqlen_q, max_seqlen_q, hq, hkv, d;  // group mode: seqlen_q is the packed total
+    float scale;
+    bool causal;
+    int dtype;
+};
+int64_t shared_prefix_workspace(const SharedPrefixParams& p);
+int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream);
 
 }  // namespace fck

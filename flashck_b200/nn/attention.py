@@ -105,6 +105,15 @@ class FlashAttention(torch.nn.Module):
                                             max_seqlen_q=max_seqlen_q, scale=self.scale, causal=self.causal,
                                             window_size=self.window_size, return_lse=return_lse)
 
+    def forward_shared_prefix(self, q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: torch.Tensor, k_cache: torch.Tensor,
+                              v_cache: torch.Tensor, seqlen_k: torch.Tensor, **kwargs):
+        """Decode over a prefix that all sequences share and their own caches (:func:`fmha_fwd_shared_prefix`)."""
+        self._check_heads(q, k_cache)
+        if self.window_size != (-1, -1):
+            raise ValueError("a window does not go with a shared prefix")
+        return self._fn("forward_shared_prefix")(q, k_prefix, v_prefix, k_cache, v_cache, seqlen_k=seqlen_k, scale=self.scale,
+                                                 causal=self.causal, **kwargs)
+
     def append_kv(self, q: Optional[torch.Tensor], k_cache: torch.Tensor, v_cache: torch.Tensor, knew: torch.Tensor,
                   vnew: torch.Tensor, seqlen_k: torch.Tensor, rotary: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
                   rope: int = RopeEnum.INTERLEAVED, **kwargs):

@@ -291,6 +291,30 @@ FLASHCK_API int FlashckPeerBufferClose(void* ptr);
 FLASHCK_API int FlashckPeerBufferFree(void* ptr);
 
 /*
+ * FmhaFwdSharedPrefix -- decode for a batch whose sequences share a prefix, which is read once for all of them (the reference
+ * has no counterpart).  Every query row attends to the whole prefix and to its sequence's own keys; the result is that of
+ * FmhaFwdSplitKV + combine over the concatenation.
+ *   q, o [b,sq,hq,d] or group mode [total_q,hq,d] (q_seq_start int64 [b+1], q_seq_len = total_q, q_max_seq_len = longest; rows
+ *      of o and lse that belong to no sequence are left as they were); lse fp32 [b,hq,sq] / [hq,total_q] or NULL
+ *   k/v_prefix: [prefix_len,hkv,d], or with prefix_table (int32, the prefix's pages in order) pools of prefix_pool_pages
+ *      pages of prefix_page tokens; prefix_len may end inside a page, and may be 0
+ *   k/v: the own caches [b,kv_seq_len,hkv,d], or with block_table (int32, rows block_table_stride apart) pools of
+ *      num_pool_pages pages of paged_block_size tokens; k_seq_len_ptr int32 [b]: own keys of each sequence (0: none)
+ *   causal: 0, or 1: query i of a sequence with n queries and m own keys sees its own keys <= m - n + i (and the prefix)
+ *   workspace: FlashckSharedPrefixWorkspace(...) bytes of device memory, 16-byte aligned, used during the call only.
+ * hdim 64 or 128, dtype 3 or 4; pages of a multiple of 16 tokens.
+ */
+FLASHCK_API int64_t FlashckSharedPrefixWorkspace(int64_t prefix_len, int64_t prefix_page, int64_t paged_block_size, int64_t batch,
+                                     int64_t q_seq_len, int64_t q_max_seq_len, int64_t q_num_heads, int64_t kv_num_heads,
+                                     int64_t head_dim, int group_mode, int dtype);
+FLASHCK_API int FmhaFwdSharedPrefix(void* q_buf_ptr, void* k_prefix_ptr, void* v_prefix_ptr, void* k_buf_ptr, void* v_buf_ptr, void* o_buf_ptr,
+                        void* lse_ptr, void* workspace, void* prefix_table, void* block_table, void* k_seq_len_ptr,
+                        int64_t* q_seq_start_ptr, int64_t prefix_len, int64_t prefix_page, int64_t prefix_pool_pages,
+                        int64_t paged_block_size, int64_t num_pool_pages, int64_t block_table_stride, int64_t kv_seq_len,
+                        int64_t batch, int64_t q_seq_len, int64_t q_max_seq_len, int64_t q_num_heads, int64_t kv_num_heads,
+                        int64_t qk_head_dim, int64_t v_head_dim, float scale, int causal, void* stream, int dtype);
+
+/*
  * FmhaFwdAppendKV -- rotary embedding of Q and the new keys, and the K/V cache write.
  * The reference names the kind (core/profiling/attention/fmha_library.h:19,41), the rotary modes
  * (fmha_library.h:195-219: 0 none, 1 interleaved, 2 half-rotated) and the table generator
