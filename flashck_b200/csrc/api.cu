@@ -140,6 +140,7 @@ inline float resolve_scale(float scale, int64_t d) {
 // which instance the last forward / prefill call of this process ran on: 1 tcgen05, 0 general (instance parameter
 // "last_instance" of family 0, read-only; the tests use it to pin a problem to the instance it is meant for)
 std::atomic<int64_t> g_last_fwd_instance{-1};
+std::atomic<int64_t> g_use_sm100_bwd{1}, g_last_bwd_instance{-1};  // instance parameters "use_sm100_bwd", "last_bwd_instance": the same of FmhaBwd
 std::atomic<int64_t> g_log_fallback{0};  // instance parameter "log_fallback": say on stderr why a call left the tcgen05 instance
 
 int run_fwd(const FwdParams& p, cudaStream_t stream) {
@@ -310,7 +311,9 @@ int FmhaBwd(void* dout, void* q, void* k, void* v, void* bias, void* o, void* ls
     p.scale = resolve_scale(scale, d);
     p.mask_type = (int)mask_type; p.wl = window_left; p.wr = window_right; p.dtype = dtype;
     p.bias = bias_enum ? bias : nullptr; p.bias_type = bias_enum; p.bias_rank = bias_rank_info; p.logits_soft_cap = logits_soft_cap;
-    return launch_bwd_generic(p, (cudaStream_t)stream);
+    const bool sm100 = g_use_sm100_bwd.load() && bwd_sm100_supported(p);
+    g_last_bwd_instance = sm100 ? 1 : 0;
+    return sm100 ? launch_bwd_sm100(p, (cudaStream_t)stream) : launch_bwd_generic(p, (cudaStream_t)stream);
 }
 
 static int batch_prefill_impl(void* q, void* k, void* v, const float* slopes, int slope_rank, void* o, int64_t* q_seq_start,
@@ -641,6 +644,7 @@ int FlashckSetInstanceParam(int family, const char* key, int64_t value) {
         return FLASHCK_OK;
     }
     if (family == 0 && !strcmp(key, "log_fallback")) { g_log_fallback = value; return FLASHCK_OK; }
+    if (family == 0 && !strcmp(key, "use_sm100_bwd")) { g_use_sm100_bwd = value; return FLASHCK_OK; }
     if (!strcmp(key, "use_pdl")) { g_use_pdl = value; return FLASHCK_OK; }
     if (family == 0) rc = fwd_set_param(key, value);
     else if (family == 2) rc = split_key_of_sm100(key) ? fwd_set_param(key, value) : splitkv_set_param(key, value);
@@ -654,6 +658,8 @@ int FlashckGetInstanceParam(int family, const char* key, int64_t* value_out) {
     if (family == 0 && !strcmp(key, "bias_rank_info")) { *value_out = g_bias_rank_info; return FLASHCK_OK; }
     if (family == 0 && !strcmp(key, "last_instance")) { *value_out = g_last_fwd_instance; return FLASHCK_OK; }
     if (family == 0 && !strcmp(key, "log_fallback")) { *value_out = g_log_fallback; return FLASHCK_OK; }
+    if (family == 0 && !strcmp(key, "use_sm100_bwd")) { *value_out = g_use_sm100_bwd; return FLASHCK_OK; }
+    if (family == 0 && !strcmp(key, "last_bwd_instance")) { *value_out = g_last_bwd_instance; return FLASHCK_OK; }
     if (!strcmp(key, "use_pdl")) { *value_out = g_use_pdl; return FLASHCK_OK; }
     if (family == 0) rc = fwd_get_param(key, value_out);
     else if (family == 2) rc = split_key_of_sm100(key) ? fwd_get_param(key, value_out) : splitkv_get_param(key, value_out);

@@ -1,0 +1,70 @@
+// Backward of fmha_fwd on the tcgen05 kernels: which calls they take, the device parameters of a call, and the launches.
+#include "fmha_bwd_sm100.cuh"
+
+namespace fck {
+
+using namespace sm100;
+
+namespace {
+
+template <typename T, int HDIM, bool EXTRA>
+int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream) {
+    constexpr size_t TILE = 128 * HDIM * 2;
+    const int64_t rows_q = p.seqstart_q ? p.seqlen_q : p.batch * p.seqlen_q, rows_k = p.seqstart_k ? p.seqlen_k : p.batch * p.seqlen_k;
+    CUtensorMap mq, mdo, mk, mv;
+    int rc;
+    if ((rc = make_map_3d(&mq, p.q, p.dtype, rows_q, p.hq, 128, HDIM))) return rc;
+    if ((rc = make_map_3d(&mdo, p.dout, p.dtype, rows_q, p.hq, 128, HDIM))) return rc;
+    if ((rc = make_map_3d(&mk, p.k, p.dtype, rows_k, p.hkv, 128, HDIM))) return rc;
+    if ((rc = make_map_3d(&mv, p.v, p.dtype, rows_k, p.hkv, 128, HDIM))) return rc;
+    auto dq = bwd_dq_sm100_kernel<T, HDIM, EXTRA>;
+    auto dkdv = bwd_dkdv_sm100_kernel<T, HDIM, EXTRA>;
+    constexpr size_t smem_dq = 1024 + 5 * TILE + 128 * sizeof(float) + sizeof(BwdCtrl);
+    constexpr size_t smem_dkdv = 7 * TILE + 512 * sizeof(float) + sizeof(BwdCtrl);
+    static_assert(smem_dq <= 227 * 1024 && smem_dkdv <= 227 * 1024, "tiles and the control block must fit the 227 KB a CTA can have");
+    static thread_local int configured_device = -1;  // per instantiation
+    int devid = 0;
+    FCK_CUDA(cudaGetDevice(&devid));
+    if (configured_device != devid) {
+        FCK_CUDA(cudaFuncSetAttribute(dq, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_dq));
+        FCK_CUDA(cudaFuncSetAttribute(dkdv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_dkdv));
+        configured_device = devid;
+    }
+    const unsigned grid_q = (unsigned)((p.max_seqlen_q + 127) / 128 * p.hq * p.batch), grid_k = (unsigned)((p.max_seqlen_k + 127) / 128 * p.hkv * p.batch);
+    FCK_CUDA(launch_dependent(dq, dim3(grid_q), dim3(kBwdThreads), smem_dq, stream, mk, mv, dev));
+    FCK_CUDA(launch_dependent(dkdv, dim3(grid_k), dim3(kBwdThreads), smem_dkdv, stream, mq, mdo, mk, mv, dev));
+    return FLASHCK_OK;
+}
+
+template <typename T>
+int launch_bwd_d(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream) {
+    const bool extra = p.bias_type == 2 || p.logits_soft_cap > 0.f;
+    if (p.d == 128) return extra ? launch_bwd_t<T, 128, true>(p, dev, stream) : launch_bwd_t<T, 128, false>(p, dev, stream);
+    return extra ? launch_bwd_t<T, 64, true>(p, dev, stream) : launch_bwd_t<T, 64, false>(p, dev, stream);
+}
+
+}  // namespace
+
+bool bwd_sm100_supported(const BwdParams& p) {
+    if (p.bias_type == 1) return false;  // an elementwise bias: the general instance
+    if (p.max_seqlen_q == 0 || p.max_seqlen_k == 0 || p.batch == 0) return false;  // (nothing to multiply)
+    if (p.wl >= (1ll << 30) || p.wr >= (1ll << 30)) return false;
+    return (p.max_seqlen_q + 127) / 128 * p.hq * p.batch < (1ll << 31) && (p.max_seqlen_k + 127) / 128 * p.hkv * p.batch < (1ll << 31);
+}
+
+int launch_bwd_sm100(const BwdParams& p, cudaStream_t stream) {
+    int* status = device_status_ptr();
+    if (!status) return FLASHCK_ERR_CUDA;
+    BwdSm100Dev dev{};
+    dev.dout = p.dout; dev.q = p.q; dev.o = p.o; dev.lse = p.lse; dev.dlse = p.dlse; dev.delta = p.delta;
+    dev.dq = p.dq; dev.dk = p.dk; dev.dv = p.dv; dev.seqstart_q = p.seqstart_q; dev.seqstart_k = p.seqstart_k; dev.status = status;
+    dev.batch = (int)p.batch; dev.seqlen_q = (int)p.seqlen_q; dev.seqlen_k = (int)p.seqlen_k; dev.hq = (int)p.hq; dev.hkv = (int)p.hkv;
+    dev.mask_type = p.mask_type; dev.wl = p.wl < 0 ? -1 : (int)p.wl; dev.wr = p.wr < 0 ? -1 : (int)p.wr;
+    dev.scale = p.scale; dev.scale_log2 = p.scale * kLog2e;
+    dev.alibi = p.bias_type == 2 ? (const float*)p.bias : nullptr; dev.alibi_rank = p.bias_rank;
+    dev.cap = p.logits_soft_cap; dev.cap_log2 = p.logits_soft_cap * kLog2e;
+    dev.two_inv_cap_log2 = p.logits_soft_cap > 0.f ? 2.f * kLog2e * (p.scale / p.logits_soft_cap) : 0.f;
+    return p.dtype == FLASHCK_DTYPE_BFLOAT16 ? launch_bwd_d<__nv_bfloat16>(p, dev, stream) : launch_bwd_d<__half>(p, dev, stream);
+}
+
+}  // namespace fck

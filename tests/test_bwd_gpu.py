@@ -10,6 +10,14 @@ pytestmark = pytest.mark.gpu
 NONE, CAUSAL = (0, -1, -1), (2, -1, 0)
 
 
+@pytest.fixture(params=["tcgen05", "general"])
+def instance(request):
+    """Both instances of the kernels take a test; a problem that the tcgen05 one does not serve runs on the other both times."""
+    _lib.set_instance_param(0, "use_sm100_bwd", int(request.param == "tcgen05"))
+    yield request.param
+    _lib.set_instance_param(0, "use_sm100_bwd", 1)
+
+
 def _options(mask):
     return dict(mask_type=mask[0], window_size=mask[1:])
 
@@ -46,13 +54,22 @@ def _check(args, mask, bias=None, slopes=None, cap=0.0, dlse=None, scale=None):
     (333, 333, (2, 17, 0)), (500, 500, (1, 64, 32)), (260, 700, (3, 5, 300)), (300, 40, (1, 20, 0)),
     (640, 640, (2, 0, 0)), (384, 512, (2, -1, 100)),
 ])
-def test_dense(dtype, d, sq, sk, mask, device_ok):
+def test_dense(dtype, d, sq, sk, mask, instance, device_ok):
     _check(_problem(2, sq, sk, 4, 2, d, dtype, mask), mask)
+
+
+def test_which_instance_serves(instance, device_ok):
+    args = _problem(1, 64, 64, 2, 2, 64, torch.bfloat16, NONE)
+    ops.fmha_bwd(*args)
+    assert _lib.get_instance_param(0, "last_bwd_instance") == int(instance == "tcgen05")
+    bias = torch.zeros(1, 1, 64, 64, device="cuda", dtype=torch.bfloat16)
+    ops.fmha_bwd(*args, bias=bias)
+    assert _lib.get_instance_param(0, "last_bwd_instance") == 0
 
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("hq,hkv", [(1, 1), (8, 1), (12, 4), (7, 7), (6, 2)])
-def test_head_groups(d, hq, hkv, device_ok):
+def test_head_groups(d, hq, hkv, instance, device_ok):
     _check(_problem(3, 200, 200, hq, hkv, d, torch.bfloat16, CAUSAL), CAUSAL)
 
 
@@ -60,7 +77,7 @@ def test_head_groups(d, hq, hkv, device_ok):
 @pytest.mark.parametrize("mask", [NONE, CAUSAL, (2, 50, 0)])
 @pytest.mark.parametrize("slopes_rank", [None, 1, 2])
 @pytest.mark.parametrize("cap", [0.0, 5.0])
-def test_alibi_and_soft_cap(d, mask, slopes_rank, cap, device_ok):
+def test_alibi_and_soft_cap(d, mask, slopes_rank, cap, instance, device_ok):
     slopes = None if slopes_rank is None else torch.rand(1 if slopes_rank == 1 else 2, 4, device="cuda") * 0.2
     _check(_problem(2, 190, 270, 4, 2, d, torch.bfloat16, mask, slopes=slopes, cap=cap), mask, slopes=slopes, cap=cap)
 
@@ -73,7 +90,7 @@ def test_bias_and_its_gradient(d, planes, sq, sk, mask, device_ok):
     _check(_problem(3, sq, sk, 4, 2, d, torch.float16, mask, bias=bias, cap=20.0), mask, bias=bias, cap=20.0)
 
 
-def test_scale_and_gradient_of_the_lse(device_ok):
+def test_scale_and_gradient_of_the_lse(instance, device_ok):
     args = _problem(2, 150, 150, 4, 2, 128, torch.bfloat16, CAUSAL, scale=0.3)
     _check(args, CAUSAL, dlse=torch.randn(2, 4, 150, device="cuda"), scale=0.3)
 
@@ -85,7 +102,7 @@ LENGTHS = [([1, 0, 130, 64, 257], [1, 0, 130, 64, 257]), ([5, 128, 3], [300, 128
 @pytest.mark.parametrize("mask", [NONE, CAUSAL, (2, 40, 0)])
 @pytest.mark.parametrize("lens", LENGTHS)
 @pytest.mark.parametrize("pad", [0, 37])
-def test_packed(d, mask, lens, pad, device_ok):
+def test_packed(d, mask, lens, pad, instance, device_ok):
     """Sequences of unequal lengths, with rows in front of the first and behind the last one that hold NaN."""
     nq, nk = lens
     hq, hkv, dtype = 4, 2, torch.bfloat16
@@ -131,7 +148,7 @@ def test_packed_bias_gradient_is_zero_outside_the_blocks(device_ok):
 
 
 @pytest.mark.parametrize("d", [64, 128])
-def test_nan_of_another_sequence_does_not_spread(d, device_ok):
+def test_nan_of_another_sequence_does_not_spread(d, instance, device_ok):
     """Tiles reach past a sequence's end into the next one, whose rows hold NaN and infinities here."""
     args = _problem(2, 100, 100, 2, 2, d, torch.bfloat16, NONE)
     for t in args[:5]:
@@ -143,14 +160,14 @@ def test_nan_of_another_sequence_does_not_spread(d, device_ok):
         assert_within(n, x[:1], w, e)
 
 
-def test_equal_calls_give_equal_bits(device_ok):
+def test_equal_calls_give_equal_bits(instance, device_ok):
     args = _problem(2, 700, 700, 8, 2, 128, torch.bfloat16, CAUSAL)
     first = ops.fmha_bwd(*args, causal=True)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, ops.fmha_bwd(*args, causal=True)))
 
 
-def test_empty_sizes(device_ok):
+def test_empty_sizes(instance, device_ok):
     def call(b, sq, sk):
         t = lambda n: torch.zeros(b, n, 2, 64, device="cuda", dtype=torch.bfloat16)  # noqa: E731
         return ops.fmha_bwd(t(sq), t(sq), t(sk), t(sk), t(sq), torch.full((b, 2, sq), -float("inf"), device="cuda"))
@@ -226,7 +243,7 @@ def test_attention_module_trains(device_ok):
         assert not attn(q, k, v).requires_grad
 
 
-def test_other_stream_and_captured(device_ok):
+def test_other_stream_and_captured(instance, device_ok):
     args = _problem(2, 300, 300, 4, 2, 128, torch.bfloat16, CAUSAL)
     want = ops.fmha_bwd(*args, causal=True)
     side = torch.cuda.Stream()
