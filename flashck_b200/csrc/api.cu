@@ -80,6 +80,13 @@ PFN_encodeTiled get_encode_tiled() {
             qres == cudaDriverEntryPointSuccess)
             fn = reinterpret_cast<PFN_encodeTiled>(sym);
     });
+    // A driver call needs a current context, which a thread that has only allocated from a framework's cache so far may not have
+    // (autograd's worker threads): the first call of a thread binds its device's.
+    static thread_local bool bound = false;
+    if (!bound) {
+        int dev = 0;
+        bound = cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess;
+    }
     return fn;
 }
 

@@ -259,3 +259,24 @@ def test_other_stream_and_captured(instance, device_ok):
         t.copy_(t.flip(1))
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(got, ops.fmha_bwd(*args, causal=True)))
+
+
+def test_first_call_of_a_thread(device_ok):
+    """A thread that has made no CUDA call of its own yet (autograd's worker threads are such): forward and backward."""
+    import threading
+    args = _problem(1, 130, 130, 2, 2, 128, torch.bfloat16, CAUSAL)
+    want = ops.fmha_bwd(*args, causal=True)
+    got, failed = [], []
+
+    def work(f):
+        try:
+            got.append(f())
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    for f in (lambda: ops.fmha_bwd(*args, causal=True), lambda: ops.fmha_fwd(*args[1:4], causal=True)):
+        t = threading.Thread(target=work, args=(f,))
+        t.start()
+        t.join()
+    assert not failed, failed
+    assert all(torch.equal(a, b) for a, b in zip(got[0], want)) and torch.isfinite(got[1]).all()
