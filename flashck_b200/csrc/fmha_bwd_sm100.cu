@@ -19,7 +19,7 @@ int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
     if ((rc = make_map_3d(&mv, p.v, p.dtype, rows_k, p.hkv, 128, HDIM))) return rc;
     auto dq = bwd_dq_sm100_kernel<T, HDIM, EXTRA>;
     auto dkdv = bwd_dkdv_sm100_kernel<T, HDIM, EXTRA>;
-    constexpr size_t smem_dq = 1024 + 5 * TILE + 128 * sizeof(float) + sizeof(BwdCtrl);
+    constexpr size_t smem_dq = 1024 + 5 * TILE + 512 * sizeof(float) + sizeof(BwdCtrl);
     constexpr size_t smem_dkdv = 7 * TILE + 512 * sizeof(float) + sizeof(BwdCtrl);
     static_assert(smem_dq <= 227 * 1024 && smem_dkdv <= 227 * 1024, "tiles and the control block must fit the 227 KB a CTA can have");
     static thread_local int configured_device = -1;  // per instantiation
@@ -30,9 +30,16 @@ int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
         FCK_CUDA(cudaFuncSetAttribute(dkdv, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_dkdv));
         configured_device = devid;
     }
-    const unsigned grid_q = (unsigned)((p.max_seqlen_q + 127) / 128 * p.hq * p.batch), grid_k = (unsigned)((p.max_seqlen_k + 127) / 128 * p.hkv * p.batch);
-    FCK_CUDA(launch_dependent(dq, dim3(grid_q), dim3(kBwdThreads), smem_dq, stream, mk, mv, dev));
-    FCK_CUDA(launch_dependent(dkdv, dim3(grid_k), dim3(kBwdThreads), smem_dkdv, stream, mq, mdo, mk, mv, dev));
+    for (int i = 0; i < 2; ++i) {
+        BwdSm100Dev d = dev;
+        const int64_t tiles = ((i ? p.max_seqlen_k : p.max_seqlen_q) + 127) / 128, items = tiles * (i ? p.hkv : p.hq) * p.batch;
+        // (one item per CTA where they all fit at once; more sequences than the schedule holds are dealt by the hardware)
+        d.listed = items > sm_count() && p.batch <= kBwdMaxBatch;
+        d.max_tiles = (int)tiles;
+        const dim3 grid((unsigned)(d.listed ? sm_count() : items));
+        if (i == 0) FCK_CUDA(launch_dependent(dq, grid, dim3(kBwdDqThreads), smem_dq, stream, mk, mv, d));
+        else FCK_CUDA(launch_dependent(dkdv, grid, dim3(kBwdDkdvThreads), smem_dkdv, stream, mq, mdo, mk, mv, d));
+    }
     return FLASHCK_OK;
 }
 
@@ -62,8 +69,11 @@ int launch_bwd_sm100(const BwdParams& p, cudaStream_t stream) {
     dev.mask_type = p.mask_type; dev.wl = p.wl < 0 ? -1 : (int)p.wl; dev.wr = p.wr < 0 ? -1 : (int)p.wr;
     dev.scale = p.scale; dev.scale_log2 = p.scale * kLog2e;
     dev.alibi = p.bias_type == 2 ? (const float*)p.bias : nullptr; dev.alibi_rank = p.bias_rank;
-    dev.cap = p.logits_soft_cap; dev.cap_log2 = p.logits_soft_cap * kLog2e;
-    dev.two_inv_cap_log2 = p.logits_soft_cap > 0.f ? 2.f * kLog2e * (p.scale / p.logits_soft_cap) : 0.f;
+    dev.soft_cap = p.logits_soft_cap;
+    if (p.logits_soft_cap > 0.f) {
+        dev.cap = soft_cap_constants(p.scale, p.logits_soft_cap);
+        dev.inv_cap_log2 = 1.f / (p.logits_soft_cap * kLog2e);
+    }
     return p.dtype == FLASHCK_DTYPE_BFLOAT16 ? launch_bwd_d<__nv_bfloat16>(p, dev, stream) : launch_bwd_d<__half>(p, dev, stream);
 }
 

@@ -141,21 +141,7 @@ int launch_fwd_sm100(const FwdParams& p, cudaStream_t stream) {
     const int expm = extra ? 0 : (int)g_exp_mode.load();
     dev.rescale_thr = expm == 1 ? 0.01f * (float)g_rescale_half_x100.load() : kRescaleThreshold;
     dev.soft_cap = p.logits_soft_cap;
-    if (p.logits_soft_cap > 0.f) {
-        const float k = p.scale * (1.f / p.logits_soft_cap), c0 = dev.scale_log2;
-        SoftCap& s = dev.cap;
-        // The coefficients carry powers of k up to the eighth, so that the raw score itself is the variable.  Where the last
-        // one leaves the range in which products keep 24 bits (a scale of 0.0884 with caps above 2000, say), the score is
-        // multiplied by k first instead, in the branch that has both forms.
-        const auto last = [&](float kk) { return 0.017135002f * (c0 * (kk * kk) * (kk * kk)); };
-        const float l = fabsf(last(k * k));
-        const bool powers = fabsf(k) < 1e3f && l > 1e-36f && l < 1e36f;
-        const float kk = powers ? k * k : 1.f;
-        s.lim = 0.5f / fabsf(k); s.lim_all = powers ? s.lim : -1.f; s.k = k;
-        s.c0 = c0; s.c1 = -0.33333069f * (c0 * kk); s.c2 = 0.13324779f * (c0 * kk * kk);
-        s.c3 = -0.052986056f * (c0 * kk * kk * kk); s.c4 = last(kk);
-        s.k2e = 2.885390081777927f * k; s.c = copysignf(p.logits_soft_cap * kLog2e, k); s.m2c = -2.f * s.c;
-    }
+    if (p.logits_soft_cap > 0.f) dev.cap = soft_cap_constants(p.scale, p.logits_soft_cap);
     dev.alibi = (p.bias && p.bias_type == 2) ? (const float*)p.bias : nullptr; dev.alibi_rank = p.bias_rank;
     if (p.dtype == FLASHCK_DTYPE_FLOAT8 || p.dtype == FLASHCK_DTYPE_BFLOAT8) {
         // The running max may lag the row max by `thr` (P up to 2^thr) only as far as P * scale_p stays inside the 8-bit

@@ -62,6 +62,23 @@ struct SoftCap {
     float k2e, c, m2c;         // the quotient form: exponent per unit of raw score, cap in base-2 units, -2 c
 };
 
+inline SoftCap soft_cap_constants(float scale, float cap) {
+    SoftCap s{};
+    const float k = scale * (1.f / cap), c0 = scale * 1.4426950408889634f;
+    // The coefficients carry powers of k up to the eighth, so that the raw score itself is the variable.  Where the last
+    // one leaves the range in which products keep 24 bits (a scale of 0.0884 with caps above 2000, say), the score is
+    // multiplied by k first instead, in the branch that has both forms.
+    const auto last = [&](float kk) { return 0.017135002f * (c0 * (kk * kk) * (kk * kk)); };
+    const float l = fabsf(last(k * k));
+    const bool powers = fabsf(k) < 1e3f && l > 1e-36f && l < 1e36f;
+    const float kk = powers ? k * k : 1.f;
+    s.lim = 0.5f / fabsf(k); s.lim_all = powers ? s.lim : -1.f; s.k = k;
+    s.c0 = c0; s.c1 = -0.33333069f * (c0 * kk); s.c2 = 0.13324779f * (c0 * kk * kk);
+    s.c3 = -0.052986056f * (c0 * kk * kk * kk); s.c4 = last(kk);
+    s.k2e = 2.885390081777927f * k; s.c = copysignf(cap * kLog2e, k); s.m2c = -2.f * s.c;
+    return s;
+}
+
 struct Sm100Dev {
     void* o;
     float* lse;

@@ -54,8 +54,8 @@ def gradients(dout, q, k, v, o, lse, scale, mask, bias=None, slopes=None, cap=0.
     """(dq, dk, dv, dT) and the bounds of their errors, all in 64 bits; dT is [b, hq, sq, sk].
 
     The bounds count, for inputs of half step u: P and dS rounded to the element type where they enter a product (u each), the
-    result rounded once (u), sums of d fp32 terms (d 2^-24 of the sum of magnitudes) in S, dP and D, and 2^-20 for the
-    exponential; the soft cap's tanh is good to 2^-21 of the cap."""
+    result rounded once (u), sums of d fp32 terms (d 2^-24 of the sum of magnitudes) in S, dP and D, and 2^-18 for the
+    exponential (the polynomial of the tcgen05 kernels is good to 2.7e-6 = 2^-18.5); the soft cap's tanh is good to 2^-21 of the cap."""
     hq, hkv, d, u = q.shape[2], k.shape[2], q.shape[3], half_step(q.dtype)
     qd, kd, vd = (_heads_first(t, hq) for t in (q, k, v))
     do, od = _heads_first(dout, hq), _heads_first(o, hq)
@@ -75,7 +75,7 @@ def gradients(dout, q, k, v, o, lse, scale, mask, bias=None, slopes=None, cap=0.
     sums = d * 2.0 ** -24
     # relative error of a P: what the sum in S moves the exponent by, the exponential itself; the largest additions in fp32
     big = x.masked_fill(torch.isneginf(x), 0.0).abs() + lse.masked_fill(torch.isneginf(lse), 0.0).abs()
-    e = sums * scale * (qd.abs() @ kd.abs().transpose(2, 3)) + 2.0 ** -20 + 2.0 ** -22 * big + (cap * 2.0 ** -21 + 2.0 ** -12 if cap else 0.0)
+    e = sums * scale * (qd.abs() @ kd.abs().transpose(2, 3)) + 2.0 ** -18 + 2.0 ** -22 * big + (cap * 2.0 ** -21 + 2.0 ** -12 if cap else 0.0)
     mag = do.abs() @ vd.abs().transpose(2, 3) + (do * od).abs().sum(-1, keepdim=True)
     e_dt = e * dt.abs() + 2 * sums * p * mag
     tiny = torch.finfo(q.dtype).smallest_normal * u if q.dtype == torch.float16 else 0.0  # (fp16: half the spacing of its subnormals)

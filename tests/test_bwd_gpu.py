@@ -129,6 +129,27 @@ def test_packed(d, mask, lens, pad, instance, device_ok):
             assert not t[: s[0]].any() and not t[s[-1]:].any()  # rows of no sequence: zeros
 
 
+@pytest.mark.parametrize("lens", [[(i * 37) % 200 for i in range(300)],               # more sequences than the schedule orders
+                                  [(i * 131) % 700 + 1 for i in range(40)],             # many items per CTA, levels of unequal size
+                                  [2000, 1, 1500, 0, 900, 128, 3]])
+@pytest.mark.parametrize("hq,hkv,d,mask", [(8, 2, 128, CAUSAL), (6, 6, 64, NONE), (8, 1, 64, (2, 300, 10))])
+def test_many_items(lens, hq, hkv, d, mask, device_ok):
+    """Several items per CTA: every sequence alone gives the same bits as in the packed call, and some are held to the formula."""
+    args = [_problem(1, n, n, hq, hkv, d, torch.bfloat16, mask, seed=i) for i, n in enumerate(lens)]
+    dout, q, k, v, o = (torch.cat([a[j][0] for a in args]) for j in range(5))
+    lse = torch.cat([a[5][0] for a in args], dim=1).contiguous()
+    cu = torch.tensor([0] + lens).cumsum(0).cuda()
+    got = ops.fmha_bwd_var_len(dout, q, k, v, o, lse, cu, cu, max(lens), max(lens), **_options(mask))
+    at = cu.tolist()
+    for i, a in enumerate(args):
+        part = [g[at[i]: at[i + 1]] for g in got]
+        if i % 10 == 0 or lens[i] > 1000:
+            want, bound = gradients(*a, d ** -0.5, mask)
+            for n, x, w, e in zip(("dq", "dk", "dv"), part, want, bound):
+                assert_within(f"{n} of sequence {i}", x, w[0], e[0])
+        assert all(torch.equal(x, y[0]) for x, y in zip(part, ops.fmha_bwd(*a, **_options(mask))))
+
+
 def test_packed_bias_gradient_is_zero_outside_the_blocks(device_ok):
     nq, nk, d, hq = [40, 90], [70, 65], 64, 2
     cu_q, cu_k = (torch.tensor([0] + n).cumsum(0).cuda() for n in (nq, nk))
