@@ -11,11 +11,13 @@
 // = 1280 clocks beside 1536 of products (Q and dO live in tensor memory, so all three products are TS); dK/dV 2 x 512 + 2 x 256 +
 // 512 = 2048 beside 2048.  P and dS go from registers to tensor memory as A operands and never through shared memory.
 //
-// The kernels are persistent (one CTA per SM).  Roles: warps 0-7 the elementwise work (thread = tensor memory lane = row; warps
-// 0-3 take columns 0-63 of a tile, 4-7 columns 64-127), warp 8 issues S and dP, another warp the products that P and dS enter (a
-// single issuer spends as long on its waits and commits as the products take, and the tensor pipe takes instructions only
-// about one ahead: 16 % slower), warp 9 the TMA copies, warp 11 finds the work items and hands them to the others through a ring.
-// dQ: warps 12-15 bring Q and dO to tensor memory and compute D.  dK/dV: warp 10 fetches LSE and D of the query columns.
+// The kernels are persistent (one CTA per SM).  Roles: warps 0-15 the elementwise work (thread = tensor memory lane = row; four
+// warpgroups, 32 columns of a 128-column tile each: four warps per scheduler, in code of 32 elements, hide each other's round trips
+// to tensor memory, where two warps with 64 elements took half as long again), warp 16 issues S, warp 17 the other products
+// (a single issuer spends as long on its waits and commits as the products take, and the tensor pipe takes instructions only
+// about one ahead: 16 % slower; dP follows the product that has read dS from its columns in one warp's order, without a
+// barrier between them), warp 18 finds the work items, hands them to the others through a ring and
+// issues the TMA copies, warp 19 computes D (dQ) or fetches LSE and D of the query columns (dK/dV).
 //   dQ works by halves h of 64 keys, each with its own barriers: one half's products run under the other's elementwise work.
 //   dK/dV: two 128-column regions change roles from step to step: P(i) and dS(i) lie in the region that S(i) came in, so that S(i+1)
 //   can take the other one as soon as dP(i) has been read from it.
@@ -83,11 +85,11 @@ __device__ __forceinline__ void bwd_issue_ts(uint32_t d, uint32_t a, uint64_t b,
     for (int ks = 0; ks < HDIM / 16; ++ks)
         umma_ts(d, a + ks * 8, b + (uint64_t)(((ks / 4) * HALF_BYTES + (ks % 4) * 32) >> 4), idesc, ks > 0 ? 1u : 0u);
 }
-// D += X B over 64 of 128 rows (half 0 / 1): X in tensor memory, 32 columns from a + 64 half; B MN-major.
+// D += X B over 64 of 128 rows (half 0 / 1): X in tensor memory, every 32 rows 16 columns in steps of 32; B MN-major.
 __device__ __forceinline__ void bwd_issue_xb(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int half, bool accumulate) {
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-        umma_ts(d, a + half * 64 + ks * 8, b + (uint64_t)(((half * 4 + ks) * 2048) >> 4), idesc, (accumulate || ks > 0) ? 1u : 0u);
+    for (int ks = half * 4; ks < half * 4 + 4; ++ks)
+        umma_ts(d, a + (ks / 2) * 32 + (ks % 2) * 8, b + (uint64_t)((ks * 2048) >> 4), idesc, (accumulate || ks > half * 4) ? 1u : 0u);
 }
 
 // 2^x on the FMA pipe for two values: x = n + f, f in [-0.5, 0.5], 2^f by the polynomial of degree 4 of least relative error
@@ -104,11 +106,12 @@ __device__ __forceinline__ float2 bwd_exp2_poly(float2 x) {
     return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
                        __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
 }
-// The exponentials of a pair: pairs `i` of every 8 below kPolyPairs go to the FMA pipe, the others to the exp2 unit, which alone would
+// The exponentials of a pair: pairs `i` of every 8 below POLY go to the FMA pipe, the others to the exp2 unit, which alone would
 // take 1024 clocks per tile.
-constexpr int kPolyPairs = 3;
+constexpr int kPolyDq = 1, kPolyDkdv = 3;
+template <int POLY>
 __device__ __forceinline__ float2 bwd_exp2(float2 y, int i) {
-    return (i & 7) < kPolyPairs ? bwd_exp2_poly(y) : make_float2(ex2_fast(y.x), ex2_fast(y.y));
+    return (i & 7) < POLY ? bwd_exp2_poly(y) : make_float2(ex2_fast(y.x), ex2_fast(y.y));
 }
 
 // Base-2 exponent of a pair of scores (raw, or with EXTRA what soft_cap_scores left of them), LSE subtracted; with a soft cap
@@ -127,18 +130,73 @@ __device__ __forceinline__ float2 bwd_exponent(const BwdSm100Dev& p, float2 x, f
     return __fadd2_rn(y, neg_lse2);
 }
 
-// 32 fp32 columns of one row, times f, as 64 bytes of the element type.
-template <typename T>
-__device__ __forceinline__ void bwd_store32(T* dst, const uint32_t (&t)[32], float f) {
+// A row of P 16-byte pieces per lane, P = 2, 4 or 8, to P lanes per row: lane l of a group of P lanes gets piece l of the rows of all
+// its group's lanes.  A row's pieces straight from its lane touch 32 lines per store instruction, and the elementwise warps
+// stood in the queue for them (4000 clocks per 128 x 128 tile); after the exchange an instruction writes whole lines.
+template <int P>
+__device__ __forceinline__ void bwd_exchange(uint4 (&x)[P], int lane) {
 #pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        uint4 w;
-        w.x = Elem<T>::pack2(__uint_as_float(t[8 * v]) * f, __uint_as_float(t[8 * v + 1]) * f);
-        w.y = Elem<T>::pack2(__uint_as_float(t[8 * v + 2]) * f, __uint_as_float(t[8 * v + 3]) * f);
-        w.z = Elem<T>::pack2(__uint_as_float(t[8 * v + 4]) * f, __uint_as_float(t[8 * v + 5]) * f);
-        w.w = Elem<T>::pack2(__uint_as_float(t[8 * v + 6]) * f, __uint_as_float(t[8 * v + 7]) * f);
-        reinterpret_cast<uint4*>(dst)[v] = w;
+    for (int s = 1; s < P; s *= 2) {
+        const bool up = lane & s;
+#pragma unroll
+        for (int i = 0; i < P; ++i) {
+            if (i & s) continue;
+            uint4 a = up ? x[i] : x[i | s];
+            a.x = __shfl_xor_sync(0xffffffffu, a.x, s);
+            a.y = __shfl_xor_sync(0xffffffffu, a.y, s);
+            a.z = __shfl_xor_sync(0xffffffffu, a.z, s);
+            a.w = __shfl_xor_sync(0xffffffffu, a.w, s);
+            if (up) x[i] = a;
+            else x[i | s] = a;
+        }
     }
+}
+// COLS fp32 accumulator columns from tensor memory, times f, packed to the element type, as the lane's row.
+template <typename T, int COLS>
+__device__ __forceinline__ void bwd_load_rows(uint32_t src, float f, uint4 (&x)[COLS / 8]) {
+    constexpr int STEP = COLS < 32 ? COLS : 32;
+#pragma unroll
+    for (int c = 0; c < COLS; c += STEP) {
+        uint32_t t[STEP];
+        if constexpr (STEP == 32) tmem_ld32(src + c, t);
+        else tmem_ld16(src + c, t);
+        tmem_wait_ld();
+#pragma unroll
+        for (int v = 0; v < STEP / 8; ++v) {
+            uint4& w = x[c / 8 + v];
+            w.x = Elem<T>::pack2(__uint_as_float(t[8 * v]) * f, __uint_as_float(t[8 * v + 1]) * f);
+            w.y = Elem<T>::pack2(__uint_as_float(t[8 * v + 2]) * f, __uint_as_float(t[8 * v + 3]) * f);
+            w.z = Elem<T>::pack2(__uint_as_float(t[8 * v + 4]) * f, __uint_as_float(t[8 * v + 5]) * f);
+            w.w = Elem<T>::pack2(__uint_as_float(t[8 * v + 6]) * f, __uint_as_float(t[8 * v + 7]) * f);
+        }
+    }
+}
+// The lanes' rows to a gradient tensor: dst is where the first of the 32 rows starts, `rows` of them exist.  Warp-collective.
+template <typename T, int P>
+__device__ __forceinline__ void bwd_store_rows(T* dst, int64_t row_stride, int rows, uint4 (&x)[P], int lane) {
+    bwd_exchange<P>(x, lane);
+    const int row0 = lane & ~(P - 1), piece = lane & (P - 1);
+#pragma unroll
+    for (int j = 0; j < P; ++j)
+        if (row0 + j < rows) *reinterpret_cast<uint4*>(dst + (row0 + j) * row_stride + piece * 8) = x[j];
+}
+// Columns lo .. hi of 32 (either may lie outside) as bits.
+__device__ __forceinline__ uint32_t bwd_column_bits(int lo, int hi) {
+    const uint32_t upto = hi < 0 ? 0u : hi >= 31 ? 0xffffffffu : 0xffffffffu >> (31 - hi);
+    return lo <= 0 ? upto : lo > 31 ? 0u : upto & (0xffffffffu << lo);
+}
+// Zeros to the hidden ones of 32 packed elements (whatever they hold: it may be a NaN).
+__device__ __forceinline__ void bwd_hide(uint32_t (&w)[16], uint32_t bits) {
+#pragma unroll
+    for (int e = 0; e < 16; ++e) w[e] &= (bits >> (2 * e) & 1u ? 0xffffu : 0u) | (bits >> (2 * e + 1) & 1u ? 0xffff0000u : 0u);
+}
+// 128 rows of a K-major tile in shared memory to tensor memory as an A operand: 8 columns (16 elements a row) per instruction.
+template <int HDIM>
+__device__ __forceinline__ void bwd_copy_to_tmem(uint32_t d, uint64_t src) {
+#pragma unroll
+    for (int ks = 0; ks < HDIM / 16; ++ks)
+        asm volatile("tcgen05.cp.cta_group::1.128x256b [%0], %1;\n" ::"r"(d + ks * 8), "l"(src + (uint64_t)(((ks / 4) * HALF_BYTES + (ks % 4) * 32) >> 4))
+                     : "memory");
 }
 
 // One tile by TMA (64-column boxes of 128 rows).  Where the sequence ends inside it, the rows behind the end are set to zero before
@@ -175,9 +233,8 @@ struct BwdCtrl {
     BwdItem items[kBwdItemRing];
     uint64_t item_full[kBwdItemRing], item_empty[kBwdItemRing];
     uint64_t a_full[3], a_empty[3], b_full[2], b_empty[2];  // rings: dQ K / V; dK/dV Q / dO
-    uint64_t own_full[2], own_free[2];  // what an item owns: dQ Q / dO in tensor memory, dK/dV the K / V tile
+    uint64_t own_full[2], own_free[2];  // what an item owns: dK/dV the K / V tile; dQ: Q / dO in the buffer that they pass through, whose release is own_free[0]
     uint64_t s_full[2], s_free[2], dp_full[2], ds_full[2];  // dQ: by half; dK/dV: [0] (s_free[0]: dP has been read)
-    uint64_t x_done[2];         // the product that reads dS is complete (dQ: by half)
     uint64_t p_full[2];         // dK/dV, by step: the elementwise warps can be one step ahead of the products that read P
     uint64_t acc_full, acc_free, tail;
     uint64_t row_full[2], row_empty[2];
@@ -185,79 +242,90 @@ struct BwdCtrl {
     int abort_flag;
 };
 
-// The scheduling warp.  Items of a level cost the same under a causal mask: level l is the row tile l of dQ (the last tiles see the
-// most keys), the tile l places in front of the last one of dK/dV (the first tiles are seen by the most queries).  Levels come
-// in decreasing order, a level's sequences in order, their heads side by side (they share tiles through L2); rounds of the grid
-// take the items in alternate directions.  Tile counts are held eight sequences a lane.
+// The schedule, kept by the warp that issues the copies.  Items of a level cost the same under a causal mask: level l is the row tile
+// l of dQ (the last tiles see the most keys), the tile l places in front of the last one of dK/dV (the first tiles are seen by
+// the most queries).  Levels come in decreasing order, a level's sequences in order, their heads side by side (they share tiles
+// through L2); rounds of the grid take the items in alternate directions.  Tile counts are held eight sequences a lane.
 template <bool DQ>
-__device__ __forceinline__ void bwd_schedule(BwdCtrl* ctrl, const BwdSm100Dev& p, int lane) {
-    const int heads = DQ ? p.hq : p.hkv;
-    uint32_t k = 0;
-    auto publish = [&](int valid, int b, int h, int row0) -> bool {
-        const int slot = k % kBwdItemRing;
-        const bool ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->item_empty[slot], ((k / kBwdItemRing) & 1u) ^ 1u, &ctrl->abort_flag, p.status, 0x10001));
-        ++k;
-        if (ok && lane == 0) {
-            BwdItem it{valid, b, h, row0, 0, 0, 0, 0};
-            if (valid) {
-                const BwdSeq s = bwd_sequence(p, b);
-                it.q0 = s.q0; it.k0 = s.k0; it.sq = s.sq; it.sk = s.sk;
+struct BwdSchedule {
+    int cnt[kBwdMaxBatch / 32], level, round;
+    int64_t base;  // first item of the level
+    uint32_t k;    // items handed out
+
+    __device__ __forceinline__ void init(const BwdSm100Dev& p, int lane) {
+        k = 0;
+        round = 0;
+        base = 0;
+        level = -1;
+        if (!p.listed) return;
+        int most = 0;
+#pragma unroll
+        for (int u = 0; u < kBwdMaxBatch / 32; ++u) {
+            cnt[u] = 0;
+            if (u * 32 + lane < p.batch) {
+                const BwdSeq s = bwd_sequence(p, u * 32 + lane);
+                cnt[u] = min(((DQ ? s.sq : s.sk) + 127) / 128, p.max_tiles);
             }
+            most = max(most, cnt[u]);
+        }
+        level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
+    }
+    // The next item, handed to the other warps as well; false: there is none (said to the others), or a wait ran out.
+    __device__ __forceinline__ bool next(BwdCtrl* ctrl, const BwdSm100Dev& p, int lane, BwdItem& it) {
+        const int heads = DQ ? p.hq : p.hkv;
+        it = BwdItem{};
+        if (!p.listed) {  // one item per CTA, by its index
+            if (round++ == 0) {
+                const int per_tile = heads * p.batch, t = (int)blockIdx.x / per_tile, rest = (int)blockIdx.x - t * per_tile;
+                it.b = rest / heads;
+                it.h = rest - it.b * heads;
+                it.row0 = (DQ ? (int)gridDim.x / per_tile - 1 - t : t) * 128;
+                it.valid = 1;
+            }
+        } else {
+            const int64_t w = (int64_t)round * gridDim.x + ((round & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            ++round;
+            for (; level >= 0; --level) {
+                int n = 0;
+#pragma unroll
+                for (int u = 0; u < kBwdMaxBatch / 32; ++u) n += __popc(__ballot_sync(0xffffffffu, cnt[u] > level));
+                if (w < base + (int64_t)n * heads) break;
+                base += (int64_t)n * heads;
+            }
+            if (level >= 0) {
+                int rank = (int)((w - base) / heads), tiles = 0;
+                it.h = (int)(w - base) - rank * heads;
+#pragma unroll
+                for (int u = 0; u < kBwdMaxBatch / 32; ++u) {
+                    const uint32_t m = __ballot_sync(0xffffffffu, cnt[u] > level);
+                    const int c = __popc(m);
+                    if (!it.valid && rank < c) {
+                        const int l = __fns(m, 0, rank + 1);
+                        it.b = u * 32 + l;
+                        tiles = __shfl_sync(0xffffffffu, cnt[u], l);
+                        it.valid = 1;
+                    }
+                    rank -= c;
+                }
+                it.row0 = (DQ ? level : tiles - 1 - level) * 128;
+            }
+        }
+        if (it.valid) {
+            const BwdSeq s = bwd_sequence(p, it.b);
+            it.q0 = s.q0; it.k0 = s.k0; it.sq = s.sq; it.sk = s.sk;
+            it.valid = it.row0 < (DQ ? s.sq : s.sk);
+        }
+        const int slot = k % kBwdItemRing;
+        if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->item_empty[slot], ((k / kBwdItemRing) & 1u) ^ 1u, &ctrl->abort_flag, p.status, 0x10001))) return false;
+        ++k;
+        if (lane == 0) {
             ctrl->items[slot] = it;
             mbar_arrive(&ctrl->item_full[slot]);
         }
         __syncwarp();
-        return ok;
-    };
-    if (!p.listed) {  // one item per CTA
-        const int per_tile = heads * p.batch, t = (int)blockIdx.x / per_tile, rest = (int)blockIdx.x - t * per_tile;
-        const int b = rest / heads, h = rest - b * heads, row0 = (DQ ? (int)gridDim.x / per_tile - 1 - t : t) * 128;
-        const BwdSeq s = bwd_sequence(p, b);
-        if (row0 < (DQ ? s.sq : s.sk) && !publish(1, b, h, row0)) return;
-        publish(0, 0, 0, 0);
-        return;
+        return it.valid != 0;
     }
-    int cnt[kBwdMaxBatch / 32], most = 0;
-#pragma unroll
-    for (int u = 0; u < kBwdMaxBatch / 32; ++u) {
-        cnt[u] = 0;
-        if (u * 32 + lane < p.batch) {
-            const BwdSeq s = bwd_sequence(p, u * 32 + lane);
-            cnt[u] = min(((DQ ? s.sq : s.sk) + 127) / 128, p.max_tiles);
-        }
-        most = max(most, cnt[u]);
-    }
-    int level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
-    int64_t base = 0;  // first item of the level
-    for (int r = 0;; ++r) {
-        const int64_t w = (int64_t)r * gridDim.x + ((r & 1) ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
-        for (; level >= 0; --level) {
-            int n = 0;
-#pragma unroll
-            for (int u = 0; u < kBwdMaxBatch / 32; ++u) n += __popc(__ballot_sync(0xffffffffu, cnt[u] > level));
-            if (w < base + (int64_t)n * heads) break;
-            base += (int64_t)n * heads;
-        }
-        if (level < 0) break;
-        int rank = (int)((w - base) / heads), b = 0, tiles = 0;
-        const int h = (int)(w - base) - rank * heads;
-        bool found = false;
-#pragma unroll
-        for (int u = 0; u < kBwdMaxBatch / 32; ++u) {
-            const uint32_t m = __ballot_sync(0xffffffffu, cnt[u] > level);
-            const int c = __popc(m);
-            if (!found && rank < c) {
-                const int l = __fns(m, 0, rank + 1);
-                b = u * 32 + l;
-                tiles = __shfl_sync(0xffffffffu, cnt[u], l);
-                found = true;
-            }
-            if (!found) rank -= c;
-        }
-        if (!publish(1, b, h, (DQ ? level : tiles - 1 - level) * 128)) return;
-    }
-    publish(0, 0, 0, 0);
-}
+};
 // The next item of a consumer warp (false: no more, or a wait ran out).
 __device__ __forceinline__ bool bwd_next_item(BwdCtrl* ctrl, const BwdSm100Dev& p, uint32_t& k, int lane, BwdItem& it) {
     const int slot = k % kBwdItemRing;
@@ -312,19 +380,20 @@ __device__ __forceinline__ void bwd_zero_outside(const BwdSm100Dev& p) {
 }
 
 
-// ---- dQ -----------------------------------------------------------------------------------------------------------------
-constexpr int kBwdDqThreads = 512;
+constexpr int kBwdThreads = 640, kBwdConsumers = 19;  // (consumers of the item ring: every warp but the one that fills it)
 
+// ---- dQ -----------------------------------------------------------------------------------------------------------------
 template <typename T, int HDIM, bool EXTRA>
-__global__ void __launch_bounds__(kBwdDqThreads, 1)
-bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const BwdSm100Dev p) {
+__global__ void __launch_bounds__(kBwdThreads, 1)
+bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const BwdSm100Dev p) {
     constexpr int TILE = 128 * HDIM * 2, KS = 3, VS = 2;
     constexpr uint32_t cS = 0, cDP = 128, cDQ = 256, cQ = 384, cDO = 448;
     extern __shared__ uint8_t smem_raw[];
-    uint8_t* base = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
-    uint8_t* sK = base;
+    uint8_t* sK = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
     uint8_t* sV = sK + KS * TILE;
-    float* sRow = reinterpret_cast<float*>(sV + VS * TILE);  // [2 items][LSE 128 | D 128] of the rows
+    uint8_t* sOwn = sV + VS * TILE;                          // Q, then dO of the next item on their way to tensor memory
+    float* sRow = reinterpret_cast<float*>(sOwn + TILE);     // [2 items][LSE 128 | D 128] of the rows
     BwdCtrl* ctrl = reinterpret_cast<BwdCtrl*>(sRow + 512);
     volatile int* abort_flag = &ctrl->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -332,29 +401,29 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (threadIdx.x == 0) {
         for (int i = 0; i < kBwdItemRing; ++i) {
             mbar_init(&ctrl->item_full[i], 1);
-            mbar_init(&ctrl->item_empty[i], 15);  // every warp but the scheduling one
+            mbar_init(&ctrl->item_empty[i], kBwdConsumers);
         }
         for (int i = 0; i < KS; ++i) { mbar_init(&ctrl->a_full[i], 1); mbar_init(&ctrl->a_empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctrl->b_full[i], 1);
             mbar_init(&ctrl->b_empty[i], 1);
-            mbar_init(&ctrl->own_full[i], 4);
-            mbar_init(&ctrl->own_free[i], 1);
             mbar_init(&ctrl->s_full[i], 1);
-            mbar_init(&ctrl->s_free[i], 4);
+            mbar_init(&ctrl->s_free[i], 8);
             mbar_init(&ctrl->dp_full[i], 1);
-            mbar_init(&ctrl->ds_full[i], 4);
-            mbar_init(&ctrl->x_done[i], 1);
-            mbar_init(&ctrl->row_full[i], 4);
-            mbar_init(&ctrl->row_empty[i], 8);
+            mbar_init(&ctrl->ds_full[i], 8);
+            mbar_init(&ctrl->row_full[i], 1);
+            mbar_init(&ctrl->row_empty[i], 16);
         }
+        mbar_init(&ctrl->own_full[0], 1);
+        mbar_init(&ctrl->own_full[1], 1);
+        mbar_init(&ctrl->own_free[0], 1);
         mbar_init(&ctrl->acc_full, 1);
-        mbar_init(&ctrl->acc_free, 8);
+        mbar_init(&ctrl->acc_free, 16);
         mbar_init(&ctrl->tail, 1);
         ctrl->abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&ctrl->tmem_base)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
     }
@@ -368,93 +437,95 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint32_t k_item = 0;
     BwdItem it{};
 
-    // Registers: launched with 512 x 128; 256 x 168 + 128 x 72 + 128 x 104 = the same 65536.
-    if (warp >= 12) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 104;\n" ::);
-        // ================ Q and dO to tensor memory, row by row; D = sum dO O - dLSE on the way ================
-        const int r = (warp & 3) * 32 + lane;
-        const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        uint32_t n_item = 0;  // items with products so far
-        while (bwd_next_item(ctrl, p, k_item, lane, it)) {
-            const int i = it.row0 + r, N = bwd_key_tiles(p, it).count;
-            const bool row_ok = i < it.sq;
-            const int64_t at = ((int64_t)(it.q0 + i) * p.hq + it.h) * HDIM;
-            const int64_t lr = (p.seqstart_q ? (int64_t)it.h * p.seqlen_q + it.q0 : ((int64_t)it.b * p.hq + it.h) * p.seqlen_q) + i;
-            uint32_t w[HDIM / 64][32];
-            auto fetch = [&](const void* src) {
-                const uint4* s4 = reinterpret_cast<const uint4*>((const T*)src + at);
-#pragma unroll
-                for (int v = 0; v < HDIM / 8; ++v) {
-                    const uint4 x = row_ok ? s4[v] : make_uint4(0u, 0u, 0u, 0u);
-                    w[v / 8][4 * (v % 8)] = x.x; w[v / 8][4 * (v % 8) + 1] = x.y; w[v / 8][4 * (v % 8) + 2] = x.z; w[v / 8][4 * (v % 8) + 3] = x.w;
-                }
-            };
-            auto put = [&](int which, uint32_t col) -> bool {
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->own_free[which], (n_item & 1u) ^ 1u, abort_flag, p.status, 0x10010))) return false;
-                tc_fence_after();
-#pragma unroll
-                for (int c = 0; c < HDIM / 64; ++c) tmem_st32(lane_addr + col + c * 32, w[c]);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctrl->own_full[which]);
-                return true;
-            };
-            float lse2 = INFINITY, dlse = 0.f;
-            if (N > 0) {
-                fetch(p.q);
-                if (row_ok) lse2 = bwd_lse_base2(p.lse[lr]);
-                if (!put(0, cQ)) break;
-            }
-            fetch(p.dout);
-            if (row_ok && p.dlse) dlse = p.dlse[lr];
-            float delta = 0.f;
-            const uint4* osrc = reinterpret_cast<const uint4*>((const T*)p.o + at);
-#pragma unroll
-            for (int v = 0; v < HDIM / 8; ++v) {
-                const uint4 y = row_ok ? osrc[v] : make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t yw[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float2 a = bias_pair<T>(w[v / 8][4 * (v % 8) + e]), o2 = bias_pair<T>(yw[e]);
-                    delta = fmaf(a.x, o2.x, fmaf(a.y, o2.y, delta));
-                }
-            }
-            delta -= dlse;
-            if (row_ok) p.delta[lr] = delta;
-            if (N == 0) continue;
-            const int slot = n_item & 1;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_empty[slot], ((n_item >> 1) & 1u) ^ 1u, abort_flag, p.status, 0x10011))) break;
-            sRow[slot * 256 + r] = lse2;
-            sRow[slot * 256 + 128 + r] = delta;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&ctrl->row_full[slot]);
-            if (!put(1, cDO)) break;
-            ++n_item;
-        }
-    } else if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;\n" ::);
-        if (warp == 11) {
-            bwd_schedule<true>(ctrl, p, lane);
-        } else if (warp == 9) {
-            // ================================ TMA producer ================================
-            uint32_t tails = 0, t = 0;
+    // Registers: launched with 640 x 96 = 512 x 104 + 128 x 64.
+    if (warp >= 16) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::);
+        if (warp == 18) {
+            // ================================ items and TMA copies ================================
+            BwdSchedule<true> schedule;
+            schedule.init(p, lane);
+            uint32_t tails = 0, t = 0, own = 0;
             bool ok = true;
-            while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
+            auto load_own = [&](int which, const CUtensorMap* map) {  // (rows behind the end of the queries stay in their own rows of dQ, which are not stored)
+                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->own_free[0], (own & 1u) ^ 1u, abort_flag, p.status, 0x10022)) &&
+                     bwd_load_tile<HDIM>(sOwn, map, &ctrl->own_full[which], &ctrl->tail, tails, it.h, it.q0 + it.row0, 128, lane, abort_flag, p.status);
+                ++own;
+                return ok;
+            };
+            // (an item is handed out while the copies of the one before it are still to come: its LSE and D are then there in time)
+            BwdItem ahead{};
+            for (bool more = schedule.next(ctrl, p, lane, ahead); ok && more;) {
+                it = ahead;
+                more = schedule.next(ctrl, p, lane, ahead);
                 const BwdRange range = bwd_key_tiles(p, it);
                 const int kh = it.h / (p.hq / p.hkv);
+                if (range.count > 0 && !load_own(0, &map_q)) break;
                 for (int j = 0; j < range.count; ++j, ++t) {
                     const int n0 = (range.begin + j) * 128, ks = t % KS, vs = t % VS;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->a_empty[ks], ((t / KS) & 1u) ^ 1u, abort_flag, p.status, 0x10020)))) break;
                     // (K rows behind the end meet dS = 0; those of V only make columns of dP that are masked by index)
                     if (!(ok = bwd_load_tile<HDIM>(sK + ks * TILE, &map_k, &ctrl->a_full[ks], &ctrl->tail, tails, kh, it.k0 + n0, it.sk - n0, lane,
                                                    abort_flag, p.status))) break;
+                    if (j == 0 && !load_own(1, &map_do)) break;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->b_empty[vs], ((t / VS) & 1u) ^ 1u, abort_flag, p.status, 0x10021)))) break;
                     bwd_load_tile<HDIM>(sV + vs * TILE, &map_v, &ctrl->b_full[vs], &ctrl->tail, tails, kh, it.k0 + n0, 128, lane, abort_flag, p.status);
                 }
             }
+        } else if (warp == 19) {
+            // ================================ D = sum dO O - dLSE, and the LSE of the rows ================================
+            constexpr int L = HDIM / 8, ROWS = 32 / L, AHEAD = 4;  // lanes a row, rows a load, loads in flight
+            const int sub = lane / L, piece = lane % L;
+            uint32_t n_item = 0;  // items with products so far
+            while (bwd_next_item(ctrl, p, k_item, lane, it)) {
+                const int N = bwd_key_tiles(p, it).count, slot = n_item & 1;
+                const int64_t lr = (p.seqstart_q ? (int64_t)it.h * p.seqlen_q + it.q0 : ((int64_t)it.b * p.hq + it.h) * p.seqlen_q) + it.row0;
+                const int64_t at = ((int64_t)(it.q0 + it.row0) * p.hq + it.h) * HDIM + piece * 8;
+                const int left = it.sq - it.row0;  // rows that exist from the tile's first on
+                if (N > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_empty[slot], ((n_item >> 1) & 1u) ^ 1u, abort_flag, p.status, 0x10011))) break;
+                float* rows = sRow + slot * 256;
+                if (N > 0)
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) rows[u * 32 + lane] = u * 32 + lane < left ? bwd_lse_base2(p.lse[lr + u * 32 + lane]) : INFINITY;
+#pragma unroll 1
+                for (int g = 0; g < min(128, left); g += ROWS * AHEAD) {
+                    uint4 x[AHEAD], y[AHEAD];
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u) {
+                        const int r = g + u * ROWS + sub;
+                        x[u] = y[u] = make_uint4(0u, 0u, 0u, 0u);
+                        if (r < left) {
+                            x[u] = *reinterpret_cast<const uint4*>((const T*)p.dout + at + (int64_t)r * p.hq * HDIM);
+                            y[u] = *reinterpret_cast<const uint4*>((const T*)p.o + at + (int64_t)r * p.hq * HDIM);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < AHEAD; ++u) {
+                        const int r = g + u * ROWS + sub;
+                        const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+                        float delta = 0.f;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float2 a = bias_pair<T>(xw[e]), o2 = bias_pair<T>(yw[e]);
+                            delta = fmaf(a.x, o2.x, fmaf(a.y, o2.y, delta));
+                        }
+#pragma unroll
+                        for (int off = L / 2; off > 0; off >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, off);
+                        if (piece == 0) {
+                            if (r < left) {
+                                if (p.dlse) delta -= p.dlse[lr + r];
+                                p.delta[lr + r] = delta;
+                            }
+                            if (N > 0) rows[128 + r] = delta;
+                        }
+                    }
+                }
+                if (N == 0) continue;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctrl->row_full[slot]);
+                ++n_item;
+            }
         } else {
-            // ================================ MMA issuers: 8 S and dP, 10 dQ ================================
+            // ================================ MMA issuers: 16 S, 17 dP and dQ ================================
             // All lanes walk the loop, the elected one issues.
             const bool leader = elect_one_sync();
             bool ok = true;
@@ -463,82 +534,91 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             };
             auto commit = [&](uint64_t* bar) { if (leader) umma_commit(bar); };
             auto at = [&](uint64_t d, uint32_t bytes) { return d + (uint64_t)(bytes >> 4); };
+            constexpr uint32_t idesc_s = make_idesc<T>(false, 64), idesc_q = make_idesc<T>(true, HDIM);
+            const uint64_t dK = make_smem_desc(smem_u32(sK), 0, 1024), dV = make_smem_desc(smem_u32(sV), 0, 1024);
+            const uint64_t dKt = make_smem_desc(smem_u32(sK), HALF_BYTES, 1024), dOwn = make_smem_desc(smem_u32(sOwn), 0, 1024);
             uint32_t t = 0, ks = 0, kph = 0, n_item = 0;  // steps so far, K slot and its phase, items with steps so far
-            if (warp == 8) {
-                constexpr uint32_t idesc_s = make_idesc<T>(false, 64);
-                const uint64_t dK = make_smem_desc(smem_u32(sK), 0, 1024), dV = make_smem_desc(smem_u32(sV), 0, 1024);
+            if (warp == 16) {
                 while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
                     const int N = bwd_key_tiles(p, it).count;
+                    if (N > 0) {  // Q, over the last item's, whose last S is complete
+                        if (!wait(&ctrl->own_full[0], n_item++ & 1u, 0x10030)) break;
+                        if (t > 0 && !wait(&ctrl->s_full[1], (t - 1) & 1u, 0x10038)) break;
+                        tc_fence_after();
+                        if (leader) bwd_copy_to_tmem<HDIM>(tmem + cQ, dOwn);
+                        commit(&ctrl->own_free[0]);
+                    }
                     for (int j = 0; j < N; ++j) {
-                        const uint32_t vs = t & 1u;
+                        if (!wait(&ctrl->a_full[ks], kph, 0x10031)) break;
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
-                            if (half == 0) {
-                                if (j == 0 && !wait(&ctrl->own_full[0], n_item & 1u, 0x10030)) break;
-                                if (!wait(&ctrl->a_full[ks], kph, 0x10031)) break;
-                            }
                             if (t > 0 && !wait(&ctrl->s_free[half], (t - 1) & 1u, 0x10032)) break;
                             tc_fence_after();
                             if (leader) bwd_issue_ts<HDIM>(tmem + cS + half * 64, tmem + cQ, at(dK, ks * TILE + half * 8192), idesc_s);
                             commit(&ctrl->s_full[half]);
-                            if (half == 1 && j + 1 == N) commit(&ctrl->own_free[0]);
-                            if (half == 0) {
-                                if (j == 0 && !wait(&ctrl->own_full[1], n_item & 1u, 0x10033)) break;
-                                if (!wait(&ctrl->b_full[vs], (t >> 1) & 1u, 0x10034)) break;
-                            }
-                            if (t > 0 && !wait(&ctrl->x_done[half], (t - 1) & 1u, 0x10035)) break;
-                            tc_fence_after();
-                            if (leader) bwd_issue_ts<HDIM>(tmem + cDP + half * 64, tmem + cDO, at(dV, vs * TILE + half * 8192), idesc_s);
-                            commit(&ctrl->dp_full[half]);
                         }
                         if (!ok) break;
-                        commit(&ctrl->b_empty[vs]);
-                        if (j + 1 == N) commit(&ctrl->own_free[1]);
                         ++t;
                         if (++ks == KS) { ks = 0; kph ^= 1u; }
                     }
-                    if (N > 0) ++n_item;
                 }
             } else {
-                constexpr uint32_t idesc_q = make_idesc<T>(true, HDIM);
-                const uint64_t dKt = make_smem_desc(smem_u32(sK), HALF_BYTES, 1024);
+                auto issue_dp = [&](uint32_t st, int half) -> bool {
+                    const uint32_t vs = st & 1u;
+                    if (half == 0 && !wait(&ctrl->b_full[vs], (st >> 1) & 1u, 0x10034)) return false;
+                    tc_fence_after();
+                    if (leader) bwd_issue_ts<HDIM>(tmem + cDP + half * 64, tmem + cDO, at(dV, vs * TILE + half * 8192), idesc_s);
+                    commit(&ctrl->dp_full[half]);
+                    if (half == 1) commit(&ctrl->b_empty[vs]);
+                    return true;
+                };
                 while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
                     const int N = bwd_key_tiles(p, it).count;
-                    if (N > 0 && n_item > 0 && !wait(&ctrl->acc_free, (n_item - 1) & 1u, 0x10036)) break;
+                    if (N == 0) continue;
+                    // dO, over the last item's, whose last dP has been read
+                    if (!wait(&ctrl->own_full[1], n_item & 1u, 0x10033)) break;
+                    tc_fence_after();
+                    if (leader) bwd_copy_to_tmem<HDIM>(tmem + cDO, dOwn);
+                    commit(&ctrl->own_free[0]);
+                    if (!issue_dp(t, 0) || !issue_dp(t, 1)) break;
+                    if (n_item > 0 && !wait(&ctrl->acc_free, (n_item - 1) & 1u, 0x10036)) break;
                     for (int j = 0; j < N; ++j) {
 #pragma unroll
                         for (int half = 0; half < 2; ++half) {
                             if (!wait(&ctrl->ds_full[half], t & 1u, 0x10037)) break;
                             tc_fence_after();
                             if (leader) bwd_issue_xb(tmem + cDQ, tmem + cDP, at(dKt, ks * TILE), idesc_q, half, j + half > 0);
-                            commit(&ctrl->x_done[half]);
+                            if (half == 1) commit(&ctrl->a_empty[ks]);
+                            if (j + 1 < N && !issue_dp(t + 1, half)) break;
                         }
                         if (!ok) break;
-                        commit(&ctrl->a_empty[ks]);
                         ++t;
                         if (++ks == KS) ks = 0;
                     }
                     if (!ok) break;
-                    if (N > 0) { commit(&ctrl->acc_full); ++n_item; }
+                    commit(&ctrl->acc_full);
+                    ++n_item;
                 }
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 168;\n" ::);
-        const int half = warp >> 2, r = (warp & 3) * 32 + lane;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::);
+        const int quarter = warp >> 2, half = quarter >> 1, r = (warp & 3) * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        const uint32_t tS = lane_addr + cS + half * 64, tDP = lane_addr + cDP + half * 64;
+        const uint32_t tS = lane_addr + cS + quarter * 32, tDP = lane_addr + cDP + quarter * 32;
         uint32_t t = 0, n_item = 0;
         bool ok = true;
         while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
+            constexpr int COLS = HDIM / 4;  // of dQ that this warp stores
             const int i = it.row0 + r, shift = p.mask_type == 2 ? it.sk - it.sq : 0;
+            const int first = it.row0 + (warp & 3) * 32;  // of this warp's rows
             const BwdRange range = bwd_key_tiles(p, it);
-            const bool row_ok = i < it.sq;
-            T* dst = (T*)p.dq + ((int64_t)(it.q0 + i) * p.hq + it.h) * HDIM + half * (HDIM / 2);
+            T* dst = (T*)p.dq + ((int64_t)(it.q0 + first) * p.hq + it.h) * HDIM + quarter * COLS;
+            uint4 out[COLS / 8];
             if (range.count == 0) {  // no row of the tile sees a key
-                if (row_ok)
 #pragma unroll
-                    for (int v = 0; v < HDIM / 16; ++v) reinterpret_cast<uint4*>(dst)[v] = make_uint4(0u, 0u, 0u, 0u);
+                for (int v = 0; v < COLS / 8; ++v) out[v] = make_uint4(0u, 0u, 0u, 0u);
+                bwd_store_rows<T>(dst, (int64_t)p.hq * HDIM, it.sq - first, out, lane);
                 continue;
             }
             const int slot = n_item & 1;
@@ -556,95 +636,71 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 if (p.wr >= 0) full_hi = min(full_hi, it.row0 + shift + p.wr);
             }
             const float2 neg_lse2 = make_float2(-lse2, -lse2), neg_delta = make_float2(-delta, -delta);
-            auto step = [&](int j, auto masked) -> bool {
-                const int key0 = (range.begin + j) * 128 + half * 64;
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->s_full[half], t & 1u, abort_flag, p.status, 0x10041))) return false;
+            for (int j = 0; j < range.count; ++j, ++t) {
+                const int n0 = (range.begin + j) * 128, key0 = n0 + quarter * 32;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->s_full[half], t & 1u, abort_flag, p.status, 0x10041)))) break;
                 tc_fence_after();
-                uint32_t x[2][32];
-                tmem_ld32(tS, x[0]);
-                tmem_ld32(tS + 32, x[1]);
+                uint32_t x[32];
+                tmem_ld32(tS, x);
                 tmem_wait_ld();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->s_free[half]);
+                if constexpr (EXTRA) {
+                    if (p.soft_cap > 0.f) soft_cap_scores<32>(x, p.cap);
+                }
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
+                for (int e = 0; e < 32; e += 2) {
+                    float2 f = make_float2(1.f, 1.f), away = f;
                     if constexpr (EXTRA) {
-                        if (p.soft_cap > 0.f) soft_cap_scores<32>(x[c], p.cap);
+                        away.x = (float)(i + it.sk - it.sq - (key0 + e));
+                        away.y = away.x - 1.f;
                     }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        float2 f = make_float2(1.f, 1.f), away = f;
-                        if constexpr (EXTRA) {
-                            away.x = (float)(i + it.sk - it.sq - (key0 + c * 32 + e));
-                            away.y = away.x - 1.f;
-                        }
-                        const float2 y = bwd_exponent<EXTRA>(p, make_float2(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), slope, away, neg_lse2, f);
-                        float2 pr = bwd_exp2(y, e / 2);
-                        if constexpr (EXTRA) pr = __fmul2_rn(pr, f);
-                        x[c][e] = __float_as_uint(pr.x);
-                        x[c][e + 1] = __float_as_uint(pr.y);
-                    }
+                    const float2 y = bwd_exponent<EXTRA>(p, make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), slope, away, neg_lse2, f);
+                    float2 pr = bwd_exp2<kPolyDq>(y, e / 2);
+                    if constexpr (EXTRA) pr = __fmul2_rn(pr, f);
+                    x[e] = __float_as_uint(pr.x);
+                    x[e + 1] = __float_as_uint(pr.y);
                 }
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->dp_full[half], t & 1u, abort_flag, p.status, 0x10042))) return false;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->dp_full[half], t & 1u, abort_flag, p.status, 0x10042)))) break;
                 tc_fence_after();
+                uint32_t dp[32], w[16];
+                tmem_ld32(tDP, dp);
+                tmem_wait_ld();
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t dp[32], w[16];
-                    tmem_ld32(tDP + c * 32, dp);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float2 d = __fadd2_rn(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), neg_delta);
-                        float2 ds = __fmul2_rn(make_float2(__uint_as_float(x[c][e]), __uint_as_float(x[c][e + 1])), d);
-                        if constexpr (decltype(masked)::value) {
-                            const int key = key0 + c * 32 + e;
-                            if (key < k_lo || key > k_hi) ds.x = 0.f;
-                            if (key + 1 < k_lo || key + 1 > k_hi) ds.y = 0.f;
-                        }
-                        w[e / 2] = Elem<T>::pack2(ds.x, ds.y);
-                    }
-                    tmem_st16(tDP + c * 16, w);  // (over columns of dP that this warp has read)
+                for (int e = 0; e < 32; e += 2) {
+                    const float2 d = __fadd2_rn(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), neg_delta);
+                    const float2 ds = __fmul2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), d);
+                    w[e / 2] = Elem<T>::pack2(ds.x, ds.y);
                 }
+                if (n0 < full_lo || n0 + 127 > full_hi) bwd_hide(w, bwd_column_bits(k_lo - key0, k_hi - key0));
+                tmem_st16(tDP, w);  // (over columns of dP that this warp has read)
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->ds_full[half]);
-                ++t;
-                return true;
-            };
-            for (int j = 0; ok && j < range.count; ++j) {
-                const int n0 = (range.begin + j) * 128;
-                ok = n0 < full_lo || n0 + 127 > full_hi ? step(j, std::true_type{}) : step(j, std::false_type{});
             }
             if (!ok || !(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->acc_full, n_item & 1u, abort_flag, p.status, 0x10043)))) break;
             ++n_item;
             tc_fence_after();
-            uint32_t acc[HDIM / 64][32];
-#pragma unroll
-            for (int c = 0; c < HDIM / 64; ++c) tmem_ld32(lane_addr + cDQ + half * (HDIM / 2) + c * 32, acc[c]);
-            tmem_wait_ld();
+            bwd_load_rows<T, COLS>(lane_addr + cDQ + quarter * COLS, p.scale, out);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctrl->acc_free);
-            if (row_ok)
-#pragma unroll
-                for (int c = 0; c < HDIM / 64; ++c) bwd_store32<T>(dst + c * 32, acc[c], p.scale);
+            bwd_store_rows<T>(dst, (int64_t)p.hq * HDIM, it.sq - first, out, lane);
         }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
     }
 }
 
 // ---- dK / dV --------------------------------------------------------------------------------------------------------------
-constexpr int kBwdDkdvThreads = 512;
-
 template <typename T, int HDIM, bool EXTRA>
-__global__ void __launch_bounds__(kBwdDkdvThreads, 1)
+__global__ void __launch_bounds__(kBwdThreads, 1)
 bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const BwdSm100Dev p) {
     constexpr int TILE = 128 * HDIM * 2, QS = 3, OS = 2;
@@ -654,7 +710,7 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     uint8_t* sV = sK + TILE;
     uint8_t* sQ = sV + TILE;
     uint8_t* sDO = sQ + QS * TILE;
-    float* sRow = reinterpret_cast<float*>(sDO + OS * TILE);  // [2 steps][LSE 128 | D 128] of the query columns
+    float* sRow = reinterpret_cast<float*>(sDO + OS * TILE);  // [2 steps][LSE 128 | D 128] of the query columns, negated
     BwdCtrl* ctrl = reinterpret_cast<BwdCtrl*>(sRow + 512);
     volatile int* abort_flag = &ctrl->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = p.hq / p.hkv;
@@ -669,30 +725,29 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     if (threadIdx.x == 0) {
         for (int i = 0; i < kBwdItemRing; ++i) {
             mbar_init(&ctrl->item_full[i], 1);
-            mbar_init(&ctrl->item_empty[i], 12);  // every warp but the scheduling and the idle ones
+            mbar_init(&ctrl->item_empty[i], kBwdConsumers);
         }
         for (int i = 0; i < QS; ++i) { mbar_init(&ctrl->a_full[i], 1); mbar_init(&ctrl->a_empty[i], 1); }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&ctrl->b_full[i], 1);
-            mbar_init(&ctrl->b_empty[i], 2);  // both products that read dO
+            mbar_init(&ctrl->b_empty[i], 1);
             mbar_init(&ctrl->own_full[i], 1);
             mbar_init(&ctrl->own_free[i], 1);
             mbar_init(&ctrl->row_full[i], 1);
-            mbar_init(&ctrl->row_empty[i], 8);
-            mbar_init(&ctrl->p_full[i], 8);
+            mbar_init(&ctrl->row_empty[i], 16);
+            mbar_init(&ctrl->p_full[i], 16);
         }
         mbar_init(&ctrl->s_full[0], 1);
-        mbar_init(&ctrl->s_free[0], 8);
+        mbar_init(&ctrl->s_free[0], 16);
         mbar_init(&ctrl->dp_full[0], 1);
-        mbar_init(&ctrl->ds_full[0], 8);
-        mbar_init(&ctrl->x_done[0], 1);
+        mbar_init(&ctrl->ds_full[0], 16);
         mbar_init(&ctrl->acc_full, 1);
-        mbar_init(&ctrl->acc_free, 8);
+        mbar_init(&ctrl->acc_free, 16);
         mbar_init(&ctrl->tail, 1);
         ctrl->abort_flag = 0;
         mbar_fence_init();
     }
-    if (warp == 8) {
+    if (warp == 16) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&ctrl->tmem_base)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
     }
@@ -703,13 +758,13 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     uint32_t k_item = 0;
     BwdItem it{};
 
-    // Registers: launched with 512 x 128 = 256 x 192 + 256 x 64.
-    if (warp >= 8) {
+    // Registers: as in the dQ kernel.
+    if (warp >= 16) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::);
-        if (warp == 11) {
-            bwd_schedule<false>(ctrl, p, lane);
-        } else if (warp == 9) {
-            // ================================ TMA producer ================================
+        if (warp == 18) {
+            // ================================ items and TMA copies ================================
+            BwdSchedule<false> schedule;
+            schedule.init(p, lane);
             uint32_t tails = 0, t = 0, n_item = 0;
             bool ok = true;
             auto own = [&](int which, uint8_t* dst, const CUtensorMap* map) -> bool {
@@ -717,7 +772,11 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 // (rows behind the end of the keys stay in their own rows of the gradients, which are not stored)
                 return bwd_load_tile<HDIM>(dst, map, &ctrl->own_full[which], &ctrl->tail, tails, it.h, it.k0 + it.row0, 128, lane, abort_flag, p.status);
             };
-            while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
+            // (an item is handed out while the copies of the one before it are still to come: its LSE and D are then there in time)
+            BwdItem ahead{};
+            for (bool more = schedule.next(ctrl, p, lane, ahead); ok && more;) {
+                it = ahead;
+                more = schedule.next(ctrl, p, lane, ahead);
                 const BwdRange range = bwd_query_tiles(p, it);
                 if (range.count == 0) continue;
                 for (int g = 0; ok && g < G; ++g)
@@ -734,7 +793,7 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     }
                 ++n_item;
             }
-        } else if (warp == 10) {
+        } else if (warp == 19) {
             // ================================ LSE and D of the query columns ================================
             pdl_wait();
             uint32_t t = 0;
@@ -763,8 +822,8 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     }
                 }
             }
-        } else if (warp == 8 || warp == 12) {
-            // ================================ MMA issuers: 8 S and dP, 12 dV and dK ================================
+        } else {
+            // ================================ MMA issuers: 16 S, 17 dP, dV and dK ================================
             const bool leader = elect_one_sync();
             bool ok = true;
             auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
@@ -772,46 +831,44 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             };
             auto commit = [&](uint64_t* bar) { if (leader) umma_commit(bar); };
             auto at = [&](uint64_t d, uint32_t bytes) { return d + (uint64_t)(bytes >> 4); };
+            constexpr uint32_t idesc_s = make_idesc<T>(false), idesc_o = make_idesc<T>(true, HDIM);
+            const uint64_t dK = make_smem_desc(smem_u32(sK), 0, 1024), dV = make_smem_desc(smem_u32(sV), 0, 1024);
+            const uint64_t dQ = make_smem_desc(smem_u32(sQ), 0, 1024), dDO = make_smem_desc(smem_u32(sDO), 0, 1024);
+            const uint64_t dQt = make_smem_desc(smem_u32(sQ), HALF_BYTES, 1024), dDOt = make_smem_desc(smem_u32(sDO), HALF_BYTES, 1024);
             uint32_t t = 0, qs = 0, qph = 0, n_item = 0;  // steps so far, Q slot and its phase, items with steps so far
-            if (warp == 8) {
-                constexpr uint32_t idesc_s = make_idesc<T>(false);
-                const uint64_t dK = make_smem_desc(smem_u32(sK), 0, 1024), dV = make_smem_desc(smem_u32(sV), 0, 1024);
-                const uint64_t dQ = make_smem_desc(smem_u32(sQ), 0, 1024), dDO = make_smem_desc(smem_u32(sDO), 0, 1024);
+            if (warp == 16) {
                 while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
                     const int N = bwd_query_tiles(p, it).count * G;
+                    if (N > 0 && !wait(&ctrl->own_full[0], n_item & 1u, 0x10130)) break;
                     for (int j = 0; j < N; ++j) {
-                        const uint32_t os = t & 1u;
-                        if (j == 0 && !wait(&ctrl->own_full[0], n_item & 1u, 0x10130)) break;
                         if (!wait(&ctrl->a_full[qs], qph, 0x10131)) break;
                         if (t > 0 && !wait(&ctrl->s_free[0], (t - 1) & 1u, 0x10132)) break;  // dP(t - 1) has been read from the region
                         tc_fence_after();
                         if (leader) bwd_issue_ss<HDIM>(tmem + (t & 1u) * 128, dK, at(dQ, qs * TILE), idesc_s);
                         commit(&ctrl->s_full[0]);
-                        if (j + 1 == N) commit(&ctrl->own_free[0]);
-                        if (j == 0 && !wait(&ctrl->own_full[1], n_item & 1u, 0x10133)) break;
-                        if (!wait(&ctrl->b_full[os], (t >> 1) & 1u, 0x10134)) break;
-                        if (t > 0 && !wait(&ctrl->x_done[0], (t - 1) & 1u, 0x10135)) break;  // P(t - 1) and dS(t - 1) have been used
-                        tc_fence_after();
-                        if (leader) bwd_issue_ss<HDIM>(tmem + ((t + 1) & 1u) * 128, dV, at(dDO, os * TILE), idesc_s);
-                        commit(&ctrl->dp_full[0]);
-                        commit(&ctrl->b_empty[os]);
-                        if (j + 1 == N) commit(&ctrl->own_free[1]);
                         ++t;
                         if (++qs == QS) { qs = 0; qph ^= 1u; }
                     }
-                    if (N > 0) ++n_item;
+                    if (!ok) break;
+                    if (N > 0) { commit(&ctrl->own_free[0]); ++n_item; }
                 }
             } else {
-                constexpr uint32_t idesc_o = make_idesc<T>(true, HDIM);
-                const uint64_t dQt = make_smem_desc(smem_u32(sQ), HALF_BYTES, 1024), dDOt = make_smem_desc(smem_u32(sDO), HALF_BYTES, 1024);
+                auto issue_dp = [&](uint32_t st) -> bool {  // to the region that P and dS of the step before have been read from
+                    if (!wait(&ctrl->b_full[st & 1u], (st >> 1) & 1u, 0x10134)) return false;
+                    tc_fence_after();
+                    if (leader) bwd_issue_ss<HDIM>(tmem + ((st + 1) & 1u) * 128, dV, at(dDO, (st & 1u) * TILE), idesc_s);
+                    commit(&ctrl->dp_full[0]);
+                    return true;
+                };
                 while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
                     const int N = bwd_query_tiles(p, it).count * G;
-                    if (N > 0 && n_item > 0 && !wait(&ctrl->acc_free, (n_item - 1) & 1u, 0x10136)) break;
+                    if (N == 0) continue;
+                    if (!wait(&ctrl->own_full[1], n_item & 1u, 0x10133) || !issue_dp(t)) break;
+                    if (n_item > 0 && !wait(&ctrl->acc_free, (n_item - 1) & 1u, 0x10136)) break;
                     for (int j = 0; j < N; ++j) {
-                        const uint32_t region = tmem + (t & 1u) * 128;  // P in its columns 0-31 and 64-95, dS in 32-63 and 96-127
+                        const uint32_t region = tmem + (t & 1u) * 128;  // of every 32 columns P has the first 16, dS the others
                         const uint32_t os = t & 1u;
-                        if (!wait(&ctrl->b_full[os], (t >> 1) & 1u, 0x10139)) break;  // (dP may still be waiting for this dO)
-                        if (!wait(&ctrl->p_full[t & 1u], (t >> 1) & 1u, 0x10137)) break;
+                        if (!wait(&ctrl->p_full[os], (t >> 1) & 1u, 0x10137)) break;
                         tc_fence_after();
                         if (leader) {
                             bwd_issue_xb(tmem + cDV, region, at(dDOt, os * TILE), idesc_o, 0, j > 0);
@@ -821,33 +878,39 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         if (!wait(&ctrl->ds_full[0], t & 1u, 0x10138)) break;
                         tc_fence_after();
                         if (leader) {
-                            bwd_issue_xb(tmem + cDK, region + 32, at(dQt, qs * TILE), idesc_o, 0, j > 0);
-                            bwd_issue_xb(tmem + cDK, region + 32, at(dQt, qs * TILE), idesc_o, 1, true);
+                            bwd_issue_xb(tmem + cDK, region + 16, at(dQt, qs * TILE), idesc_o, 0, j > 0);
+                            bwd_issue_xb(tmem + cDK, region + 16, at(dQt, qs * TILE), idesc_o, 1, true);
                         }
-                        commit(&ctrl->x_done[0]);
                         commit(&ctrl->a_empty[qs]);
+                        if (j + 1 < N && !issue_dp(t + 1)) break;
                         ++t;
                         if (++qs == QS) qs = 0;
                     }
                     if (!ok) break;
-                    if (N > 0) { commit(&ctrl->acc_full); ++n_item; }
+                    commit(&ctrl->own_free[1]);
+                    commit(&ctrl->acc_full);
+                    ++n_item;
                 }
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 192;\n" ::);
-        const int half = warp >> 2, r = (warp & 3) * 32 + lane;
-        const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + half * 64;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::);
+        const int quarter = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
         uint32_t t = 0, n_item = 0;
         bool ok = true;
         while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
+            constexpr int COLS = HDIM / 2;  // of dV (warps 0-7) or dK (8-15) that this warp stores
+            const bool is_dk = quarter >= 2;
             const int key = it.row0 + r, shift = p.mask_type == 2 ? it.sk - it.sq : 0;
+            const int first = it.row0 + (warp & 3) * 32;  // of this warp's rows
             const BwdRange range = bwd_query_tiles(p, it);
-            T* dst = (T*)(half ? p.dk : p.dv) + ((int64_t)(it.k0 + key) * p.hkv + it.h) * HDIM;  // warps 0-3 store dV, 4-7 dK
+            T* dst = (T*)(is_dk ? p.dk : p.dv) + ((int64_t)(it.k0 + first) * p.hkv + it.h) * HDIM + (quarter & 1) * COLS;
+            uint4 out[COLS / 8];
             if (range.count == 0) {  // nobody sees these keys
-                if (key < it.sk)
 #pragma unroll
-                    for (int v = 0; v < HDIM / 8; ++v) reinterpret_cast<uint4*>(dst)[v] = make_uint4(0u, 0u, 0u, 0u);
+                for (int v = 0; v < COLS / 8; ++v) out[v] = make_uint4(0u, 0u, 0u, 0u);
+                bwd_store_rows<T>(dst, (int64_t)p.hkv * HDIM, it.sk - first, out, lane);
                 continue;
             }
             // query rows that see all of the tile's keys
@@ -856,84 +919,71 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 if (p.wr >= 0) full_lo = it.row0 + 127 - shift - p.wr;
                 if (p.wl >= 0) full_hi = it.row0 - shift + p.wl;
             }
-            auto step = [&](int m0, float slope, auto masked) -> bool {
-                // columns of this half that see the key: i >= key - shift - wr, i <= key - shift + wl
-                int c_lo = 0, c_hi = 0x3fffffff;
-                if constexpr (decltype(masked)::value) {
-                    const int i0 = m0 + half * 64;
-                    c_lo = p.wr >= 0 ? key - shift - p.wr - i0 : 0;
-                    c_hi = p.wl >= 0 ? key - shift + p.wl - i0 : 0x3fffffff;
-                }
-                const float* rows = sRow + (t & 1) * 256 + half * 64;
-                const uint32_t tS = lane_addr + (t & 1u) * 128, tDP = lane_addr + ((t + 1) & 1u) * 128;
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_full[t & 1], (t >> 1) & 1u, abort_flag, p.status, 0x10140))) return false;
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->s_full[0], t & 1u, abort_flag, p.status, 0x10141))) return false;
+            for (int g = 0, m = 0; g < G; ++t) {
+                const int m0 = (range.begin + m) * 128, i0 = m0 + quarter * 32;
+                const bool masked = m0 < full_lo || m0 + 127 > full_hi;
+                const float slope = EXTRA && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h * G + g] * kLog2e : 0.f;
+                if (++m == range.count) { m = 0; ++g; }
+                // columns of this quarter that see the key: i >= key - shift - wr, i <= key - shift + wl
+                uint32_t seen = 0xffffffffu;
+                if (masked) seen = bwd_column_bits(p.wr >= 0 ? key - shift - p.wr - i0 : 0, p.wl >= 0 ? key - shift + p.wl - i0 : 31);
+                const float* rows = sRow + (t & 1) * 256 + quarter * 32;
+                const uint32_t tS = lane_addr + (t & 1u) * 128 + quarter * 32, tDP = lane_addr + ((t + 1) & 1u) * 128 + quarter * 32;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_full[t & 1], (t >> 1) & 1u, abort_flag, p.status, 0x10140)))) break;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->s_full[0], t & 1u, abort_flag, p.status, 0x10141)))) break;
                 tc_fence_after();
-                uint32_t x[2][32];
-                tmem_ld32(tS, x[0]);
-                tmem_ld32(tS + 32, x[1]);
+                uint32_t x[32], w[16];
+                tmem_ld32(tS, x);
                 tmem_wait_ld();
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[16];
-                    if constexpr (EXTRA) {
-                        if (p.soft_cap > 0.f) soft_cap_scores<32>(x[c], p.cap);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 l4 = *reinterpret_cast<const float4*>(rows + c * 32 + e);
-#pragma unroll
-                        for (int u = 0; u < 4; u += 2) {
-                            const int col = c * 32 + e + u;
-                            float2 f = make_float2(1.f, 1.f), away = f;
-                            if constexpr (EXTRA) {
-                                away.x = (float)(m0 + half * 64 + col + it.sk - it.sq - key);
-                                away.y = away.x + 1.f;
-                            }
-                            const float2 y = bwd_exponent<EXTRA>(p, make_float2(__uint_as_float(x[c][e + u]), __uint_as_float(x[c][e + u + 1])), slope,
-                                                                 away, u ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), f);
-                            float2 pr = bwd_exp2(y, (e + u) / 2);
-                            if constexpr (decltype(masked)::value) {
-                                if (col < c_lo || col > c_hi) pr.x = 0.f;
-                                if (col + 1 < c_lo || col + 1 > c_hi) pr.y = 0.f;
-                            }
-                            w[(e + u) / 2] = Elem<T>::pack2(pr.x, pr.y);
-                            if constexpr (EXTRA) pr = __fmul2_rn(pr, f);  // (from here on P serves dS alone)
-                            x[c][e + u] = __float_as_uint(pr.x);
-                            x[c][e + u + 1] = __float_as_uint(pr.y);
-                        }
-                    }
-                    tmem_st16(tS + c * 16, w);
+                if constexpr (EXTRA) {
+                    if (p.soft_cap > 0.f) soft_cap_scores<32>(x, p.cap);
                 }
+#pragma unroll
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 l4 = *reinterpret_cast<const float4*>(rows + e);
+#pragma unroll
+                    for (int u = 0; u < 4; u += 2) {
+                        float2 f = make_float2(1.f, 1.f), away = f;
+                        if constexpr (EXTRA) {
+                            away.x = (float)(i0 + e + u + it.sk - it.sq - key);
+                            away.y = away.x + 1.f;
+                        }
+                        const float2 y = bwd_exponent<EXTRA>(p, make_float2(__uint_as_float(x[e + u]), __uint_as_float(x[e + u + 1])), slope, away,
+                                                             u ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), f);
+                        float2 pr = bwd_exp2<kPolyDkdv>(y, (e + u) / 2);
+                        w[(e + u) / 2] = Elem<T>::pack2(pr.x, pr.y);
+                        if constexpr (EXTRA) pr = __fmul2_rn(pr, f);  // (from here on P serves dS alone)
+                        x[e + u] = __float_as_uint(pr.x);
+                        x[e + u + 1] = __float_as_uint(pr.y);
+                    }
+                }
+                if (masked) bwd_hide(w, seen);
+                tmem_st16(tS, w);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->p_full[t & 1u]);
-                if (!__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->dp_full[0], t & 1u, abort_flag, p.status, 0x10142))) return false;
+                if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->dp_full[0], t & 1u, abort_flag, p.status, 0x10142)))) break;
                 tc_fence_after();
-                uint32_t dp[2][32];
-                tmem_ld32(tDP, dp[0]);
-                tmem_ld32(tDP + 32, dp[1]);
+                uint32_t dp[32];
+                tmem_ld32(tDP, dp);
                 tmem_wait_ld();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->s_free[0]);
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t w[16];
+                for (int e = 0; e < 32; e += 4) {
+                    const float4 d4 = *reinterpret_cast<const float4*>(rows + 128 + e);
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) {
-                        const float4 d4 = *reinterpret_cast<const float4*>(rows + 128 + c * 32 + e);
-#pragma unroll
-                        for (int u = 0; u < 4; u += 2) {
-                            const float2 d = __fadd2_rn(make_float2(__uint_as_float(dp[c][e + u]), __uint_as_float(dp[c][e + u + 1])),
-                                                        u ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y));
-                            const float2 ds = __fmul2_rn(make_float2(__uint_as_float(x[c][e + u]), __uint_as_float(x[c][e + u + 1])), d);
-                            w[(e + u) / 2] = Elem<T>::pack2(ds.x, ds.y);
-                        }
+                    for (int u = 0; u < 4; u += 2) {
+                        const float2 d = __fadd2_rn(make_float2(__uint_as_float(dp[e + u]), __uint_as_float(dp[e + u + 1])),
+                                                    u ? make_float2(d4.z, d4.w) : make_float2(d4.x, d4.y));
+                        const float2 ds = __fmul2_rn(make_float2(__uint_as_float(x[e + u]), __uint_as_float(x[e + u + 1])), d);
+                        w[(e + u) / 2] = Elem<T>::pack2(ds.x, ds.y);
                     }
-                    tmem_st16(tS + 32 + c * 16, w);
                 }
+                if (masked) bwd_hide(w, seen);
+                tmem_st16(tS + 16, w);
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -941,35 +991,21 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     mbar_arrive(&ctrl->ds_full[0]);
                     mbar_arrive(&ctrl->row_empty[t & 1]);
                 }
-                ++t;
-                return true;
-            };
-            for (int g = 0; ok && g < G; ++g) {
-                const float slope = EXTRA && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h * G + g] * kLog2e : 0.f;
-                for (int m = 0; ok && m < range.count; ++m) {
-                    const int m0 = (range.begin + m) * 128;
-                    ok = m0 < full_lo || m0 + 127 > full_hi ? step(m0, slope, std::true_type{}) : step(m0, slope, std::false_type{});
-                }
             }
             if (!ok || !(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->acc_full, n_item & 1u, abort_flag, p.status, 0x10143)))) break;
             ++n_item;
             tc_fence_after();
-            uint32_t acc[HDIM / 32][32];
-#pragma unroll
-            for (int c = 0; c < HDIM / 32; ++c) tmem_ld32(lane_addr - half * 64 + (half ? cDK : cDV) + c * 32, acc[c]);
-            tmem_wait_ld();
+            bwd_load_rows<T, COLS>(lane_addr + (is_dk ? cDK : cDV) + (quarter & 1) * COLS, is_dk ? p.scale : 1.f, out);
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctrl->acc_free);
-            if (key < it.sk)
-#pragma unroll
-                for (int c = 0; c < HDIM / 32; ++c) bwd_store32<T>(dst + c * 32, acc[c], half ? p.scale : 1.f);
+            bwd_store_rows<T>(dst, (int64_t)p.hkv * HDIM, it.sk - first, out, lane);
         }
     }
     pdl_wait();
     tc_fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == 16) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
     }
