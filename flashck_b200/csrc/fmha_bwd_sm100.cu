@@ -19,7 +19,7 @@ int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
     if ((rc = make_map_3d(&mv, p.v, p.dtype, rows_k, p.hkv, 128, HDIM))) return rc;
     auto dq = bwd_dq_sm100_kernel<T, HDIM, EXTRA>;
     auto dkdv = bwd_dkdv_sm100_kernel<T, HDIM, EXTRA>;
-    constexpr size_t smem_dq = 1024 + 6 * TILE + 512 * sizeof(float) + sizeof(BwdCtrl);
+    constexpr size_t smem_dq = 7 * TILE + 256 * sizeof(float) + sizeof(BwdCtrl);
     constexpr size_t smem_dkdv = 7 * TILE + 512 * sizeof(float) + sizeof(BwdCtrl);
     static_assert(smem_dq <= 227 * 1024 && smem_dkdv <= 227 * 1024, "tiles and the control block must fit the 227 KB a CTA can have");
     static thread_local int configured_device = -1;  // per instantiation

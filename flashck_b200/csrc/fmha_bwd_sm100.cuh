@@ -17,7 +17,8 @@
 // (a single issuer spends as long on its waits and commits as the products take, and the tensor pipe takes instructions only
 // about one ahead: 16 % slower; dP follows the product that has read dS from its columns in one warp's order, without a
 // barrier between them), warp 18 finds the work items, hands them to the others through a ring and
-// issues the TMA copies, warp 19 computes D (dQ) or fetches LSE and D of the query columns (dK/dV).
+// issues the TMA copies, warp 19 requests the next item's O from memory (dQ) or
+// fetches LSE and D of the query columns (dK/dV).  D is computed by the elementwise warps of dQ, eight rows each.
 //   dQ works by halves h of 64 keys, each with its own barriers: one half's products run under the other's elementwise work.
 //   dK/dV: two 128-column regions change roles from step to step: P(i) and dS(i) lie in the region that S(i) came in, so that S(i+1)
 //   can take the other one as soon as dP(i) has been read from it.
@@ -233,7 +234,7 @@ struct BwdCtrl {
     BwdItem items[kBwdItemRing];
     uint64_t item_full[kBwdItemRing], item_empty[kBwdItemRing];
     uint64_t a_full[3], a_empty[3], b_full[2], b_empty[2];  // rings: dQ K / V; dK/dV Q / dO
-    uint64_t own_full[2], own_free[2];  // what an item owns: dK/dV the K / V tile; dQ: Q / dO in the buffer that they pass through, whose release is own_free[0]
+    uint64_t own_full[2], own_free[2];  // what an item owns: dK/dV the K / V tile; dQ: Q / dO on their way to tensor memory
     uint64_t s_full[2], s_free[2], dp_full[2], ds_full[2];  // dQ: by half; dK/dV: [0] (s_free[0]: dP has been read)
     uint64_t p_full[2];         // dK/dV, by step: the elementwise warps can be one step ahead of the products that read P
     uint64_t acc_full, acc_free, tail;
@@ -389,15 +390,21 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const BwdSm100Dev p) {
     constexpr int TILE = 128 * HDIM * 2, KS = 3, VS = 2;
     constexpr uint32_t cS = 0, cDP = 128, cDQ = 256, cQ = 384, cDO = 448;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* sK = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* sK = smem_raw;  // (no room for slack: that it starts on a 1024-byte boundary is checked below)
     uint8_t* sV = sK + KS * TILE;
-    uint8_t* sOwn = sV + VS * TILE;                          // Q, then dO of the next item on their way to tensor memory
-    float* sRow = reinterpret_cast<float*>(sOwn + TILE);     // [2 items][LSE 128 | D 128] of the rows
-    BwdCtrl* ctrl = reinterpret_cast<BwdCtrl*>(sRow + 512);
+    uint8_t* sQ = sV + VS * TILE;                            // Q and dO of the next item on their way to tensor memory
+    uint8_t* sDO = sQ + TILE;
+    float* sDelta = reinterpret_cast<float*>(sDO + TILE);    // [2 items][128 rows]
+    BwdCtrl* ctrl = reinterpret_cast<BwdCtrl*>(sDelta + 256);
     volatile int* abort_flag = &ctrl->abort_flag;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    if ((smem_u32(smem_raw) & 1023u) != 0) {
+        if (threadIdx.x == 0) atomicOr(p.status, 0x10100);
+        pdl_wait();
+        return;
+    }
     if (threadIdx.x == 0) {
         for (int i = 0; i < kBwdItemRing; ++i) {
             mbar_init(&ctrl->item_full[i], 1);
@@ -411,12 +418,12 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             mbar_init(&ctrl->s_free[i], 8);
             mbar_init(&ctrl->dp_full[i], 1);
             mbar_init(&ctrl->ds_full[i], 8);
-            mbar_init(&ctrl->row_full[i], 1);
-            mbar_init(&ctrl->row_empty[i], 16);
+            mbar_init(&ctrl->row_full[i], 16);
         }
         mbar_init(&ctrl->own_full[0], 1);
         mbar_init(&ctrl->own_full[1], 1);
         mbar_init(&ctrl->own_free[0], 1);
+        mbar_init(&ctrl->own_free[1], 17);  // copied to tensor memory, and read for D by the elementwise warps
         mbar_init(&ctrl->acc_full, 1);
         mbar_init(&ctrl->acc_free, 16);
         mbar_init(&ctrl->tail, 1);
@@ -444,85 +451,47 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             // ================================ items and TMA copies ================================
             BwdSchedule<true> schedule;
             schedule.init(p, lane);
-            uint32_t tails = 0, t = 0, own = 0;
+            uint32_t tails = 0, t = 0, n_own = 0;
             bool ok = true;
-            auto load_own = [&](int which, const CUtensorMap* map) {  // (rows behind the end of the queries stay in their own rows of dQ, which are not stored)
-                ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->own_free[0], (own & 1u) ^ 1u, abort_flag, p.status, 0x10022)) &&
-                     bwd_load_tile<HDIM>(sOwn, map, &ctrl->own_full[which], &ctrl->tail, tails, it.h, it.q0 + it.row0, 128, lane, abort_flag, p.status);
-                ++own;
-                return ok;
+            auto load_own = [&](const BwdItem& item) {  // (rows behind the end of the queries stay in their own rows of dQ, which are not stored)
+                for (int i = 0; ok && i < 2; ++i)
+                    ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->own_free[i], (n_own & 1u) ^ 1u, abort_flag, p.status, 0x10022)) &&
+                         bwd_load_tile<HDIM>(i ? sDO : sQ, i ? &map_do : &map_q, &ctrl->own_full[i], &ctrl->tail, tails, item.h, item.q0 + item.row0,
+                                             128, lane, abort_flag, p.status);
+                ++n_own;
             };
-            // (an item is handed out while the copies of the one before it are still to come: its LSE and D are then there in time)
+            // An item is handed out, and its Q and dO are fetched, while the copies of the one before it are still to come: its D is
+            // then there in time.
             BwdItem ahead{};
-            for (bool more = schedule.next(ctrl, p, lane, ahead); ok && more;) {
+            bool more = schedule.next(ctrl, p, lane, ahead);
+            if (more && bwd_key_tiles(p, ahead).count > 0) load_own(ahead);
+            while (ok && more) {
                 it = ahead;
                 more = schedule.next(ctrl, p, lane, ahead);
+                const bool fetch = more && bwd_key_tiles(p, ahead).count > 0;
                 const BwdRange range = bwd_key_tiles(p, it);
                 const int kh = it.h / (p.hq / p.hkv);
-                if (range.count > 0 && !load_own(0, &map_q)) break;
                 for (int j = 0; j < range.count; ++j, ++t) {
                     const int n0 = (range.begin + j) * 128, ks = t % KS, vs = t % VS;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->a_empty[ks], ((t / KS) & 1u) ^ 1u, abort_flag, p.status, 0x10020)))) break;
                     // (K rows behind the end meet dS = 0; those of V only make columns of dP that are masked by index)
                     if (!(ok = bwd_load_tile<HDIM>(sK + ks * TILE, &map_k, &ctrl->a_full[ks], &ctrl->tail, tails, kh, it.k0 + n0, it.sk - n0, lane,
                                                    abort_flag, p.status))) break;
-                    if (j == 0 && !load_own(1, &map_do)) break;
                     if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->b_empty[vs], ((t / VS) & 1u) ^ 1u, abort_flag, p.status, 0x10021)))) break;
                     bwd_load_tile<HDIM>(sV + vs * TILE, &map_v, &ctrl->b_full[vs], &ctrl->tail, tails, kh, it.k0 + n0, 128, lane, abort_flag, p.status);
+                    if (fetch && j == min(KS, range.count) - 1) load_own(ahead);
+                    if (!ok) break;
                 }
+                if (ok && fetch && range.count == 0) load_own(ahead);
             }
         } else if (warp == 19) {
-            // ================================ D = sum dO O - dLSE, and the LSE of the rows ================================
-            constexpr int L = HDIM / 8, ROWS = 32 / L, AHEAD = 4;  // lanes a row, rows a load, loads in flight
-            const int sub = lane / L, piece = lane % L;
-            uint32_t n_item = 0;  // items with products so far
+            // ================================ O of the coming item on its way to L2 ================================
             while (bwd_next_item(ctrl, p, k_item, lane, it)) {
-                const int N = bwd_key_tiles(p, it).count, slot = n_item & 1;
-                const int64_t lr = (p.seqstart_q ? (int64_t)it.h * p.seqlen_q + it.q0 : ((int64_t)it.b * p.hq + it.h) * p.seqlen_q) + it.row0;
-                const int64_t at = ((int64_t)(it.q0 + it.row0) * p.hq + it.h) * HDIM + piece * 8;
-                const int left = it.sq - it.row0;  // rows that exist from the tile's first on
-                if (N > 0 && !__all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_empty[slot], ((n_item >> 1) & 1u) ^ 1u, abort_flag, p.status, 0x10011))) break;
-                float* rows = sRow + slot * 256;
-                if (N > 0)
+                for (int r = lane; r < min(128, it.sq - it.row0); r += 32) {
+                    const T* row = (const T*)p.o + ((int64_t)(it.q0 + it.row0 + r) * p.hq + it.h) * HDIM;
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) rows[u * 32 + lane] = u * 32 + lane < left ? bwd_lse_base2(p.lse[lr + u * 32 + lane]) : INFINITY;
-#pragma unroll 1
-                for (int g = 0; g < min(128, left); g += ROWS * AHEAD) {
-                    uint4 x[AHEAD], y[AHEAD];
-#pragma unroll
-                    for (int u = 0; u < AHEAD; ++u) {
-                        const int r = g + u * ROWS + sub;
-                        x[u] = y[u] = make_uint4(0u, 0u, 0u, 0u);
-                        if (r < left) {
-                            x[u] = *reinterpret_cast<const uint4*>((const T*)p.dout + at + (int64_t)r * p.hq * HDIM);
-                            y[u] = *reinterpret_cast<const uint4*>((const T*)p.o + at + (int64_t)r * p.hq * HDIM);
-                        }
-                    }
-#pragma unroll
-                    for (int u = 0; u < AHEAD; ++u) {
-                        const int r = g + u * ROWS + sub;
-                        const uint32_t xw[4] = {x[u].x, x[u].y, x[u].z, x[u].w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
-                        float delta = 0.f;
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float2 a = bias_pair<T>(xw[e]), o2 = bias_pair<T>(yw[e]);
-                            delta = fmaf(a.x, o2.x, fmaf(a.y, o2.y, delta));
-                        }
-#pragma unroll
-                        for (int off = L / 2; off > 0; off >>= 1) delta += __shfl_xor_sync(0xffffffffu, delta, off);
-                        if (piece == 0) {
-                            if (r < left) {
-                                if (p.dlse) delta -= p.dlse[lr + r];
-                                p.delta[lr + r] = delta;
-                            }
-                            if (N > 0) rows[128 + r] = delta;
-                        }
-                    }
+                    for (int c = 0; c < HDIM; c += 64) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(row + c));
                 }
-                if (N == 0) continue;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&ctrl->row_full[slot]);
-                ++n_item;
             }
         } else {
             // ================================ MMA issuers: 16 S, 17 dP and dQ ================================
@@ -536,7 +505,8 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             auto at = [&](uint64_t d, uint32_t bytes) { return d + (uint64_t)(bytes >> 4); };
             constexpr uint32_t idesc_s = make_idesc<T>(false, 64), idesc_q = make_idesc<T>(true, HDIM);
             const uint64_t dK = make_smem_desc(smem_u32(sK), 0, 1024), dV = make_smem_desc(smem_u32(sV), 0, 1024);
-            const uint64_t dKt = make_smem_desc(smem_u32(sK), HALF_BYTES, 1024), dOwn = make_smem_desc(smem_u32(sOwn), 0, 1024);
+            const uint64_t dKt = make_smem_desc(smem_u32(sK), HALF_BYTES, 1024);
+            const uint64_t dQ = make_smem_desc(smem_u32(sQ), 0, 1024), dDO = make_smem_desc(smem_u32(sDO), 0, 1024);
             uint32_t t = 0, ks = 0, kph = 0, n_item = 0;  // steps so far, K slot and its phase, items with steps so far
             if (warp == 16) {
                 while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
@@ -545,7 +515,7 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         if (!wait(&ctrl->own_full[0], n_item++ & 1u, 0x10030)) break;
                         if (t > 0 && !wait(&ctrl->s_full[1], (t - 1) & 1u, 0x10038)) break;
                         tc_fence_after();
-                        if (leader) bwd_copy_to_tmem<HDIM>(tmem + cQ, dOwn);
+                        if (leader) bwd_copy_to_tmem<HDIM>(tmem + cQ, dQ);
                         commit(&ctrl->own_free[0]);
                     }
                     for (int j = 0; j < N; ++j) {
@@ -578,8 +548,8 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     // dO, over the last item's, whose last dP has been read
                     if (!wait(&ctrl->own_full[1], n_item & 1u, 0x10033)) break;
                     tc_fence_after();
-                    if (leader) bwd_copy_to_tmem<HDIM>(tmem + cDO, dOwn);
-                    commit(&ctrl->own_free[0]);
+                    if (leader) bwd_copy_to_tmem<HDIM>(tmem + cDO, dDO);
+                    commit(&ctrl->own_free[1]);
                     if (!issue_dp(t, 0) || !issue_dp(t, 1)) break;
                     if (n_item > 0 && !wait(&ctrl->acc_free, (n_item - 1) & 1u, 0x10036)) break;
                     for (int j = 0; j < N; ++j) {
@@ -614,6 +584,45 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const int first = it.row0 + (warp & 3) * 32;  // of this warp's rows
             const BwdRange range = bwd_key_tiles(p, it);
             T* dst = (T*)p.dq + ((int64_t)(it.q0 + first) * p.hq + it.h) * HDIM + quarter * COLS;
+            // D = sum dO O - dLSE of rows warp * 8 .. + 7, dO from its tile (or from memory, where the item has no products)
+            const int64_t lr = (p.seqstart_q ? (int64_t)it.h * p.seqlen_q + it.q0 : ((int64_t)it.b * p.hq + it.h) * p.seqlen_q) + it.row0;
+            const int slot = n_item & 1, left = it.sq - it.row0;
+            const float lse2 = r < left ? bwd_lse_base2(p.lse[lr + r]) : INFINITY;
+            {
+                constexpr int L = HDIM / 8, ROWS = 32 / L, LOADS = 8 / ROWS;  // lanes a row, rows a load
+                const int sub = lane / L, piece = lane % L;
+                const int64_t at = ((int64_t)(it.q0 + it.row0) * p.hq + it.h) * HDIM + piece * 8, stride = (int64_t)p.hq * HDIM;
+                uint4 y[LOADS];
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u) {
+                    const int row = warp * 8 + u * ROWS + sub;
+                    y[u] = row < left ? *reinterpret_cast<const uint4*>((const T*)p.o + at + row * stride) : make_uint4(0u, 0u, 0u, 0u);
+                }
+                if (range.count > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->own_full[1], n_item & 1u, abort_flag, p.status, 0x10040)))) break;
+#pragma unroll
+                for (int u = 0; u < LOADS; ++u) {
+                    const int row = warp * 8 + u * ROWS + sub;
+                    uint4 x = make_uint4(0u, 0u, 0u, 0u);
+                    if (range.count > 0) x = *reinterpret_cast<const uint4*>(sDO + (piece / 8) * HALF_BYTES + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+                    else if (row < left) x = *reinterpret_cast<const uint4*>((const T*)p.dout + at + row * stride);
+                    const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float2 a = bias_pair<T>(xw[e]), o2 = bias_pair<T>(yw[e]);
+                        sum = fmaf(a.x, o2.x, fmaf(a.y, o2.y, sum));
+                    }
+#pragma unroll
+                    for (int off = L / 2; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+                    if (piece == 0) {
+                        if (row < left) {
+                            if (p.dlse) sum -= p.dlse[lr + row];
+                            p.delta[lr + row] = sum;
+                        }
+                        sDelta[slot * 128 + row] = sum;
+                    }
+                }
+            }
             uint4 out[COLS / 8];
             if (range.count == 0) {  // no row of the tile sees a key
 #pragma unroll
@@ -621,11 +630,11 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 bwd_store_rows<T>(dst, (int64_t)p.hq * HDIM, it.sq - first, out, lane);
                 continue;
             }
-            const int slot = n_item & 1;
-            if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_full[slot], (n_item >> 1) & 1u, abort_flag, p.status, 0x10040)))) break;
-            const float lse2 = sRow[slot * 256 + r], delta = sRow[slot * 256 + 128 + r];
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ctrl->row_empty[slot]);
+            if (lane == 0) mbar_arrive(&ctrl->own_free[1]);
+            if (lane == 0) mbar_arrive(&ctrl->row_full[slot]);
+            if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_full[slot], (n_item >> 1) & 1u, abort_flag, p.status, 0x10044)))) break;
+            const float delta = sDelta[slot * 128 + r];
             const float slope = EXTRA && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h] * kLog2e : 0.f;
             // visible keys of this row; key tiles that every row of the tile sees whole
             const int k_lo = p.mask_type != 0 && p.wl >= 0 ? i + shift - p.wl : 0;
