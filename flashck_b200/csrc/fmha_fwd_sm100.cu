@@ -9,7 +9,7 @@ namespace fck {
 namespace sm100 {
 
 #define FCK_EXTERN(T, E, V, S, H) extern FCK_SM100_INST(T, E, V, S, H)
-#define FCK_EXTERN_SPLIT(T, S, E) extern FCK_SM100_INST_SPLIT(T, S, E)
+#define FCK_EXTERN_SPLIT(T, S, E, H) extern FCK_SM100_INST_SPLIT(T, S, E, H)
 FCK_SM100_PLAIN(FCK_EXTERN, __half) FCK_SM100_PLAIN(FCK_EXTERN, __nv_bfloat16)
 FCK_SM100_HDIM64(FCK_EXTERN, __half) FCK_SM100_HDIM64(FCK_EXTERN, __nv_bfloat16)
 FCK_SM100_EXTRA(FCK_EXTERN, __half) FCK_SM100_EXTRA(FCK_EXTERN, __nv_bfloat16)
@@ -18,6 +18,7 @@ FCK_SM100_BIAS(FCK_EXTERN, __half) FCK_SM100_BIAS(FCK_EXTERN, __nv_bfloat16)
 FCK_SM100_TMA_BIAS(FCK_EXTERN, __half) FCK_SM100_TMA_BIAS(FCK_EXTERN, __nv_bfloat16)
 FCK_SM100_FP8(FCK_EXTERN, f8e4m3_t) FCK_SM100_FP8(FCK_EXTERN, f8e5m2_t)
 FCK_SM100_SPLIT(FCK_EXTERN_SPLIT, __half) FCK_SM100_SPLIT(FCK_EXTERN_SPLIT, __nv_bfloat16)
+FCK_SM100_SPLIT64(FCK_EXTERN_SPLIT, __half) FCK_SM100_SPLIT64(FCK_EXTERN_SPLIT, __nv_bfloat16)
 
 }  // namespace sm100
 
@@ -50,6 +51,8 @@ int64_t split_cap_tiles(const SplitKVParams& p) {  // key tiles of the longest s
     const int64_t cap = p.block_table ? p.bt_stride * p.page : p.seqlen_k_cap;
     return (cap + BN - 1) / BN;
 }
+// packed rows of a tile: whole tokens
+int64_t split_rows_per_tile(const SplitKVParams& p, int64_t rows) { return std::max<int64_t>(rows / (p.hq / p.hkv), 1) * (p.hq / p.hkv); }
 // At most 64 packed rows and room for two splits per piece: the rows are duplicated (kernel mode 2).
 bool split_duplicates_rows(const SplitKVParams& p) {
     return p.max_seqlen_q * (p.hq / p.hkv) <= 64 && p.num_splits >= 2;
@@ -201,12 +204,14 @@ int launch_fwd_sm100(const FwdParams& p, cudaStream_t stream) {
 bool splitkv_sm100_supported(const SplitKVParams& p) {
     if (!g_use_sm100_splitkv.load()) return false;
     if (p.alibi_slopes) return false;  // ALiBi runs on the mma.sync decode kernel
-    if (p.d != HD || p.dv != HD || p.batch <= 0 || p.batch > kMaxBatch || p.hq > 1023) return false;
+    // hdim 64 and groups that do not divide a tile: a shared prefix's rows only (other calls keep the kernel that they have)
+    if (p.d != p.dv || !(p.d == HD || (p.d == 64 && p.shared_prefix)) || p.batch <= 0 || p.batch > kMaxBatch || p.hq > 1023) return false;
     const int64_t group = p.hq / p.hkv;
-    if (group > BM || BM % group != 0) return false;
+    if (group > BM || (BM % group != 0 && !p.shared_prefix)) return false;
+    const int64_t rpt = split_rows_per_tile(p, BM);
     // one 16-row tile of (token, group head) rows is what the mma.sync decode kernel serves at the HBM rate
     if (p.max_seqlen_q * group <= 16) return false;
-    if ((p.max_seqlen_q * group + BM - 1) / BM > 16) return false;
+    if ((p.max_seqlen_q * group + rpt - 1) / rpt > 16) return false;
     if (p.seqstart_k) return false;                           // paged or [rows, seqlen_k, hkv, d] caches
     if (p.mask_type > 2 || (p.mask_type != 0 && !(p.wl < 0 && p.wr == 0))) return false;  // none or causal
     if (p.block_table) {
@@ -220,8 +225,8 @@ bool splitkv_sm100_supported(const SplitKVParams& p) {
     // piece of w units reaches into at most w / item_cost + 2 streams, and w is at most the larger of the line's
     // 148th, the shortest piece, and what keeps the longest possible stream within the workspace's splits.
     const int64_t cap_tiles = split_cap_tiles(p);
-    const int64_t streams = p.batch * p.hkv * ((p.max_seqlen_q * group + BM - 1) / BM);
-    const int64_t item_cost = g_split_item_cost.load(), min_piece = g_split_min_piece_tiles.load();
+    const int64_t streams = p.batch * p.hkv * ((p.max_seqlen_q * group + rpt - 1) / rpt);
+    const int64_t item_cost = g_split_item_cost.load(), min_piece = p.shared_prefix ? p.min_piece_tiles : g_split_min_piece_tiles.load();
     const int64_t line = streams * (cap_tiles + item_cost);
     if (line >= (1ll << 31)) return false;
     const int64_t max_pieces = std::max<int64_t>(1, split_duplicates_rows(p) ? p.num_splits / 2 : p.num_splits);
@@ -259,7 +264,15 @@ int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream) {
     const bool bf16 = p.dtype == FLASHCK_DTYPE_BFLOAT16;
     const bool hexp = g_exp_mode_splitkv.load() == 1;
     dev.rescale_thr = hexp ? 0.01f * (float)g_rescale_half_x100.load() : kRescaleThreshold;
-    if (split_duplicates_rows(p)) {
+    const bool twice = split_duplicates_rows(p);
+    dev.rpt = (int)split_rows_per_tile(p, twice ? 64 : BM);
+    if (p.shared_prefix) dev.piece_tiles = (int)p.min_piece_tiles;
+    if (p.d == 64) {  // (fp32 exponentials)
+        dev.rescale_thr = kRescaleThreshold;
+        if (twice) return bf16 ? launch_split_t<__nv_bfloat16, 2, 0, 64>(p, dev, stream) : launch_split_t<__half, 2, 0, 64>(p, dev, stream);
+        return bf16 ? launch_split_t<__nv_bfloat16, 1, 0, 64>(p, dev, stream) : launch_split_t<__half, 1, 0, 64>(p, dev, stream);
+    }
+    if (twice) {
         if (hexp) return bf16 ? launch_split_t<__nv_bfloat16, 2, 1>(p, dev, stream) : launch_split_t<__half, 2, 1>(p, dev, stream);
         return bf16 ? launch_split_t<__nv_bfloat16, 2, 0>(p, dev, stream) : launch_split_t<__half, 2, 0>(p, dev, stream);
     }

@@ -101,6 +101,7 @@ struct Sm100Dev {
     float* o_acc;
     float* lse_acc;
     int num_splits, piece_tiles, group, sq_cap;
+    int rpt;          // packed rows of a tile: 128, or fewer where the group does not divide it (64 in mode 2)
     int item_cost;    // units of the work line that stand for an item's fixed cost (see kItemCostDefault)
     int causal;       // mask type: 0 none, 1 top-left, 2 bottom-right, 3 window with top-left alignment
     int wl, wr;       // window of a masked problem: keys [i + shift - wl, i + shift + wr] of row i; -1 = unbounded
@@ -522,11 +523,11 @@ constexpr int kItemCostDefault = 6;   // instance parameter "split_item_cost" (1
 
 // key tiles the rows of row block `rb` of a sequence see
 __device__ __forceinline__ int split_stream_tiles(const Sm100Dev& p, int sq, int sk, int rb) {
-    const int first_tok = rb * BM / p.group;
+    const int first_tok = rb * p.rpt / p.group;
     if (first_tok >= sq || sk <= 0) return 0;
     int hi_key = sk - 1;
     if (p.causal) {
-        const int last_tok = min(sq, (rb * BM + BM + p.group - 1) / p.group) - 1;
+        const int last_tok = min(sq, (rb * p.rpt + p.rpt + p.group - 1) / p.group) - 1;
         hi_key = min(hi_key, last_tok + ((p.causal == 2) ? sk - sq : 0));
     }
     return hi_key >= 0 ? hi_key / BN + 1 : 0;
@@ -549,7 +550,7 @@ __device__ __forceinline__ void expand_item_split(const Ctrl* ctrl, const Sm100D
     it.kh = kh;
     it.h[0] = kh * p.group;  // first q head of the group
     it.h[1] = piece;         // split slot of the result
-    it.row0[0] = rb * BM;    // first packed row (token * group + group head)
+    it.row0[0] = rb * p.rpt;    // first packed row (token * group + group head)
     it.row0[1] = 0x3fffffff; // tile 1 does not exist
     it.shift = (p.causal == 2) ? it.sk - it.sq : 0;
     const int lo = rnd == 0 ? ctrl->split_first_lo : 0;
@@ -862,7 +863,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     constexpr bool F8 = ElemInfo<T>::f8;
     constexpr int ES = ElemInfo<T>::bytes;
     constexpr int HD = HDIM, RB = HD * ES, TILE_BYTES = BM * RB, HB = RB / 128, XB = 128 / ES, KK = 32 / ES;
-    static_assert(HDIM == 128 || (HDIM == 64 && SPLIT == 0), "hdim 64 is built for the prefill forms only");
+    static_assert(HDIM == 128 || HDIM == 64, "");
     static_assert(!F8 || (HDIM == 128 && SPLIT == 0 && (VAR & 6) == 0 && EXPM == 0),
                   "the 8-bit instances: hdim 128, prefill forms, fp32 exponentials, no score additions");
     constexpr bool WINDOW = (VAR & 1) != 0;  // the mask has a second bound (see above)
@@ -966,7 +967,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         ctrl->seq_sk[b] = sk;
         const int rows_per_block = p.pair_heads ? BM : 2 * BM;
         if (SPLIT) {  // units of the work line this sequence takes, and its longest stream
-            const int rbc = (sq * p.group + BM - 1) / BM;
+            const int rbc = (sq * p.group + p.rpt - 1) / p.rpt;
             int cost = 0, nmax = 0;
             for (int rb = 0; rb < rbc; ++rb) {
                 const int n = split_stream_tiles(p, sq, sk, rb);
@@ -1009,7 +1010,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
                 for (; b < p.batch && ctrl->level_start[b] < hi; ++b) {
                     const int sq = ctrl->seq_sq[b], sk = ctrl->seq_sk[b];
-                    const int rbc = (sq * p.group + BM - 1) / BM;
+                    const int rbc = (sq * p.group + p.rpt - 1) / p.rpt;
                     int seg0 = ctrl->level_start[b];
                     for (int rb = 0; rb < rbc && seg0 < hi; ++rb) {
                         const int n = split_stream_tiles(p, sq, sk, rb), c = n + p.item_cost;
@@ -1125,7 +1126,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     if (ok && SPLIT) {
                         // one box of (64 columns, group heads, 128/group tokens) per half: the rows land in
                         // (token, group head) order
-                        mbar_expect_tx(&ctrl->q_full, TILE_BYTES);
+                        mbar_expect_tx(&ctrl->q_full, (SPLIT == 2 ? 2 : 1) * p.rpt * RB);
                         for (int hb = 0; hb < HB; ++hb) {
                             if (SPLIT == 2) {  // the box holds 64 rows: once for tile rows 0-63, once for 64-127
                                 tma_load_4d(sQ + hb * HALF_BYTES, &map_q, &ctrl->q_full, hb * XB, 0, it.kh, it.q0);
@@ -1465,7 +1466,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             // overwrite the buffer) that this product is complete.
             if (warp == 4) {  // (all lanes walk the loop, the elected one issues)
                 const bool lead4 = elect_one_sync();
-                constexpr uint32_t idesc_pv = make_idesc<T>(true);
+                constexpr uint32_t idesc_pv = make_idesc<T>(true, HD);
                 const uint64_t dV0 = make_smem_desc(smem_u32(sV), HALF_BYTES, 1024);
                 const uint64_t dV1 = make_smem_desc(smem_u32(sV + TILE_BYTES), HALF_BYTES, 1024);
                 uint32_t kv_cnt = 0, g = 0;
@@ -1501,16 +1502,16 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const int max_pieces = max(1, p.num_splits / kDup), w = ctrl->split_w;
                 for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
                     const int sq = ctrl->seq_sq[b], sk = ctrl->seq_sk[b], q0 = ctrl->seq_q0[b];
-                    const int rbc = (sq * p.group + BM - 1) / BM;
+                    const int rbc = (sq * p.group + p.rpt - 1) / p.rpt;
                     int seg0 = ctrl->level_start[b];
                     for (int rb = 0; rb < rbc; ++rb) {
                         const int n = split_stream_tiles(p, sq, sk, rb), c = n + p.item_cost;
-                        const int rows = min(BM, sq * p.group - rb * BM);
+                        const int rows = min(p.rpt, sq * p.group - rb * p.rpt);
                         for (int kh = 0; kh < p.hkv; ++kh) {
                             const int used = split_stream_pieces(seg0 + kh * c, n, w, max_pieces, p.item_cost) * kDup;
                             const int cnt = (p.num_splits - used) * rows;
                             for (int e = (int)threadIdx.x - 160; e < cnt; e += 96) {
-                                const int sp = used + e / rows, pr = rb * BM + e % rows;
+                                const int sp = used + e / rows, pr = rb * p.rpt + e % rows;
                                 const int tok = pr / p.group, h = kh * p.group + (pr - tok * p.group);
                                 const int64_t slot = p.seqstart_q ? ((int64_t)h * p.num_splits + sp) * p.total_q + q0 + tok
                                                                   : (((int64_t)b * p.hq + h) * p.num_splits + sp) * p.sq_cap + tok;
@@ -1537,7 +1538,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             const int khalf = SPLIT == 2 ? (r >> 6) : 0;  // which 64 keys of every tile this thread's copy of the row takes
             const int tile_first_row = SPLIT ? packed_first / group : packed_first;
             const int row = SPLIT ? (packed_first + rr) / group : packed_first + r;      // row inside the sequence
-            const bool row_ok = row < sq;
+            const bool row_ok = row < sq && (SPLIT == 0 || rr < p.rpt);
             if (SPLIT) head += (packed_first + rr) - row * group;
             // visible keys of this row: [first_key, limit]
             const int wr = WINDOW ? p.wr : 0, wl = WINDOW ? p.wl : -1;
@@ -1860,7 +1861,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     const unsigned long long my_ptr = row_ok ? (unsigned long long)(p.o_acc + slot * HD) : 0ull;
                     float* stage = reinterpret_cast<float*>(sStage + (warp & 3) * 4096);
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
+                    for (int c = 0; c < HD / 32; ++c) {
                         uint32_t t[32];
                         if (Ni > 0) {
                             tmem_ld32(tO + c * 32, t);
@@ -2088,11 +2089,11 @@ int launch_t(const FwdParams& p, const Sm100Dev& dev, cudaStream_t stream) {
 
 // ---- split-KV with several query rows per kv head (append + decode, speculative decoding, chunked prefill) ----
 // Q [tokens, hkv, group, 128] as boxes of (64 columns, group heads, 1 kv head, 128/group tokens).
-inline int make_map_q_packed(CUtensorMap* map, const void* base, int dtype, int64_t tokens, int64_t hkv, int64_t group, int rows) {
+inline int make_map_q_packed(CUtensorMap* map, const void* base, int dtype, int64_t tokens, int64_t hkv, int64_t group, int rows, int hd) {
     PFN_encodeTiled enc = get_encode_tiled();
     FCK_REQUIRE(enc != nullptr, FLASHCK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint64_t dims[4] = {(cuuint64_t)HD, (cuuint64_t)group, (cuuint64_t)hkv, (cuuint64_t)(tokens > 0 ? tokens : 1)};
-    const cuuint64_t strides[3] = {(cuuint64_t)(HD * 2), (cuuint64_t)(group * HD * 2), (cuuint64_t)(hkv * group * HD * 2)};
+    const cuuint64_t dims[4] = {(cuuint64_t)hd, (cuuint64_t)group, (cuuint64_t)hkv, (cuuint64_t)(tokens > 0 ? tokens : 1)};
+    const cuuint64_t strides[3] = {(cuuint64_t)(hd * 2), (cuuint64_t)(group * hd * 2), (cuuint64_t)(hkv * group * hd * 2)};
     const cuuint32_t box[4] = {64, (cuuint32_t)group, 1, (cuuint32_t)(rows / group)};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
     const CUtensorMapDataType dt =
@@ -2103,22 +2104,22 @@ inline int make_map_q_packed(CUtensorMap* map, const void* base, int dtype, int6
     return FLASHCK_OK;
 }
 
-template <typename T, int SPLIT, int EXPM>
+template <typename T, int SPLIT, int EXPM, int HDIM = 128>
 int launch_split_t(const SplitKVParams& p, const Sm100Dev& dev, cudaStream_t stream) {
     const int64_t tokens = p.seqstart_q ? p.total_q : p.batch * p.seqlen_q;
     const int box_k = p.block_table ? (int)std::min<int64_t>(p.page, BN) : BN;
     CUtensorMap mq, mk, mv;
     int rc;
-    if ((rc = make_map_q_packed(&mq, p.q, p.dtype, tokens, p.hkv, p.hq / p.hkv, SPLIT == 2 ? 64 : BM))) return rc;
+    if ((rc = make_map_q_packed(&mq, p.q, p.dtype, tokens, p.hkv, p.hq / p.hkv, SPLIT == 2 ? 64 : BM, HDIM))) return rc;
     // Paged pools: the map ends with the pool (num_pages pages: a page id beyond it reads as zeros), and a copy never
     // leaves its page.  Contiguous cache [batch, capacity, hkv, 128]: the last 128-token chunk of a row reaches past the
     // row's end, and past the end of the buffer in the last row; the map carries the true row count so that those rows
     // are not read (they come as zeros).
     const int64_t cache_rows = p.block_table ? std::max<int64_t>(p.num_pages, 1) * p.page : p.batch * p.seqlen_k_cap;
-    if ((rc = make_map_3d(&mk, p.k, p.dtype, cache_rows, p.hkv, box_k))) return rc;
-    if ((rc = make_map_3d(&mv, p.v, p.dtype, cache_rows, p.hkv, box_k))) return rc;
-    auto kern = fmha_fwd_sm100_kernel<T, EXPM, 0, SPLIT>;
-    const size_t smem = 1024 + (size_t)(2 + 2 * KV_SLOTS) * TILE_BYTES + 8 * STAGE_BYTES + sizeof(Ctrl);
+    if ((rc = make_map_3d(&mk, p.k, p.dtype, cache_rows, p.hkv, box_k, HDIM))) return rc;
+    if ((rc = make_map_3d(&mv, p.v, p.dtype, cache_rows, p.hkv, box_k, HDIM))) return rc;
+    auto kern = fmha_fwd_sm100_kernel<T, EXPM, 0, SPLIT, HDIM>;
+    const size_t smem = 1024 + (size_t)(2 + 2 * KV_SLOTS) * (BM * HDIM * 2) + 8 * STAGE_BYTES + sizeof(Ctrl);
     static thread_local int configured_device = -1;
     int devid = 0;
     FCK_CUDA(cudaGetDevice(&devid));
@@ -2131,7 +2132,7 @@ int launch_split_t(const SplitKVParams& p, const Sm100Dev& dev, cudaStream_t str
 }
 
 // The instances, one explicit instantiation each (fmha_fwd_sm100_*.cu; a compilation of several minutes otherwise).
-// FCK_SM100_PREFILL(X) lists launch_t<T, EXPM, VAR, SPLIT, HDIM>, FCK_SM100_SPLIT(X) launch_split_t<T, SPLIT, EXPM>.
+// FCK_SM100_PREFILL(X) lists launch_t<T, EXPM, VAR, SPLIT, HDIM>, FCK_SM100_SPLIT(X) launch_split_t<T, SPLIT, EXPM, HDIM>.
 #define FCK_SM100_PLAIN(X, T) X(T, 0, 0, 0, 128) X(T, 1, 0, 0, 128) X(T, 11, 0, 0, 128) X(T, 12, 0, 0, 128) X(T, 13, 0, 0, 128) \
     X(T, 0, 1, 0, 128) X(T, 1, 1, 0, 128)
 #define FCK_SM100_HDIM64(X, T) X(T, 0, 0, 0, 64) X(T, 0, 1, 0, 64)
@@ -2140,9 +2141,10 @@ int launch_split_t(const SplitKVParams& p, const Sm100Dev& dev, cudaStream_t str
 #define FCK_SM100_BIAS(X, T) X(T, 0, 4, 0, 128) X(T, 0, 5, 0, 128)
 #define FCK_SM100_TMA_BIAS(X, T) X(T, 0, 12, 0, 128) X(T, 0, 13, 0, 128)
 #define FCK_SM100_FP8(X, T) X(T, 0, 0, 0, 128) X(T, 0, 1, 0, 128)
-#define FCK_SM100_SPLIT(X, T) X(T, 1, 0) X(T, 1, 1) X(T, 2, 0) X(T, 2, 1)
+#define FCK_SM100_SPLIT(X, T) X(T, 1, 0, 128) X(T, 1, 1, 128) X(T, 2, 0, 128) X(T, 2, 1, 128)
+#define FCK_SM100_SPLIT64(X, T) X(T, 1, 0, 64) X(T, 2, 0, 64)
 #define FCK_SM100_INST(T, E, V, S, H) template int launch_t<T, E, V, S, H>(const FwdParams&, const Sm100Dev&, cudaStream_t);
-#define FCK_SM100_INST_SPLIT(T, S, E) template int launch_split_t<T, S, E>(const SplitKVParams&, const Sm100Dev&, cudaStream_t);
+#define FCK_SM100_INST_SPLIT(T, S, E, H) template int launch_split_t<T, S, E, H>(const SplitKVParams&, const Sm100Dev&, cudaStream_t);
 
 }  // namespace sm100
 

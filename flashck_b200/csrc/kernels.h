@@ -64,7 +64,10 @@ struct SplitKVParams {
     // the score of query i and key j gets -slope * |i + sk - sq - j| added
     const float* alibi_slopes;
     int alibi_rank;
-    bool one_length = false;  // paged: no length array, every sequence holds seqlen_k_cap keys
+    // the pass over a shared prefix: one sequence of seqlen_k_cap keys, paged or not, without a length array; the shortest piece (tiles of
+    // 128 keys) the tcgen05 split mode cuts it into
+    bool shared_prefix = false;
+    int64_t min_piece_tiles = 0;
 };
 int launch_splitkv_decode(const SplitKVParams& p, cudaStream_t stream);
 // instance parameters (see FlashckSetInstanceParam): "stages", "ctas_per_sm_x100" ...

@@ -4,7 +4,7 @@
 //
 // over the partials s of the prefix and of the sequence's own cache.  1. The prefix: the query rows of all sequences as those of
 // one sequence (rows x group per kv head fill whole tiles, so the split kernels read the prefix once per 128 rows instead
-// of once per sequence).  2. The own caches, as any split-KV call.  3. The merge of both sets of partials, here.
+// of once per sequence; the tcgen05 split mode takes 16 tiles of rows in one launch, so more rows go in runs).  2. The own caches, as any split-KV call.  3. The merge of both sets of partials, here.
 #include <algorithm>
 
 #include "kernels.h"
@@ -13,7 +13,7 @@ namespace fck {
 
 namespace {
 
-constexpr int64_t kRowsPerLaunch = 2048;  // query rows per kv head that the tcgen05 split mode takes in one launch (16 tiles)
+constexpr int64_t kMinPieceTiles = 2;     // shortest run of 128-key tiles that a CTA takes of the prefix
 
 struct MergeDev {
     const float* lse1;  // prefix: runs of `chunk` rows one behind the other, each [hq, S1, rows of the run]
@@ -108,7 +108,7 @@ SplitKVParams prefix_pass(const SharedPrefixParams& p, int64_t row0, int64_t row
     s.k = p.k_prefix; s.v = p.v_prefix;
     s.block_table = p.prefix_table;
     s.batch = 1; s.seqlen_q = s.max_seqlen_q = s.total_q = rows;
-    s.seqlen_k_cap = p.prefix_len; s.one_length = true;
+    s.seqlen_k_cap = p.prefix_len; s.shared_prefix = true; s.min_piece_tiles = kMinPieceTiles;
     s.hq = p.hq; s.hkv = p.hkv; s.d = s.dv = p.d;
     s.num_pages = p.prefix_table ? p.prefix_pool_pages : 1;
     s.bt_stride = p.prefix_table ? (p.prefix_len + p.prefix_page - 1) / p.prefix_page : 0;
@@ -128,15 +128,16 @@ Plan plan(const SharedPrefixParams& p) {
     r.chunk = r.rows;
     if (p.prefix_len > 0 && r.rows > 0) {
         const int64_t sms = sm_count();
-        r.chunk = std::min(r.rows, std::max<int64_t>(1, kRowsPerLaunch / group));
+        const int64_t rpt = group <= 128 ? 128 / group * group : group;  // rows of a tile: whole tokens
+        r.chunk = std::min(r.rows, std::max<int64_t>(1, 16 * rpt / group));
         SplitKVParams s = prefix_pass(p, 0, r.chunk);
         s.num_splits = 2;
         s.lse_acc = reinterpret_cast<float*>(16);  // (only asked whether there is one)
-        const int64_t row_tiles = (r.chunk * group + 127) / 128;
+        const int64_t row_tiles = (r.chunk * group + rpt - 1) / rpt;
         if (splitkv_sm100_supported(s)) {
-            // a stream (kv head, row tile) is cut into 148 / streams pieces of at least 1024 keys and one more; with at most 64
-            // rows each piece leaves two partials
-            r.s1 = std::min((sms + p.hkv * row_tiles - 1) / (p.hkv * row_tiles) + 1, (p.prefix_len + 1023) / 1024 + 1);
+            // a stream (kv head, row tile) is cut into 148 / streams pieces of at least kMinPieceTiles tiles and one more; with at
+            // most 64 rows each piece leaves two partials
+            r.s1 = std::min((sms + p.hkv * row_tiles - 1) / (p.hkv * row_tiles) + 1, (p.prefix_len + 128 * kMinPieceTiles - 1) / (128 * kMinPieceTiles) + 1);
             if (r.chunk * group <= 64) r.s1 *= 2;
         } else {
             r.chunk = r.rows;

@@ -664,7 +664,7 @@ int launch_splitkv_decode(const SplitKVParams& p, cudaStream_t stream) {
     FCK_REQUIRE(p.batch >= 1 && p.batch <= 8192, FLASHCK_ERR_UNSUPPORTED, "splitkv: batch must be in [1,8192]");
     FCK_REQUIRE(!p.block_table || (p.page > 0 && p.page % kTok == 0), FLASHCK_ERR_UNSUPPORTED,
                 "splitkv: page_block_size must be a positive multiple of %d (got %lld)", kTok, (long long)p.page);
-    FCK_REQUIRE(!p.block_table || p.seqlen_k || p.one_length, FLASHCK_ERR_INVALID_ARGUMENT,
+    FCK_REQUIRE(!p.block_table || p.seqlen_k || p.shared_prefix, FLASHCK_ERR_INVALID_ARGUMENT,
                 "splitkv: paged K/V needs per-sequence lengths (k_seq_len_ptr)");
     int* status = device_status_ptr();
     if (!status) return FLASHCK_ERR_CUDA;
