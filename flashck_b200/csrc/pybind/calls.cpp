@@ -330,6 +330,113 @@ PyObject* call_append_kv(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     END_HANDLE_TH_ERRORS
 }
 
+// (dout, q, k, v, o, lse, cu_seqlens_q | None, cu_seqlens_k | None, max_seqlen_q, max_seqlen_k, scale, causal, window_size, mask_type,
+//  cap, dlse | None) -> (dq, dk, dv)
+PyObject* call_backward(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (!plain_state()) Py_RETURN_NONE;
+    Reader r{args, nargs};
+    const at::Tensor* dout = r.need(at::ScalarType::Undefined);
+    if (!r.ok || !elem16(dout)) Py_RETURN_NONE;
+    const at::ScalarType elem = dout->scalar_type();
+    const int64_t dim = dout->dim();
+    const at::Tensor *q = r.need(elem, dim), *k = r.need(elem, dim), *v = r.need(elem, dim), *o = r.need(elem, dim), *lse = r.need(at::kFloat);
+    const at::Tensor *cu_q = r.maybe(at::kLong), *cu_k = r.maybe(at::kLong);
+    const int64_t max_q = r.integer(), max_k = r.integer();
+    const double scale = r.real(true);
+    uint32_t mt;
+    int64_t wl, wr;
+    r.mask(mt, wl, wr);
+    const double cap = r.real(false);
+    const at::Tensor* dlse = r.maybe(at::kFloat);
+    if (!r.ok || r.i != nargs) Py_RETURN_NONE;
+    const bool group = cu_q != nullptr;
+    if (dim != (group ? 3 : 4) || group != (cu_k != nullptr)) Py_RETURN_NONE;
+    if (q->sizes() != dout->sizes() || o->sizes() != q->sizes() || v->sizes() != k->sizes() || k->size(-1) != q->size(-1)) Py_RETURN_NONE;
+    const int64_t hq = q->size(-2), d = q->size(-1), hkv = k->size(-2);
+    int64_t batch, sq, sk;
+    if (group) {
+        if (cu_q->numel() != cu_k->numel() || cu_q->numel() < 2 || lse->sizes() != at::IntArrayRef({hq, q->size(0)})) Py_RETURN_NONE;
+        batch = cu_q->numel() - 1;
+        sq = q->size(0);
+        sk = k->size(0);
+    } else {
+        batch = q->size(0);
+        sq = q->size(1);
+        sk = k->size(1);
+        if (k->size(0) != batch || lse->sizes() != at::IntArrayRef({batch, hq, sq})) Py_RETURN_NONE;
+    }
+    if (dlse && dlse->sizes() != lse->sizes()) Py_RETURN_NONE;
+    at::Tensor dq, dk, dv, delta;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(r.device);
+        dq = empty(q->sizes(), elem, r.device);
+        dk = empty(k->sizes(), elem, r.device);
+        dv = empty(k->sizes(), elem, r.device);
+        delta = empty({lse->numel()}, at::kFloat, r.device);
+        rc = FmhaBwd(ptr(dout), ptr(q), ptr(k), ptr(v), nullptr, ptr(o), ptr(lse), ptr(dlse), ptr(dq), ptr(dk), ptr(dv), nullptr, ptr(delta),
+                     (int64_t*)ptr(cu_q), (int64_t*)ptr(cu_k), batch, sq, sk, hq, hkv, d, d, group ? max_q : 0, group ? max_k : 0, (float)scale,
+                     wl, wr, mt, stream_of(r.device), dtype_code(*q), 0, 0, (float)cap);
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    PyObject* t[3] = {THPVariable_Wrap(dq), THPVariable_Wrap(dk), THPVariable_Wrap(dv)};
+    PyObject* all = t[0] && t[1] && t[2] ? PyTuple_Pack(3, t[0], t[1], t[2]) : nullptr;
+    for (PyObject* x : t) Py_XDECREF(x);
+    return all;
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, k_prefix, v_prefix, k_cache, v_cache, seqlen_k, prefix_len | None, prefix_table | None, block_table | None, cu_seqlens_q | None,
+//  max_seqlen_q, scale, causal, return_lse)
+PyObject* call_shared_prefix(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (!plain_state()) Py_RETURN_NONE;
+    Reader r{args, nargs};
+    const at::Tensor* q = r.need(at::ScalarType::Undefined);
+    if (!r.ok || !elem16(q)) Py_RETURN_NONE;
+    const at::ScalarType elem = q->scalar_type();
+    const at::Tensor *kp = r.need(elem), *vp = r.need(elem), *k = r.need(elem, 4), *v = r.need(elem, 4), *sl = r.need(at::kInt);
+    PyObject* len = r.next();
+    int64_t prefix = r.ok && len != Py_None ? r.integer(len) : -1;
+    const at::Tensor *table = r.maybe(at::kInt, 1), *bt = r.maybe(at::kInt, 2), *cu_q = r.maybe(at::kLong);
+    const int64_t max_q = r.integer();
+    const double scale = r.real(true);
+    const bool causal = r.flag(), with_lse = r.flag();
+    if (!r.ok || r.i != nargs || (len != Py_None && prefix < 0)) Py_RETURN_NONE;
+    const bool group = cu_q != nullptr;
+    const int64_t batch = sl->numel();
+    if (q->dim() != (group ? 3 : 4) || (group ? cu_q->numel() != batch + 1 : q->size(0) != batch)) Py_RETURN_NONE;
+    const int64_t sq = q->size(-3), hq = q->size(-2), d = q->size(-1), hkv = k->size(2);
+    if (k->size(3) != d || v->sizes() != k->sizes() || kp->dim() != (table ? 4 : 3) || kp->size(-2) != hkv || kp->size(-1) != d ||
+        vp->sizes() != kp->sizes() || hkv == 0)
+        Py_RETURN_NONE;
+    const int64_t p_page = table ? kp->size(1) : 0, page = bt ? k->size(1) : 0;
+    if (table ? len == Py_None || table->numel() * p_page < prefix : prefix > kp->size(0)) Py_RETURN_NONE;
+    if (prefix < 0) prefix = kp->size(0);
+    if ((bt ? bt->size(0) : k->size(0)) != batch) Py_RETURN_NONE;
+    at::Tensor o, lse, work;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(r.device);
+        const int64_t bytes = FlashckSharedPrefixWorkspace(prefix, p_page, page, batch, sq, max_q, hq, hkv, d, group, dtype_code(*q));
+        rc = bytes < 0 ? FLASHCK_ERR_INVALID_ARGUMENT : 0;
+        if (rc == 0) {
+            work = empty({std::max<int64_t>(bytes, 16)}, at::kByte, r.device);
+            o = empty(q->sizes(), elem, r.device);
+            if (with_lse) lse = group ? empty({hq, sq}, at::kFloat, r.device) : empty({batch, hq, sq}, at::kFloat, r.device);
+            rc = FmhaFwdSharedPrefix(ptr(q), ptr(kp), ptr(vp), ptr(k), ptr(v), ptr(o), ptr(lse), ptr(work), ptr(table), ptr(bt), ptr(sl),
+                                     (int64_t*)ptr(cu_q), prefix, p_page, kp->size(0), page, k->size(0), bt ? bt->size(1) : 0,
+                                     page ? 0 : k->size(1), batch, sq, max_q, hq, hkv, d, d, (float)scale, causal, stream_of(r.device),
+                                     dtype_code(*q));
+        }
+    }
+    return result(rc, o, lse);
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* num_splits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Reader r{args, nargs};
     const int64_t b = r.integer(), rows = r.integer();
@@ -342,6 +449,8 @@ PyMethodDef methods[] = {
     {"_call_paged_prefill", (PyCFunction)(void (*)(void))call_paged_prefill, METH_FASTCALL, nullptr},
     {"_call_splitkv", (PyCFunction)(void (*)(void))call_splitkv, METH_FASTCALL, nullptr},
     {"_call_append_kv", (PyCFunction)(void (*)(void))call_append_kv, METH_FASTCALL, nullptr},
+    {"_call_backward", (PyCFunction)(void (*)(void))call_backward, METH_FASTCALL, nullptr},
+    {"_call_shared_prefix", (PyCFunction)(void (*)(void))call_shared_prefix, METH_FASTCALL, nullptr},
     {"_num_splits", (PyCFunction)(void (*)(void))num_splits, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

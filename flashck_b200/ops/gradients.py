@@ -83,6 +83,11 @@ def fmha_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tens
 
     dout and o ``[b, sq, hq, d]``, q, k, v and the options as the forward had them, lse fp32 ``[b, hq, sq]`` -> ``(dq, dk, dv)``,
     with ``return_dbias`` the bias tensor's gradient as a fourth.  ``dlse``: the gradient of the LSE where it was used too."""
+    native = _f._native()
+    if native and bias is None and alibi_slopes is None and not return_dbias:
+        r = native._call_backward(dout, q, k, v, o, lse, None, None, 0, 0, scale, causal, window_size, mask_type, logits_soft_cap, dlse)
+        if r is not None:
+            return r if r.__class__ is not int else _lib.check(r, "FmhaBwd")
     _qkv(q, k, v, 4, "[batch, seqlen, heads, hdim]")
     b, sq = q.shape[:2]
     if k.shape[0] != b:
@@ -101,6 +106,12 @@ def fmha_bwd_var_len(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
 
     ``max_seqlen_*`` bound the longest sequences (0: the packed totals).  Rows that belong to no sequence get zeros; elements
     of the bias gradient outside the sequences' blocks too."""
+    native = _f._native()
+    if native and bias is None and alibi_slopes is None and not return_dbias and cu_seqlens_q is not None:
+        r = native._call_backward(dout, q, k, v, o, lse, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, scale, causal, window_size,
+                                  mask_type, logits_soft_cap, dlse)
+        if r is not None:
+            return r if r.__class__ is not int else _lib.check(r, "FmhaBwd")
     _qkv(q, k, v, 3, "packed [total_tokens, heads, hdim]")
     cu_q, cu_k = _f._as_i64("cu_seqlens_q", cu_seqlens_q), _f._as_i64("cu_seqlens_k", cu_seqlens_k)
     if cu_q.numel() != cu_k.numel() or cu_q.numel() < 2:

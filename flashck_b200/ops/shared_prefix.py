@@ -29,6 +29,12 @@ def fmha_fwd_shared_prefix(q: torch.Tensor, k_prefix: torch.Tensor, v_prefix: to
     sees the whole prefix and its own keys up to ``seqlen_k - sq + i``.
 
     Returns o like q (and LSE ``[b, hq, sq]`` / ``[hq, total_q]``); packed rows that belong to no sequence are not written."""
+    native = _f._native()
+    if native:
+        r = native._call_shared_prefix(q, k_prefix, v_prefix, k_cache, v_cache, seqlen_k, prefix_len, prefix_table, block_table, cu_seqlens_q,
+                                       max_seqlen_q, scale, causal, return_lse)
+        if r is not None:
+            return r if r.__class__ is not int else _lib.check(r, "FmhaFwdSharedPrefix")
     for n, t in (("q", q), ("k_prefix", k_prefix), ("v_prefix", v_prefix), ("k_cache", k_cache), ("v_cache", v_cache), ("seqlen_k", seqlen_k)):
         if t is None:
             raise TypeError(f"{n} must be a torch.Tensor")
