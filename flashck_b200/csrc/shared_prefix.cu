@@ -165,6 +165,9 @@ int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream) {
     if (r.rows == 0) return FLASHCK_OK;
     FCK_REQUIRE(r.rows * p.hq < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSharedPrefix: %lld rows of %lld heads (fewer than 2^31)",
                 (long long)r.rows, (long long)p.hq);
+    // (no more partials than pieces of two 16-key tiles in the room that a sequence has: short caches leave fewer slots to mark and merge)
+    const int64_t room = p.block_table ? p.bt_stride * p.page : p.seqlen_k_cap;
+    r.s2 = std::min(r.s2, std::max<int64_t>(2, (room + 31) / 32 + 1));
     float* o1 = (float*)p.workspace;
     float* o2 = o1 + r.floats1 * p.d;
     float* lse1 = o2 + r.floats2 * p.d;
@@ -184,7 +187,7 @@ int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream) {
     s.num_pages = p.block_table ? p.pool_pages : p.batch;
     s.bt_stride = p.bt_stride; s.page = p.page; s.scale = p.scale;
     s.mask_type = p.causal ? 2 : 0; s.wl = -1; s.wr = p.causal ? 0 : -1; s.dtype = p.dtype;
-    if (p.block_table ? p.bt_stride == 0 : p.seqlen_k_cap == 0) r.s2 = 0;  // caches without room: no sequence has own keys
+    if (room == 0) r.s2 = 0;  // caches without room: no sequence has own keys
     else if (int rc = splitkv_sm100_supported(s) ? launch_splitkv_sm100(s, stream) : launch_splitkv_decode(s, stream)) return rc;
     MergeDev m{};
     m.lse1 = lse1; m.o1 = o1; m.lse2 = lse2; m.o2 = o2; m.o = p.o; m.lse = p.lse; m.seqstart_q = p.seqstart_q;
