@@ -1,4 +1,6 @@
 // Backward of fmha_fwd on the tcgen05 kernels: which calls they take, the device parameters of a call, and the launches.
+#include <algorithm>
+
 #include "fmha_bwd_sm100.cuh"
 
 namespace fck {
@@ -7,7 +9,13 @@ using namespace sm100;
 
 namespace {
 
-template <typename T, int HDIM, bool EXTRA>
+// 128 x 128 tiles of all planes (group mode: of every sequence's block in them)
+int64_t bias_items(const BwdParams& p) {
+    const int64_t planes = (p.bias_rank >= 1 ? p.hq : 1) * (p.bias_rank == 2 || p.seqstart_q ? p.batch : 1);
+    return (p.max_seqlen_q + 127) / 128 * ((p.max_seqlen_k + 127) / 128) * planes;
+}
+
+template <typename T, int HDIM, int VAR>
 int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream) {
     constexpr size_t TILE = 128 * HDIM * 2;
     const int64_t rows_q = p.seqstart_q ? p.seqlen_q : p.batch * p.seqlen_q, rows_k = p.seqstart_k ? p.seqlen_k : p.batch * p.seqlen_k;
@@ -17,8 +25,8 @@ int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
     if ((rc = make_map_3d(&mdo, p.dout, p.dtype, rows_q, p.hq, 128, HDIM))) return rc;
     if ((rc = make_map_3d(&mk, p.k, p.dtype, rows_k, p.hkv, 128, HDIM))) return rc;
     if ((rc = make_map_3d(&mv, p.v, p.dtype, rows_k, p.hkv, 128, HDIM))) return rc;
-    auto dq = bwd_dq_sm100_kernel<T, HDIM, EXTRA>;
-    auto dkdv = bwd_dkdv_sm100_kernel<T, HDIM, EXTRA>;
+    auto dq = bwd_dq_sm100_kernel<T, HDIM, VAR>;
+    auto dkdv = bwd_dkdv_sm100_kernel<T, HDIM, VAR>;
     constexpr size_t smem_dq = 7 * TILE + 256 * sizeof(float) + sizeof(BwdCtrl);
     constexpr size_t smem_dkdv = 7 * TILE + 512 * sizeof(float) + sizeof(BwdCtrl);
     static_assert(smem_dq <= 227 * 1024 && smem_dkdv <= 227 * 1024, "tiles and the control block must fit the 227 KB a CTA can have");
@@ -40,20 +48,30 @@ int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
         if (i == 0) FCK_CUDA(launch_dependent(dq, grid, dim3(kBwdThreads), smem_dq, stream, mk, mv, mq, mdo, d));
         else FCK_CUDA(launch_dependent(dkdv, grid, dim3(kBwdThreads), smem_dkdv, stream, mq, mdo, mk, mv, d));
     }
+    if constexpr (VAR == 2) {
+        if (p.dbias) {
+            auto dbias = bwd_dbias_sm100_kernel<T, HDIM>;
+            constexpr size_t smem = 1024 + 6 * TILE + sizeof(BwdCtrl);
+            FCK_CUDA(cudaFuncSetAttribute(dbias, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+            const int64_t tq = (p.max_seqlen_q + 127) / 128, tk = (p.max_seqlen_k + 127) / 128, items = bias_items(p);
+            FCK_CUDA(launch_dependent(dbias, dim3((unsigned)std::min<int64_t>(items, sm_count())), dim3(kBwdThreads), smem, stream, mq, mdo, mk, mv, dev,
+                                      (int)tq, (int)tk, items));
+        }
+    }
     return FLASHCK_OK;
 }
 
 template <typename T>
 int launch_bwd_d(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream) {
-    const bool extra = p.bias_type == 2 || p.logits_soft_cap > 0.f;
-    if (p.d == 128) return extra ? launch_bwd_t<T, 128, true>(p, dev, stream) : launch_bwd_t<T, 128, false>(p, dev, stream);
-    return extra ? launch_bwd_t<T, 64, true>(p, dev, stream) : launch_bwd_t<T, 64, false>(p, dev, stream);
+    const int var = p.bias_type == 1 ? 2 : p.bias_type == 2 || p.logits_soft_cap > 0.f ? 1 : 0;
+    if (p.d == 128)
+        return var == 2 ? launch_bwd_t<T, 128, 2>(p, dev, stream) : var ? launch_bwd_t<T, 128, 1>(p, dev, stream) : launch_bwd_t<T, 128, 0>(p, dev, stream);
+    return var == 2 ? launch_bwd_t<T, 64, 2>(p, dev, stream) : var ? launch_bwd_t<T, 64, 1>(p, dev, stream) : launch_bwd_t<T, 64, 0>(p, dev, stream);
 }
 
 }  // namespace
 
 bool bwd_sm100_supported(const BwdParams& p) {
-    if (p.bias_type == 1) return false;  // an elementwise bias: the general instance
     if (p.max_seqlen_q == 0 || p.max_seqlen_k == 0 || p.batch == 0) return false;  // (nothing to multiply)
     if (p.wl >= (1ll << 30) || p.wr >= (1ll << 30)) return false;
     return (p.max_seqlen_q + 127) / 128 * p.hq * p.batch < (1ll << 31) && (p.max_seqlen_k + 127) / 128 * p.hkv * p.batch < (1ll << 31);
@@ -68,6 +86,8 @@ int launch_bwd_sm100(const BwdParams& p, cudaStream_t stream) {
     dev.batch = (int)p.batch; dev.seqlen_q = (int)p.seqlen_q; dev.seqlen_k = (int)p.seqlen_k; dev.hq = (int)p.hq; dev.hkv = (int)p.hkv;
     dev.mask_type = p.mask_type; dev.wl = p.wl < 0 ? -1 : (int)p.wl; dev.wr = p.wr < 0 ? -1 : (int)p.wr;
     dev.scale = p.scale; dev.scale_log2 = p.scale * kLog2e;
+    dev.bias = p.bias_type == 1 ? p.bias : nullptr; dev.dbias = p.dbias; dev.bias_rank = p.bias_rank;
+    dev.bias_sq = p.seqlen_q; dev.bias_sk = p.seqlen_k;
     dev.alibi = p.bias_type == 2 ? (const float*)p.bias : nullptr; dev.alibi_rank = p.bias_rank;
     dev.soft_cap = p.logits_soft_cap;
     if (p.logits_soft_cap > 0.f) {

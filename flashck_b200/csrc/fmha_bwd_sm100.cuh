@@ -50,6 +50,10 @@ struct BwdSm100Dev {
     int alibi_rank;
     float soft_cap, inv_cap_log2;  // the soft cap c (0: off), 1 / (c log2(e))
     SoftCap cap;                   // constants of soft_cap_scores
+    const void* bias;              // VAR 2: an elementwise bias, planes of bias_sq x bias_sk (group mode: the packed totals)
+    void* dbias;
+    int bias_rank;                 // 0 one plane, 1 one per head, 2 one per (batch, head)
+    int64_t bias_sq, bias_sk;
     int listed;                    // items are found in order of cost by a persistent grid; 0: one per CTA, by its index
     int max_tiles;                 // tiles of the longest sequence
 };
@@ -115,11 +119,12 @@ __device__ __forceinline__ float2 bwd_exp2(float2 y, int i) {
     return (i & 7) < POLY ? bwd_exp2_poly(y) : make_float2(ex2_fast(y.x), ex2_fast(y.y));
 }
 
-// Base-2 exponent of a pair of scores (raw, or with EXTRA what soft_cap_scores left of them), LSE subtracted; with a soft cap
-// f is what dS gets from it, 1 - tanh^2.
-template <bool EXTRA>
-__device__ __forceinline__ float2 bwd_exponent(const BwdSm100Dev& p, float2 x, float slope_log2, float2 away, float2 neg_lse2, float2& f) {
-    if constexpr (!EXTRA) return __ffma2_rn(x, make_float2(p.scale_log2, p.scale_log2), neg_lse2);
+// Score additions (template parameter VAR of the kernels): 0 none, 1 ALiBi and / or a soft cap, 2 a bias tensor and / or a soft cap.
+// Base-2 exponent of a pair of scores (raw, or behind a soft cap what soft_cap_scores left of them), LSE subtracted; with a soft
+// cap f is what dS gets from it, 1 - tanh^2.  `add`: distances from the diagonal, or bias values.
+template <int VAR>
+__device__ __forceinline__ float2 bwd_exponent(const BwdSm100Dev& p, float2 x, float slope_log2, float2 add, float2 neg_lse2, float2& f) {
+    if constexpr (VAR == 0) return __ffma2_rn(x, make_float2(p.scale_log2, p.scale_log2), neg_lse2);
     float2 y = x;
     if (p.soft_cap > 0.f) {
         const float2 t = __fmul2_rn(x, make_float2(p.inv_cap_log2, p.inv_cap_log2));
@@ -127,8 +132,15 @@ __device__ __forceinline__ float2 bwd_exponent(const BwdSm100Dev& p, float2 x, f
     } else {
         y = __fmul2_rn(x, make_float2(p.scale_log2, p.scale_log2));
     }
-    y = __ffma2_rn(make_float2(-slope_log2, -slope_log2), make_float2(fabsf(away.x), fabsf(away.y)), y);
+    if constexpr (VAR == 2) y = __ffma2_rn(make_float2(kLog2e, kLog2e), add, y);
+    else y = __ffma2_rn(make_float2(-slope_log2, -slope_log2), make_float2(fabsf(add.x), fabsf(add.y)), y);
     return __fadd2_rn(y, neg_lse2);
+}
+// Element (0, 0) of the bias block of a (sequence, head).
+__device__ __forceinline__ int64_t bwd_bias_block(const BwdSm100Dev& p, int b, int h, int64_t q0, int64_t k0) {
+    const int64_t plane = p.bias_sq * p.bias_sk;
+    return (p.bias_rank >= 1 ? (int64_t)h * plane : 0) + (p.bias_rank == 2 ? (int64_t)b * p.hq * plane : 0) +
+           (p.seqstart_q ? q0 * p.bias_sk + k0 : 0);
 }
 
 // A row of P 16-byte pieces per lane, P = 2, 4 or 8, to P lanes per row: lane l of a group of P lanes gets piece l of the rows of all
@@ -384,7 +396,7 @@ __device__ __forceinline__ void bwd_zero_outside(const BwdSm100Dev& p) {
 constexpr int kBwdThreads = 640, kBwdConsumers = 19;  // (consumers of the item ring: every warp but the one that fills it)
 
 // ---- dQ -----------------------------------------------------------------------------------------------------------------
-template <typename T, int HDIM, bool EXTRA>
+template <typename T, int HDIM, int VAR>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do, const BwdSm100Dev p) {
@@ -635,7 +647,7 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if (lane == 0) mbar_arrive(&ctrl->row_full[slot]);
             if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_full[slot], (n_item >> 1) & 1u, abort_flag, p.status, 0x10044)))) break;
             const float delta = sDelta[slot * 128 + r];
-            const float slope = EXTRA && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h] * kLog2e : 0.f;
+            const float slope = VAR == 1 && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h] * kLog2e : 0.f;
             // visible keys of this row; key tiles that every row of the tile sees whole
             const int k_lo = p.mask_type != 0 && p.wl >= 0 ? i + shift - p.wl : 0;
             const int k_hi = p.mask_type != 0 && p.wr >= 0 ? min(it.sk - 1, i + shift + p.wr) : it.sk - 1;
@@ -647,6 +659,12 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const float2 neg_lse2 = make_float2(-lse2, -lse2), neg_delta = make_float2(-delta, -delta);
             for (int j = 0; j < range.count; ++j, ++t) {
                 const int n0 = (range.begin + j) * 128, key0 = n0 + quarter * 32;
+                [[maybe_unused]] uint4 bw[VAR == 2 ? 4 : 1];  // the row's 32 bias values, requested before the wait for S
+                if constexpr (VAR == 2) {
+                    const unsigned short* row = r < left ? (const unsigned short*)p.bias + bwd_bias_block(p, it.b, it.h, it.q0, it.k0) + i * p.bias_sk : nullptr;
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) bw[v] = load_bias_piece(row, key0 + v * 8, it.sk - key0 - v * 8);
+                }
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->s_full[half], t & 1u, abort_flag, p.status, 0x10041)))) break;
                 tc_fence_after();
                 uint32_t x[32];
@@ -655,19 +673,21 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&ctrl->s_free[half]);
-                if constexpr (EXTRA) {
+                if constexpr (VAR != 0) {
                     if (p.soft_cap > 0.f) soft_cap_scores<32>(x, p.cap);
                 }
 #pragma unroll
                 for (int e = 0; e < 32; e += 2) {
                     float2 f = make_float2(1.f, 1.f), away = f;
-                    if constexpr (EXTRA) {
+                    if constexpr (VAR == 1) {
                         away.x = (float)(i + it.sk - it.sq - (key0 + e));
                         away.y = away.x - 1.f;
+                    } else if constexpr (VAR == 2) {
+                        away = bias_pair<T>((&bw[e / 8].x)[e / 2 % 4]);
                     }
-                    const float2 y = bwd_exponent<EXTRA>(p, make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), slope, away, neg_lse2, f);
+                    const float2 y = bwd_exponent<VAR>(p, make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), slope, away, neg_lse2, f);
                     float2 pr = bwd_exp2<kPolyDq>(y, e / 2);
-                    if constexpr (EXTRA) pr = __fmul2_rn(pr, f);
+                    if constexpr (VAR != 0) pr = __fmul2_rn(pr, f);
                     x[e] = __float_as_uint(pr.x);
                     x[e + 1] = __float_as_uint(pr.y);
                 }
@@ -708,7 +728,7 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 }
 
 // ---- dK / dV --------------------------------------------------------------------------------------------------------------
-template <typename T, int HDIM, bool EXTRA>
+template <typename T, int HDIM, int VAR>
 __global__ void __launch_bounds__(kBwdThreads, 1)
 bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const BwdSm100Dev p) {
@@ -931,11 +951,22 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             for (int g = 0, m = 0; g < G; ++t) {
                 const int m0 = (range.begin + m) * 128, i0 = m0 + quarter * 32;
                 const bool masked = m0 < full_lo || m0 + 127 > full_hi;
-                const float slope = EXTRA && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h * G + g] * kLog2e : 0.f;
+                const float slope = VAR == 1 && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h * G + g] * kLog2e : 0.f;
+                [[maybe_unused]] const int head = g;  // of the group
                 if (++m == range.count) { m = 0; ++g; }
                 // columns of this quarter that see the key: i >= key - shift - wr, i <= key - shift + wl
                 uint32_t seen = 0xffffffffu;
                 if (masked) seen = bwd_column_bits(p.wr >= 0 ? key - shift - p.wr - i0 : 0, p.wl >= 0 ? key - shift + p.wl - i0 : 31);
+                [[maybe_unused]] uint32_t bw[VAR == 2 ? 16 : 1];  // the key's bias values in the 32 query columns
+                if constexpr (VAR == 2) {  // (a row of the tensor at a time: the warp's 32 keys lie side by side)
+                    const unsigned short* at = (const unsigned short*)p.bias + bwd_bias_block(p, it.b, it.h * G + head, it.q0, it.k0) + i0 * p.bias_sk + key;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const uint32_t lo = key < it.sk && i0 + e < it.sq ? __ldg(at + e * p.bias_sk) : 0u;
+                        const uint32_t hi = key < it.sk && i0 + e + 1 < it.sq ? __ldg(at + (e + 1) * p.bias_sk) : 0u;
+                        bw[e / 2] = lo | hi << 16;
+                    }
+                }
                 const float* rows = sRow + (t & 1) * 256 + quarter * 32;
                 const uint32_t tS = lane_addr + (t & 1u) * 128 + quarter * 32, tDP = lane_addr + ((t + 1) & 1u) * 128 + quarter * 32;
                 if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_full[t & 1], (t >> 1) & 1u, abort_flag, p.status, 0x10140)))) break;
@@ -944,7 +975,7 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 uint32_t x[32], w[16];
                 tmem_ld32(tS, x);
                 tmem_wait_ld();
-                if constexpr (EXTRA) {
+                if constexpr (VAR != 0) {
                     if (p.soft_cap > 0.f) soft_cap_scores<32>(x, p.cap);
                 }
 #pragma unroll
@@ -953,15 +984,17 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 #pragma unroll
                     for (int u = 0; u < 4; u += 2) {
                         float2 f = make_float2(1.f, 1.f), away = f;
-                        if constexpr (EXTRA) {
+                        if constexpr (VAR == 1) {
                             away.x = (float)(i0 + e + u + it.sk - it.sq - key);
                             away.y = away.x + 1.f;
+                        } else if constexpr (VAR == 2) {
+                            away = bias_pair<T>(bw[(e + u) / 2]);
                         }
-                        const float2 y = bwd_exponent<EXTRA>(p, make_float2(__uint_as_float(x[e + u]), __uint_as_float(x[e + u + 1])), slope, away,
+                        const float2 y = bwd_exponent<VAR>(p, make_float2(__uint_as_float(x[e + u]), __uint_as_float(x[e + u + 1])), slope, away,
                                                              u ? make_float2(l4.z, l4.w) : make_float2(l4.x, l4.y), f);
                         float2 pr = bwd_exp2<kPolyDkdv>(y, (e + u) / 2);
                         w[(e + u) / 2] = Elem<T>::pack2(pr.x, pr.y);
-                        if constexpr (EXTRA) pr = __fmul2_rn(pr, f);  // (from here on P serves dS alone)
+                        if constexpr (VAR != 0) pr = __fmul2_rn(pr, f);  // (from here on P serves dS alone)
                         x[e + u] = __float_as_uint(pr.x);
                         x[e + u + 1] = __float_as_uint(pr.y);
                     }
@@ -1012,6 +1045,216 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         }
     }
     pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 16) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;\n" ::"r"(tmem));
+    }
+}
+
+// ---- the gradient of a bias tensor --------------------------------------------------------------------------------------------
+// dbias = dT = P (dP - D), summed over the heads and sequences that share a plane.  A work item is a 128 x 128 tile of one plane (group
+// mode: of one sequence's block): its CTA walks the sharers in order, S = Q K^T and dP = dO V^T into two buffers each, and
+// adds up in registers.  Four tiles are copied for two products, so shared memory (2048 clocks a step) and L2 bound it.
+struct BwdBiasItem {
+    int valid, row0, key0, b_begin, b_end, h_begin, h_end, steps;
+    BwdSeq s;  // of the first sharer (the sharers' lengths are equal)
+};
+__device__ __forceinline__ BwdBiasItem bwd_bias_item(const BwdSm100Dev& p, int64_t item, int tiles_q, int tiles_k) {
+    BwdBiasItem it;
+    it.key0 = (int)(item % tiles_k) * 128;
+    item /= tiles_k;
+    it.row0 = (int)(item % tiles_q) * 128;
+    item /= tiles_q;
+    const int planes_h = p.bias_rank >= 1 ? p.hq : 1, ph = (int)(item % planes_h), pb = (int)(item / planes_h);
+    const bool own_b = p.bias_rank == 2 || p.seqstart_q;
+    it.b_begin = own_b ? pb : 0;
+    it.b_end = own_b ? pb + 1 : p.batch;
+    it.h_begin = p.bias_rank >= 1 ? ph : 0;
+    it.h_end = p.bias_rank >= 1 ? ph + 1 : p.hq;
+    it.s = bwd_sequence(p, it.b_begin);
+    it.valid = it.row0 < it.s.sq && it.key0 < it.s.sk;
+    bool seen = it.valid;  // by some row: the first key of the last row's window, the last key of the last row
+    if (p.mask_type != 0) {
+        const int last = min(it.s.sq, it.row0 + 128) - 1;
+        if (p.wr >= 0 && it.key0 > last + it.s.shift + p.wr) seen = false;
+        if (p.wl >= 0 && min(it.s.sk, it.key0 + 128) - 1 < it.row0 + it.s.shift - p.wl) seen = false;
+    }
+    it.steps = seen ? (it.b_end - it.b_begin) * (it.h_end - it.h_begin) : 0;
+    return it;
+}
+
+template <typename T, int HDIM>
+__global__ void __launch_bounds__(kBwdThreads, 1)
+bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
+                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const BwdSm100Dev p, int tiles_q,
+                       int tiles_k, int64_t items) {
+    constexpr int TILE = 128 * HDIM * 2;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* sQ = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));  // 2 x (Q, K)
+    uint8_t* sDO = sQ + 4 * TILE;                                                             // dO, V
+    BwdCtrl* ctrl = reinterpret_cast<BwdCtrl*>(sDO + 2 * TILE);
+    volatile int* abort_flag = &ctrl->abort_flag;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&ctrl->a_full[i], 1);
+            mbar_init(&ctrl->a_empty[i], 1);
+            mbar_init(&ctrl->s_full[i], 1);
+            mbar_init(&ctrl->dp_full[i], 1);
+            mbar_init(&ctrl->s_free[i], 16);
+        }
+        mbar_init(&ctrl->b_full[0], 1);
+        mbar_init(&ctrl->b_empty[0], 1);
+        ctrl->abort_flag = 0;
+        mbar_fence_init();
+    }
+    if (warp == 16) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;\n" ::"r"(smem_u32(&ctrl->tmem_base)));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::);
+    }
+    pdl_wait();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctrl->tmem_base;  // S in columns 0-127 and 128-255, dP in 256-383 and 384-511
+    const int G = p.hq / p.hkv;
+    bool ok = true;
+    uint32_t t = 0;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        return ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, p.status, code)) != 0;
+    };
+    // Registers: as in the dQ kernel.
+    if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::);
+    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::);
+    if (warp == 18) {
+        // ================================ TMA producer ================================
+        // (Rows behind a sequence's end make rows and columns of dT that are not stored.)
+        auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
+#pragma unroll
+            for (int hb = 0; hb < HDIM / 64; ++hb) tma_load_3d(dst + hb * HALF_BYTES, map, bar, hb * 64, head, row);
+        };
+        for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+            const BwdBiasItem it = bwd_bias_item(p, item, tiles_q, tiles_k);
+            int b = it.b_begin, h = it.h_begin;
+            for (int j = 0; j < it.steps; ++j, ++t) {
+                const BwdSeq s = bwd_sequence(p, b);
+                const int kh = h / G, slot = t & 1;
+                if (!wait(&ctrl->a_empty[slot], ((t >> 1) & 1u) ^ 1u, 0x10201)) break;
+                if (lane == 0) {
+                    mbar_expect_tx(&ctrl->a_full[slot], 2 * TILE);
+                    load(sQ + slot * 2 * TILE, &map_q, &ctrl->a_full[slot], h, s.q0 + it.row0);
+                    load(sQ + slot * 2 * TILE + TILE, &map_k, &ctrl->a_full[slot], kh, s.k0 + it.key0);
+                }
+                if (!wait(&ctrl->b_empty[0], (t & 1u) ^ 1u, 0x10202)) break;
+                if (lane == 0) {
+                    mbar_expect_tx(&ctrl->b_full[0], 2 * TILE);
+                    load(sDO, &map_do, &ctrl->b_full[0], h, s.q0 + it.row0);
+                    load(sDO + TILE, &map_v, &ctrl->b_full[0], kh, s.k0 + it.key0);
+                }
+                if (++h == it.h_end) { h = it.h_begin; ++b; }
+            }
+        }
+    } else if (warp == 16) {
+        // ================================ MMA issuer ================================
+        constexpr uint32_t idesc = make_idesc<T>(false);
+        const bool leader = elect_one_sync();
+        auto commit = [&](uint64_t* bar) { if (leader) umma_commit(bar); };
+        const uint64_t dQ = make_smem_desc(smem_u32(sQ), 0, 1024), dDO = make_smem_desc(smem_u32(sDO), 0, 1024);
+        for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+            const int steps = bwd_bias_item(p, item, tiles_q, tiles_k).steps;
+            for (int j = 0; j < steps; ++j, ++t) {
+                const uint32_t buf = t & 1u, par = (t >> 1) & 1u;
+                if (!wait(&ctrl->a_full[buf], par, 0x10211) || !wait(&ctrl->s_free[buf], par ^ 1u, 0x10212)) break;
+                tc_fence_after();
+                if (leader) bwd_issue_ss<HDIM>(tmem + buf * 128, dQ + ((buf * 2 * TILE) >> 4), dQ + ((buf * 2 * TILE + TILE) >> 4), idesc);
+                commit(&ctrl->s_full[buf]);
+                commit(&ctrl->a_empty[buf]);
+                if (!wait(&ctrl->b_full[0], t & 1u, 0x10213)) break;
+                tc_fence_after();
+                if (leader) bwd_issue_ss<HDIM>(tmem + 256 + buf * 128, dDO, dDO + (TILE >> 4), idesc);
+                commit(&ctrl->dp_full[buf]);
+                commit(&ctrl->b_empty[0]);
+            }
+        }
+    } else if (warp < 16) {
+        const int quarter = warp >> 2, r = (warp & 3) * 32 + lane;
+        const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + quarter * 32;
+        for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
+            const BwdBiasItem it = bwd_bias_item(p, item, tiles_q, tiles_k);
+            if (!it.valid) continue;
+            const int i = it.row0 + r, key0 = it.key0 + quarter * 32, left = it.s.sq - it.row0;
+            const int64_t block = bwd_bias_block(p, it.b_begin, it.h_begin, it.s.q0, it.s.k0);
+            uint32_t bw[16];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                const uint4 x = load_bias_piece(r < left ? (const unsigned short*)p.bias + block + i * p.bias_sk : nullptr, key0 + v * 8, it.s.sk - key0 - v * 8);
+                bw[4 * v] = x.x; bw[4 * v + 1] = x.y; bw[4 * v + 2] = x.z; bw[4 * v + 3] = x.w;
+            }
+            const int k_lo = p.mask_type != 0 && p.wl >= 0 ? i + it.s.shift - p.wl : 0;
+            const int k_hi = p.mask_type != 0 && p.wr >= 0 ? min(it.s.sk - 1, i + it.s.shift + p.wr) : it.s.sk - 1;
+            const uint32_t seen = bwd_column_bits(k_lo - key0, k_hi - key0);
+            float2 acc[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[e] = make_float2(0.f, 0.f);
+            int b = it.b_begin, h = it.h_begin;
+            for (int j = 0; j < it.steps; ++j, ++t) {
+                const BwdSeq s = bwd_sequence(p, b);
+                const int64_t lr = (p.seqstart_q ? (int64_t)h * p.seqlen_q + s.q0 : ((int64_t)b * p.hq + h) * p.seqlen_q) + i;
+                const float lse2 = r < left ? bwd_lse_base2(p.lse[lr]) : INFINITY, delta = r < left ? p.delta[lr] : 0.f;
+                if (++h == it.h_end) { h = it.h_begin; ++b; }
+                const uint32_t buf = t & 1u, par = (t >> 1) & 1u;
+                if (!wait(&ctrl->s_full[buf], par, 0x10221) || !wait(&ctrl->dp_full[buf], par, 0x10222)) break;
+                tc_fence_after();
+#pragma unroll
+                for (int c = 0; c < 32; c += 16) {
+                    uint32_t x[16], dp[16];
+                    tmem_ld16(lane_addr + buf * 128 + c, x);
+                    tmem_ld16(lane_addr + 256 + buf * 128 + c, dp);
+                    tmem_wait_ld();
+                    if (p.soft_cap > 0.f) soft_cap_scores<16>(x, p.cap);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        float2 f;
+                        const float2 y = bwd_exponent<2>(p, make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), 0.f, bias_pair<T>(bw[(c + e) / 2]),
+                                                         make_float2(-lse2, -lse2), f);
+                        const float2 dt = __fadd2_rn(make_float2(__uint_as_float(dp[e]), __uint_as_float(dp[e + 1])), make_float2(-delta, -delta));
+                        float2& a = acc[(c + e) / 2];
+                        if (seen >> (c + e) & 1u) a.x = fmaf(ex2_fast(y.x), dt.x, a.x);
+                        if (seen >> (c + e + 1) & 1u) a.y = fmaf(ex2_fast(y.y), dt.y, a.y);
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&ctrl->s_free[buf]);
+            }
+            if (!ok) break;
+            uint4 out[4];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+                out[v].x = Elem<T>::pack2(acc[4 * v].x, acc[4 * v].y);
+                out[v].y = Elem<T>::pack2(acc[4 * v + 1].x, acc[4 * v + 1].y);
+                out[v].z = Elem<T>::pack2(acc[4 * v + 2].x, acc[4 * v + 2].y);
+                out[v].w = Elem<T>::pack2(acc[4 * v + 3].x, acc[4 * v + 3].y);
+            }
+            bwd_exchange<4>(out, lane);
+            const int first = (warp & 3) * 32 + (lane & ~3), col = key0 + (lane & 3) * 8;  // this lane: 8 elements of rows first .. + 3
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (first + j >= left) continue;
+                unsigned short* dst = (unsigned short*)p.dbias + block + (int64_t)(it.row0 + first + j) * p.bias_sk + col;
+                if (col + 8 <= it.s.sk && (reinterpret_cast<uintptr_t>(dst) & 15u) == 0) {
+                    *reinterpret_cast<uint4*>(dst) = out[j];
+                } else {
+                    const uint32_t w[4] = {out[j].x, out[j].y, out[j].z, out[j].w};
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (col + e < it.s.sk) dst[e] = (unsigned short)(w[e / 2] >> (16 * (e & 1)));
+                }
+            }
+        }
+    }
     tc_fence_before();
     __syncthreads();
     if (warp == 16) {

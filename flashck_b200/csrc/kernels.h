@@ -147,7 +147,7 @@ struct BwdParams {
     float logits_soft_cap;
 };
 int launch_bwd_generic(const BwdParams& p, cudaStream_t stream);
-// the tcgen05 kernels (fmha_bwd_sm100.cu): everything but an elementwise bias
+// the tcgen05 kernels (fmha_bwd_sm100.cu): every call with something to multiply
 bool bwd_sm100_supported(const BwdParams& p);
 int launch_bwd_sm100(const BwdParams& p, cudaStream_t stream);
 

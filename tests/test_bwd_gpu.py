@@ -64,6 +64,8 @@ def test_which_instance_serves(instance, device_ok):
     assert _lib.get_instance_param(0, "last_bwd_instance") == int(instance == "tcgen05")
     bias = torch.zeros(1, 1, 64, 64, device="cuda", dtype=torch.bfloat16)
     ops.fmha_bwd(*args, bias=bias)
+    assert _lib.get_instance_param(0, "last_bwd_instance") == int(instance == "tcgen05")
+    ops.fmha_bwd(args[0], args[1], args[2][:, :0].contiguous(), args[3][:, :0].contiguous(), *args[4:])  # (no key: the general one)
     assert _lib.get_instance_param(0, "last_bwd_instance") == 0
 
 
@@ -84,10 +86,11 @@ def test_alibi_and_soft_cap(d, mask, slopes_rank, cap, instance, device_ok):
 
 @pytest.mark.parametrize("d", [64, 128])
 @pytest.mark.parametrize("planes", [(1, 1), (1, 4), (3, 4)])
-@pytest.mark.parametrize("sq,sk,mask", [(70, 131, NONE), (130, 130, CAUSAL)])
-def test_bias_and_its_gradient(d, planes, sq, sk, mask, device_ok):
-    bias = torch.randn(*planes, sq, sk, device="cuda", dtype=torch.float16)
-    _check(_problem(3, sq, sk, 4, 2, d, torch.float16, mask, bias=bias, cap=20.0), mask, bias=bias, cap=20.0)
+@pytest.mark.parametrize("sq,sk,mask", [(70, 131, NONE), (130, 130, CAUSAL), (1, 1, NONE), (300, 264, (2, 60, 5)), (128, 256, NONE)])
+@pytest.mark.parametrize("dtype,cap", [(torch.float16, 20.0), (torch.bfloat16, 0.0)])
+def test_bias_and_its_gradient(d, planes, sq, sk, mask, dtype, cap, instance, device_ok):
+    bias = torch.randn(*planes, sq, sk, device="cuda", dtype=dtype)
+    _check(_problem(3, sq, sk, 4, 2, d, dtype, mask, bias=bias, cap=cap), mask, bias=bias, cap=cap)
 
 
 def test_scale_and_gradient_of_the_lse(instance, device_ok):
@@ -150,10 +153,11 @@ def test_many_items(lens, hq, hkv, d, mask, device_ok):
         assert all(torch.equal(x, y[0]) for x, y in zip(part, ops.fmha_bwd(*a, **_options(mask))))
 
 
-def test_packed_bias_gradient_is_zero_outside_the_blocks(device_ok):
-    nq, nk, d, hq = [40, 90], [70, 65], 64, 2
+@pytest.mark.parametrize("planes", [1, 2])
+def test_packed_bias_gradient_is_zero_outside_the_blocks(planes, instance, device_ok):
+    nq, nk, d, hq = [40, 190], [170, 65], 64, 2
     cu_q, cu_k = (torch.tensor([0] + n).cumsum(0).cuda() for n in (nq, nk))
-    bias = torch.randn(1, hq, sum(nq), sum(nk), device="cuda", dtype=torch.bfloat16)
+    bias = torch.randn(1, planes, sum(nq), sum(nk), device="cuda", dtype=torch.bfloat16)
     parts = [_problem(1, a, c, hq, hq, d, torch.bfloat16, NONE, seed=n, bias=bias[:, :, cu_q[n]: cu_q[n + 1], cu_k[n]: cu_k[n + 1]])
              for n, (a, c) in enumerate(zip(nq, nk))]
     dout, q, k, v, o = (torch.cat([p[n][0] for p in parts]) for n in range(5))
@@ -163,7 +167,8 @@ def test_packed_bias_gradient_is_zero_outside_the_blocks(device_ok):
     for n, p in enumerate(parts):
         block = (slice(None), slice(None), slice(cu_q[n], cu_q[n + 1]), slice(cu_k[n], cu_k[n + 1]))
         want, bound = gradients(*p, d ** -0.5, NONE, bias=bias[block])
-        assert_within("dbias", got[block], want[3], bound[3] + half_step(bias.dtype) * want[3].abs())
+        w, e = (t.sum(1, keepdim=True) if planes == 1 else t for t in (want[3], bound[3]))
+        assert_within("dbias", got[block], w, e + half_step(bias.dtype) * w.abs())
         outside[block] = False
     assert not got[outside].any()
 
