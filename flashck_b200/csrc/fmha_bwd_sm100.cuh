@@ -590,33 +590,42 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const uint32_t tS = lane_addr + cS + quarter * 32, tDP = lane_addr + cDP + quarter * 32;
         uint32_t t = 0, n_item = 0;
         bool ok = true;
-        while (ok && bwd_next_item(ctrl, p, k_item, lane, it)) {
-            constexpr int COLS = HDIM / 4;  // of dQ that this warp stores
-            const int i = it.row0 + r, shift = p.mask_type == 2 ? it.sk - it.sq : 0;
-            const int first = it.row0 + (warp & 3) * 32;  // of this warp's rows
-            const BwdRange range = bwd_key_tiles(p, it);
-            T* dst = (T*)p.dq + ((int64_t)(it.q0 + first) * p.hq + it.h) * HDIM + quarter * COLS;
-            // D = sum dO O - dLSE of rows warp * 8 .. + 7, dO from its tile (or from memory, where the item has no products)
-            const int64_t lr = (p.seqstart_q ? (int64_t)it.h * p.seqlen_q + it.q0 : ((int64_t)it.b * p.hq + it.h) * p.seqlen_q) + it.row0;
-            const int slot = n_item & 1, left = it.sq - it.row0;
-            const float lse2 = r < left ? bwd_lse_base2(p.lse[lr + r]) : INFINITY;
-            {
-                constexpr int L = HDIM / 8, ROWS = 32 / L, LOADS = 8 / ROWS;  // lanes a row, rows a load
-                const int sub = lane / L, piece = lane % L;
-                const int64_t at = ((int64_t)(it.q0 + it.row0) * p.hq + it.h) * HDIM + piece * 8, stride = (int64_t)p.hq * HDIM;
-                uint4 y[LOADS];
+        constexpr int COLS = HDIM / 4;                                        // of dQ that a warp stores
+        constexpr int L = HDIM / 8, ROWS = 32 / L, LOADS = 8 / ROWS;          // D: lanes a row, rows a load
+        const int sub = lane / L, piece = lane % L;
+        // What an item's D needs from memory: O of rows warp * 8 .. + 7 (8 columns a lane), the row's LSE.  It is requested in front of the
+        // stores of the item before.
+        uint4 y[LOADS];
+        float lse2;
+        auto request = [&]() {
+            const int left = it.sq - it.row0;
+            const T* at = (const T*)p.o + ((int64_t)(it.q0 + it.row0) * p.hq + it.h) * HDIM + piece * 8;
 #pragma unroll
-                for (int u = 0; u < LOADS; ++u) {
-                    const int row = warp * 8 + u * ROWS + sub;
-                    y[u] = row < left ? *reinterpret_cast<const uint4*>((const T*)p.o + at + row * stride) : make_uint4(0u, 0u, 0u, 0u);
-                }
+            for (int u = 0; u < LOADS; ++u) {
+                const int row = warp * 8 + u * ROWS + sub;
+                y[u] = row < left ? *reinterpret_cast<const uint4*>(at + row * ((int64_t)p.hq * HDIM)) : make_uint4(0u, 0u, 0u, 0u);
+            }
+            const int64_t lr = (p.seqstart_q ? (int64_t)it.h * p.seqlen_q + it.q0 : ((int64_t)it.b * p.hq + it.h) * p.seqlen_q) + it.row0;
+            lse2 = r < left ? bwd_lse_base2(p.lse[lr + r]) : INFINITY;
+        };
+        bool more = bwd_next_item(ctrl, p, k_item, lane, it);
+        if (more) request();
+        while (ok && more) {
+            const int i = it.row0 + r, shift = p.mask_type == 2 ? it.sk - it.sq : 0;
+            const int rows = it.sq - it.row0 - (warp & 3) * 32;  // of this warp's 32 that exist
+            const BwdRange range = bwd_key_tiles(p, it);
+            T* dst = (T*)p.dq + ((int64_t)(it.q0 + it.row0 + (warp & 3) * 32) * p.hq + it.h) * HDIM + quarter * COLS;
+            // D = sum dO O - dLSE, dO from its tile (or from memory, where the item has no products)
+            const int slot = n_item & 1, left = it.sq - it.row0;
+            {
+                const int64_t lr = (p.seqstart_q ? (int64_t)it.h * p.seqlen_q + it.q0 : ((int64_t)it.b * p.hq + it.h) * p.seqlen_q) + it.row0;
                 if (range.count > 0 && !(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->own_full[1], n_item & 1u, abort_flag, p.status, 0x10040)))) break;
 #pragma unroll
                 for (int u = 0; u < LOADS; ++u) {
                     const int row = warp * 8 + u * ROWS + sub;
                     uint4 x = make_uint4(0u, 0u, 0u, 0u);
                     if (range.count > 0) x = *reinterpret_cast<const uint4*>(sDO + (piece / 8) * HALF_BYTES + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
-                    else if (row < left) x = *reinterpret_cast<const uint4*>((const T*)p.dout + at + row * stride);
+                    else if (row < left) x = *reinterpret_cast<const uint4*>((const T*)p.dout + ((int64_t)(it.q0 + it.row0 + row) * p.hq + it.h) * HDIM + piece * 8);
                     const uint32_t xw[4] = {x.x, x.y, x.z, x.w}, yw[4] = {y[u].x, y[u].y, y[u].z, y[u].w};
                     float sum = 0.f;
 #pragma unroll
@@ -639,12 +648,16 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if (range.count == 0) {  // no row of the tile sees a key
 #pragma unroll
                 for (int v = 0; v < COLS / 8; ++v) out[v] = make_uint4(0u, 0u, 0u, 0u);
-                bwd_store_rows<T>(dst, (int64_t)p.hq * HDIM, it.sq - first, out, lane);
+                bwd_store_rows<T>(dst, (int64_t)p.hq * HDIM, rows, out, lane);
+                more = bwd_next_item(ctrl, p, k_item, lane, it);
+                if (more) request();
                 continue;
             }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&ctrl->own_free[1]);
-            if (lane == 0) mbar_arrive(&ctrl->row_full[slot]);
+            if (lane == 0) {
+                mbar_arrive(&ctrl->own_free[1]);
+                mbar_arrive(&ctrl->row_full[slot]);
+            }
             if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->row_full[slot], (n_item >> 1) & 1u, abort_flag, p.status, 0x10044)))) break;
             const float delta = sDelta[slot * 128 + r];
             const float slope = VAR == 1 && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h] * kLog2e : 0.f;
@@ -716,7 +729,9 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&ctrl->acc_free);
-            bwd_store_rows<T>(dst, (int64_t)p.hq * HDIM, it.sq - first, out, lane);
+            more = bwd_next_item(ctrl, p, k_item, lane, it);
+            if (more) request();
+            bwd_store_rows<T>(dst, (int64_t)p.hq * HDIM, rows, out, lane);
         }
     }
     tc_fence_before();
