@@ -54,7 +54,7 @@ int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
             constexpr size_t smem = 1024 + 6 * TILE + sizeof(BwdCtrl);
             FCK_CUDA(cudaFuncSetAttribute(dbias, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
             const int64_t tq = (p.max_seqlen_q + 127) / 128, tk = (p.max_seqlen_k + 127) / 128, items = bias_items(p);
-            FCK_CUDA(launch_dependent(dbias, dim3((unsigned)std::min<int64_t>(items, sm_count())), dim3(kBwdThreads), smem, stream, mq, mdo, mk, mv, dev,
+            FCK_CUDA(launch_dependent(dbias, dim3((unsigned)std::min<int64_t>(items, sm_count())), dim3(kBwdBiasThreads), smem, stream, mq, mdo, mk, mv, dev,
                                       (int)tq, (int)tk, items));
         }
     }

@@ -1072,6 +1072,12 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // dbias = dT = P (dP - D), summed over the heads and sequences that share a plane.  A work item is a 128 x 128 tile of one plane (group
 // mode: of one sequence's block): its CTA walks the sharers in order, S = Q K^T and dP = dO V^T into two buffers each, and
 // adds up in registers.  Four tiles are copied for two products, so shared memory (2048 clocks a step) and L2 bound it.
+__device__ __forceinline__ void bwd_tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(taddr)
+                 : "memory");
+}
 struct BwdBiasItem {
     int valid, row0, key0, b_begin, b_end, h_begin, h_end, steps;
     BwdSeq s;  // of the first sharer (the sharers' lengths are equal)
@@ -1100,8 +1106,10 @@ __device__ __forceinline__ BwdBiasItem bwd_bias_item(const BwdSm100Dev& p, int64
     return it;
 }
 
+constexpr int kBwdBiasThreads = 576;  // warps 0-15 elementwise, 16 products, 17 copies
+
 template <typename T, int HDIM>
-__global__ void __launch_bounds__(kBwdThreads, 1)
+__global__ void __launch_bounds__(kBwdBiasThreads, 1)
 bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
                        const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const BwdSm100Dev p, int tiles_q,
                        int tiles_k, int64_t items) {
@@ -1140,10 +1148,7 @@ bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
         return ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, p.status, code)) != 0;
     };
-    // Registers: as in the dQ kernel.
-    if (warp >= 16) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;\n" ::);
-    else asm volatile("setmaxnreg.inc.sync.aligned.u32 104;\n" ::);
-    if (warp == 18) {
+    if (warp == 17) {
         // ================================ TMA producer ================================
         // (Rows behind a sequence's end make rows and columns of dT that are not stored.)
         auto load = [&](uint8_t* dst, const CUtensorMap* map, uint64_t* bar, int head, int row) {
@@ -1223,14 +1228,14 @@ bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
                 if (!wait(&ctrl->s_full[buf], par, 0x10221) || !wait(&ctrl->dp_full[buf], par, 0x10222)) break;
                 tc_fence_after();
 #pragma unroll
-                for (int c = 0; c < 32; c += 16) {
-                    uint32_t x[16], dp[16];
-                    tmem_ld16(lane_addr + buf * 128 + c, x);
-                    tmem_ld16(lane_addr + 256 + buf * 128 + c, dp);
+                for (int c = 0; c < 32; c += 8) {
+                    uint32_t x[8], dp[8];
+                    bwd_tmem_ld8(lane_addr + buf * 128 + c, x);
+                    bwd_tmem_ld8(lane_addr + 256 + buf * 128 + c, dp);
                     tmem_wait_ld();
-                    if (p.soft_cap > 0.f) soft_cap_scores<16>(x, p.cap);
+                    if (p.soft_cap > 0.f) soft_cap_scores<8>(x, p.cap);
 #pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
+                    for (int e = 0; e < 8; e += 2) {
                         float2 f;
                         const float2 y = bwd_exponent<2>(p, make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), 0.f, bias_pair<T>(bw[(c + e) / 2]),
                                                          make_float2(-lse2, -lse2), f);
