@@ -25,6 +25,7 @@ SIGNATURES = {
     "FmhaFwdBias": ([_P] * 8 + [_I64] * 8 + [_F, _I64, _I64, _U32, _P, _P, _I, _I, _I, _F], _I),
     "FmhaFwdFp8": ([_P] * 6 + [_I64] * 8 + [_F, _F, _F, _I64, _I64, _U32, _P, _P, _I, _I], _I),
     "FmhaBwd": ([_P] * 15 + [_I64] * 9 + [_F, _I64, _I64, _U32, _P, _I, _I, _I, _F], _I),
+    "FmhaZeroOutside": ([_P] * 3 + [_I64] * 4 + [_P, _I], _I),
     "FmhaFwdBatchPrefill": ([_P] * 9 + [_I64] * 9 + [_F, _I64, _I64, _U32, _P, _P, _I], _I),
     "FmhaFwdPagedKVPrefill": ([_P] * 9 + [_I64] * 9 + [_F, _I64, _I64, _U32, _P, _P, _I], _I),
     "FmhaFwdSplitKV": ([_P] * 11 + [_I64] * 11 + [_F, _I64, _I64, _U32, _P, _I], _I),

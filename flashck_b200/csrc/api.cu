@@ -323,6 +323,16 @@ int FmhaBwd(void* dout, void* q, void* k, void* v, void* bias, void* o, void* ls
     return sm100 ? launch_bwd_sm100(p, (cudaStream_t)stream) : launch_bwd_generic(p, (cudaStream_t)stream);
 }
 
+int FmhaZeroOutside(void* o, void* lse, int64_t* q_seq_start, int64_t batch, int64_t q_seq_len, int64_t hq, int64_t dv, void* stream, int dtype) {
+    FCK_REQUIRE(dtype == FLASHCK_DTYPE_FLOAT16 || dtype == FLASHCK_DTYPE_BFLOAT16, FLASHCK_ERR_UNSUPPORTED,
+                "FmhaZeroOutside: dtype must be 3 (fp16) or 4 (bf16), got %d", dtype);
+    FCK_REQUIRE(batch >= 0 && q_seq_len >= 0 && hq >= 0 && dv >= 0, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaZeroOutside: negative size");
+    if (q_seq_len == 0 || hq == 0 || dv == 0) return FLASHCK_OK;
+    FCK_REQUIRE(o && q_seq_start, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaZeroOutside: null pointer argument");
+    FCK_REQUIRE(((uintptr_t)o & 15) == 0 && hq * dv % 8 == 0, FLASHCK_ERR_UNSUPPORTED, "FmhaZeroOutside: o and its rows must lie on 16-byte boundaries");
+    return launch_zero_outside(o, (float*)lse, q_seq_start, batch, q_seq_len, hq, hq * dv * 2, (cudaStream_t)stream);
+}
+
 static int batch_prefill_impl(void* q, void* k, void* v, const float* slopes, int slope_rank, void* o, int64_t* q_seq_start,
                               void* kv_indptr, void* kv_page_indices, void* kv_last_page_len, int64_t batch,
                               int64_t q_seq_len, int64_t hq, int64_t hkv, int64_t d, int64_t dv, int64_t q_max_seq_len,

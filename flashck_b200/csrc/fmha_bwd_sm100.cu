@@ -69,7 +69,25 @@ int launch_bwd_d(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
     return var == 2 ? launch_bwd_t<T, 64, 2>(p, dev, stream) : var ? launch_bwd_t<T, 64, 1>(p, dev, stream) : launch_bwd_t<T, 64, 0>(p, dev, stream);
 }
 
+// (a batch without padding costs its launch: 2 us)
+__global__ void __launch_bounds__(256) zero_outside_kernel(uint4* o, float* lse, const int64_t* seqstart, int64_t batch, int64_t total, int64_t hq,
+                                                           int64_t row_vecs) {
+    pdl_wait();
+    const int64_t tid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, threads = (int64_t)gridDim.x * blockDim.x;
+    const int64_t first = min(max(seqstart[0], (int64_t)0), total), end = min(max(seqstart[batch], first), total), n = total - end + first;
+    auto outside = [&](int64_t i) { return i < first ? i : i - first + end; };  // i-th row that belongs to no sequence
+    for (int64_t e = tid; e < n * row_vecs; e += threads) o[outside(e / row_vecs) * row_vecs + e % row_vecs] = make_uint4(0u, 0u, 0u, 0u);
+    if (lse)
+        for (int64_t e = tid; e < n * hq; e += threads) lse[e / n * total + outside(e % n)] = 0.f;
+}
+
 }  // namespace
+
+int launch_zero_outside(void* o, float* lse, const int64_t* seqstart, int64_t batch, int64_t total, int64_t hq, int64_t row_bytes, cudaStream_t stream) {
+    FCK_CUDA(launch_dependent(zero_outside_kernel, dim3((unsigned)sm_count()), dim3(256), 0, stream, (uint4*)o, lse, seqstart, batch, total, hq,
+                              row_bytes / 16));
+    return FLASHCK_OK;
+}
 
 bool bwd_sm100_supported(const BwdParams& p) {
     if (p.max_seqlen_q == 0 || p.max_seqlen_k == 0 || p.batch == 0) return false;  // (nothing to multiply)

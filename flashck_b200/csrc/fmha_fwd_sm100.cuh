@@ -863,7 +863,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     constexpr bool F8 = ElemInfo<T>::f8;
     constexpr int ES = ElemInfo<T>::bytes;
     constexpr int HD = HDIM, RB = HD * ES, TILE_BYTES = BM * RB, HB = RB / 128, XB = 128 / ES, KK = 32 / ES;
-    static_assert(HDIM == 128 || HDIM == 64, "");
+    static_assert(HDIM == 128 || HDIM == 64, "hdim 128 or 64");
     static_assert(!F8 || (HDIM == 128 && SPLIT == 0 && (VAR & 6) == 0 && EXPM == 0),
                   "the 8-bit instances: hdim 128, prefill forms, fp32 exponentials, no score additions");
     constexpr bool WINDOW = (VAR & 1) != 0;  // the mask has a second bound (see above)

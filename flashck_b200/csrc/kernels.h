@@ -121,7 +121,7 @@ int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream);
 int fwd_set_param(const char* key, int64_t value);
 int fwd_get_param(const char* key, int64_t* value);
 
-// ---- backward of the forward (fmha_bwd_generic.cu) ----------------------------------------------------------
+// ---- backward of the forward (fmha_bwd_sm100.cu; fmha_bwd_generic.cu) ----------------------------------------------------------
 struct BwdParams {
     const void* dout;
     const void* q;
@@ -150,6 +150,9 @@ int launch_bwd_generic(const BwdParams& p, cudaStream_t stream);
 // the tcgen05 kernels (fmha_bwd_sm100.cu): every call with something to multiply
 bool bwd_sm100_supported(const BwdParams& p);
 int launch_bwd_sm100(const BwdParams& p, cudaStream_t stream);
+
+// zeros to the packed rows of o and the entries of the LSE [hq, total] (or nullptr) that belong to no sequence
+int launch_zero_outside(void* o, float* lse, const int64_t* seqstart, int64_t batch, int64_t total, int64_t hq, int64_t row_bytes, cudaStream_t stream);
 
 // ---- decode over a prefix that all sequences share (shared_prefix.cu) ------------------------------------------
 struct SharedPrefixParams {

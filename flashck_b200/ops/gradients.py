@@ -120,14 +120,34 @@ def fmha_bwd_var_len(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
                       int(max_seqlen_k), scale, causal, window_size, mask_type, bias, alibi_slopes, logits_soft_cap, dlse, return_dbias)
 
 
+# A leaf's gradient is accumulated on the stream where the first graph that uses the leaf was recorded, for as long as a graph holds
+# the leaf's node.  Where that is the default stream, a captured backward pass would make it wait for the capture, which
+# ends the process.  The node carries a mark, and the captured pass is refused.
+_ON_DEFAULT_STREAM = "flashck_b200: recorded on the default stream"
+
+
+def _mark_leaves(*tensors: Optional[torch.Tensor]) -> list:
+    """The nodes of the leaves among the tensors, marked; they have to be held until the graph holds them."""
+    leaves = [t for t in tensors if t is not None and t.is_cuda and t.is_leaf and t.requires_grad]
+    nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves]
+    if nodes and torch.cuda.current_stream(leaves[0].device).cuda_stream == 0:
+        for n in nodes:
+            n.metadata[_ON_DEFAULT_STREAM] = True
+    return nodes
+
+
 class _Attention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, bias, alibi_slopes, cu_q, cu_k, max_sq, max_sk, options):
         if cu_q is None:
             o, lse = _f.fmha_fwd(q, k, v, return_lse=True, bias=bias, alibi_slopes=alibi_slopes, **options)
         else:
+            cu_q, cu_k = _f._as_i64("cu_seqlens_q", cu_q), _f._as_i64("cu_seqlens_k", cu_k)
             o, lse = _f.fmha_fwd_var_len(q, k, v, cu_q, cu_k, max_sq or q.shape[0], max_sk, return_lse=True, bias=bias,
                                          alibi_slopes=alibi_slopes, **options)
+            with _f._on(q.device):
+                _lib.check(_lib.lib().FmhaZeroOutside(_f._ptr(o), _f._ptr(lse), _f._ptr(cu_q), cu_q.numel() - 1, *o.shape, _f._stream(),
+                                                      _f._dtype_code(o)), "FmhaZeroOutside")
         ctx.save_for_backward(q, k, v, bias, alibi_slopes, cu_q, cu_k, o, lse)
         ctx.max_sq, ctx.max_sk, ctx.options = max_sq, max_sk, options
         ctx.set_materialize_grads(False)
@@ -139,7 +159,12 @@ class _Attention(torch.autograd.Function):
         q, k, v, bias, alibi_slopes, cu_q, cu_k, o, lse = ctx.saved_tensors
         if dout is None and dlse is None:
             return (None,) * 10
+        if torch.cuda.is_current_stream_capturing() and any(n.metadata.get(_ON_DEFAULT_STREAM) for n, _ in ctx.next_functions if n is not None):
+            raise RuntimeError("this backward pass is being captured, but an input's gradient belongs to a graph that was recorded on the default "
+                               "stream and still lives: release that graph's outputs, or record it on a side stream")
         dout = torch.zeros_like(o) if dout is None else dout.contiguous()
+        if dout.data_ptr() % 16:
+            dout = dout.clone()
         more = dict(bias=bias, alibi_slopes=alibi_slopes, dlse=None if dlse is None else dlse.contiguous(),
                     return_dbias=bias is not None and ctx.needs_input_grad[3], **ctx.options)
         g = (fmha_bwd(dout, q, k, v, o, lse, **more) if cu_q is None else
@@ -151,6 +176,7 @@ class _Attention(torch.autograd.Function):
 def _differentiable(q, k, v, bias, alibi_slopes, cu_q, cu_k, max_sq, max_sk, return_lse, options):
     if alibi_slopes is not None and alibi_slopes.requires_grad:
         raise ValueError("alibi_slopes are constants: their gradient is not computed")
+    held = _mark_leaves(q, k, v, bias) if torch.is_grad_enabled() else None  # noqa: F841
     o, lse = _Attention.apply(q, k, v, bias, alibi_slopes, cu_q, cu_k, max_sq, max_sk, options)
     return (o, lse) if return_lse else o
 
@@ -161,8 +187,8 @@ def fmha_autograd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: O
     """:func:`fmha_fwd` as a function that autograd differentiates: same arguments and results, with gradients for q, k, v and
     the bias tensor, through the output and (``return_lse``) the LSE.
 
-    A captured backward pass: call :func:`fmha_bwd` in the capture, or capture the whole step after a warm-up on a side stream
-    with no eager graph of the same leaves alive, as autograd requires of every function."""
+    A backward pass in a CUDA graph: capture the whole step after a warm-up on a side stream, or call :func:`fmha_bwd` in the
+    capture.  A captured pass is refused while a graph of the same leaves that was recorded on the default stream lives."""
     return _differentiable(q, k, v, bias, alibi_slopes, None, None, 0, 0, return_lse,
                            dict(scale=scale, causal=causal, window_size=tuple(window_size), mask_type=mask_type, logits_soft_cap=logits_soft_cap))
 
@@ -172,6 +198,7 @@ def fmha_autograd_var_len(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_
                           window_size: Sequence[int] = (-1, -1), mask_type: Optional[int] = None, return_lse: bool = False,
                           bias: Optional[torch.Tensor] = None, alibi_slopes: Optional[torch.Tensor] = None,
                           logits_soft_cap: float = 0.0):
-    """:func:`fmha_fwd_var_len` as a function that autograd differentiates (see :func:`fmha_autograd`)."""
+    """:func:`fmha_fwd_var_len` as a function that autograd differentiates (see :func:`fmha_autograd`).  Rows of the output
+    and entries of the LSE that belong to no sequence are zero."""
     return _differentiable(q, k, v, bias, alibi_slopes, cu_seqlens_q, cu_seqlens_k, int(max_seqlen_q), int(max_seqlen_k), return_lse,
                            dict(scale=scale, causal=causal, window_size=tuple(window_size), mask_type=mask_type, logits_soft_cap=logits_soft_cap))

@@ -145,6 +145,14 @@ FLASHCK_API int FmhaBwd(void* do_buf_ptr, void* q_buf_ptr, void* k_buf_ptr, void
             uint32_t mask_type, void* stream, int dtype, int bias_enum, int bias_rank_info, float logits_soft_cap);
 
 /*
+ * FmhaZeroOutside -- zeros to the rows of a packed output [q_seq_len, hq, dv] and the entries of its LSE [hq, q_seq_len] (or NULL)
+ * in front of the first and behind the last sequence, which the forward leaves as they were.  A product with the gradient of a
+ * padded output (zero there) would otherwise meet whatever the memory held.
+ */
+FLASHCK_API int FmhaZeroOutside(void* o_buf_ptr, void* lse_ptr, int64_t* q_seq_start_ptr, int64_t batch, int64_t q_seq_len, int64_t q_num_heads,
+            int64_t v_head_dim, void* stream, int dtype);
+
+/*
  * FmhaFwdBatchPrefill -- varlen prefill whose K/V sit behind an SGLang-style page table.
  * The reference emits this family (core/profiling/attention/fmha_fwd_batch_prefill/
  * fmha_fwd_batch_prefill_codegen.cc:93-162, problem ..._problem.h:20-99 `num_total_pages`) but its glue

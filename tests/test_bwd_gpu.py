@@ -306,3 +306,67 @@ def test_first_call_of_a_thread(device_ok):
         t.join()
     assert not failed, failed
     assert all(torch.equal(a, b) for a, b in zip(got[0], want)) and torch.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_bias_that_hides(d, instance, device_ok):
+    """Infinities in a bias: whole rows, whole key tiles, single keys.  What is hidden gets nothing at all."""
+    bias = torch.randn(2, 4, 200, 300, device="cuda").to(torch.bfloat16)
+    bias[:, :, 5:9] = -torch.inf
+    bias[0, :, :, 128:256] = -torch.inf
+    bias[1, 2, :, 7] = -torch.inf
+    bias[:, :, 40, ::2] = -torch.inf
+    got = _check(_problem(2, 200, 300, 4, 2, d, torch.bfloat16, NONE, bias=bias), NONE, bias=bias)
+    assert not got[0][:, 5:9].any() and not got[1][0, 128:256].any() and not got[2][0, 128:256].any()
+    assert not got[3][torch.isneginf(bias)].any()
+
+
+def test_padding_of_a_differentiable_output_is_zero(device_ok):
+    """The output is multiplied by weights whose gradient is o^T times zeros there: what the memory held must not count."""
+    total, cu = 300, torch.tensor([7, 40, 200], device="cuda")
+    q, k, v = (torch.randn(total, h, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for h in (4, 2, 2))
+    for _ in range(2):
+        old = torch.full((total, 4, 64), float("nan"), device="cuda", dtype=torch.bfloat16), torch.full((4, total), float("nan"), device="cuda")
+        del old  # (the outputs may lie where these did)
+        o, lse = ops.fmha_autograd_var_len(q, k, v, cu, cu, 160, 160, causal=True, return_lse=True)
+        for rows in (slice(0, 7), slice(200, None)):
+            assert not o[rows].any() and not lse[:, rows].any()
+        plain, plain_lse = ops.fmha_fwd_var_len(q, k, v, cu, cu, 160, 160, causal=True, return_lse=True)
+        assert torch.equal(o[7:200], plain[7:200]) and torch.equal(lse[:, 7:200], plain_lse[:, 7:200])
+    # starts in 32 bits; no padding; a batch without a token
+    for starts in ([0, 100, total], [0, 0, 0]):
+        c = torch.tensor(starts, device="cuda", dtype=torch.int32)
+        o = ops.fmha_autograd_var_len(q, k, v, c, c, total, total)
+        assert torch.equal(o, ops.fmha_fwd_var_len(q, k, v, c, c, total, total)) if starts[-1] else not o.any()
+
+
+def test_gradient_that_starts_off_a_boundary(device_ok):
+    q, k, v = (torch.randn(1, 70, 2, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for _ in range(3))
+    w = torch.randn(q.numel() + 1, device="cuda", dtype=torch.bfloat16)[1:].view_as(q)
+    got, want = (torch.autograd.grad(ops.fmha_autograd(q, k, v), (q, k, v), x) for x in (w, w.clone()))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_step(device_ok):
+    """Forward and backward in one graph; refused while a graph of the same leaves from the default stream lives."""
+    q, k, v = (torch.randn(2, 130, h, 64, device="cuda", dtype=torch.bfloat16, requires_grad=True) for h in (4, 2, 2))
+    w = torch.randn_like(q)
+    alive = ops.fmha_autograd(q, k, v, causal=True)
+    with pytest.raises(RuntimeError, match="recorded on the default stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            ops.fmha_autograd(q, k, v, causal=True).backward(w)
+    del alive
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        torch.autograd.grad(ops.fmha_autograd(q, k, v, causal=True), (q, k, v), w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(ops.fmha_autograd(q, k, v, causal=True), (q, k, v), w)
+    with torch.no_grad():
+        for t in (q, w):
+            t.copy_(t.flip(1))
+    graph.replay()
+    want = torch.autograd.grad(ops.fmha_autograd(q, k, v, causal=True), (q, k, v), w)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

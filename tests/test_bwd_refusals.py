@@ -34,6 +34,16 @@ def test_nothing_to_do_is_no_error():
     assert _call(sq=0, sk=0, dout=0, q=0, k=0, v=0, o=0, lse=0, dq=0, dk=0, dv=0, delta=0)[0] == 0
 
 
+@pytest.mark.parametrize("change,code,said", [
+    (dict(dtype=1), 2, "dtype"), (dict(batch=-1), 1, "negative"), (dict(o=0), 1, "null"), (dict(cu=0), 1, "null"), (dict(o=P + 8), 2, "16-byte"),
+    (dict(hq=1, dv=4), 2, "16-byte"), (dict(total=0, o=0), 0, ""),
+])
+def test_zero_outside_refuses(change, code, said):
+    a = dict(o=P, lse=P, cu=P, batch=1, total=4, hq=2, dv=64, stream=0, dtype=4)
+    a.update(change)
+    assert _lib.lib().FmhaZeroOutside(*a.values()) == code and (code == 0 or said in _lib.last_error())
+
+
 def test_functions_refuse_before_launch():
     q = torch.zeros(1, 4, 2, 64, dtype=torch.bfloat16)
     lse = torch.zeros(1, 2, 4)
