@@ -1,5 +1,8 @@
 // Backward of fmha_fwd -- the general instance: every call that the forward takes on contiguous K/V (hdim 64 / 128, fp16 / bf16,
-// batch and group mode, GQA, the four masks, elementwise bias with its gradient, ALiBi, soft cap).
+// batch and group mode, GQA, the four masks, elementwise bias with its gradient, ALiBi, soft cap).  It serves what the tcgen05
+// kernels leave (no keys or no queries at all, windows of 2^30 and more) and is the second instance that "use_sm100_bwd" = 0
+// selects, against which the other can be checked: 6155 us on 2 x 4096 causal tokens of 32 / 8 heads of 128, where the tcgen05
+// kernels take 770.
 //
 // With S = scale Q K^T, S' = cap tanh(S / cap), T = S' + bias, P = exp(T - LSE) (recomputed, 0 where masked),
 //     D_i = sum_c dO_ic O_ic - dLSE_i      dP = dO V^T      dT = P (dP - D)      dS = dT (1 - (S' / cap)^2)

@@ -19,6 +19,7 @@ FCK_SM100_TMA_BIAS(FCK_EXTERN, __half) FCK_SM100_TMA_BIAS(FCK_EXTERN, __nv_bfloa
 FCK_SM100_FP8(FCK_EXTERN, f8e4m3_t) FCK_SM100_FP8(FCK_EXTERN, f8e5m2_t)
 FCK_SM100_SPLIT(FCK_EXTERN_SPLIT, __half) FCK_SM100_SPLIT(FCK_EXTERN_SPLIT, __nv_bfloat16)
 FCK_SM100_SPLIT64(FCK_EXTERN_SPLIT, __half) FCK_SM100_SPLIT64(FCK_EXTERN_SPLIT, __nv_bfloat16)
+FCK_SM100_SPLIT_PAIR(FCK_EXTERN_SPLIT, __half) FCK_SM100_SPLIT_PAIR(FCK_EXTERN_SPLIT, __nv_bfloat16)
 
 }  // namespace sm100
 
@@ -239,6 +240,19 @@ bool splitkv_sm100_supported(const SplitKVParams& p) {
     return true;
 }
 
+bool splitkv_sm100_pairs_tiles(const SplitKVParams& p) {
+    const int64_t group = p.hq / p.hkv;
+    return p.shared_prefix && p.max_seqlen_q * group > split_rows_per_tile(p, BM);
+}
+
+int64_t splitkv_sm100_prefix_splits(const SplitKVParams& p) {
+    const int64_t group = p.hq / p.hkv, rpt = split_rows_per_tile(p, BM), per_stream = splitkv_sm100_pairs_tiles(p) ? 2 * rpt : rpt;
+    const int64_t tiles = (p.seqlen_k_cap + BN - 1) / BN, cost = g_split_item_cost.load();
+    const int64_t streams = p.hkv * ((p.max_seqlen_q * group + per_stream - 1) / per_stream);
+    const int64_t w = std::max<int64_t>((streams * (tiles + cost) + sm_count() - 1) / sm_count(), p.min_piece_tiles + cost);
+    return ((tiles + w - 1) / w + 1) * (split_duplicates_rows(p) ? 2 : 1);
+}
+
 int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream) {
     int* status = device_status_ptr();
     if (!status) return FLASHCK_ERR_CUDA;
@@ -266,7 +280,14 @@ int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream) {
     dev.rescale_thr = hexp ? 0.01f * (float)g_rescale_half_x100.load() : kRescaleThreshold;
     const bool twice = split_duplicates_rows(p);
     dev.rpt = (int)split_rows_per_tile(p, twice ? 64 : BM);
+    dev.rpb = dev.rpt;
     if (p.shared_prefix) dev.piece_tiles = (int)p.min_piece_tiles;
+    if (splitkv_sm100_pairs_tiles(p)) {  // (fp32 exponentials)
+        dev.rpb = 2 * dev.rpt;
+        dev.rescale_thr = kRescaleThreshold;
+        if (p.d == 64) return bf16 ? launch_split_t<__nv_bfloat16, 3, 0, 64>(p, dev, stream) : launch_split_t<__half, 3, 0, 64>(p, dev, stream);
+        return bf16 ? launch_split_t<__nv_bfloat16, 3, 0>(p, dev, stream) : launch_split_t<__half, 3, 0>(p, dev, stream);
+    }
     if (p.d == 64) {  // (fp32 exponentials)
         dev.rescale_thr = kRescaleThreshold;
         if (twice) return bf16 ? launch_split_t<__nv_bfloat16, 2, 0, 64>(p, dev, stream) : launch_split_t<__half, 2, 0, 64>(p, dev, stream);

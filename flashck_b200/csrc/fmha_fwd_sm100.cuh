@@ -102,6 +102,7 @@ struct Sm100Dev {
     float* lse_acc;
     int num_splits, piece_tiles, group, sq_cap;
     int rpt;          // packed rows of a tile: 128, or fewer where the group does not divide it (64 in mode 2)
+    int rpb;          // packed rows of a stream: a tile's, mode 3: two tiles'
     int item_cost;    // units of the work line that stand for an item's fixed cost (see kItemCostDefault)
     int causal;       // mask type: 0 none, 1 top-left, 2 bottom-right, 3 window with top-left alignment
     int wl, wr;       // window of a masked problem: keys [i + shift - wl, i + shift + wr] of row i; -1 = unbounded
@@ -513,7 +514,7 @@ __device__ __forceinline__ int item_of_round(int rnd, int cta, int g) {
 static_assert(1024 + (2 + 2 * KV_SLOTS) * TILE_BYTES + 8 * STAGE_BYTES + sizeof(Ctrl) <= 227 * 1024,
               "tiles, staging buffers and the control block must fit the 227 KB a CTA can have");
 
-// Split modes.  A stream is the key tiles one (sequence, 128-row block of the packed rows, kv head) needs; all streams,
+// Split modes.  A stream is the key tiles one (sequence, row block of the packed rows: one tile, mode 3: two, kv head) needs; all streams,
 // in that order, each preceded by item_cost units (kItemCostDefault) that stand for an item's fixed cost (Q load, pipeline fill, epilogue),
 // form one line that is cut into equal pieces of split_w units, one per CTA, so that the SMs finish together whatever
 // the lengths are.  The part of a stream inside one CTA's piece is a work item and one split of the result; a stream
@@ -523,11 +524,11 @@ constexpr int kItemCostDefault = 6;   // instance parameter "split_item_cost" (1
 
 // key tiles the rows of row block `rb` of a sequence see
 __device__ __forceinline__ int split_stream_tiles(const Sm100Dev& p, int sq, int sk, int rb) {
-    const int first_tok = rb * p.rpt / p.group;
+    const int first_tok = rb * p.rpb / p.group;
     if (first_tok >= sq || sk <= 0) return 0;
     int hi_key = sk - 1;
     if (p.causal) {
-        const int last_tok = min(sq, (rb * p.rpt + p.rpt + p.group - 1) / p.group) - 1;
+        const int last_tok = min(sq, (rb * p.rpb + p.rpb + p.group - 1) / p.group) - 1;
         hi_key = min(hi_key, last_tok + ((p.causal == 2) ? sk - sq : 0));
     }
     return hi_key >= 0 ? hi_key / BN + 1 : 0;
@@ -539,6 +540,7 @@ __device__ __forceinline__ int split_stream_pieces(int g0, int n, int w, int max
     return (g0 + item_cost + n - 1) / w - (g0 + item_cost) / w + 1;
 }
 
+template <int SPLIT>
 __device__ __forceinline__ void expand_item_split(const Ctrl* ctrl, const Sm100Dev& p, uint32_t packed, int rnd, Item& it) {
     it.valid = packed >> 31;
     const int b = (packed >> 22) & 0x1ff, kh = (packed >> 12) & 0x3ff, piece = (packed >> 4) & 0xff, rb = packed & 0xf;
@@ -550,15 +552,45 @@ __device__ __forceinline__ void expand_item_split(const Ctrl* ctrl, const Sm100D
     it.kh = kh;
     it.h[0] = kh * p.group;  // first q head of the group
     it.h[1] = piece;         // split slot of the result
-    it.row0[0] = rb * p.rpt;    // first packed row (token * group + group head)
-    it.row0[1] = 0x3fffffff; // tile 1 does not exist
+    it.row0[0] = rb * p.rpb;    // first packed row (token * group + group head)
+    it.row0[1] = 0x3fffffff; // tile 1 does not exist (modes 1 and 2)
+    if (SPLIT == 3 && it.row0[0] + p.rpt < it.sq * p.group) it.row0[1] = it.row0[0] + p.rpt;
     it.shift = (p.causal == 2) ? it.sk - it.sq : 0;
     const int lo = rnd == 0 ? ctrl->split_first_lo : 0;
     const int hi = rnd == ctrl->split_items - 1 ? ctrl->split_last_hi : split_stream_tiles(p, it.sq, it.sk, rb);
     it.n0 = lo;
     it.nt[0] = hi - lo;
-    it.nt[1] = 0;
+    it.nt[1] = SPLIT == 3 && it.row0[1] != 0x3fffffff ? it.nt[0] : 0;  // (mode 3 has no mask: its tiles see the same keys)
     it.N = it.nt[0];
+}
+
+// LSE = -inf to the splits a stream does not use, so that the merge gives them no weight: threads `first` of `threads`.
+__device__ __forceinline__ void split_mark_unused(const Ctrl* ctrl, const Sm100Dev& p, int dup, int first, int threads) {
+    const int max_pieces = max(1, p.num_splits / dup), w = ctrl->split_w;
+    // (a sequence's streams are shared out over gridDim.x / batch CTAs: by one of them, those of a prefix that 1024 rows share took 30 us)
+    const int parts = max(1, (int)gridDim.x / p.batch), part = parts > 1 ? (int)blockIdx.x / p.batch : 0;
+    for (int b = parts > 1 ? (int)blockIdx.x % p.batch : (int)blockIdx.x; b < p.batch && part < parts; b += gridDim.x) {
+        const int sq = ctrl->seq_sq[b], sk = ctrl->seq_sk[b], q0 = ctrl->seq_q0[b];
+        const int rbc = (sq * p.group + p.rpb - 1) / p.rpb;
+        int seg0 = ctrl->level_start[b];
+        for (int rb = 0; rb < rbc; ++rb) {
+            const int n = split_stream_tiles(p, sq, sk, rb), c = n + p.item_cost;
+            const int rows = min(p.rpb, sq * p.group - rb * p.rpb);
+            for (int kh = 0; kh < p.hkv; ++kh) {
+                if ((rb * p.hkv + kh) % parts != part) continue;
+                const int used = split_stream_pieces(seg0 + kh * c, n, w, max_pieces, p.item_cost) * dup;
+                const int cnt = (p.num_splits - used) * rows;
+                for (int e = first; e < cnt; e += threads) {
+                    const int sp = used + e / rows, pr = rb * p.rpb + e % rows;
+                    const int tok = pr / p.group, h = kh * p.group + (pr - tok * p.group);
+                    const int64_t slot = p.seqstart_q ? ((int64_t)h * p.num_splits + sp) * p.total_q + q0 + tok
+                                                      : (((int64_t)b * p.hq + h) * p.num_splits + sp) * p.sq_cap + tok;
+                    p.lse_acc[slot] = -INFINITY;
+                }
+            }
+            seg0 += p.hkv * c;
+        }
+    }
 }
 
 // Item `w` of the order by levels (hdim 64, and the lists of prefill_work_list that are neither uniform nor sorted):
@@ -647,7 +679,7 @@ __device__ __forceinline__ uint32_t group_cost(const Ctrl* ctrl, const Sm100Dev&
 // The work item of round `rnd` of this CTA, from the table filled at start-up.
 template <int SPLIT = 0>
 __device__ __forceinline__ void get_item(const Ctrl* ctrl, const Sm100Dev& p, int rnd, int total_items, int lane, Item& it) {
-    if (SPLIT) expand_item_split(ctrl, p, ctrl->items[rnd], rnd, it);
+    if (SPLIT) expand_item_split<SPLIT>(ctrl, p, ctrl->items[rnd], rnd, it);
     else expand_item(ctrl, p, ctrl->items[rnd], it);
 }
 
@@ -844,6 +876,10 @@ __device__ __noinline__ void prefill_work_list_call(Ctrl* ctrl, const Sm100Dev& 
 //          0-63 takes keys 0-63 of every 128-key tile, the copy in rows 64-127 takes keys 64-127, each as a split of its
 //          own (2 * piece, 2 * piece + 1).  Every softmax thread then handles 64 columns instead of 128 with half of the
 //          threads idle, which halves the softmax part of the per-tile chain.
+// SPLIT 3: two row tiles of one kv head per stream, for a shared prefix of more rows than a tile has.  Both tiles meet a K/V tile
+//          once it is in shared memory, with the roles of the prefill forms (one issuer, a softmax warpgroup per tile), but a
+//          producer warp each for K, V and Q (which writes LSE = -inf to the unused splits when it is done).  A prefix of 131072
+//          keys in pages of 64 under 32 sequences of 8 heads a kv head: with both kernels around it 254 -> 200 us.
 // EXPM: how the softmax takes its exponentials.  0: one fp32 exp2 per element on the exp2 unit; 1: two per issue
 //       through the unit's packed f16x2 form (see pack_f16x2); 11, 12, 13: fp32, with 1, 2 or 3 of every 8 column pairs
 //       on a polynomial on the FMA pipe instead.
@@ -872,6 +908,8 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     static_assert(!TMA_BIAS || (BIAS && HDIM == 128), "a bias through shared memory takes the room of a K and a V slot of hdim 128");
     constexpr bool EXTRA = (VAR & 2) != 0 || BIAS;   // ALiBi and / or a logits soft cap on the scaled scores
     static_assert(!BIAS || (SPLIT == 0 && EXPM == 0 && !F8), "the bias instances are prefill forms with fp32 exponentials");
+    static_assert(SPLIT != 3 || VAR == 0, "two row tiles per stream: no mask, no score additions");
+    constexpr bool ONE_TILE = SPLIT == 1 || SPLIT == 2;  // the split forms with one Q tile and two S buffers
     constexpr int NPOLY8 = EXPM >= 11 ? EXPM - 10 : 0;
     constexpr bool HEXP = EXPM == 1;
     // Score additions (not the bias tensors) make a step so long that a second copy of it for masked tiles (see the loop over the
@@ -884,8 +922,8 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     // 18.5 / 18.7.
     constexpr bool ONE_STEP = EXTRA && !BIAS;
     constexpr bool RESCALE_HERE = ONE_STEP && (HDIM == 128) != WINDOW;
-    constexpr int RESCALE_COLS = SPLIT || (ONE_STEP && WINDOW) ? 32 : 16;  // (by the call; see rescale_rows)
-    constexpr bool HALVES = FCK_P_HALVES != 0 && SPLIT == 0;  // P reaches the PV in two halves of 64 keys
+    constexpr int RESCALE_COLS = ONE_TILE || (ONE_STEP && WINDOW) ? 32 : 16;  // (by the call; see rescale_rows)
+    constexpr bool HALVES = FCK_P_HALVES != 0 && !ONE_TILE;  // P reaches the PV in two halves of 64 keys
 
     // ---- shared memory carve-up ----
     const uint32_t raw = smem_u32(smem_raw);
@@ -893,9 +931,9 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
     uint8_t* sQ = base;                                  // 2 tiles
     // The split modes have one Q tile; the room of the second one is a third K slot: with a single tile per item
     // the step is short, and two K tiles ahead keep the loads in flight that the HBM rate needs.
-    constexpr int KS = SPLIT ? 3 : TMA_BIAS ? 1 : 2;
+    constexpr int KS = ONE_TILE ? 3 : TMA_BIAS ? 1 : 2;
     constexpr int KV_SLOTS = TMA_BIAS ? 1 : 2;  // (V slots)
-    uint8_t* sK = base + (SPLIT ? 1 : 2) * TILE_BYTES;   // KS tiles
+    uint8_t* sK = base + (ONE_TILE ? 1 : 2) * TILE_BYTES;   // KS tiles
     uint8_t* sV = sK + KS * TILE_BYTES;                  // KV_SLOTS tiles
     uint8_t* sBias = sV + KV_SLOTS * TILE_BYTES;         // TMA_BIAS: 2 tiles
     uint8_t* sStage = sBias + (TMA_BIAS ? 2 * TILE_BYTES : 0);  // 8 x STAGE_BYTES: O chunks of the softmax warps
@@ -967,7 +1005,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         ctrl->seq_sk[b] = sk;
         const int rows_per_block = p.pair_heads ? BM : 2 * BM;
         if (SPLIT) {  // units of the work line this sequence takes, and its longest stream
-            const int rbc = (sq * p.group + p.rpt - 1) / p.rpt;
+            const int rbc = (sq * p.group + p.rpb - 1) / p.rpb;
             int cost = 0, nmax = 0;
             for (int rb = 0; rb < rbc; ++rb) {
                 const int n = split_stream_tiles(p, sq, sk, rb);
@@ -1010,7 +1048,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
                 for (; b < p.batch && ctrl->level_start[b] < hi; ++b) {
                     const int sq = ctrl->seq_sq[b], sk = ctrl->seq_sk[b];
-                    const int rbc = (sq * p.group + p.rpt - 1) / p.rpt;
+                    const int rbc = (sq * p.group + p.rpb - 1) / p.rpb;
                     int seg0 = ctrl->level_start[b];
                     for (int rb = 0; rb < rbc && seg0 < hi; ++rb) {
                         const int n = split_stream_tiles(p, sq, sk, rb), c = n + p.item_cost;
@@ -1089,7 +1127,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         // whole pool -- at 80 registers the producer and the issuing thread spill ~90 bytes, which costs the kernel
         // 1-2 % (the issuing thread's time between MMAs is idle time of the tensor pipe); the softmax warps would need
         // 216 to be free of spills, which the pool does not hold.  Split modes: 256 x 208 + 128 x 80.
-        if constexpr (SPLIT == 0) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::);
+        if constexpr (!ONE_TILE) asm volatile("setmaxnreg.dec.sync.aligned.u32 88;\n" ::);
         else asm volatile("setmaxnreg.dec.sync.aligned.u32 80;\n" ::);
         // In the split modes a step is short and the copies are many small boxes whose issue takes a warp a good part
         // of it, so K, V and Q have a producer warp each (9, 10, 11): the K producer then runs ahead into the next item
@@ -1126,13 +1164,15 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     if (ok && SPLIT) {
                         // one box of (64 columns, group heads, 128/group tokens) per half: the rows land in
                         // (token, group head) order
-                        mbar_expect_tx(&ctrl->q_full, (SPLIT == 2 ? 2 : 1) * p.rpt * RB);
+                        mbar_expect_tx(&ctrl->q_full, (SPLIT == 2 || it.nt[1] > 0 ? 2 : 1) * p.rpt * RB);
                         for (int hb = 0; hb < HB; ++hb) {
                             if (SPLIT == 2) {  // the box holds 64 rows: once for tile rows 0-63, once for 64-127
                                 tma_load_4d(sQ + hb * HALF_BYTES, &map_q, &ctrl->q_full, hb * XB, 0, it.kh, it.q0);
                                 tma_load_4d(sQ + hb * HALF_BYTES + 64 * 128, &map_q, &ctrl->q_full, hb * XB, 0, it.kh, it.q0);
                             } else {
                                 tma_load_4d(sQ + hb * HALF_BYTES, &map_q, &ctrl->q_full, hb * XB, 0, it.kh, it.q0 + it.row0[0] / p.group);
+                                if (SPLIT == 3 && it.nt[1] > 0)
+                                    tma_load_4d(sQ + TILE_BYTES + hb * HALF_BYTES, &map_q, &ctrl->q_full, hb * XB, 0, it.kh, it.q0 + it.row0[1] / p.group);
                             }
                         }
                     } else if (ok) {
@@ -1260,6 +1300,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 ++q_cnt;
                 if (!ok) break;
             }
+            if (SPLIT == 3 && q_role && p.lse_acc) split_mark_unused(ctrl, p, 1, lane, 32);
         } else if (warp == 8) {
             // ================================ MMA issuer ================================
             constexpr uint32_t idesc_qk = make_idesc<T>(false);
@@ -1323,7 +1364,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             };
             // running counts give ring slots and barrier parities across work items
             uint32_t kv_cnt = 0, q_cnt = 0, sc0 = 0, sc1 = 0;
-            if (SPLIT) {
+            if (ONE_TILE) {
                 // Split modes: this warp issues only the QK^T (all lanes walk the loop, the elected one issues), warp 4 the PV (the warps of tile 1's
                 // softmax warpgroup have nothing else to do there).  Each polls its own barriers while the other's
                 // block of MMAs runs, which a single issuer could not do (the tensor pipe takes instructions only about
@@ -1351,7 +1392,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                     sc0 += N;
                     ++q_cnt;
                 }
-            } else if (!SPLIT) {
+            } else {
                 // All 32 lanes walk the loop and poll the barriers together; one elected lane issues the MMAs and the
                 // commits.  The control flow, the counters and the descriptors are then the same in every lane, which
                 // lets them live in the warp's uniform registers instead of one thread's vector registers (an item with
@@ -1459,7 +1500,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
         const uint32_t tS = lane_addr + i * 128, tO = lane_addr + 256 + i * 128;
         uint32_t sc = 0, oc = 0;  // S tiles and O accumulators consumed so far (barrier parities)
         bool ok = true;
-        if (SPLIT && i == 1) {
+        if (ONE_TILE && i == 1) {
             // Split modes have no second Q tile; the first thread of this warpgroup issues the PV products instead
             // (the QK^T come from warp 8): O += P V from S/P buffer g & 1 once V has landed and the softmax has
             // handed P over, then pv_done tells the softmax (which may rescale O) and the QK^T issuer (which may
@@ -1496,31 +1537,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 }
             }
             else if (warp > 4 && p.lse_acc) {
-                // (warps 5-7, while the others work) splits a stream does not use: LSE = -inf, so that the merge gives
-                // them no weight
-                constexpr int kDup = SPLIT == 2 ? 2 : 1;
-                const int max_pieces = max(1, p.num_splits / kDup), w = ctrl->split_w;
-                for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-                    const int sq = ctrl->seq_sq[b], sk = ctrl->seq_sk[b], q0 = ctrl->seq_q0[b];
-                    const int rbc = (sq * p.group + p.rpt - 1) / p.rpt;
-                    int seg0 = ctrl->level_start[b];
-                    for (int rb = 0; rb < rbc; ++rb) {
-                        const int n = split_stream_tiles(p, sq, sk, rb), c = n + p.item_cost;
-                        const int rows = min(p.rpt, sq * p.group - rb * p.rpt);
-                        for (int kh = 0; kh < p.hkv; ++kh) {
-                            const int used = split_stream_pieces(seg0 + kh * c, n, w, max_pieces, p.item_cost) * kDup;
-                            const int cnt = (p.num_splits - used) * rows;
-                            for (int e = (int)threadIdx.x - 160; e < cnt; e += 96) {
-                                const int sp = used + e / rows, pr = rb * p.rpt + e % rows;
-                                const int tok = pr / p.group, h = kh * p.group + (pr - tok * p.group);
-                                const int64_t slot = p.seqstart_q ? ((int64_t)h * p.num_splits + sp) * p.total_q + q0 + tok
-                                                                  : (((int64_t)b * p.hq + h) * p.num_splits + sp) * p.sq_cap + tok;
-                                p.lse_acc[slot] = -INFINITY;
-                            }
-                        }
-                        seg0 += p.hkv * c;
-                    }
-                }
+                split_mark_unused(ctrl, p, SPLIT == 2 ? 2 : 1, (int)threadIdx.x - 160, 96);  // (warps 5-7, while the others work)
             }
             ok = false;  // nothing else for this warpgroup
         }
@@ -1529,7 +1546,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             get_item<SPLIT>(ctrl, p, rnd, total_items, lane, it);
             if (!it.valid) continue;
             const int Ni = i ? it.nt[1] : it.nt[0];
-            int head = i ? it.h[1] : it.h[0];
+            int head = i && !SPLIT ? it.h[1] : it.h[0];
             const int sq = it.sq, sk = it.sk, shift = it.shift;
             // split mode packs (token, group head) into the rows; `row` is the query token either way
             const int packed_first = i ? it.row0[1] : it.row0[0];
@@ -1565,8 +1582,8 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 // step n+1 is issued before the PV of step n, so the next S is there when P has been handed over.
                 // Buffer and barrier index are the step's parity there, the Q tile otherwise.
                 const uint32_t gstep = sc + n;
-                const int sb = SPLIT ? (int)(gstep & 1u) : i;
-                const uint32_t tSb = SPLIT ? lane_addr + sb * 128 : tS;
+                const int sb = ONE_TILE ? (int)(gstep & 1u) : i;
+                const uint32_t tSb = ONE_TILE ? lane_addr + sb * 128 : tS;
                 const int key0 = (it.n0 + n) * BN + khalf * 64;
                 [[maybe_unused]] const bool capped = EXTRA && p.soft_cap > 0.f;
                 [[maybe_unused]] uint4 bw[BIAS && !TMA_BIAS ? 16 : 1];  // the 128 bias values of this thread's row and key tile
@@ -1582,7 +1599,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                         if (key0 + BN + 127 < sk) asm volatile("prefetch.global.L2 [%0];\n" ::"l"(nx + 127));
                     }
                 }
-                const uint32_t s_parity = (SPLIT ? (gstep >> 1) : gstep) & 1u;
+                const uint32_t s_parity = (ONE_TILE ? (gstep >> 1) : gstep) & 1u;
                 // (one vote where S is there at the first look: hdim 64, 4 x 4096 tokens causal 392 -> 382 us, all keys 716 -> 708; the
                 // 16-bit instances of hdim 128 came out 1 % slower with it)
                 constexpr bool ONE_VOTE = F8 || (HDIM == 64 && VAR == 0 && EXPM == 0);
@@ -1687,7 +1704,7 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 [[maybe_unused]] float alpha = 1.f;
                 [[maybe_unused]] bool rescale = false;  // (warp-uniform) 8-bit instances: O is rescaled under the exponentials
                 if (n > 0 && __any_sync(0xffffffffu, grow)) {
-                    if (SPLIT) {
+                    if (ONE_TILE) {
                         // O must be at rest: the PV of step n-1 may still be running, S of this step was computed ahead
                         // of it.
                         ok = __all_sync(0xffffffffu, mbar_wait_bounded(&ctrl->pv_done[sb ^ 1], ((gstep - 1u) >> 1) & 1u,
@@ -1849,40 +1866,42 @@ fmha_fwd_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
             }
             if (SPLIT) {
                 // fp32 partial of this split, normalised inside the split, and its LSE (natural log)
-                if (i == 0 && tile_first_row < sq) {
+                if ((i == 0 || !ONE_TILE) && tile_first_row < sq) {
                     const float inv = l > 0.f ? 1.f / l : 0.f;
                     const int split = SPLIT == 2 ? 2 * it.h[1] + khalf : it.h[1];
                     const int64_t slot = p.seqstart_q
                         ? ((int64_t)head * p.num_splits + split) * p.total_q + it.q0 + row
                         : (((int64_t)it.b * p.hq + head) * p.num_splits + split) * p.sq_cap + row;
                     // The rows of a warp go to 32 different places of the workspace (one per token and head), 512
-                    // bytes each.  They pass through shared memory (32 rows x 32 columns, 16-byte pieces rotated by
-                    // row against bank conflicts) so that eight lanes write one row's 128 bytes together.
+                    // bytes each.  They pass through shared memory (32 rows x 32 or 16 columns, 16-byte pieces rotated by
+                    // row against bank conflicts) so that eight (four) lanes write one row's bytes together.
                     const unsigned long long my_ptr = row_ok ? (unsigned long long)(p.o_acc + slot * HD) : 0ull;
-                    float* stage = reinterpret_cast<float*>(sStage + (warp & 3) * 4096);
+                    constexpr int EC = ONE_TILE ? 32 : 16, PC = EC / 4;  // columns at a time (the room is 4 x 4096 or 8 x 2048 bytes)
+                    float* stage = reinterpret_cast<float*>(sStage + (ONE_TILE ? (warp & 3) * 4096 : warp * 2048));
 #pragma unroll
-                    for (int c = 0; c < HD / 32; ++c) {
-                        uint32_t t[32];
+                    for (int c = 0; c < HD / EC; ++c) {
+                        uint32_t t[EC];
                         if (Ni > 0) {
-                            tmem_ld32(tO + c * 32, t);
+                            if constexpr (EC == 32) tmem_ld32(tO + c * EC, t);
+                            else tmem_ld16(tO + c * EC, t);
                             tmem_wait_ld();
                         } else {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) t[j] = 0u;
+                            for (int j = 0; j < EC; ++j) t[j] = 0u;
                         }
                         __syncwarp();  // the previous chunk has been read out of the staging rows
 #pragma unroll
-                        for (int v4 = 0; v4 < 8; ++v4)
-                            *reinterpret_cast<float4*>(stage + lane * 32 + ((v4 ^ (lane & 7)) << 2)) =
+                        for (int v4 = 0; v4 < PC; ++v4)
+                            *reinterpret_cast<float4*>(stage + lane * EC + ((v4 ^ (lane & (PC - 1))) << 2)) =
                                 make_float4(__uint_as_float(t[v4 * 4 + 0]) * inv, __uint_as_float(t[v4 * 4 + 1]) * inv,
                                             __uint_as_float(t[v4 * 4 + 2]) * inv, __uint_as_float(t[v4 * 4 + 3]) * inv);
                         __syncwarp();
 #pragma unroll
-                        for (int g4 = 0; g4 < 8; ++g4) {  // four rows per pass: lane = (row in the pass, 16-byte piece)
-                            const int srow = g4 * 4 + (lane >> 3), piece = lane & 7;
+                        for (int g4 = 0; g4 < PC; ++g4) {  // 32 / PC rows per pass: lane = (row in the pass, 16-byte piece)
+                            const int srow = g4 * (32 / PC) + lane / PC, piece = lane & (PC - 1);
                             const unsigned long long dst = __shfl_sync(0xffffffffu, my_ptr, srow);
-                            const float4 val = *reinterpret_cast<const float4*>(stage + srow * 32 + ((piece ^ (srow & 7)) << 2));
-                            if (dst) *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + c * 32 + piece * 4) = val;
+                            const float4 val = *reinterpret_cast<const float4*>(stage + srow * EC + ((piece ^ (srow & (PC - 1))) << 2));
+                            if (dst) *reinterpret_cast<float4*>(reinterpret_cast<float*>(dst) + c * EC + piece * 4) = val;
                         }
                     }
                     if (p.lse_acc && row_ok)
@@ -2143,6 +2162,7 @@ int launch_split_t(const SplitKVParams& p, const Sm100Dev& dev, cudaStream_t str
 #define FCK_SM100_FP8(X, T) X(T, 0, 0, 0, 128) X(T, 0, 1, 0, 128)
 #define FCK_SM100_SPLIT(X, T) X(T, 1, 0, 128) X(T, 1, 1, 128) X(T, 2, 0, 128) X(T, 2, 1, 128)
 #define FCK_SM100_SPLIT64(X, T) X(T, 1, 0, 64) X(T, 2, 0, 64)
+#define FCK_SM100_SPLIT_PAIR(X, T) X(T, 3, 0, 128) X(T, 3, 0, 64)
 #define FCK_SM100_INST(T, E, V, S, H) template int launch_t<T, E, V, S, H>(const FwdParams&, const Sm100Dev&, cudaStream_t);
 #define FCK_SM100_INST_SPLIT(T, S, E, H) template int launch_split_t<T, S, E, H>(const SplitKVParams&, const Sm100Dev&, cudaStream_t);
 

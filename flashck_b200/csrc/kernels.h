@@ -117,6 +117,8 @@ bool fwd_sm100_supported(const FwdParams& p);
 int launch_fwd_sm100(const FwdParams& p, cudaStream_t stream);
 // the same kernel as a split-KV backend for several query rows per kv head (partials into the caller's workspaces)
 bool splitkv_sm100_supported(const SplitKVParams& p);
+bool splitkv_sm100_pairs_tiles(const SplitKVParams& p);  // a shared prefix of more rows than one tile has: two tiles per stream
+int64_t splitkv_sm100_prefix_splits(const SplitKVParams& p);  // the most splits that a stream of a shared prefix is cut into
 int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream);
 int fwd_set_param(const char* key, int64_t value);
 int fwd_get_param(const char* key, int64_t* value);

@@ -127,18 +127,13 @@ Plan plan(const SharedPrefixParams& p) {
     r.rows = p.seqstart_q ? p.seqlen_q : p.batch * p.seqlen_q;
     r.chunk = r.rows;
     if (p.prefix_len > 0 && r.rows > 0) {
-        const int64_t sms = sm_count();
         const int64_t rpt = group <= 128 ? 128 / group * group : group;  // rows of a tile: whole tokens
         r.chunk = std::min(r.rows, std::max<int64_t>(1, 16 * rpt / group));
         SplitKVParams s = prefix_pass(p, 0, r.chunk);
         s.num_splits = 2;
         s.lse_acc = reinterpret_cast<float*>(16);  // (only asked whether there is one)
-        const int64_t row_tiles = (r.chunk * group + rpt - 1) / rpt;
         if (splitkv_sm100_supported(s)) {
-            // a stream (kv head, row tile) is cut into 148 / streams pieces of at least kMinPieceTiles tiles and one more; with at
-            // most 64 rows each piece leaves two partials
-            r.s1 = std::min((sms + p.hkv * row_tiles - 1) / (p.hkv * row_tiles) + 1, (p.prefix_len + 128 * kMinPieceTiles - 1) / (128 * kMinPieceTiles) + 1);
-            if (r.chunk * group <= 64) r.s1 *= 2;
+            r.s1 = splitkv_sm100_prefix_splits(s);
         } else {
             r.chunk = r.rows;
             r.s1 = std::min<int64_t>(128, (p.prefix_len + 31) / 32 + 1);  // the decode kernel: a piece per SM, of two tiles of 16 keys or more

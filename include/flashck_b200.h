@@ -382,7 +382,8 @@ FLASHCK_API int FmhaFwdSplitKVStatic(void* q_buf_ptr, void* k_buf_ptr, void* v_b
  *     running max for exp_mode 1), "poly8" (read-only view of the polynomial share), "bias_enum" / "bias_rank_info"
  *     (meaning of the bias pointer of the reference-shaped FmhaFwd symbol), "log_fallback" (1: a call that leaves the
  *     tcgen05 instances says why on stderr), "last_instance" (read-only: 1 if the last forward call ran on a tcgen05
- *     instance);
+ *     instance), "use_sm100_bwd" (1: FmhaBwd runs on the tcgen05 kernels wherever there is something to multiply, 0: on the
+ *     mma.sync kernels), "last_bwd_instance" (read-only: 1 if the last FmhaBwd ran on the tcgen05 kernels);
  *   family 2 -- "stages" (0 = as many as fit), "ctas_per_sm_x100", "heads_per_cta", "row_tiles" (decode kernel tiling; 0 =
  *     chosen per call), "use_sm100_splitkv" (1: calls with more than 16 query rows per kv head run on the tcgen05 split
  *     modes), "exp_mode_splitkv", "split_item_cost", "split_min_piece_tiles" (work cut of the split modes);

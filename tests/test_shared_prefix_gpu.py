@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from attention_reference import assert_within, forward, half_step
-from flashck_b200 import ops
+from flashck_b200 import _lib, ops
 from flashck_b200.nn import FlashAttention
 
 pytestmark = pytest.mark.gpu
@@ -197,3 +197,26 @@ def test_sample_and_train(device_ok):
     assert ((decoded.double() - trained.double()).abs() <= 2 * u * (v.detach().double().abs().amax() + trained.double().abs())).all()
     o.sum().backward()
     assert all(torch.isfinite(t.grad).all() and t.grad.any() for t in (q, k, v))
+
+
+@pytest.mark.parametrize("page,hq,hkv", [(16, 32, 8), (64, 16, 2)])
+def test_split_kv_repeats(page, hq, hkv, device_ok):
+    """The decode kernel gives a stage of the ring back only when all of it has been read: equal calls, equal bits."""
+    lens, tokens, d = [2000, 40, 1300, 0, 129, 3100], [16, 7, 1, 3, 40, 33], 128
+    per = -(-max(lens) // page)
+    g = torch.Generator("cuda").manual_seed(1)
+    k, v = (torch.randn(6 * per, page, hkv, d, device="cuda", generator=g).bfloat16() for _ in range(2))
+    table = torch.randperm(6 * per, device="cuda", generator=g).int().view(6, per)
+    cu = torch.tensor([0] + tokens).cumsum(0).cuda()
+    q = torch.randn(sum(tokens), hq, d, device="cuda", generator=g).bfloat16()
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    _lib.set_instance_param(2, "use_sm100_splitkv", 0)
+    try:
+        call = lambda: ops.fmha_fwd_splitkv(q, k, v, seqlen_k=sl, block_table=table, cu_seqlens_q=cu, max_seqlen_q=40, num_splits=3)  # noqa: E731
+        first = call()
+        differ = torch.zeros((), device="cuda", dtype=torch.int64)
+        for _ in range(8000):
+            differ += (call() != first).any()
+    finally:
+        _lib.set_instance_param(2, "use_sm100_splitkv", 1)
+    assert int(differ) == 0
