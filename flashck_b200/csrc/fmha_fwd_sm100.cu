@@ -227,7 +227,7 @@ bool splitkv_sm100_supported(const SplitKVParams& p) {
     // 148th, the shortest piece, and what keeps the longest possible stream within the workspace's splits.
     const int64_t cap_tiles = split_cap_tiles(p);
     const int64_t streams = p.batch * p.hkv * ((p.max_seqlen_q * group + rpt - 1) / rpt);
-    const int64_t item_cost = g_split_item_cost.load(), min_piece = p.shared_prefix ? p.min_piece_tiles : g_split_min_piece_tiles.load();
+    const int64_t item_cost = g_split_item_cost.load(), min_piece = p.shared_prefix ? p.min_piece_tiles - item_cost : g_split_min_piece_tiles.load();
     const int64_t line = streams * (cap_tiles + item_cost);
     if (line >= (1ll << 31)) return false;
     const int64_t max_pieces = std::max<int64_t>(1, split_duplicates_rows(p) ? p.num_splits / 2 : p.num_splits);
@@ -249,7 +249,7 @@ int64_t splitkv_sm100_prefix_splits(const SplitKVParams& p) {
     const int64_t group = p.hq / p.hkv, rpt = split_rows_per_tile(p, BM), per_stream = splitkv_sm100_pairs_tiles(p) ? 2 * rpt : rpt;
     const int64_t tiles = (p.seqlen_k_cap + BN - 1) / BN, cost = g_split_item_cost.load();
     const int64_t streams = p.hkv * ((p.max_seqlen_q * group + per_stream - 1) / per_stream);
-    const int64_t w = std::max<int64_t>((streams * (tiles + cost) + sm_count() - 1) / sm_count(), p.min_piece_tiles + cost);
+    const int64_t w = std::max<int64_t>((streams * (tiles + cost) + sm_count() - 1) / sm_count(), p.min_piece_tiles);
     return ((tiles + w - 1) / w + 1) * (split_duplicates_rows(p) ? 2 : 1);
 }
 
@@ -281,7 +281,7 @@ int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream) {
     const bool twice = split_duplicates_rows(p);
     dev.rpt = (int)split_rows_per_tile(p, twice ? 64 : BM);
     dev.rpb = dev.rpt;
-    if (p.shared_prefix) dev.piece_tiles = (int)p.min_piece_tiles;
+    if (p.shared_prefix) dev.piece_tiles = (int)p.min_piece_tiles - dev.item_cost;
     if (splitkv_sm100_pairs_tiles(p)) {  // (fp32 exponentials)
         dev.rpb = 2 * dev.rpt;
         dev.rescale_thr = kRescaleThreshold;

@@ -13,7 +13,10 @@ namespace fck {
 
 namespace {
 
-constexpr int64_t kMinPieceTiles = 2;     // shortest run of 128-key tiles that a CTA takes of the prefix
+// Shortest run of 128-key tiles that a CTA takes of the prefix.  2, 3, 4, 6 or 8 tiles, us in a graph: 1000 keys under 8 sequences of 4
+// heads a kv head 28.3, 29.1, 29.2, 31.4, 31.4; 4000 keys under 48 sequences of 1-4 tokens, hdim 64, 44.0, 44.1, 44.2, 45.3, 47.3;
+// 2000 keys under 256 sequences 87.5, 87.5, 87.6, 87.5, 89.3; 8192 under 64 103.1, 103.5, 103.0, 102.1, 101.8.
+constexpr int64_t kMinPieceTiles = 2;
 
 struct MergeDev {
     const float* lse1;  // prefix: runs of `chunk` rows one behind the other, each [hq, S1, rows of the run]
