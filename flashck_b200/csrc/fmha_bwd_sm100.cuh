@@ -13,9 +13,10 @@
 //
 // The kernels are persistent (one CTA per SM).  Roles: warps 0-15 the elementwise work (thread = tensor memory lane = row; four
 // warpgroups, 32 columns of a 128-column tile each: four warps per scheduler, in code of 32 elements, hide each other's round trips
-// to tensor memory, where two warps with 64 elements took half as long again), warp 16 issues S, warp 17 the other products
-// (a single issuer spends as long on its waits and commits as the products take, and the tensor pipe takes instructions only
-// about one ahead: 16 % slower; dP follows the product that has read dS from its columns in one warp's order, without a
+// to tensor memory; with two warps of 64 elements 2 x 5000 tokens behind a window with a soft cap took 1100 us instead of 902, 16 x 1025
+// of hdim 64 568 instead of 503), warp 16 issues S, warp 17 the other products (a single issuer spends as long on its waits and
+// commits as the products take, and the tensor pipe takes instructions only about one ahead: 2 x 4096 causal tokens of 32 / 8
+// heads 927 us instead of 789; dP follows the product that has read dS from its columns in one warp's order, without a
 // barrier between them), warp 18 finds the work items, hands them to the others through a ring and
 // issues the TMA copies, warp 19 requests the next item's O from memory (dQ) or
 // fetches LSE and D of the query columns (dK/dV).  D is computed by the elementwise warps of dQ, eight rows each.
@@ -396,6 +397,9 @@ __device__ __forceinline__ void bwd_zero_outside(const BwdSm100Dev& p) {
 
 constexpr int kBwdThreads = 640, kBwdConsumers = 19;  // (consumers of the item ring: every warp but the one that fills it)
 
+// 2 x 4096 causal tokens of 32 / 8 heads of 128: 350 us, 589 TFLOP/s of its three products, the tensor pipe busy 66 % of the time, at 1700
+// clocks a step beside the 1536 of the products and 8-9k clocks between two items (code that runs once an item comes from memory
+// again each time).
 // ---- dQ -----------------------------------------------------------------------------------------------------------------
 template <typename T, int HDIM, int VAR>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -743,6 +747,9 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
 }
 
+// The same tokens: 449 us, 612 TFLOP/s of its four products, the tensor pipe busy 70 %.  A step takes 2600 clocks beside the 2048 of
+// shared memory and of the products: S(i+1) waits for dP(i) to be read, so the elementwise work of a step (S and dP from tensor
+// memory, 32 exponentials and two conversions a thread, P and dS back) lies on the chain.
 // ---- dK / dV --------------------------------------------------------------------------------------------------------------
 template <typename T, int HDIM, int VAR>
 __global__ void __launch_bounds__(kBwdThreads, 1)
@@ -1072,7 +1079,9 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
 // ---- the gradient of a bias tensor --------------------------------------------------------------------------------------------
 // dbias = dT = P (dP - D), summed over the heads and sequences that share a plane.  A work item is a 128 x 128 tile of one plane (group
 // mode: of one sequence's block): its CTA walks the sharers in order, S = Q K^T and dP = dO V^T into two buffers each, and
-// adds up in registers.  Four tiles are copied for two products, so shared memory (2048 clocks a step) and L2 bound it.
+// adds up in registers.  Four tiles are copied for two products, so shared memory (2048 clocks a step) and L2 bound it: 56 us for
+// 2 x 1024 tokens of 16 heads of 128 with a plane per head.  With a bias tensor, dQ takes 63 us there and dK/dV 134: transposed, a
+// thread reads its 32 bias values a step two bytes at a time.
 __device__ __forceinline__ void bwd_tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])

@@ -3,8 +3,12 @@
 //     O = sum_s w_s O_s,   w_s = exp(LSE_s - LSE),   LSE = log sum_s exp(LSE_s)
 //
 // over the partials s of the prefix and of the sequence's own cache.  1. The prefix: the query rows of all sequences as those of
-// one sequence (rows x group per kv head fill whole tiles, so the split kernels read the prefix once per 128 rows instead
-// of once per sequence; the tcgen05 split mode takes 16 tiles of rows in one launch, so more rows go in runs).  2. The own caches, as any split-KV call.  3. The merge of both sets of partials, here.
+// one sequence (rows x group per kv head fill whole tiles, so the split kernels read the prefix once per 128 or 256 rows instead
+// of once per sequence; the tcgen05 split mode takes 16 tiles of rows in one launch, so more rows go in runs).  2. The own caches,
+// as any split-KV call.  3. The merge of both sets of partials, here.
+// 131072 keys under 32 sequences of 64 / 8 heads with 1-4096 keys of their own: 199 us; the prefix 125 (537 MB at 4.3 TB/s, 1100 TFLOP/s:
+// bound by the steps, as the prefill forms are), the own caches 59 (5.2 TB/s), the merge 13.  8192 keys under 64 sequences of 32 / 8 heads
+// with 64-2048 keys of their own: 103 us; 24, 58 and 12.
 #include <algorithm>
 
 #include "kernels.h"
