@@ -370,3 +370,19 @@ def test_captured_step(device_ok):
     graph.replay()
     want = torch.autograd.grad(ops.fmha_autograd(q, k, v, causal=True), (q, k, v), w)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_two_streams_at_once(device_ok):
+    """Calls of different problems on two streams, in flight together."""
+    problems = [_problem(2, 700, 700, 4, 2, d, torch.bfloat16, CAUSAL, seed=d) for d in (64, 128)]
+    want = [ops.fmha_bwd(*x, causal=True) for x in problems]
+    streams = [torch.cuda.Stream() for _ in problems]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (x, s) in enumerate(zip(problems, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(ops.fmha_bwd(*x, causal=True))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for w, gs in zip(want, got) for g in gs for a, b in zip(g, w))
+    assert _lib.device_status() == 0
