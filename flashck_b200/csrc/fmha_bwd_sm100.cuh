@@ -981,14 +981,16 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 uint32_t seen = 0xffffffffu;
                 if (masked) seen = bwd_column_bits(p.wr >= 0 ? key - shift - p.wr - i0 : 0, p.wl >= 0 ? key - shift + p.wl - i0 : 31);
                 [[maybe_unused]] uint32_t bw[VAR == 2 ? 16 : 1];  // the key's bias values in the 32 query columns
-                if constexpr (VAR == 2) {  // (a row of the tensor at a time: the warp's 32 keys lie side by side)
-                    const unsigned short* at = (const unsigned short*)p.bias + bwd_bias_block(p, it.b, it.h * G + head, it.q0, it.k0) + i0 * p.bias_sk + key;
+                if constexpr (VAR == 2) {
+                    // A row of the tensor at a time: the warp's 32 keys lie side by side.  Every address is inside the block, so that no load
+                    // waits for a test and all of them are in flight together; what lies outside is zeroed afterwards.
+                    const unsigned short* at = (const unsigned short*)p.bias + bwd_bias_block(p, it.b, it.h * G + head, it.q0, it.k0) + min(key, it.sk - 1);
+                    unsigned short raw[32];
 #pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const uint32_t lo = key < it.sk && i0 + e < it.sq ? __ldg(at + e * p.bias_sk) : 0u;
-                        const uint32_t hi = key < it.sk && i0 + e + 1 < it.sq ? __ldg(at + (e + 1) * p.bias_sk) : 0u;
-                        bw[e / 2] = lo | hi << 16;
-                    }
+                    for (int e = 0; e < 32; ++e) raw[e] = __ldg(at + min(i0 + e, it.sq - 1) * p.bias_sk);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) bw[e / 2] = raw[e] | (uint32_t)raw[e + 1] << 16;
+                    if (key >= it.sk || i0 + 32 > it.sq) bwd_hide(bw, key < it.sk ? bwd_column_bits(0, it.sq - 1 - i0) : 0u);
                 }
                 const float* rows = sRow + (t & 1) * 256 + quarter * 32;
                 const uint32_t tS = lane_addr + (t & 1u) * 128 + quarter * 32, tDP = lane_addr + ((t + 1) & 1u) * 128 + quarter * 32;
