@@ -54,6 +54,9 @@ int64_t split_cap_tiles(const SplitKVParams& p) {  // key tiles of the longest s
 }
 // packed rows of a tile: whole tokens
 int64_t split_rows_per_tile(const SplitKVParams& p, int64_t rows) { return std::max<int64_t>(rows / (p.hq / p.hkv), 1) * (p.hq / p.hkv); }
+// A shared prefix is cut by its sizes alone: its workspace is sized in a call of its own, and an instance parameter that changed in
+// between would make the pass write more partials than there is room for.
+int64_t split_item_cost(const SplitKVParams& p) { return p.shared_prefix ? kItemCostDefault : g_split_item_cost.load(); }
 // At most 64 packed rows and room for two splits per piece: the rows are duplicated (kernel mode 2).
 bool split_duplicates_rows(const SplitKVParams& p) {
     return p.max_seqlen_q * (p.hq / p.hkv) <= 64 && p.num_splits >= 2;
@@ -203,7 +206,7 @@ int launch_fwd_sm100(const FwdParams& p, cudaStream_t stream) {
 }
 
 bool splitkv_sm100_supported(const SplitKVParams& p) {
-    if (!g_use_sm100_splitkv.load()) return false;
+    if (!p.shared_prefix && !g_use_sm100_splitkv.load()) return false;
     if (p.alibi_slopes) return false;  // ALiBi runs on the mma.sync decode kernel
     // hdim 64 and groups that do not divide a tile: a shared prefix's rows only (other calls keep the kernel that they have)
     if (p.d != p.dv || !(p.d == HD || (p.d == 64 && p.shared_prefix)) || p.batch <= 0 || p.batch > kMaxBatch || p.hq > 1023) return false;
@@ -227,7 +230,7 @@ bool splitkv_sm100_supported(const SplitKVParams& p) {
     // 148th, the shortest piece, and what keeps the longest possible stream within the workspace's splits.
     const int64_t cap_tiles = split_cap_tiles(p);
     const int64_t streams = p.batch * p.hkv * ((p.max_seqlen_q * group + rpt - 1) / rpt);
-    const int64_t item_cost = g_split_item_cost.load(), min_piece = p.shared_prefix ? p.min_piece_tiles - item_cost : g_split_min_piece_tiles.load();
+    const int64_t item_cost = split_item_cost(p), min_piece = p.shared_prefix ? p.min_piece_tiles - item_cost : g_split_min_piece_tiles.load();
     const int64_t line = streams * (cap_tiles + item_cost);
     if (line >= (1ll << 31)) return false;
     const int64_t max_pieces = std::max<int64_t>(1, split_duplicates_rows(p) ? p.num_splits / 2 : p.num_splits);
@@ -247,7 +250,7 @@ bool splitkv_sm100_pairs_tiles(const SplitKVParams& p) {
 
 int64_t splitkv_sm100_prefix_splits(const SplitKVParams& p) {
     const int64_t group = p.hq / p.hkv, rpt = split_rows_per_tile(p, BM), per_stream = splitkv_sm100_pairs_tiles(p) ? 2 * rpt : rpt;
-    const int64_t tiles = (p.seqlen_k_cap + BN - 1) / BN, cost = g_split_item_cost.load();
+    const int64_t tiles = (p.seqlen_k_cap + BN - 1) / BN, cost = split_item_cost(p);
     const int64_t streams = p.hkv * ((p.max_seqlen_q * group + per_stream - 1) / per_stream);
     const int64_t w = std::max<int64_t>((streams * (tiles + cost) + sm_count() - 1) / sm_count(), p.min_piece_tiles);
     return ((tiles + w - 1) / w + 1) * (split_duplicates_rows(p) ? 2 : 1);
@@ -269,7 +272,7 @@ int launch_splitkv_sm100(const SplitKVParams& p, cudaStream_t stream) {
     dev.bt_stride = (int)p.bt_stride;
     dev.o_acc = p.o_acc; dev.lse_acc = p.lse_acc; dev.num_splits = (int)p.num_splits;
     dev.piece_tiles = (int)g_split_min_piece_tiles.load();
-    dev.item_cost = (int)g_split_item_cost.load();
+    dev.item_cost = (int)split_item_cost(p);
     dev.group = (int)(p.hq / p.hkv);
     dev.sq_cap = (int)p.seqlen_q;
     dev.causal = p.mask_type; dev.wl = -1; dev.wr = p.mask_type ? 0 : -1;

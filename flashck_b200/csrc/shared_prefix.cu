@@ -124,6 +124,7 @@ SplitKVParams prefix_pass(const SharedPrefixParams& p, int64_t row0, int64_t row
     return s;
 }
 
+// Nothing in it may depend on what can change between the sizing of the workspace and the call (the instance parameters do).
 struct Plan {
     int64_t rows, chunk, s1, s2, floats1, floats2;  // workspace: LSEs and rows of the prefix's partials, then of the others
 };
@@ -157,7 +158,13 @@ Plan plan(const SharedPrefixParams& p) {
 }  // namespace
 
 int64_t shared_prefix_workspace(const SharedPrefixParams& p) {
-    const Plan r = plan(p);
+    Plan r = plan(p);
+    if (p.prefix_table) {  // a page size is all that is known here: the call is paged if it has a table
+        SharedPrefixParams q = p;
+        q.prefix_table = nullptr;
+        q.prefix_page = 0;
+        r.floats1 = std::max(r.floats1, plan(q).floats1);
+    }
     // rows of 16 bytes first, LSEs behind them
     return (r.floats1 + r.floats2) * (p.d + 1) * (int64_t)sizeof(float);
 }

@@ -309,7 +309,9 @@ FLASHCK_API int FlashckPeerBufferFree(void* ptr);
  *   k/v: the own caches [b,kv_seq_len,hkv,d], or with block_table (int32, rows block_table_stride apart) pools of
  *      num_pool_pages pages of paged_block_size tokens; k_seq_len_ptr int32 [b]: own keys of each sequence (0: none)
  *   causal: 0, or 1: query i of a sequence with n queries and m own keys sees its own keys <= m - n + i (and the prefix)
- *   workspace: FlashckSharedPrefixWorkspace(...) bytes of device memory, 16-byte aligned, used during the call only.
+ *   workspace: FlashckSharedPrefixWorkspace(...) bytes of device memory, 16-byte aligned, used during the call only.  The size follows
+ *      from the sizes of the call and the current device, no instance parameter changes it: one asked for once serves every call of
+ *      these sizes on that device.
  * hdim 64 or 128, dtype 3 or 4; pages of a multiple of 16 tokens.
  */
 FLASHCK_API int64_t FlashckSharedPrefixWorkspace(int64_t prefix_len, int64_t prefix_page, int64_t paged_block_size, int64_t batch,
@@ -386,7 +388,7 @@ FLASHCK_API int FmhaFwdSplitKVStatic(void* q_buf_ptr, void* k_buf_ptr, void* v_b
  *     mma.sync kernels), "last_bwd_instance" (read-only: 1 if the last FmhaBwd ran on the tcgen05 kernels);
  *   family 2 -- "stages" (0 = as many as fit), "ctas_per_sm_x100", "heads_per_cta", "row_tiles" (decode kernel tiling; 0 =
  *     chosen per call), "use_sm100_splitkv" (1: calls with more than 16 query rows per kv head run on the tcgen05 split
- *     modes), "exp_mode_splitkv", "split_item_cost", "split_min_piece_tiles" (work cut of the split modes);
+ *     modes; the pass of FmhaFwdSharedPrefix over the prefix goes by its sizes alone), "exp_mode_splitkv", "split_item_cost", "split_min_piece_tiles" (work cut of the split modes);
  *   any family -- "use_pdl" (1: the kernels of a decode step and the prefill kernel are launched as programmatic
  *     dependents of the kernel before them in the stream, see csrc/common.cuh).
  * Unknown keys return FLASHCK_ERR_INVALID_ARGUMENT.  Set before launching; not thread-safe against launches.
