@@ -966,10 +966,10 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 continue;
             }
             // query rows that see all of the tile's keys
-            int full_lo = 0, full_hi = 0x3fffffff;
+            int full_lo = 0, full_hi = it.sq - 1;
             if (p.mask_type != 0) {
                 if (p.wr >= 0) full_lo = it.row0 + 127 - shift - p.wr;
-                if (p.wl >= 0) full_hi = it.row0 - shift + p.wl;
+                if (p.wl >= 0) full_hi = min(full_hi, it.row0 - shift + p.wl);
             }
             for (int g = 0, m = 0; g < G; ++t) {
                 const int m0 = (range.begin + m) * 128, i0 = m0 + quarter * 32;
@@ -977,9 +977,14 @@ bwd_dkdv_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_co
                 const float slope = VAR == 1 && p.alibi ? p.alibi[(p.alibi_rank ? it.b * p.hq : 0) + it.h * G + g] * kLog2e : 0.f;
                 [[maybe_unused]] const int head = g;  // of the group
                 if (++m == range.count) { m = 0; ++g; }
-                // columns of this quarter that see the key: i >= key - shift - wr, i <= key - shift + wl
+                // columns of this quarter that see the key: i >= key - shift - wr, i <= key - shift + wl.  (Columns behind the last query are
+                // zeros, but a key that nobody sees may hold a NaN.)
                 uint32_t seen = 0xffffffffu;
-                if (masked) seen = bwd_column_bits(p.wr >= 0 ? key - shift - p.wr - i0 : 0, p.wl >= 0 ? key - shift + p.wl - i0 : 31);
+                if (masked) {
+                    const bool bounded = p.mask_type != 0;
+                    seen = bwd_column_bits(bounded && p.wr >= 0 ? key - shift - p.wr - i0 : 0,
+                                           (bounded && p.wl >= 0 ? min(it.sq - 1, key - shift + p.wl) : it.sq - 1) - i0);
+                }
                 [[maybe_unused]] uint32_t bw[VAR == 2 ? 16 : 1];  // the key's bias values in the 32 query columns
                 if constexpr (VAR == 2) {
                     // A row of the tensor at a time: the warp's 32 keys lie side by side.  Every address is inside the block, so that no load
