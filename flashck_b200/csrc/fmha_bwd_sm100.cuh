@@ -99,18 +99,24 @@ __device__ __forceinline__ void bwd_issue_xb(uint32_t d, uint32_t a, uint64_t b,
 }
 
 // 2^x on the FMA pipe for two values: x = n + f, f in [-0.5, 0.5], 2^f by the polynomial of degree 4 of least relative error
-// (2.7e-6 with its fp32 rounding), n added to the exponent.  x above -126 (2^-126 stands for everything below).
+// (2.7e-6 with its fp32 rounding), times 2^n put together from its bits.  x above -126 (2^-126 stands for everything below).  A NaN
+// stays one: the maximum hands it on, and a product with it is NaN whatever the bits of n have become (added to the exponent,
+// n would turn it into the largest finite number).
+__device__ __forceinline__ float bwd_max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 __device__ __forceinline__ float2 bwd_exp2_poly(float2 x) {
-    x.x = fmaxf(x.x, -126.f);
-    x.y = fmaxf(x.y, -126.f);
+    x.x = bwd_max_nan(x.x, -126.f);
+    x.y = bwd_max_nan(x.y, -126.f);
     const float2 t = __fadd2_rn(x, make_float2(12582912.f, 12582912.f));  // 1.5 * 2^23: n lands in the low mantissa bits
     const float2 f = __fadd2_rn(x, __fadd2_rn(make_float2(12582912.f, 12582912.f), make_float2(-t.x, -t.y)));
     float2 q = __ffma2_rn(make_float2(0.009570076f, 0.009570076f), f, make_float2(0.05591789f, 0.05591789f));
     q = __ffma2_rn(q, f, make_float2(0.24024746f, 0.24024746f));
     q = __ffma2_rn(q, f, make_float2(0.6931218f, 0.6931218f));
     q = __ffma2_rn(q, f, make_float2(0.9999993f, 0.9999993f));
-    return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
-                       __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+    return __fmul2_rn(q, make_float2(__int_as_float((__float_as_int(t.x) << 23) + 0x3f800000), __int_as_float((__float_as_int(t.y) << 23) + 0x3f800000)));
 }
 // The exponentials of a pair: pairs `i` of every 8 below POLY go to the FMA pipe, the others to the exp2 unit, which alone would
 // take 1024 clocks per 128 x 128 tile.  Shares of 8 measured (dQ, dK/dV; us of 2 x 4096 causal tokens of 32 / 8 heads, and of 37k ragged

@@ -46,3 +46,30 @@ def test_keys_that_no_query_sees(d, mask, sq, sk, add, instance, device_ok):
     assert not dk[:, unseen:].any() and not dv[:, unseen:].any()
     for n, x, w, e in (("dk", dk, want[1], bound[1]), ("dv", dv, want[2], bound[2])):
         assert_within(n, x, w, e)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("where", ["q", "lse"])
+def test_a_nan_in_any_query_row_shows(d, where, instance, device_ok):
+    """Sequence i has it in row i.  Its P are NaN, so all of dV and dK are, and the row's dQ; other rows' dQ are not."""
+    n = 64
+    dout, q, k, v, o, lse = _problem(n, n, 70, 1, d, NONE)
+    rows = torch.arange(n, device="cuda")
+    (q[:, :, 0, 0] if where == "q" else lse[:, 0])[rows, rows] = float("nan")
+    dq, dk, dv = ops.fmha_bwd(dout, q, k, v, o, lse)
+    assert torch.isnan(dv).all() and torch.isnan(dk).all()
+    hit = torch.isnan(dq).all(-1)[..., 0]
+    assert torch.equal(hit, torch.eye(n, dtype=torch.bool, device="cuda")) and torch.isfinite(dq[~hit]).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_nan_in_any_key_shows(d, instance, device_ok):
+    n = 64
+    dout, q, k, v, o, lse = _problem(n, 70, n, 1, d, NONE)
+    rows = torch.arange(n, device="cuda")
+    k[rows, rows, 0, 0] = float("nan")
+    dq, dk, dv = ops.fmha_bwd(dout, q, k, v, o, lse)
+    assert torch.isnan(dq).all()
+    hit = torch.isnan(dv).all(-1)[..., 0]
+    assert torch.equal(hit, torch.eye(n, dtype=torch.bool, device="cuda")) and torch.isfinite(dv[~hit]).all()
+    assert torch.equal(torch.isnan(dk).all(-1)[..., 0], hit) and torch.isfinite(dk[~hit]).all()
