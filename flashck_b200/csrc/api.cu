@@ -588,8 +588,9 @@ int FmhaFwdSharedPrefix(void* q, void* k_prefix, void* v_prefix, void* k, void* 
     FCK_REQUIRE(batch >= 0 && q_seq_len >= 0 && q_max_seq_len >= 0 && prefix_len >= 0 && kv_seq_len >= 0, FLASHCK_ERR_INVALID_ARGUMENT,
                 "FmhaFwdSharedPrefix: negative size");
     if (batch == 0 || q_seq_len == 0) return FLASHCK_OK;
-    FCK_REQUIRE(q && k && v && o && k_seq_len && workspace && (prefix_len == 0 || (k_prefix && v_prefix)), FLASHCK_ERR_INVALID_ARGUMENT,
-                "FmhaFwdSharedPrefix: null pointer argument");
+    const bool no_room = (block_table ? block_table_stride : kv_seq_len) == 0;  // caches that hold nothing have no address
+    FCK_REQUIRE(q && (no_room || (k && v)) && o && k_seq_len && workspace && (prefix_len == 0 || (k_prefix && v_prefix)),
+                FLASHCK_ERR_INVALID_ARGUMENT, "FmhaFwdSharedPrefix: null pointer argument");
     FCK_REQUIRE(((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)k_prefix | (uintptr_t)v_prefix | (uintptr_t)o | (uintptr_t)workspace) & 15) == 0),
                 FLASHCK_ERR_INVALID_ARGUMENT, "FmhaFwdSharedPrefix: the tensors must start on 16-byte boundaries");
     FCK_REQUIRE(prefix_len < (1ll << 31) - 256, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSharedPrefix: prefix_len must stay below 2^31");

@@ -307,7 +307,8 @@ FLASHCK_API int FlashckPeerBufferFree(void* ptr);
  *   k/v_prefix: [prefix_len,hkv,d], or with prefix_table (int32, the prefix's pages in order) pools of prefix_pool_pages
  *      pages of prefix_page tokens; prefix_len may end inside a page, and may be 0
  *   k/v: the own caches [b,kv_seq_len,hkv,d], or with block_table (int32, rows block_table_stride apart) pools of
- *      num_pool_pages pages of paged_block_size tokens; k_seq_len_ptr int32 [b]: own keys of each sequence (0: none)
+ *      num_pool_pages pages of paged_block_size tokens; k_seq_len_ptr int32 [b]: own keys of each sequence (0: none).  Caches without
+ *      room (kv_seq_len or block_table_stride 0) may be NULL
  *   causal: 0, or 1: query i of a sequence with n queries and m own keys sees its own keys <= m - n + i (and the prefix)
  *   workspace: FlashckSharedPrefixWorkspace(...) bytes of device memory, 16-byte aligned, used during the call only.  The size follows
  *      from the sizes of the call and the current device, no instance parameter changes it: one asked for once serves every call of
