@@ -14,7 +14,9 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
@@ -437,6 +439,17 @@ PyObject* call_shared_prefix(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
+// (leaf) -> whether its gradient is accumulated on the default stream: where the node that does it was made, which need not be by a
+// call of this package
+PyObject* accumulates_on_default_stream(PyObject*, PyObject* leaf) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(THPVariable_Check(leaf), "a tensor is needed");
+    const auto node = torch::autograd::impl::grad_accumulator(THPVariable_Unpack(leaf));
+    const auto stream = node ? node->stream() : std::nullopt;
+    return PyBool_FromLong(stream && stream->device_type() == c10::kCUDA && c10::cuda::CUDAStream(*stream).stream() == nullptr);
+    END_HANDLE_TH_ERRORS
+}
+
 PyObject* num_splits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     Reader r{args, nargs};
     const int64_t b = r.integer(), rows = r.integer();
@@ -451,6 +464,7 @@ PyMethodDef methods[] = {
     {"_call_append_kv", (PyCFunction)(void (*)(void))call_append_kv, METH_FASTCALL, nullptr},
     {"_call_backward", (PyCFunction)(void (*)(void))call_backward, METH_FASTCALL, nullptr},
     {"_call_shared_prefix", (PyCFunction)(void (*)(void))call_shared_prefix, METH_FASTCALL, nullptr},
+    {"_accumulates_on_default_stream", (PyCFunction)accumulates_on_default_stream, METH_O, nullptr},
     {"_num_splits", (PyCFunction)(void (*)(void))num_splits, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

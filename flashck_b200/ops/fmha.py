@@ -87,7 +87,8 @@ def _on(device: torch.device):
 # Plain calls run in the compiled binding (csrc/pybind/calls.cpp: the same checks, allocations and C call; 2 x 128 tokens 24 us a
 # call in Python, 7.0 there).  It answers None for a call that it cannot check completely; the code below then takes it.
 _NATIVE = None  # the binding, or False where there is none of this package's age that loads
-_NATIVE_CALLS = ("_call_forward", "_call_paged_prefill", "_call_splitkv", "_call_append_kv", "_call_backward", "_call_shared_prefix")
+_NATIVE_CALLS = ("_call_forward", "_call_paged_prefill", "_call_splitkv", "_call_append_kv", "_call_backward", "_call_shared_prefix",
+                 "_accumulates_on_default_stream")
 _TUNING_DIR = flags.flag("FC_TUNING_DB_DIR")  # (set: the call may have to tune first)
 
 

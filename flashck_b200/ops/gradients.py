@@ -120,19 +120,22 @@ def fmha_bwd_var_len(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: to
                       int(max_seqlen_k), scale, causal, window_size, mask_type, bias, alibi_slopes, logits_soft_cap, dlse, return_dbias)
 
 
-# A leaf's gradient is accumulated on the stream where the first graph that uses the leaf was recorded, for as long as a graph holds
-# the leaf's node.  Where that is the default stream, a captured backward pass would make it wait for the capture, which
+# A leaf's gradient is accumulated on the stream where its node was made (by the first graph that uses the leaf), for as long as a
+# graph holds the node.  Where that is the default stream, a captured backward pass would make it wait for the capture, which
 # ends the process.  The node carries a mark, and the captured pass is refused.
-_ON_DEFAULT_STREAM = "flashck_b200: recorded on the default stream"
+_ON_DEFAULT_STREAM = "flashck_b200: made on the default stream"
 
 
 def _mark_leaves(*tensors: Optional[torch.Tensor]) -> list:
     """The nodes of the leaves among the tensors, marked; they have to be held until the graph holds them."""
     leaves = [t for t in tensors if t is not None and t.is_cuda and t.is_leaf and t.requires_grad]
     nodes = [torch.autograd.graph.get_gradient_edge(t).node for t in leaves]
-    if nodes and torch.cuda.current_stream(leaves[0].device).cuda_stream == 0:
-        for n in nodes:
-            n.metadata[_ON_DEFAULT_STREAM] = True
+    native = _f._native()
+    for t, n in zip(leaves, nodes):
+        if native:
+            n.metadata[_ON_DEFAULT_STREAM] = native._accumulates_on_default_stream(t)
+        else:  # what made the node cannot be asked: the first call here that meets it is taken for it
+            n.metadata.setdefault(_ON_DEFAULT_STREAM, torch.cuda.current_stream(t.device).cuda_stream == 0)
     return nodes
 
 
