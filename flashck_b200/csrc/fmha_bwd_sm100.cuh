@@ -55,7 +55,7 @@ struct BwdSm100Dev {
     void* dbias;
     int bias_rank;                 // 0 one plane, 1 one per head, 2 one per (batch, head)
     int64_t bias_sq, bias_sk;
-    int listed;                    // items are found in order of cost by a persistent grid; 0: one per CTA, by its index
+    int listed;                    // a persistent grid finds the items, 1: in order of cost, 2: sequence after sequence; 0: one per CTA, by its index
     int max_tiles;                 // tiles of the longest sequence
 };
 
@@ -266,12 +266,20 @@ struct BwdCtrl {
 // The schedule, kept by the warp that issues the copies.  Items of a level cost the same under a causal mask: level l is the row tile
 // l of dQ (the last tiles see the most keys), the tile l places in front of the last one of dK/dV (the first tiles are seen by
 // the most queries).  Levels come in decreasing order, a level's sequences in order, their heads side by side (they share tiles
-// through L2); rounds of the grid take the items in alternate directions.  Tile counts are held eight sequences a lane.
+// through L2); rounds of the grid take the items in alternate directions.  Tile counts are held eight sequences a lane.  More sequences
+// than that come in their own order, 32 at a time, the tiles of a sequence one after the other: the tiles that exist, not those that
+// the longest sequence would have.
 template <bool DQ>
 struct BwdSchedule {
-    int cnt[kBwdMaxBatch / 32], level, round;
-    int64_t base;  // first item of the level
+    int cnt[kBwdMaxBatch / 32], level, round;  // (listed 2: cnt[0] is sequence level + lane's)
+    int64_t base;  // first item of the level (listed 2: of the 32 sequences)
     uint32_t k;    // items handed out
+
+    __device__ __forceinline__ int tiles_of(const BwdSm100Dev& p, int b) {
+        if (b >= p.batch) return 0;
+        const BwdSeq s = bwd_sequence(p, b);
+        return min(((DQ ? s.sq : s.sk) + 127) / 128, p.max_tiles);
+    }
 
     __device__ __forceinline__ void init(const BwdSm100Dev& p, int lane) {
         k = 0;
@@ -279,14 +287,15 @@ struct BwdSchedule {
         base = 0;
         level = -1;
         if (!p.listed) return;
+        if (p.listed == 2) {
+            level = 0;
+            cnt[0] = tiles_of(p, lane);
+            return;
+        }
         int most = 0;
 #pragma unroll
         for (int u = 0; u < kBwdMaxBatch / 32; ++u) {
-            cnt[u] = 0;
-            if (u * 32 + lane < p.batch) {
-                const BwdSeq s = bwd_sequence(p, u * 32 + lane);
-                cnt[u] = min(((DQ ? s.sq : s.sk) + 127) / 128, p.max_tiles);
-            }
+            cnt[u] = tiles_of(p, u * 32 + lane);
             most = max(most, cnt[u]);
         }
         level = (int)__reduce_max_sync(0xffffffffu, (unsigned)most) - 1;
@@ -301,6 +310,31 @@ struct BwdSchedule {
                 it.b = rest / heads;
                 it.h = rest - it.b * heads;
                 it.row0 = (DQ ? (int)gridDim.x / per_tile - 1 - t : t) * 128;
+                it.valid = 1;
+            }
+        } else if (p.listed == 2) {
+            const int64_t w = (int64_t)round * gridDim.x + blockIdx.x;
+            ++round;
+            int total;
+            while (true) {
+                total = __reduce_add_sync(0xffffffffu, cnt[0]);
+                if (w < base + (int64_t)total * heads || level + 32 >= p.batch) break;
+                base += (int64_t)total * heads;
+                level += 32;
+                cnt[0] = tiles_of(p, level + lane);
+            }
+            if (w < base + (int64_t)total * heads) {
+                const int at = (int)((w - base) / heads);  // tile of the 32 sequences
+                int end = cnt[0];                          // tiles up to and with the lane's
+#pragma unroll
+                for (int off = 1; off < 32; off *= 2) {
+                    const int before = __shfl_up_sync(0xffffffffu, end, off);
+                    if (lane >= off) end += before;
+                }
+                const int l = __ffs(__ballot_sync(0xffffffffu, end > at)) - 1;
+                it.b = level + l;
+                it.h = (int)(w - base) - at * heads;
+                it.row0 = (at - __shfl_sync(0xffffffffu, end - cnt[0], l)) * 128;
                 it.valid = 1;
             }
         } else {
