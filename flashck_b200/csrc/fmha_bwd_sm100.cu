@@ -9,7 +9,7 @@ using namespace sm100;
 
 namespace {
 
-// 128 x 128 tiles of all planes (group mode: of every sequence's block in them)
+// 128 x 128 tiles of all planes (group mode: of every sequence's block in them, as if all were as long as the longest)
 int64_t bias_items(const BwdParams& p) {
     const int64_t planes = (p.bias_rank >= 1 ? p.hq : 1) * (p.bias_rank == 2 || p.seqstart_q ? p.batch : 1);
     return (p.max_seqlen_q + 127) / 128 * ((p.max_seqlen_k + 127) / 128) * planes;
@@ -56,9 +56,8 @@ int launch_bwd_t(const BwdParams& p, const BwdSm100Dev& dev, cudaStream_t stream
             auto dbias = bwd_dbias_sm100_kernel<T, HDIM>;
             constexpr size_t smem = 1024 + 6 * TILE + sizeof(BwdCtrl);
             FCK_CUDA(cudaFuncSetAttribute(dbias, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-            const int64_t tq = (p.max_seqlen_q + 127) / 128, tk = (p.max_seqlen_k + 127) / 128, items = bias_items(p);
-            FCK_CUDA(launch_dependent(dbias, dim3((unsigned)std::min<int64_t>(items, sm_count())), dim3(kBwdBiasThreads), smem, stream, mq, mdo, mk, mv, dev,
-                                      (int)tq, (int)tk, items));
+            FCK_CUDA(launch_dependent(dbias, dim3((unsigned)std::min<int64_t>(bias_items(p), sm_count())), dim3(kBwdBiasThreads), smem, stream, mq, mdo,
+                                      mk, mv, dev));
         }
     }
     return FLASHCK_OK;

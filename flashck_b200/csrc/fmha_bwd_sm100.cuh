@@ -1138,24 +1138,38 @@ __device__ __forceinline__ void bwd_tmem_ld8(uint32_t taddr, uint32_t (&r)[8]) {
                  : "memory");
 }
 struct BwdBiasItem {
-    int valid, row0, key0, b_begin, b_end, h_begin, h_end, steps;
+    int row0, key0, b_begin, b_end, h_begin, h_end, steps;
     BwdSeq s;  // of the first sharer (the sharers' lengths are equal)
 };
-__device__ __forceinline__ BwdBiasItem bwd_bias_item(const BwdSm100Dev& p, int64_t item, int tiles_q, int tiles_k) {
+// The items of a CTA: those tiles of plane after plane that lie inside the plane's sequence (planes: heads, or none, inside sequences,
+// or none), dealt in turn.  Every role walks them for itself.
+struct BwdBiasWalk {
+    int pb, ph, tiles_k;
+    int at, tiles;  // the next item of this CTA, and the tiles, of the plane (a plane that memory holds has fewer than 2^25)
+
+    __device__ __forceinline__ void plane(const BwdSm100Dev& p) {
+        const BwdSeq s = bwd_sequence(p, pb);
+        tiles_k = (s.sk + 127) / 128;
+        tiles = (s.sq + 127) / 128 * tiles_k;
+    }
+    __device__ __forceinline__ void init(const BwdSm100Dev& p) {
+        pb = ph = 0;
+        at = blockIdx.x;
+        plane(p);
+    }
+    __device__ __forceinline__ bool next(const BwdSm100Dev& p, BwdBiasItem& it);
+};
+__device__ __forceinline__ BwdBiasItem bwd_bias_item(const BwdSm100Dev& p, int pb, int ph, int tile_q, int tile_k) {
     BwdBiasItem it;
-    it.key0 = (int)(item % tiles_k) * 128;
-    item /= tiles_k;
-    it.row0 = (int)(item % tiles_q) * 128;
-    item /= tiles_q;
-    const int planes_h = p.bias_rank >= 1 ? p.hq : 1, ph = (int)(item % planes_h), pb = (int)(item / planes_h);
+    it.key0 = tile_k * 128;
+    it.row0 = tile_q * 128;
     const bool own_b = p.bias_rank == 2 || p.seqstart_q;
     it.b_begin = own_b ? pb : 0;
     it.b_end = own_b ? pb + 1 : p.batch;
     it.h_begin = p.bias_rank >= 1 ? ph : 0;
     it.h_end = p.bias_rank >= 1 ? ph + 1 : p.hq;
     it.s = bwd_sequence(p, it.b_begin);
-    it.valid = it.row0 < it.s.sq && it.key0 < it.s.sk;
-    bool seen = it.valid;  // by some row: the first key of the last row's window, the last key of the last row
+    bool seen = true;  // by some row: the first key of the last row's window, the last key of the last row
     if (p.mask_type != 0) {
         const int last = min(it.s.sq, it.row0 + 128) - 1;
         if (p.wr >= 0 && it.key0 > last + it.s.shift + p.wr) seen = false;
@@ -1164,14 +1178,28 @@ __device__ __forceinline__ BwdBiasItem bwd_bias_item(const BwdSm100Dev& p, int64
     it.steps = seen ? (it.b_end - it.b_begin) * (it.h_end - it.h_begin) : 0;
     return it;
 }
+__device__ __forceinline__ bool BwdBiasWalk::next(const BwdSm100Dev& p, BwdBiasItem& it) {
+    const int planes_h = p.bias_rank >= 1 ? p.hq : 1, planes_b = p.bias_rank == 2 || p.seqstart_q ? p.batch : 1;
+    while (at >= tiles) {
+        at -= tiles;
+        if (++ph == planes_h) {
+            ph = 0;
+            if (++pb >= planes_b) return false;
+            plane(p);
+        }
+    }
+    const int tile_q = at / tiles_k;
+    it = bwd_bias_item(p, pb, ph, tile_q, at - tile_q * tiles_k);
+    at += gridDim.x;
+    return true;
+}
 
 constexpr int kBwdBiasThreads = 576;  // warps 0-15 elementwise, 16 products, 17 copies
 
 template <typename T, int HDIM>
 __global__ void __launch_bounds__(kBwdBiasThreads, 1)
 bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_do,
-                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const BwdSm100Dev p, int tiles_q,
-                       int tiles_k, int64_t items) {
+                       const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const BwdSm100Dev p) {
     constexpr int TILE = 128 * HDIM * 2;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* sQ = smem_raw + (((smem_u32(smem_raw) + 1023u) & ~1023u) - smem_u32(smem_raw));  // 2 x (Q, K)
@@ -1204,6 +1232,9 @@ bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     const int G = p.hq / p.hkv;
     bool ok = true;
     uint32_t t = 0;
+    BwdBiasWalk walk;
+    BwdBiasItem it;
+    walk.init(p);
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
         return ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, p.status, code)) != 0;
     };
@@ -1214,8 +1245,7 @@ bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
 #pragma unroll
             for (int hb = 0; hb < HDIM / 64; ++hb) tma_load_3d(dst + hb * HALF_BYTES, map, bar, hb * 64, head, row);
         };
-        for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-            const BwdBiasItem it = bwd_bias_item(p, item, tiles_q, tiles_k);
+        while (ok && walk.next(p, it)) {
             int b = it.b_begin, h = it.h_begin;
             for (int j = 0; j < it.steps; ++j, ++t) {
                 const BwdSeq s = bwd_sequence(p, b);
@@ -1241,9 +1271,8 @@ bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
         const bool leader = elect_one_sync();
         auto commit = [&](uint64_t* bar) { if (leader) umma_commit(bar); };
         const uint64_t dQ = make_smem_desc(smem_u32(sQ), 0, 1024), dDO = make_smem_desc(smem_u32(sDO), 0, 1024);
-        for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-            const int steps = bwd_bias_item(p, item, tiles_q, tiles_k).steps;
-            for (int j = 0; j < steps; ++j, ++t) {
+        while (ok && walk.next(p, it)) {
+            for (int j = 0; j < it.steps; ++j, ++t) {
                 const uint32_t buf = t & 1u, par = (t >> 1) & 1u;
                 if (!wait(&ctrl->a_full[buf], par, 0x10211) || !wait(&ctrl->s_free[buf], par ^ 1u, 0x10212)) break;
                 tc_fence_after();
@@ -1260,9 +1289,7 @@ bwd_dbias_sm100_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_c
     } else if (warp < 16) {
         const int quarter = warp >> 2, r = (warp & 3) * 32 + lane;
         const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + quarter * 32;
-        for (int64_t item = blockIdx.x; ok && item < items; item += gridDim.x) {
-            const BwdBiasItem it = bwd_bias_item(p, item, tiles_q, tiles_k);
-            if (!it.valid) continue;
+        while (ok && walk.next(p, it)) {
             const int i = it.row0 + r, key0 = it.key0 + quarter * 32, left = it.s.sq - it.row0;
             const int64_t block = bwd_bias_block(p, it.b_begin, it.h_begin, it.s.q0, it.s.k0);
             uint32_t bw[16];

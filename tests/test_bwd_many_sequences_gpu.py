@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from attention_reference import assert_within, forward, gradients
+from attention_reference import assert_within, forward, gradients, half_step
 from flashck_b200 import _lib, ops
 
 pytestmark = pytest.mark.gpu
@@ -81,3 +81,41 @@ def test_a_dense_batch_of_many_sequences(device_ok):
     want, bound = gradients(*args, 0.125, CAUSAL)
     for name, x, w, e in zip(("dq", "dk", "dv"), ops.fmha_bwd(*args, causal=True), want, bound):
         assert_within(name, x, w, e)
+
+
+def _milliseconds(call):
+    times = []
+    for _ in range(7):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        call()
+        b.record()
+        b.synchronize()
+        times.append(a.elapsed_time(b))
+    return sorted(times)[3]
+
+
+@pytest.mark.parametrize("heads,planes,d", [(2, 1, 64), (2, 2, 128)])
+def test_bias_gradient_of_many_sequences(heads, planes, d, device_ok):
+    """The blocks of 500 sequences in one plane, with and without the longest one stated: the same bits, in about the same time
+    (tiles of the whole plane, sequence by sequence, are some four million here)."""
+    lens = [i * 7 % 41 for i in range(500)]
+    total, cu = sum(lens), torch.tensor([0] + lens).cumsum(0).cuda()
+    q, k, v, dout = (torch.randn(total, heads, d, device="cuda").bfloat16() for _ in range(4))
+    bias = torch.randn(1, planes, total, total, device="cuda").bfloat16()
+    o, lse = ops.fmha_fwd_var_len(q, k, v, cu, cu, max(lens), max(lens), return_lse=True, bias=bias)
+    call = lambda *longest: ops.fmha_bwd_var_len(dout, q, k, v, o, lse, cu, cu, *longest, bias=bias, return_dbias=True)  # noqa: E731
+    got = call()
+    assert all(torch.equal(a, b) for a, b in zip(got, call(max(lens), max(lens))))
+    at, outside = cu.tolist(), torch.ones_like(bias, dtype=torch.bool)
+    for i, n in enumerate(lens):
+        block = (slice(None), slice(None), slice(at[i], at[i + 1]), slice(at[i], at[i + 1]))
+        outside[block] = False
+        if n and i % 25 == 0:
+            rows = block[2]
+            part = [t[None, rows] for t in (dout, q, k, v, o)] + [lse[None, :, rows]]
+            want, bound = gradients(*part, d ** -0.5, (0, -1, -1), bias=bias[block])
+            w, e = (t.sum(1, keepdim=True) if planes == 1 else t for t in (want[3], bound[3]))
+            assert_within(f"dbias of sequence {i}", got[3][block], w, e + half_step(bias.dtype) * w.abs() + 2.0 ** -25)
+    assert not got[3][outside].any()
+    assert _milliseconds(call) <= 2 * _milliseconds(lambda: call(max(lens), max(lens)))
