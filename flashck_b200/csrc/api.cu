@@ -7,6 +7,7 @@
 #include <stdio.h>
 #include <string.h>
 
+#include <algorithm>
 #include <atomic>
 #include <mutex>
 
@@ -316,7 +317,8 @@ int FmhaBwd(void* dout, void* q, void* k, void* v, void* bias, void* o, void* ls
     p.max_seqlen_q = q_seq_start && q_max_seq_len > 0 && q_max_seq_len < q_seq_len ? q_max_seq_len : q_seq_len;
     p.max_seqlen_k = q_seq_start && kv_max_seq_len > 0 && kv_max_seq_len < kv_seq_len ? kv_max_seq_len : kv_seq_len;
     p.scale = resolve_scale(scale, d);
-    p.mask_type = (int)mask_type; p.wl = window_left; p.wr = window_right; p.dtype = dtype;
+    constexpr int64_t kFar = (1ll << 30) - 1;  // (reaches over every tensor that fits the memory)
+    p.mask_type = (int)mask_type; p.wl = std::min(window_left, kFar); p.wr = std::min(window_right, kFar); p.dtype = dtype;
     p.bias = bias_enum ? bias : nullptr; p.bias_type = bias_enum; p.bias_rank = bias_rank_info; p.logits_soft_cap = logits_soft_cap;
     const bool sm100 = g_use_sm100_bwd.load() && bwd_sm100_supported(p);
     g_last_bwd_instance = sm100 ? 1 : 0;

@@ -142,7 +142,7 @@ struct BwdParams {
     int64_t batch, seqlen_q, seqlen_k, hq, hkv, d, max_seqlen_q, max_seqlen_k;  // group mode: seqlen_q / seqlen_k are totals
     float scale;
     int mask_type;
-    int64_t wl, wr;
+    int64_t wl, wr;     // -1 or below 2^30
     int dtype;
     const void* bias;   // as in FwdParams
     int bias_type, bias_rank;
