@@ -120,7 +120,8 @@ __device__ __forceinline__ float2 bwd_exp2_poly(float2 x) {
 }
 // The exponentials of a pair: pairs `i` of every 8 below POLY go to the FMA pipe, the others to the exp2 unit, which alone would
 // take 1024 clocks per 128 x 128 tile.  Shares of 8 measured (dQ, dK/dV; us of 2 x 4096 causal tokens of 32 / 8 heads, and of 37k ragged
-// ones): (0, 3) 780, 2512; (1, 3) 773, 2489; (1, 4) 774, 2502; (2, 2) 780, 2525.  None with a bias tensor: its -inf must give a P of 0.
+// ones): (0, 3) 780, 2512; (1, 3) 773, 2489; (1, 4) 774, 2502; (2, 2) 780, 2525 (before the product that keeps a
+// NaN, with which the packed ones take 1 % more).  None with a bias tensor: its -inf must give a P of 0.
 constexpr int kPolyDq = 1, kPolyDkdv = 3;
 template <int POLY>
 __device__ __forceinline__ float2 bwd_exp2(float2 y, int i) {
@@ -437,7 +438,7 @@ __device__ __forceinline__ void bwd_zero_outside(const BwdSm100Dev& p) {
 
 constexpr int kBwdThreads = 640, kBwdConsumers = 19;  // (consumers of the item ring: every warp but the one that fills it)
 
-// 2 x 4096 causal tokens of 32 / 8 heads of 128: 350 us, 589 TFLOP/s of its three products, the tensor pipe busy 66 % of the time, at 1700
+// 2 x 4096 causal tokens of 32 / 8 heads of 128: 322 us, 1280 TFLOP/s of its three products, the tensor pipe busy 66 % of the time, at 1700
 // clocks a step beside the 1536 of the products and 8-9k clocks between two items (code that runs once an item comes from memory
 // again each time).
 // ---- dQ -----------------------------------------------------------------------------------------------------------------
@@ -787,7 +788,7 @@ bwd_dq_sm100_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
 }
 
-// The same tokens: 449 us, 612 TFLOP/s of its four products, the tensor pipe busy 70 %.  A step takes 2600 clocks beside the 2048 of
+// The same tokens: 422 us, 1300 TFLOP/s of its four products, the tensor pipe busy 70 %.  A step takes 2600 clocks beside the 2048 of
 // shared memory and of the products: S(i+1) waits for dP(i) to be read, so the elementwise work of a step (S and dP from tensor
 // memory, 32 exponentials and two conversions a thread, P and dS back) lies on the chain.
 // ---- dK / dV --------------------------------------------------------------------------------------------------------------

@@ -6,9 +6,9 @@
 // one sequence (rows x group per kv head fill whole tiles, so the split kernels read the prefix once per 128 or 256 rows instead
 // of once per sequence; the tcgen05 split mode takes 16 tiles of rows in one launch, so more rows go in runs).  2. The own caches,
 // as any split-KV call.  3. The merge of both sets of partials, here.
-// 131072 keys under 32 sequences of 64 / 8 heads with 1-4096 keys of their own: 199 us; the prefix 125 (537 MB at 4.3 TB/s, 1100 TFLOP/s:
-// bound by the steps, as the prefill forms are), the own caches 59 (5.2 TB/s), the merge 13.  8192 keys under 64 sequences of 32 / 8 heads
-// with 64-2048 keys of their own: 103 us; 24, 58 and 12.
+// 131072 keys under 32 sequences of 64 / 8 heads with 1-4096 keys of their own: 217 us a call; by themselves the prefix 125 (537 MB at
+// 4.3 TB/s, 1100 TFLOP/s: bound by the steps, as the prefill forms are), the own caches 59 (5.2 TB/s), the merge 13.  8192 keys under
+// 64 sequences of 32 / 8 heads with 64-2048 keys of their own: 103 us; 24, 58 and 12.
 #include <algorithm>
 
 #include "kernels.h"
