@@ -45,6 +45,10 @@ SIGNATURES = {
     "FlashckSharedPrefixWorkspace": ([_I64] * 9 + [_I, _I], _I64),
     "FmhaFwdSharedPrefix": ([_P] * 12 + [_I64] * 14 + [_F, _I, _P, _I], _I),
     "FmhaFwdAppendKV": ([_P] * 12 + [_I64] * 9 + [_I, _I64, _I64, _P, _I], _I),
+    "FmhaFwdAppendKVInt4": ([_P] * 19 + [_I64] * 10 + [_I] + [_I64] * 3 + [_P, _I], _I),
+    "FmhaFwdSplitKVInt4": ([_P] * 11 + [_I64] * 11 + [_F, _I64, _I64, _U32, _P, _I], _I),
+    "FmhaReadKVInt4": ([_P] * 10 + [_I64] * 8 + [_P, _I], _I),
+    "FmhaRotary": ([_P] * 8 + [_I64] * 7 + [_I, _I, _P, _I], _I),
     "FlashckSetInstanceParam": ([_I, ctypes.c_char_p, _I64], _I),
     "FlashckGetInstanceParam": ([_I, ctypes.c_char_p, ctypes.POINTER(_I64)], _I),
 }

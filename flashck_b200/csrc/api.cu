@@ -650,6 +650,106 @@ int FmhaFwdAppendKV(void* q, void* k_cache, void* knew, void* v_cache, void* vne
     return launch_appendkv(p, (cudaStream_t)stream);
 }
 
+// The parts of a 4-bit cache that its three entry points share.
+static int int4_cache(const char* fn, Int4Cache& c, const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                      const void* k_seq_len, const void* block_table, const int64_t* cache_batch_idx, int64_t batch, int64_t hkv, int64_t d,
+                      int64_t group, int64_t bt_stride, int64_t page, int64_t pool, int dtype) {
+    FCK_REQUIRE(k_codes && k_params && v_codes && v_params && k_seq_len, FLASHCK_ERR_INVALID_ARGUMENT, "%s: null cache or length pointer", fn);
+    const auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+    FCK_REQUIRE(aligned(k_codes) && aligned(k_params) && aligned(v_codes) && aligned(v_params), FLASHCK_ERR_INVALID_ARGUMENT,
+                "%s: codes and params of the caches must be 16-byte aligned", fn);
+    FCK_REQUIRE(batch > 0, FLASHCK_ERR_INVALID_ARGUMENT, "%s: batch must be positive", fn);
+    FCK_REQUIRE(group > 0 && d % group == 0, FLASHCK_ERR_INVALID_ARGUMENT, "%s: the group must divide the head dim", fn);
+    FCK_REQUIRE(batch < (1ll << 31) && bt_stride >= 0, FLASHCK_ERR_INVALID_ARGUMENT, "%s: bad batch or block table", fn);
+    c = Int4Cache{};
+    c.k_codes = const_cast<void*>(k_codes); c.k_params = const_cast<void*>(k_params);
+    c.v_codes = const_cast<void*>(v_codes); c.v_params = const_cast<void*>(v_params);
+    c.seqlen = (const int32_t*)k_seq_len; c.block_table = (const int32_t*)block_table; c.cache_batch_idx = cache_batch_idx;
+    c.batch = batch; c.hkv = hkv; c.d = d; c.group = group; c.bt_stride = block_table ? bt_stride : 0; c.page = page; c.pool = pool;
+    c.dtype = dtype;
+    return FLASHCK_OK;
+}
+
+int FmhaFwdAppendKVInt4(const void* q, void* q_out, void* k_codes, void* k_params, const void* knew, void* v_codes, void* v_params,
+                        const void* vnew, void* k_held, void* v_held, const void* k_seq_len, const int64_t* q_seq_start,
+                        const int64_t* knew_seq_start, const void* positions, const void* rotary_cos, const void* rotary_sin,
+                        const void* pair_axis, const void* block_table, const int64_t* cache_batch_idx, int64_t batch, int64_t q_seq_len,
+                        int64_t knew_seq_len, int64_t hq, int64_t hkv, int64_t d, int64_t group, int64_t axes, int64_t rotary_dim,
+                        int64_t rotary_rows, int rope_type, int64_t block_table_stride, int64_t page, int64_t pool, void* stream, int dtype) {
+    const char* fn = "FmhaFwdAppendKVInt4";
+    AppendInt4Params p{};
+    if (int rc = check_common(fn, dtype, q ? hq : hkv, hkv, d, d, nullptr)) return rc;
+    if (int rc = int4_cache(fn, p.cache, k_codes, k_params, v_codes, v_params, k_seq_len, block_table, cache_batch_idx, batch, hkv, d, group,
+                            block_table_stride, page, pool, dtype)) return rc;
+    FCK_REQUIRE(knew_seq_len >= 0 && q_seq_len >= 0 && knew_seq_len < (1ll << 31) && q_seq_len < (1ll << 31), FLASHCK_ERR_INVALID_ARGUMENT,
+                "%s: bad number of tokens", fn);
+    FCK_REQUIRE(knew_seq_len == 0 || (knew && vnew), FLASHCK_ERR_INVALID_ARGUMENT, "%s: knew/vnew must not be null", fn);
+    FCK_REQUIRE(!q || q_out, FLASHCK_ERR_INVALID_ARGUMENT, "%s: q_out must not be null", fn);
+    FCK_REQUIRE(!q || (q_seq_start == nullptr) == (knew_seq_start == nullptr), FLASHCK_ERR_INVALID_ARGUMENT,
+                "%s: q_seq_start_ptr and knew_seq_start_ptr go together (group mode)", fn);
+    p.q = q; p.q_out = q_out; p.knew = knew; p.vnew = vnew; p.k_held = k_held; p.v_held = v_held;
+    p.seqstart_q = q_seq_start; p.seqstart_knew = knew_seq_start; p.positions = (const int32_t*)positions;
+    p.rotary_cos = rotary_cos; p.rotary_sin = rotary_sin; p.pair_axis = (const uint8_t*)pair_axis;
+    p.seqlen_q = q_seq_len; p.seqlen_knew = knew_seq_len; p.hq = hq; p.axes = axes;
+    p.rotary_dim = rotary_dim; p.rotary_rows = rotary_rows; p.rope_type = rope_type;
+    return launch_append_int4(p, (cudaStream_t)stream);
+}
+
+int FmhaFwdSplitKVInt4(const void* q, const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, void* lse_acc,
+                       void* o_acc, const int64_t* q_seq_start, const void* k_seq_len, const void* block_table,
+                       const int64_t* cache_batch_idx, int64_t batch, int64_t q_seq_len, int64_t q_max_seq_len, int64_t hq, int64_t hkv,
+                       int64_t d, int64_t group, int64_t num_splits, int64_t block_table_stride, int64_t page, int64_t pool, float scale,
+                       int64_t window_left, int64_t window_right, uint32_t mask_type, void* stream, int dtype) {
+    const char* fn = "FmhaFwdSplitKVInt4";
+    SplitKVInt4Params p{};
+    if (int rc = check_common(fn, dtype, hq, hkv, d, d, nullptr)) return rc;
+    if (int rc = int4_cache(fn, p.cache, k_codes, k_params, v_codes, v_params, k_seq_len, block_table, cache_batch_idx, batch, hkv, d, group,
+                            block_table_stride, page, pool, dtype)) return rc;
+    FCK_REQUIRE(q && lse_acc && o_acc, FLASHCK_ERR_INVALID_ARGUMENT, "%s: null query or workspace pointer", fn);
+    FCK_REQUIRE((reinterpret_cast<uintptr_t>(q) & 15u) == 0 && (reinterpret_cast<uintptr_t>(o_acc) & 15u) == 0, FLASHCK_ERR_INVALID_ARGUMENT,
+                "%s: q and o_acc must be 16-byte aligned", fn);
+    FCK_REQUIRE(num_splits >= 1 && num_splits <= 4096 && mask_type <= 3, FLASHCK_ERR_INVALID_ARGUMENT, "%s: bad num_splits or mask_type", fn);
+    FCK_REQUIRE(q_seq_len > 0 && (q_seq_start ? q_max_seq_len > 0 : true), FLASHCK_ERR_INVALID_ARGUMENT, "%s: no query rows", fn);
+    p.q = q; p.o_acc = (float*)o_acc; p.lse_acc = (float*)lse_acc; p.seqstart_q = q_seq_start;
+    p.seqlen_q = q_seq_len; p.max_seqlen_q = q_seq_start ? std::min(q_max_seq_len, q_seq_len) : q_seq_len;
+    p.total_q = q_seq_start ? q_seq_len : batch * q_seq_len;
+    p.hq = hq; p.num_splits = num_splits; p.scale = resolve_scale(scale, d); p.mask_type = (int)mask_type;
+    p.wl = window_left; p.wr = window_right;
+    return launch_splitkv_int4(p, (cudaStream_t)stream);
+}
+
+int FmhaReadKVInt4(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, void* k_out, void* v_out,
+                   const void* k_seq_len, const int64_t* out_seq_start, const void* block_table, const int64_t* cache_batch_idx, int64_t batch,
+                   int64_t out_tokens, int64_t hkv, int64_t d, int64_t group, int64_t block_table_stride, int64_t page, int64_t pool,
+                   void* stream, int dtype) {
+    const char* fn = "FmhaReadKVInt4";
+    ReadInt4Params p{};
+    if (int rc = check_common(fn, dtype, hkv, hkv, d, d, nullptr)) return rc;
+    if (int rc = int4_cache(fn, p.cache, k_codes, k_params, v_codes, v_params, k_seq_len, block_table, cache_batch_idx, batch, hkv, d, group,
+                            block_table_stride, page, pool, dtype)) return rc;
+    FCK_REQUIRE(out_tokens >= 0, FLASHCK_ERR_INVALID_ARGUMENT, "%s: bad number of tokens", fn);
+    FCK_REQUIRE(out_tokens == 0 || (k_out && v_out), FLASHCK_ERR_INVALID_ARGUMENT, "%s: null output pointer", fn);
+    FCK_REQUIRE(((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15u) == 0, FLASHCK_ERR_INVALID_ARGUMENT,
+                "%s: the outputs must be 16-byte aligned", fn);
+    p.k = k_out; p.v = v_out; p.seqstart = out_seq_start; p.tokens = out_tokens;
+    return launch_read_int4(p, (cudaStream_t)stream);
+}
+
+int FmhaRotary(const void* q, void* q_out, const void* k, void* k_out, const void* positions, const void* rotary_cos, const void* rotary_sin,
+               const void* pair_axis, int64_t axes, int64_t tokens, int64_t hq, int64_t hkv, int64_t d, int64_t rotary_dim,
+               int64_t rotary_rows, int rope_type, int inverse, void* stream, int dtype) {
+    FCK_REQUIRE(dtype == FLASHCK_DTYPE_FLOAT16 || dtype == FLASHCK_DTYPE_BFLOAT16, FLASHCK_ERR_UNSUPPORTED,
+                "FmhaRotary: dtype must be 3 (float16) or 4 (bfloat16), got %d", dtype);
+    FCK_REQUIRE(tokens >= 0 && hq >= 0 && hkv >= 0, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaRotary: bad sizes");
+    FCK_REQUIRE(tokens == 0 || (q && q_out && positions && (!k || k_out)), FLASHCK_ERR_INVALID_ARGUMENT, "FmhaRotary: null pointer");
+    RotaryParams p{};
+    p.q = q; p.q_out = q_out; p.k = k; p.k_out = k_out; p.positions = (const int32_t*)positions;
+    p.rotary_cos = rotary_cos; p.rotary_sin = rotary_sin; p.pair_axis = (const uint8_t*)pair_axis; p.axes = axes; p.tokens = tokens;
+    p.hq = hq; p.hkv = hkv; p.d = d; p.rotary_dim = rotary_dim; p.rotary_rows = rotary_rows;
+    p.rope_type = rope_type; p.inverse = inverse; p.dtype = dtype;
+    return launch_rotary(p, (cudaStream_t)stream);
+}
+
 int FlashckSetInstanceParam(int family, const char* key, int64_t value) {
     FCK_REQUIRE(key != nullptr, FLASHCK_ERR_INVALID_ARGUMENT, "FlashckSetInstanceParam: null key");
     int rc = FLASHCK_ERR_INVALID_ARGUMENT;

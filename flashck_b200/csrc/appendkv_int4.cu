@@ -1,0 +1,370 @@
+// The write of a 4-bit key/value cache, and its way back to 16-bit keys and values.
+//
+// Append: the queries and the new keys are turned (int4.cuh), the turned keys and the values quantised group by group and written
+// through the block table.  One pass: a lane holds 8 channels of a head, 4 to 16 lanes a group, whose least and greatest value take 2
+// to 4 shuffles each.  A half-rotated pair's other half is read a second time (from L1) instead of exchanged.
+// Read: the same layout of lanes, 4 bytes of codes in and 16 bytes of values out.
+//
+// A job is one token's keys and values, or its queries; 1 to 8 warps share it.  What bounds the append of a decode step are three
+// memory round trips (sequence starts; length and page; the row), what bounds a long one is its traffic.
+#include <algorithm>
+#include <type_traits>
+
+#include "int4.cuh"
+
+namespace fck {
+
+int fill_rotary(const char* fn, RotaryDev& r, const void* cosr, const void* sinr, int64_t rows, int64_t rotary_dim, int64_t d, int rope_type,
+                const uint8_t* pair_axis, int64_t axes, bool rows_aligned) {
+    r = RotaryDev{};
+    r.type = rope_type;
+    r.vec = rows_aligned;
+    if (rope_type == 0) return FLASHCK_OK;
+    FCK_REQUIRE(rope_type == 1 || rope_type == 2, FLASHCK_ERR_INVALID_ARGUMENT, "%s: rope_type must be 0..2", fn);
+    FCK_REQUIRE(rotary_dim > 0 && rotary_dim <= d && rotary_dim % 2 == 0 && rotary_dim <= 2 * kMaxPairs, FLASHCK_ERR_INVALID_ARGUMENT,
+                "%s: rotary_dim must be even and in (0, hdim], at most %d (got %lld)", fn, 2 * kMaxPairs, (long long)rotary_dim);
+    FCK_REQUIRE(cosr && sinr, FLASHCK_ERR_INVALID_ARGUMENT, "%s: rotary tables must not be null when rope_type != 0", fn);
+    FCK_REQUIRE(rows >= 0 && rows < (1ll << 31), FLASHCK_ERR_INVALID_ARGUMENT, "%s: bad number of rows of the rotary tables", fn);
+    FCK_REQUIRE(axes >= 1 && axes <= kMaxAxes, FLASHCK_ERR_UNSUPPORTED, "%s: 1 to %d axes of positions (got %lld)", fn, kMaxAxes, (long long)axes);
+    r.cosr = cosr; r.sinr = sinr;
+    r.rows = (int)rows; r.half = (int)(rotary_dim / 2);
+    const auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+    r.vec = rows_aligned && aligned(cosr) && aligned(sinr) && rotary_dim % (rope_type == 1 ? 8 : 16) == 0;
+    for (int i = 0; pair_axis && i < r.half; ++i) {
+        FCK_REQUIRE(pair_axis[i] < axes, FLASHCK_ERR_INVALID_ARGUMENT, "%s: pair %d turns with axis %d of %lld", fn, i, (int)pair_axis[i],
+                    (long long)axes);
+        r.axis[i >> 4] |= (uint32_t)pair_axis[i] << (2 * (i & 15));
+    }
+    return FLASHCK_OK;
+}
+
+namespace {
+
+struct CacheDev {
+    uint8_t* codes[2];   // K, V
+    uint32_t* params[2];
+    const int32_t* seqlen;
+    const int32_t* block_table;
+    const int64_t* cache_batch_idx;
+    int batch, hkv, d, group, bt_stride, page, pool;
+};
+
+// The cache row of token `pos` of sequence b, or -1: behind the cache's end, or on a page that the pool does not have.
+__device__ __forceinline__ int64_t cache_row(const CacheDev& c, int b, int64_t pos) {
+    const int64_t bphys = c.cache_batch_idx ? c.cache_batch_idx[b] : b;
+    if (pos < 0) return -1;
+    if (!c.block_table) return pos < c.page && (uint64_t)bphys < (uint64_t)c.pool ? bphys * c.page + pos : -1;
+    const int64_t slot = pos / c.page;
+    if (slot >= c.bt_stride) return -1;
+    const int32_t pg = c.block_table[bphys * c.bt_stride + slot];
+    return (uint32_t)pg < (uint32_t)c.pool ? (int64_t)pg * c.page + (pos - slot * c.page) : -1;
+}
+
+// The sequence of packed row t, by the whole warp: the number of starts 1 .. batch - 1 at or below t.
+__device__ __forceinline__ int sequence_of(const int64_t* seqstart, int batch, int64_t t, int lane) {
+    int n = 0;
+    for (int i = 1 + lane; i < batch; i += 32) n += seqstart[i] <= t;
+    return __reduce_add_sync(0xffffffffu, n);
+}
+
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float r;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// (x - lo) / scale to the nearest code, ties to even, without rounding the quotient: a multiple h of one half is compared with it by the
+// sign of r - h scale, which one FMA gives exactly.
+__device__ __noinline__ uint32_t exact_code(float r, float s) {
+    uint32_t k = 0;
+    if (!(s > 0.f)) return 0;
+#pragma unroll 1
+    for (int i = 0; i < 15; ++i) {
+        const float e = fmaf(-(i + 0.5f), s, r);
+        k += e > 0.f || (e == 0.f && (i & 1));
+    }
+    return k;
+}
+
+// 8 channels of a group of `lanes` lanes: codes, scale and least value; `x` becomes what they stand for.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise(Vec8<T>& x, int lanes, T& scale_t, T& lo_t) {
+    float f[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f32(x.e[i]);
+    float lo = f[0], hi = f[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) { lo = min_nan(lo, f[i]); hi = max_nan(hi, f[i]); }
+    for (int off = 1; off < lanes; off <<= 1) {
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
+    }
+    lo_t = Elem<T>::from_f32(lo);
+    const float range = hi - lo;
+    scale_t = Elem<T>::from_f32(range < INFINITY ? __fdiv_rn(range, 15.f) : NAN);  // (a group that is not finite is NaN as a whole)
+    const float s = Elem<T>::to_f32(scale_t);
+    // quotients are off by a few 2^-22; where one is closer than 1e-4 to half way between two codes (0.2 in a thousand), or the
+    // reciprocal may overflow, the comparison above decides
+    const float inv = __frcp_rn(s);
+    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the rounded integer
+    float away = 0.f;
+    uint32_t word = 0;
+    uint32_t code[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float quotient = fminf((f[i] - lo) * inv, 15.f), t = quotient + kRound;
+        away = fmaxf(away, fabsf(quotient - (t - kRound)));
+        code[i] = __float_as_uint(t) & 15u;
+    }
+    if (away > 0.4999f || !(s > 1e-30f)) {
+        for (int i = 0; i < 8; ++i) code[i] = exact_code(f[i] - lo, s);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        word |= code[i] << (4 * i);
+        x.e[i] = Elem<T>::from_f32(fmaf(s, (float)code[i], lo));
+    }
+    return word;
+}
+
+struct AppendInt4Dev {
+    CacheDev cache;
+    RotaryDev rot;
+    const void* q;
+    void* q_out;
+    const void* knew;
+    const void* vnew;
+    void* k_held;
+    void* v_held;
+    const int64_t* seqstart_q;
+    const int64_t* seqstart_knew;
+    const int32_t* positions;
+    int* status;
+    int seqlen_q, seqlen_knew, hq, warps_per_job;
+    int64_t total_new, total_q;
+};
+
+template <typename T>
+__device__ __forceinline__ Vec8<T> load8(const T* p, bool vec) {
+    Vec8<T> x;
+    if (vec) {
+        x.v = *reinterpret_cast<const uint4*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.e[i] = p[i];
+    }
+    return x;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const Vec8<T>& x, bool vec) {
+    if (vec) {
+        *reinterpret_cast<uint4*>(p) = x.v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = x.e[i];
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) append_int4_kernel(const AppendInt4Dev a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const CacheDev& c = a.cache;
+    const int lane = threadIdx.x & 31, w = a.warps_per_job;
+    const int64_t job = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
+    const int part = (threadIdx.x >> 5) % w;
+    if (job >= a.total_new + a.total_q) return;  // (whole warps)
+    const bool queries = job >= a.total_new;
+    const int64_t t = queries ? job - a.total_new : job;
+    // ---- the token: its sequence b, its place j among the sequence's new tokens ----
+    const int64_t* starts = queries ? a.seqstart_q : a.seqstart_knew;
+    const int64_t each = queries ? a.seqlen_q : a.seqlen_knew;
+    int b;
+    int64_t j, n, first = 0;  // n: rows of the sequence in this tensor; first: packed row of its first new token
+    if (starts) {
+        b = sequence_of(starts, c.batch, t, lane);
+        const int64_t s0 = starts[b];
+        j = t - s0;
+        n = starts[b + 1] - s0;
+        first = queries ? a.seqstart_knew[b] : s0;
+    } else {
+        b = (int)(t / each);
+        j = t - b * each;
+        n = each;
+        first = (int64_t)b * a.seqlen_knew;
+    }
+    const bool real = j >= 0 && j < n;  // (a row that belongs to no sequence leaves as zeros)
+    if (queries) j += (a.seqstart_knew ? a.seqstart_knew[b + 1] - first : (int64_t)a.seqlen_knew) - n;  // the last new tokens are the queries'
+    const int64_t at = real ? c.seqlen[b] + j : -1;  // place in the cache
+    const int64_t token = first + j;
+    auto pos = [&](int axis) -> int64_t {
+        if (!a.positions) return at;
+        return j >= 0 && token < a.total_new ? a.positions[axis * a.total_new + token] : -1;
+    };
+    const int pieces = c.d >> 3, sub = lane / pieces, e0 = (lane - sub * pieces) << 3, heads_at_once = 32 / pieces;
+    const bool vec = a.rot.vec;
+    const int heads = queries ? a.hq : c.hkv, partner = partner_of(a.rot, e0);
+    const int64_t row = !queries && real ? cache_row(c, b, at) : -1;
+    if (!queries && real && row < 0 && lane == 0 && part == 0) atomicOr(a.status, FLASHCK_STATUS_APPEND_OVERFLOW);
+    const T* src = (const T*)(queries ? a.q : a.knew) + t * heads * c.d;
+    const int group_lanes = c.group >> 3;
+    for (int h0 = part * heads_at_once; h0 < heads; h0 += w * heads_at_once) {
+        const int h = h0 + sub;
+        const bool mine = h < heads;
+        Vec8<T> x, y;
+        x.v = make_uint4(0, 0, 0, 0);
+        if (real && mine) {
+            const T* p = src + (int64_t)h * c.d;
+            if (a.rot.type == 0) {
+                x = load8(p + e0, vec);
+            } else if (vec) {
+                const Vec8<T> own = load8(p + e0, true), other = load8(p + partner, true);
+                turn_piece<T>(a.rot, e0, pos, own, other, x);
+            } else {
+                turn_piece_any<T>(a.rot, e0, pos, p, x);
+            }
+        }
+        if (queries) {
+            if (mine) store8((T*)a.q_out + (t * heads + h) * c.d + e0, x, vec);
+            continue;
+        }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            if (kv == 1) {
+                x.v = make_uint4(0, 0, 0, 0);
+                if (real && mine) x = load8((const T*)a.vnew + (t * heads + h) * c.d + e0, vec);
+            }
+            T scale, lo;
+            const uint32_t word = quantise<T>(x, group_lanes, scale, lo);
+            if (!mine) continue;
+            if (row >= 0) {
+                const int64_t place = row * c.hkv + h;
+                reinterpret_cast<uint32_t*>(c.codes[kv])[(place * c.d + e0) >> 3] = word;
+                if ((e0 & (c.group - 1)) == 0) {
+                    T two[2] = {scale, lo};
+                    c.params[kv][(place * c.d + e0) / c.group] = *reinterpret_cast<const uint32_t*>(two);
+                }
+            }
+            void* held = kv ? a.v_held : a.k_held;
+            if (held) store8((T*)held + (t * heads + h) * c.d + e0, x, vec);
+        }
+    }
+}
+
+struct ReadInt4Dev {
+    CacheDev cache;
+    void* out[2];
+    const int64_t* seqstart;
+    int64_t tokens, total;
+    int warps_per_job;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) read_int4_kernel(const ReadInt4Dev a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const CacheDev& c = a.cache;
+    const int lane = threadIdx.x & 31, w = a.warps_per_job;
+    const int64_t t = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
+    const int part = (threadIdx.x >> 5) % w;
+    if (t >= a.total) return;
+    int b;
+    int64_t j, n;
+    if (a.seqstart) {
+        b = sequence_of(a.seqstart, c.batch, t, lane);
+        j = t - a.seqstart[b];
+        n = min((int64_t)c.seqlen[b], a.seqstart[b + 1] - a.seqstart[b]);
+    } else {
+        b = (int)(t / a.tokens);
+        j = t - b * a.tokens;
+        n = c.seqlen[b];
+    }
+    const int64_t row = j >= 0 && j < n ? cache_row(c, b, j) : -1;  // (no such token: zeros)
+    const int per_row = c.hkv * c.d >> 3;  // 8 channels each
+    for (int i = part * 32 + lane; i < per_row; i += w * 32) {
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+            Vec8<T> x;
+            x.v = make_uint4(0, 0, 0, 0);
+            if (row >= 0) {
+                const uint32_t word = reinterpret_cast<const uint32_t*>(c.codes[kv])[row * per_row + i];
+                const uint32_t two = c.params[kv][(row * per_row + i) / (c.group >> 3)];
+                const float s = Elem<T>::to_f32(reinterpret_cast<const T*>(&two)[0]), lo = Elem<T>::to_f32(reinterpret_cast<const T*>(&two)[1]);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) x.e[k] = Elem<T>::from_f32(fmaf(s, (float)((word >> (4 * k)) & 15u), lo));
+            }
+            *reinterpret_cast<uint4*>((T*)a.out[kv] + (t * per_row + i) * 8) = x.v;
+        }
+    }
+}
+
+int fill_cache(const char* fn, const Int4Cache& p, CacheDev& c) {
+    FCK_REQUIRE(p.d == 64 || p.d == 128, FLASHCK_ERR_UNSUPPORTED, "%s: hdim 64 or 128 (got %lld)", fn, (long long)p.d);
+    FCK_REQUIRE((p.group == 32 || p.group == 64 || p.group == 128) && p.group <= p.d, FLASHCK_ERR_UNSUPPORTED,
+                "%s: groups of 32, 64 or 128 channels of a head (got %lld of %lld)", fn, (long long)p.group, (long long)p.d);
+    FCK_REQUIRE(p.page > 0 && p.page < (1ll << 31) && p.pool >= 0 && p.pool < (1ll << 31) && p.bt_stride < (1ll << 31), FLASHCK_ERR_INVALID_ARGUMENT,
+                "%s: bad page, pool or block table size", fn);
+    FCK_REQUIRE(p.hkv <= 1024, FLASHCK_ERR_UNSUPPORTED, "%s: at most 1024 kv heads", fn);
+    c.codes[0] = (uint8_t*)p.k_codes; c.codes[1] = (uint8_t*)p.v_codes;
+    c.params[0] = (uint32_t*)p.k_params; c.params[1] = (uint32_t*)p.v_params;
+    c.seqlen = p.seqlen; c.block_table = p.block_table; c.cache_batch_idx = p.cache_batch_idx;
+    c.batch = (int)p.batch; c.hkv = (int)p.hkv; c.d = (int)p.d; c.group = (int)p.group;
+    c.bt_stride = (int)p.bt_stride; c.page = (int)p.page; c.pool = (int)p.pool;
+    return FLASHCK_OK;
+}
+
+// Warps that share a job: enough to fill the SMs with few jobs, one with many (what they all work out is worked out fewer times).
+int warps_for(int64_t jobs, int64_t most) {
+    int w = 8;
+    while (w > 1 && (w > most || jobs * w > (int64_t)sm_count() * 32)) w >>= 1;
+    return w;
+}
+
+}  // namespace
+
+int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream) {
+    AppendInt4Dev a{};
+    if (int rc = fill_cache("FmhaFwdAppendKVInt4", p.cache, a.cache)) return rc;
+    const auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+    const bool rows = aligned(p.q) && aligned(p.q_out) && aligned(p.knew) && aligned(p.vnew) && aligned(p.k_held) && aligned(p.v_held);
+    if (int rc = fill_rotary("FmhaFwdAppendKVInt4", a.rot, p.rotary_cos, p.rotary_sin, p.rotary_rows, p.rotary_dim, p.cache.d, p.rope_type,
+                             p.pair_axis, p.positions ? p.axes : 1, rows)) return rc;
+    a.status = device_status_ptr();
+    if (!a.status) return FLASHCK_ERR_CUDA;
+    a.q = p.q; a.q_out = p.q_out; a.knew = p.knew; a.vnew = p.vnew; a.k_held = p.k_held; a.v_held = p.v_held;
+    a.seqstart_q = p.seqstart_q; a.seqstart_knew = p.seqstart_knew; a.positions = p.positions;
+    a.seqlen_q = (int)p.seqlen_q; a.seqlen_knew = (int)p.seqlen_knew; a.hq = (int)p.hq;
+    a.total_new = p.seqstart_knew ? p.seqlen_knew : p.cache.batch * p.seqlen_knew;
+    a.total_q = !p.q ? 0 : p.seqstart_q ? p.seqlen_q : p.cache.batch * p.seqlen_q;
+    const int64_t jobs = a.total_new + a.total_q;
+    if (jobs == 0) return FLASHCK_OK;
+    a.warps_per_job = warps_for(jobs, std::max<int64_t>(1, std::max(p.hq, p.cache.hkv) * p.cache.d / 256));
+    const int64_t blocks = (jobs * a.warps_per_job + 7) / 8;
+    FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdAppendKVInt4: too many tokens");
+    const dim3 grid((unsigned)blocks), block(256);
+    if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_dependent(append_int4_kernel<__nv_bfloat16>, grid, block, 0, stream, a));
+    else FCK_CUDA(launch_dependent(append_int4_kernel<__half>, grid, block, 0, stream, a));
+    return FLASHCK_OK;
+}
+
+int launch_read_int4(const ReadInt4Params& p, cudaStream_t stream) {
+    ReadInt4Dev a{};
+    if (int rc = fill_cache("FmhaReadKVInt4", p.cache, a.cache)) return rc;
+    a.out[0] = p.k; a.out[1] = p.v; a.seqstart = p.seqstart; a.tokens = p.tokens;
+    a.total = p.seqstart ? p.tokens : p.cache.batch * p.tokens;
+    if (a.total == 0) return FLASHCK_OK;
+    a.warps_per_job = warps_for(a.total, std::max<int64_t>(1, p.cache.hkv * p.cache.d / 256));
+    const int64_t blocks = (a.total * a.warps_per_job + 7) / 8;
+    FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaReadKVInt4: too many tokens");
+    const dim3 grid((unsigned)blocks), block(256);
+    if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_dependent(read_int4_kernel<__nv_bfloat16>, grid, block, 0, stream, a));
+    else FCK_CUDA(launch_dependent(read_int4_kernel<__half>, grid, block, 0, stream, a));
+    return FLASHCK_OK;
+}
+
+}  // namespace fck

@@ -179,4 +179,73 @@ struct SharedPrefixParams {
 int64_t shared_prefix_workspace(const SharedPrefixParams& p);
 int launch_shared_prefix(const SharedPrefixParams& p, cudaStream_t stream);
 
+// ---- the 4-bit cache (appendkv_int4.cu, splitkv_int4.cu) and the rotation by itself (rotary.cu) ---------------------------------------
+struct Int4Cache {
+    void* k_codes;  // uint8 [rows, hkv, d / 2]; rows: pages * page, or cache rows * capacity
+    void* k_params;  // T [rows, hkv, d / group, 2]
+    void* v_codes;
+    void* v_params;
+    const int32_t* seqlen;          // [batch]
+    const int32_t* block_table;     // [., bt_stride] or nullptr: contiguous
+    const int64_t* cache_batch_idx;
+    int64_t batch, hkv, d, group;
+    int64_t bt_stride, page;        // contiguous: page is the capacity of a row
+    int64_t pool;                   // pages of the pools, or rows of contiguous caches
+    int dtype;
+};
+struct AppendInt4Params {
+    Int4Cache cache;                // seqlen: before the append
+    const void* q;
+    void* q_out;
+    const void* knew;
+    const void* vnew;
+    void* k_held;                   // what the cache holds for the new tokens, like knew, or nullptr
+    void* v_held;
+    const int64_t* seqstart_q;
+    const int64_t* seqstart_knew;
+    const int32_t* positions;       // [axes, total_new] or nullptr: the place in the cache
+    const void* rotary_cos;
+    const void* rotary_sin;
+    const uint8_t* pair_axis;       // host memory, one entry per pair, or nullptr
+    int64_t seqlen_q, seqlen_knew, hq, axes, rotary_dim, rotary_rows;
+    int rope_type;
+};
+int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream);
+
+struct ReadInt4Params {
+    Int4Cache cache;
+    void* k;
+    void* v;
+    const int64_t* seqstart;  // of the packed output, or nullptr: [batch, tokens, hkv, d]
+    int64_t tokens;           // of the packed output, or of a row of the other
+};
+int launch_read_int4(const ReadInt4Params& p, cudaStream_t stream);
+
+struct RotaryParams {
+    const void* q;
+    void* q_out;
+    const void* k;  // or nullptr
+    void* k_out;
+    const int32_t* positions;  // [axes, tokens]
+    const void* rotary_cos;
+    const void* rotary_sin;
+    const uint8_t* pair_axis;
+    int64_t axes, tokens, hq, hkv, d, rotary_dim, rotary_rows;
+    int rope_type, inverse, dtype;
+};
+int launch_rotary(const RotaryParams& p, cudaStream_t stream);
+
+struct SplitKVInt4Params {
+    Int4Cache cache;
+    const void* q;
+    float* o_acc;    // as in SplitKVParams
+    float* lse_acc;
+    const int64_t* seqstart_q;
+    int64_t seqlen_q, max_seqlen_q, total_q, hq, num_splits;
+    float scale;
+    int mask_type;
+    int64_t wl, wr;
+};
+int launch_splitkv_int4(const SplitKVInt4Params& p, cudaStream_t stream);
+
 }  // namespace fck

@@ -439,6 +439,274 @@ PyObject* call_shared_prefix(PyObject*, PyObject* const* args, Py_ssize_t nargs)
     END_HANDLE_TH_ERRORS
 }
 
+// The tensors and sizes of a 4-bit cache, as ops.int4 checks them.
+struct Int4Args {
+    const at::Tensor *k, *kp, *v, *vp, *sl = nullptr, *bt = nullptr;
+    int64_t batch = 0, hkv = 0, d = 0, group = 0;
+
+    void read(Reader& r, at::ScalarType elem) {
+        k = r.need(at::kByte, 4);
+        kp = r.need(elem, 5);
+        v = r.need(at::kByte, 4);
+        vp = r.need(elem, 5);
+    }
+    bool fits(int64_t unit) {
+        batch = sl->numel();
+        hkv = k->size(2);
+        d = 2 * k->size(3);
+        const int64_t groups = kp->size(3);
+        if (sl->dim() != 1 || batch < 1 || hkv < 1 || (d != 64 && d != 128) || (groups != 1 && groups != 2 && groups != 4) || d / groups < 32 ||
+            kp->size(4) != 2 || kp->sizes().slice(0, 3) != k->sizes().slice(0, 3) || v->sizes() != k->sizes() || vp->sizes() != kp->sizes())
+            return false;
+        group = d / groups;
+        for (const at::Tensor* t : {k, kp, v, vp})
+            if ((uintptr_t)t->data_ptr() % 16) return false;
+        return bt ? bt->size(0) >= batch && k->size(1) % unit == 0 : k->size(0) >= batch;
+    }
+    int64_t stride() const { return bt ? bt->size(1) : 0; }
+};
+
+// sections, interleaved_sections and positions -> axes and the axis of each pair, as ops.rotary._pair_axes has them
+struct Axes {
+    int64_t axes = 1;
+    bool one = true;  // all pairs turn with the first
+    uint8_t pair[128];
+
+    static void parse(Reader& r, PyObject*& sections, bool& dealt) {
+        sections = r.next();
+        dealt = r.flag();
+    }
+    bool fill(Reader& r, PyObject* sections, bool dealt, const at::Tensor* positions, int64_t tokens, int64_t half) {
+        if (positions) {
+            axes = tokens > 0 ? positions->numel() / tokens : 1;
+            if (positions->numel() != axes * tokens || axes < 1 || axes > 4 || (axes > 1 && positions->size(0) != axes)) return false;
+        }
+        if (sections == Py_None) return axes == 1;
+        if (!PyTuple_CheckExact(sections) || PyTuple_GET_SIZE(sections) != axes || half > 128) return false;
+        int64_t left[4], sum = 0;
+        for (int64_t a = 0; a < axes; ++a) {
+            left[a] = r.integer(PyTuple_GET_ITEM(sections, a));
+            if (!r.ok || left[a] < 0 || left[a] > half) return false;
+            sum += left[a];
+        }
+        if (sum != half) return false;
+        one = false;
+        for (int64_t i = 0; i < half;)
+            for (int64_t a = 0; a < axes; ++a)
+                for (; left[a] > 0; ) {
+                    pair[i++] = (uint8_t)a;
+                    --left[a];
+                    if (dealt) break;
+                }
+        return true;
+    }
+    const void* get() const { return one ? nullptr : pair; }
+};
+
+PyObject* wrap(std::initializer_list<at::Tensor> all) {
+    PyObject* t = PyTuple_New((Py_ssize_t)all.size());
+    Py_ssize_t i = 0;
+    for (const at::Tensor& x : all) {
+        PyObject* o = nullptr;
+        if (t && x.defined()) o = THPVariable_Wrap(x);
+        else if (t) Py_INCREF(o = Py_None);
+        if (!o) {
+            Py_XDECREF(t);
+            return nullptr;
+        }
+        PyTuple_SET_ITEM(t, i++, o);
+    }
+    return t;
+}
+
+// (q | None, k_cache, k_params, v_cache, v_params, knew, vnew, seqlen_k, rotary_cos | None, rotary_sin | None, rope, rotary_dim | None,
+//  positions | None, sections | None, interleaved_sections, block_table | None, cu_seqlens_q | None, cu_seqlens_knew | None, return_kv)
+PyObject* call_append_kv_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (!plain_state()) Py_RETURN_NONE;
+    Reader r{args, nargs};
+    const at::Tensor* q = r.maybe(at::ScalarType::Undefined);
+    if (nargs < 3 || !THPVariable_CheckExact(args[2])) Py_RETURN_NONE;
+    const at::ScalarType elem = THPVariable_Unpack(args[2]).scalar_type();
+    if (elem != at::kHalf && elem != at::kBFloat16) Py_RETURN_NONE;
+    Int4Args c;
+    c.read(r, elem);
+    const at::Tensor *knew = r.need(elem), *vnew = r.need(elem);
+    c.sl = r.need(at::kInt);
+    const at::Tensor *cos = r.maybe(elem, 2), *sin = r.maybe(elem, 2);
+    const int64_t rope = r.integer();
+    PyObject* width = r.next();
+    const int64_t asked = r.ok && width != Py_None ? r.integer(width) : -1;
+    const at::Tensor* pos = r.maybe(at::kInt);
+    PyObject* sections;
+    bool dealt;
+    Axes::parse(r, sections, dealt);
+    c.bt = r.maybe(at::kInt, 2);
+    const at::Tensor *cu_q = r.maybe(at::kLong), *cu_n = r.maybe(at::kLong);
+    const bool held = r.flag();
+    if (!r.ok || r.i != nargs || (q && q->scalar_type() != elem) || !c.fits(1)) Py_RETURN_NONE;
+    if ((q && (cu_q != nullptr) != (cu_n != nullptr)) || (!q && cu_q)) Py_RETURN_NONE;
+    const int64_t dim = cu_n ? 3 : 4;
+    if (knew->dim() != dim || vnew->sizes() != knew->sizes() || knew->size(-2) != c.hkv || knew->size(-1) != c.d) Py_RETURN_NONE;
+    if (q && (q->dim() != dim || q->size(-1) != c.d)) Py_RETURN_NONE;
+    if (cu_n ? cu_n->numel() != c.batch + 1 || (cu_q && cu_q->numel() != c.batch + 1) : knew->size(0) != c.batch || (q && q->size(0) != c.batch))
+        Py_RETURN_NONE;
+    const int64_t n_new = cu_n ? knew->size(0) : knew->size(1), tokens = cu_n ? n_new : c.batch * n_new;
+    Axes axes;
+    int64_t rotary_dim = 0;
+    if (rope != 0) {
+        if (!cos || !sin || cos->sizes() != sin->sizes()) Py_RETURN_NONE;
+        rotary_dim = 2 * cos->size(1);
+        if ((width != Py_None && asked != rotary_dim) || !axes.fill(r, sections, dealt, pos, tokens, rotary_dim / 2)) Py_RETURN_NONE;
+    } else if (pos || sections != Py_None) {
+        Py_RETURN_NONE;
+    }
+    at::Tensor q_out, kh, vh;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(r.device);
+        if (q) q_out = empty(q->sizes(), elem, r.device);
+        if (held) {
+            kh = empty(knew->sizes(), elem, r.device);
+            vh = empty(knew->sizes(), elem, r.device);
+        }
+        rc = FmhaFwdAppendKVInt4(ptr(q), ptr(q_out), ptr(c.k), ptr(c.kp), ptr(knew), ptr(c.v), ptr(c.vp), ptr(vnew), ptr(kh), ptr(vh), ptr(c.sl),
+                                 (int64_t*)ptr(cu_q), (int64_t*)ptr(cu_n), ptr(pos), ptr(cos), ptr(sin), axes.get(), ptr(c.bt), nullptr, c.batch,
+                                 !q ? 0 : cu_n ? q->size(0) : q->size(1), n_new, q ? q->size(-2) : 0, c.hkv, c.d, c.group, axes.axes, rotary_dim,
+                                 cos ? cos->size(0) : 0, (int)rope, c.stride(), c.k->size(1), c.k->size(0), stream_of(r.device), dtype_code(*knew));
+    }
+    if (rc != 0) return PyLong_FromLong(rc);
+    if (held) return wrap({q_out, kh, vh});
+    if (q) return THPVariable_Wrap(q_out);
+    return PyLong_FromLong(0);
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, k_cache, k_params, v_cache, v_params, seqlen_k, block_table | None, cu_seqlens_q | None, max_seqlen_q, num_splits, scale, causal,
+//  window_size, mask_type, return_lse)
+PyObject* call_splitkv_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (!plain_state()) Py_RETURN_NONE;
+    Reader r{args, nargs};
+    const at::Tensor* q = r.need(at::ScalarType::Undefined);
+    if (!r.ok || !elem16(q)) Py_RETURN_NONE;
+    const at::ScalarType elem = q->scalar_type();
+    Int4Args c;
+    c.read(r, elem);
+    c.sl = r.need(at::kInt);
+    c.bt = r.maybe(at::kInt, 2);
+    const at::Tensor* cu_q = r.maybe(at::kLong);
+    int64_t max_q = r.integer(), splits = r.integer();
+    const double scale = r.real(true);
+    uint32_t mt;
+    int64_t wl, wr;
+    r.mask(mt, wl, wr);
+    const bool with_lse = r.flag();
+    if (!r.ok || r.i != nargs || !c.fits(16)) Py_RETURN_NONE;
+    const bool group = cu_q != nullptr;
+    if (q->dim() != (group ? 3 : 4) || q->size(-1) != c.d || (group ? cu_q->numel() != c.batch + 1 : q->size(0) != c.batch)) Py_RETURN_NONE;
+    const int64_t hq = q->size(-2), sq = q->size(-3), bs = group ? 1 : c.batch;
+    if (q->numel() == 0 || hq % c.hkv != 0 || c.k->numel() == 0 || (uintptr_t)q->data_ptr() % 16) Py_RETURN_NONE;
+    max_q = group && max_q > 0 ? std::min(max_q, sq) : sq;
+    if (splits <= 0) splits = num_splits_for(c.batch, 1);
+    at::Tensor o, lse, work;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(r.device);
+        void* stream = stream_of(r.device);
+        // one workspace: the partial rows, then their LSEs
+        const int64_t rows = bs * hq * splits * sq;
+        work = empty({rows * (c.d + 1)}, at::kFloat, r.device);
+        float* o_acc = (float*)work.data_ptr();
+        float* lse_acc = o_acc + rows * c.d;
+        rc = FmhaFwdSplitKVInt4(ptr(q), ptr(c.k), ptr(c.kp), ptr(c.v), ptr(c.vp), lse_acc, o_acc, (int64_t*)ptr(cu_q), ptr(c.sl), ptr(c.bt), nullptr,
+                                c.batch, sq, max_q, hq, c.hkv, c.d, c.group, splits, c.stride(), c.k->size(1), c.k->size(0), (float)scale, wl, wr,
+                                mt, stream, dtype_code(*q));
+        if (rc == 0) {
+            o = empty(q->sizes(), elem, r.device);
+            if (with_lse) lse = group ? empty({hq, sq}, at::kFloat, r.device) : empty({c.batch, hq, sq}, at::kFloat, r.device);
+            rc = FmhaFwdSplitKVCombine(lse_acc, o_acc, ptr(o), nullptr, bs, sq, hq, c.d, sq, splits, stream, ptr(lse), dtype_code(*q));
+            if (rc != 0) rc = -rc;  // (which of the two calls it was)
+        }
+    }
+    return result(rc, o, lse);
+    END_HANDLE_TH_ERRORS
+}
+
+// (k_cache, k_params, v_cache, v_params, seqlen_k, block_table | None, cu_seqlens_k | None, total_k | None, max_seqlen_k | None)
+PyObject* call_read_kv_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (!plain_state()) Py_RETURN_NONE;
+    Reader r{args, nargs};
+    if (nargs < 2 || !THPVariable_CheckExact(args[1])) Py_RETURN_NONE;
+    const at::ScalarType elem = THPVariable_Unpack(args[1]).scalar_type();
+    if (elem != at::kHalf && elem != at::kBFloat16) Py_RETURN_NONE;
+    Int4Args c;
+    c.read(r, elem);
+    c.sl = r.need(at::kInt);
+    c.bt = r.maybe(at::kInt, 2);
+    const at::Tensor* cu = r.maybe(at::kLong);
+    PyObject *total = r.next(), *most = r.next();
+    if (!r.ok || r.i != nargs || !c.fits(1) || (cu != nullptr) != (total != Py_None) || (cu != nullptr) == (most != Py_None)) Py_RETURN_NONE;
+    const int64_t tokens = r.integer(cu ? total : most);
+    if (!r.ok || tokens < 0 || (cu && cu->numel() != c.batch + 1)) Py_RETURN_NONE;
+    at::Tensor k, v;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(r.device);
+        if (cu) {
+            k = empty({tokens, c.hkv, c.d}, elem, r.device);
+            v = empty({tokens, c.hkv, c.d}, elem, r.device);
+        } else {
+            k = empty({c.batch, tokens, c.hkv, c.d}, elem, r.device);
+            v = empty({c.batch, tokens, c.hkv, c.d}, elem, r.device);
+        }
+        rc = FmhaReadKVInt4(ptr(c.k), ptr(c.kp), ptr(c.v), ptr(c.vp), ptr(k), ptr(v), ptr(c.sl), (int64_t*)ptr(cu), ptr(c.bt), nullptr, c.batch, tokens,
+                            c.hkv, c.d, c.group, c.stride(), c.k->size(1), c.k->size(0), stream_of(r.device), dtype_code(*c.kp));
+    }
+    return rc != 0 ? PyLong_FromLong(rc) : wrap({k, v});
+    END_HANDLE_TH_ERRORS
+}
+
+// (q, k | None, positions, rotary_cos, rotary_sin, sections | None, interleaved_sections, rope, inverse) -> (q, k | None)
+PyObject* call_rotary(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    HANDLE_TH_ERRORS
+    if (!plain_state()) Py_RETURN_NONE;
+    Reader r{args, nargs};
+    const at::Tensor* q = r.need(at::ScalarType::Undefined);
+    if (!r.ok || !elem16(q)) Py_RETURN_NONE;
+    const at::ScalarType elem = q->scalar_type();
+    const at::Tensor *k = r.maybe(elem, q->dim()), *pos = r.need(at::kInt), *cos = r.need(elem, 2), *sin = r.need(elem, 2);
+    PyObject* sections;
+    bool dealt;
+    Axes::parse(r, sections, dealt);
+    const int64_t rope = r.integer();
+    const bool inverse = r.flag();
+    if (!r.ok || r.i != nargs || q->dim() < 3 || (rope != 1 && rope != 2)) Py_RETURN_NONE;
+    const int64_t hq = q->size(-2), d = q->size(-1), lead = q->dim() - 2;
+    if (k && (k->sizes().slice(0, lead) != q->sizes().slice(0, lead) || k->size(-1) != d)) Py_RETURN_NONE;
+    int64_t tokens = 1;
+    for (int64_t i = 0; i < lead; ++i) tokens *= q->size(i);
+    if (cos->sizes() != sin->sizes() || 2 * cos->size(1) > d) Py_RETURN_NONE;
+    Axes axes;
+    if (!axes.fill(r, sections, dealt, pos, tokens, cos->size(1))) Py_RETURN_NONE;
+    at::Tensor q_out, k_out;
+    int rc;
+    {
+        pybind11::gil_scoped_release no_gil;
+        const c10::cuda::CUDAGuard guard(r.device);
+        q_out = empty(q->sizes(), elem, r.device);
+        if (k) k_out = empty(k->sizes(), elem, r.device);
+        rc = FmhaRotary(ptr(q), ptr(q_out), ptr(k), ptr(k_out), ptr(pos), ptr(cos), ptr(sin), axes.get(), axes.axes, tokens, hq, k ? k->size(-2) : 0, d,
+                        2 * cos->size(1), cos->size(0), (int)rope, inverse, stream_of(r.device), dtype_code(*q));
+    }
+    return rc != 0 ? PyLong_FromLong(rc) : wrap({q_out, k_out});
+    END_HANDLE_TH_ERRORS
+}
+
 // (leaf) -> whether its gradient is accumulated on the default stream: where the node that does it was made, which need not be by a
 // call of this package
 PyObject* accumulates_on_default_stream(PyObject*, PyObject* leaf) {
@@ -464,6 +732,10 @@ PyMethodDef methods[] = {
     {"_call_append_kv", (PyCFunction)(void (*)(void))call_append_kv, METH_FASTCALL, nullptr},
     {"_call_backward", (PyCFunction)(void (*)(void))call_backward, METH_FASTCALL, nullptr},
     {"_call_shared_prefix", (PyCFunction)(void (*)(void))call_shared_prefix, METH_FASTCALL, nullptr},
+    {"_call_append_kv_int4", (PyCFunction)(void (*)(void))call_append_kv_int4, METH_FASTCALL, nullptr},
+    {"_call_splitkv_int4", (PyCFunction)(void (*)(void))call_splitkv_int4, METH_FASTCALL, nullptr},
+    {"_call_read_kv_int4", (PyCFunction)(void (*)(void))call_read_kv_int4, METH_FASTCALL, nullptr},
+    {"_call_rotary", (PyCFunction)(void (*)(void))call_rotary, METH_FASTCALL, nullptr},
     {"_accumulates_on_default_stream", (PyCFunction)accumulates_on_default_stream, METH_O, nullptr},
     {"_num_splits", (PyCFunction)(void (*)(void))num_splits, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},

@@ -1,0 +1,81 @@
+// Rotation of queries and keys by the positions of their tokens, along one or several axes (int4.cuh has the arithmetic).
+//
+// Bound by its traffic: each row read and written once.  A lane holds 8 channels of a head and keeps its cosines and sines for all heads
+// of the token; a half-rotated pair's other half is read a second time, from L1.
+#include <algorithm>
+#include <type_traits>
+
+#include "int4.cuh"
+
+namespace fck {
+
+namespace {
+
+struct RotaryCall {
+    RotaryDev rot;
+    const void* src[2];  // q, k
+    void* dst[2];
+    const int32_t* positions;
+    int64_t tokens;
+    int heads[2], d, warps_per_job;
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall a) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int w = a.warps_per_job, lane = threadIdx.x & 31;
+    const int64_t t = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
+    const int part = (threadIdx.x >> 5) % w;
+    if (t >= a.tokens) return;
+    auto pos = [&](int axis) -> int64_t { return a.positions[axis * a.tokens + t]; };
+    const int pieces = a.d >> 3;
+    for (int i = 0; i < 2; ++i) {
+        const T* src = (const T*)a.src[i] + t * a.heads[i] * a.d;
+        T* dst = (T*)a.dst[i] + t * a.heads[i] * a.d;
+        for (int p = part * 32 + lane; p < a.heads[i] * pieces; p += w * 32) {
+            const int h = p / pieces, e0 = (p - h * pieces) << 3;
+            const T* row = src + (int64_t)h * a.d;
+            Vec8<T> x, out;
+            if (a.rot.vec) {
+                Vec8<T> y;
+                x.v = *reinterpret_cast<const uint4*>(row + e0);
+                y.v = *reinterpret_cast<const uint4*>(row + partner_of(a.rot, e0));
+                turn_piece<T>(a.rot, e0, pos, x, y, out);
+                *reinterpret_cast<uint4*>(dst + (int64_t)h * a.d + e0) = out.v;
+            } else {
+                turn_piece_any<T>(a.rot, e0, pos, row, out);
+                for (int k = 0; k < 8; ++k) dst[(int64_t)h * a.d + e0 + k] = out.e[k];
+            }
+        }
+    }
+}
+
+}  // namespace
+
+int launch_rotary(const RotaryParams& p, cudaStream_t stream) {
+    FCK_REQUIRE(p.d > 0 && p.d % 8 == 0 && p.d <= 1024, FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: hdim must be a multiple of 8, at most 1024 (got %lld)",
+                (long long)p.d);
+    FCK_REQUIRE(p.rope_type != 0, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaRotary: rope_type must be 1 or 2");
+    FCK_REQUIRE(p.hq <= 65536 && p.hkv <= 65536, FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: at most 65536 heads");
+    RotaryCall a{};
+    const auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
+    if (int rc = fill_rotary("FmhaRotary", a.rot, p.rotary_cos, p.rotary_sin, p.rotary_rows, p.rotary_dim, p.d, p.rope_type, p.pair_axis, p.axes,
+                             aligned(p.q) && aligned(p.q_out) && aligned(p.k) && aligned(p.k_out))) return rc;
+    a.rot.back = p.inverse != 0;
+    a.src[0] = p.q; a.src[1] = p.k; a.dst[0] = p.q_out; a.dst[1] = p.k_out;
+    a.positions = p.positions; a.tokens = p.tokens; a.d = (int)p.d;
+    a.heads[0] = (int)p.hq; a.heads[1] = p.k ? (int)p.hkv : 0;
+    if (p.tokens == 0 || a.heads[0] + a.heads[1] == 0) return FLASHCK_OK;
+    const int64_t most = std::max<int64_t>(1, (p.hq + a.heads[1]) * p.d / 256);
+    int w = 8;
+    while (w > 1 && (w > most || p.tokens * w > (int64_t)sm_count() * 32)) w >>= 1;
+    a.warps_per_job = w;
+    const int64_t blocks = (p.tokens * w + 7) / 8;
+    FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: too many tokens");
+    if (p.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_dependent(rotary_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0, stream, a));
+    else FCK_CUDA(launch_dependent(rotary_kernel<__half>, dim3((unsigned)blocks), dim3(256), 0, stream, a));
+    return FLASHCK_OK;
+}
+
+}  // namespace fck

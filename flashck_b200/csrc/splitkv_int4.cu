@@ -1,0 +1,814 @@
+// fmha_fwd_splitkv over a 4-bit cache: partial attention of a few query rows per kv head, one partial (O_s, LSE_s) per split.
+//
+// A token of a kv head is d codes u (4 bits) and, for each group of channels, (scale s, least value m):  k_c = m + s u_c.  So
+//     q . k = sum_g ( s_g sum_{c in g} q_c u_c  +  m_g sum_{c in g} q_c ),
+//     O_c   = sum_j p_j (m_j + s_j u_jc) = sum_j (p_j s_j) (u_jc - 8)  +  sum_j p_j (m_j + 8 s_j),
+// and no key or value is ever written out: the products run over the codes themselves, scales and least values come in once per key.
+// The second sum of O is one number per row and group; with 8 taken off, what the rounding of p s to 16 bits costs is in proportion to
+// the values' spread, not to their distance from the least one (the rounded weights are summed by an MMA against ones for it).
+//
+// Codes become MMA operands in 0.6 (K) and 0.75 (V) instructions each: a 4-bit field in the low mantissa bits of a half IS u * 2^-24 (a
+// subnormal, which the tensor cores multiply exactly), one four bits higher u * 2^-20; so a mask gives two operands, a shift by 8 the next
+// two, and the powers of two go to Q, or to O at the end.  Two keys' codes of one channel are put side by side by one byte permutation.
+// Both products are taken transposed (S^T = K Q^T, O^T = V^T P^T): m16n8k16 then has 16 keys or channels against 8 query rows, which a
+// group of 4 or 8 heads fills, instead of 16 rows half empty.  P^T's fragments come from S^T's by movmatrix.
+//
+// Halves have no range for arbitrary Q and scales.  A row of Q is scaled by a power of two.  The weights p s are kept in range by the row's
+// reference R (p' = exp2(x - R)): it follows the largest x + log2 s seen, moves when a weight passes 2^13, and then everything the row
+// has summed is rescaled.  Moves are rare, and what decides one is a maximum over packed halves and a vote, without a shuffle.
+//
+// Bound by the cache's bytes in HBM: 136 a token and head at hdim 128 with one group, for 370 issue slots of an SM's four schedulers per 16
+// keys, of which about half are used.  A CTA per SM: a producer warp and 8 or 16 consumer warps.  A stage is 256 (head, token) pairs --
+// 32 tokens of 8 heads, 256 of one -- of K and V codes, by TMA (boxes of up to 256 tokens of a page, 64- or 32-byte swizzle: a warp's reads
+// meet no bank twice), and their scales, by 4- to 16-byte asynchronous copies.  8 consumer warps take 32 tokens of one head each; with 16,
+// two teams take stages in turn.  The warps of a head meet once per segment, in shared memory.  The work is cut as in splitkv_decode.cu.
+#include <algorithm>
+#include <type_traits>
+
+#include "kernels.h"
+
+namespace fck {
+
+namespace {
+
+constexpr int kPairs = 256;  // (head, token) pairs of a stage
+constexpr int kUnit = 32;    // tokens a warp takes of it
+constexpr int kCentre = 4;   // units between two centrings
+constexpr uint32_t kLowCodes = 0x000f000fu, kHighCodes = 0x00f000f0u;
+
+struct Int4Dev {
+    const void* q;
+    float* o_acc;
+    float* lse_acc;
+    const int64_t* seqstart_q;
+    const int32_t* seqlen_k;
+    const int32_t* block_table;
+    const int64_t* cache_batch_idx;
+    const uint8_t* k_params;
+    const uint8_t* v_params;
+    int* status;
+    int batch, seqlen_q, hq, hkv, num_splits, total_q, bt_stride, page, pool, room;  // room: tokens that a sequence's part of the cache has
+    int mask_type, wl, wr;
+    int heads_log2, chunk_log2, stages;  // kv heads of a CTA; tokens of a box
+    float scale_log2;
+};
+
+__device__ __forceinline__ int len_q(const Int4Dev& p, int b) {
+    return p.seqstart_q ? (int)(p.seqstart_q[b + 1] - p.seqstart_q[b]) : p.seqlen_q;
+}
+__device__ __forceinline__ int len_k(const Int4Dev& p, int b) { return min(p.seqlen_k[b], p.room); }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
+}
+__device__ __forceinline__ void arrive_after_copies(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint32_t halves(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Shared memory of a stage: K codes, V codes, K params, V params [heads][tokens + 1][NG] (the extra entry keeps the producer's lanes, which
+// walk the heads, off one bank).
+template <int D, int NG>
+struct Stage {
+    static constexpr int kCodes = kPairs * (D / 2);
+    static constexpr int kParams = (kPairs + 8) * NG * 4;
+    static constexpr int kBytes = (2 * kCodes + 2 * kParams + 1023) / 1024 * 1024;
+};
+
+// What one warp has summed over its keys, for rows 2t and 2t + 1 (t = lane % 4) of each of NT tiles of 8 rows.
+template <int D, int NG, int NT>
+struct Sums {
+    float o[NT][D / 32][2][4];  // sum w u, w = p' s, over 2^24 ([0]: channels 4g, 4g + 2) or 2^20 ([1]: 4g + 1, 4g + 3 of 32)
+    float ones[NT][NG][4];      // sum w since the last centring (entries 0 and 1; the fragment's lower rows repeat them)
+    float mid[NT][NG][2];       // sum p' (m + 8 s) over the lane's keys
+    float l[NT][2];             // sum p' over the lane's keys
+    float m[NT][2], j[NT][2], ref[NT][2];  // largest x, largest x + log2 s, and R at its last move
+};
+
+template <typename T, int D, int NG, int NT, int TEAMS>
+__global__ void __launch_bounds__((8 * TEAMS + 1) * 32, 1)
+splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Int4Dev p) {
+    constexpr int ROW = D / 2, GR = D / 32, PER = GR / NG;  // bytes of a row; 16-byte pieces (32 channels) of it; of them per group
+    constexpr int kConsumers = 8 * TEAMS;
+    using St = Stage<D, NG>;
+    extern __shared__ uint8_t smem_raw[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int G = p.hq / p.hkv, stages = p.stages;
+    const int heads = 1 << p.heads_log2, tok_log2 = 8 - p.heads_log2, toks = 1 << tok_log2;
+
+    uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+    float4* meet = reinterpret_cast<float4*>(ring + (size_t)stages * St::kBytes);  // [4 TEAMS or 8][row pair floats]: the warps' sums
+    constexpr int kMeetWarps = TEAMS == 2 ? 8 : 4, kMeetFloat4 = NT * 2 * GR;      // float4 per lane
+    float* meet_stats = reinterpret_cast<float*>(meet + kMeetWarps * kMeetFloat4 * 32);  // [warp][NT][2][8 rows: ref, l]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(meet_stats + kMeetWarps * NT * 16);
+    uint64_t* full = bars;
+    uint64_t* empty = bars + stages;
+    int* prefix = reinterpret_cast<int*>(bars + 2 * stages);  // [batch + 1] tiles before each sequence
+    int* tile0 = prefix + p.batch + 1;
+    volatile int* abort_flag = tile0 + p.batch;
+    int* longest = const_cast<int*>(abort_flag) + 1;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < stages; ++s) {
+            mbar_init(&full[s], 33);  // the lanes' copies of scales, and the byte count of the boxes
+            mbar_init(&empty[s], 8);
+        }
+        *abort_flag = 0;
+        mbar_fence_init();
+    }
+    pdl_launch_dependents();
+    pdl_wait();
+    // ---- schedule: tiles (stages) per sequence and their prefix sums ----
+    if (warp == 0) {
+        int run = 0, mx = 0;
+        for (int base = 0; base < p.batch; base += 32) {
+            const int b = base + lane;
+            int n = 0, t0 = 0;
+            if (b < p.batch) {
+                const int len = len_k(p, b);
+                if (len > 0) {
+                    int first = 0;
+                    if (p.mask_type != 0 && p.wl >= 0) first = max(0, min(len - 1, (p.mask_type == 2 ? len - len_q(p, b) : 0) - p.wl));
+                    t0 = first >> tok_log2;
+                    n = ((len - 1) >> tok_log2) + 1 - t0;
+                }
+                tile0[b] = t0;
+            }
+            int incl = n;
+#pragma unroll
+            for (int off = 1; off < 32; off <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, incl, off);
+                if (lane >= off) incl += y;
+            }
+            if (b < p.batch) prefix[b] = run + incl - n;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+            mx = max(mx, __reduce_max_sync(0xffffffffu, n));
+        }
+        if (lane == 0) {
+            prefix[p.batch] = run;
+            *longest = mx;
+        }
+    }
+    __syncthreads();
+
+    const int total = prefix[p.batch];
+    const bool per_sequence = p.num_splits <= 1;
+    const int even = (total + (int)gridDim.x - 1) / (int)gridDim.x;
+    const int cap = per_sequence ? 0 : (*longest + p.num_splits - 2) / (p.num_splits - 1);
+    const int piece_len = max(1, max(even, cap));
+    const int pieces = per_sequence ? p.batch : (total + piece_len - 1) / piece_len;
+    auto begin_piece = [&](int piece, int& lo, int& hi) {  // its tiles, and the sequence it starts in
+        if (per_sequence) {
+            lo = prefix[piece];
+            hi = prefix[piece + 1];
+            return piece;
+        }
+        lo = piece * piece_len;
+        hi = min(total, lo + piece_len);
+        int a = 0, z = p.batch - 1;
+        while (a < z) {
+            const int mid = (a + z + 1) >> 1;
+            if (prefix[mid] <= lo) a = mid; else z = mid - 1;
+        }
+        return a;
+    };
+    const int head0 = blockIdx.z << p.heads_log2;
+    const int row0 = blockIdx.y * 8 * NT;  // first (token, group head) row of this CTA's tiles
+
+    if (warp == kConsumers) {
+        // =========================== producer warp ===========================================
+        if (lane == 0) {
+            tma_prefetch_desc(&map_k);
+            tma_prefetch_desc(&map_v);
+        }
+        const int chunk = 1 << p.chunk_log2, box = heads * chunk * ROW;
+        uint32_t it = 0;
+        bool ok = true;
+        for (int piece = blockIdx.x; piece < pieces && ok; piece += gridDim.x) {
+            int lo, hi, b = begin_piece(piece, lo, hi);
+            for (; b < p.batch && prefix[b] < hi && ok; ++b) {
+                const int ta = max(lo, prefix[b]) - prefix[b], tb = min(hi, prefix[b + 1]) - prefix[b];
+                if (tb <= ta || row0 >= len_q(p, b) * G) continue;  // (the consumers skip the same segments)
+                const int len = len_k(p, b);
+                const int64_t bphys = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
+                // lane c looks after chunk c of a tile (at most 16), one tile ahead: its page, or one that is not there
+                auto entry = [&](int t, int& pg, int& tok) {
+                    const int token = ((tile0[b] + t) << tok_log2) + (lane << p.chunk_log2);
+                    pg = p.pool;
+                    tok = 0;
+                    if (t >= tb || token >= len || lane >= (toks >> p.chunk_log2)) return;
+                    if (p.block_table) {
+                        const int slot = token / p.page;
+                        tok = token - slot * p.page;
+                        const int id = slot < p.bt_stride ? p.block_table[bphys * p.bt_stride + slot] : -1;
+                        if ((uint32_t)id < (uint32_t)p.pool) pg = id;
+                    } else {
+                        tok = token;
+                        if ((uint64_t)bphys < (uint64_t)p.pool) pg = (int)bphys;
+                    }
+                };
+                int pg_next, tok_next;
+                entry(ta, pg_next, tok_next);
+                for (int t = ta; t < tb; ++t, ++it) {
+                    const int pg = pg_next, tok = tok_next, s = it % stages;
+                    entry(t + 1, pg_next, tok_next);
+                    const int token0 = (tile0[b] + t) << tok_log2;
+                    const int chunks = min(toks >> p.chunk_log2, (len - token0 + chunk - 1) >> p.chunk_log2);
+                    if (!mbar_wait_bounded(&empty[s], ((it / stages) & 1u) ^ 1u, abort_flag, p.status, 0x100)) { ok = false; break; }
+                    uint8_t* st = ring + (size_t)s * St::kBytes;
+                    if (lane == 0) mbar_expect_tx(&full[s], 2 * chunks * box);
+                    __syncwarp();
+                    if (lane < chunks) {
+                        tma_load_4d(st + lane * box, &map_k, &full[s], 0, tok, head0, pg);
+                        tma_load_4d(st + St::kCodes + lane * box, &map_v, &full[s], 0, tok, head0, pg);
+                    }
+                    const int64_t at = pg < p.pool ? (int64_t)pg * p.page + tok : -1;  // row of the chunk's first token
+                    const uint32_t dst = smem_u32(st + 2 * St::kCodes);
+#pragma unroll
+                    for (int i = 0; i < kPairs / 32; ++i) {
+                        const int e = i * 32 + lane, k = e >> p.heads_log2, h = e & (heads - 1);  // token of the tile, head of the CTA
+                        const int64_t row = __shfl_sync(0xffffffffu, at, k >> p.chunk_log2);
+                        const bool there = row >= 0 && token0 + k < len;  // (the rest of a tile has scales of zero)
+                        const int64_t off = there ? ((row + (k & (chunk - 1))) * p.hkv + head0 + h) * (4 * NG) : 0;
+                        const uint32_t to = dst + (h * (toks + 1) + k) * (4 * NG);
+                        copy_async<4 * NG>(to, p.k_params + off, there);
+                        copy_async<4 * NG>(to + St::kParams, p.v_params + off, there);
+                    }
+                    arrive_after_copies(&full[s]);
+                }
+            }
+        }
+        // ---- unused splits get LSE = -inf (see splitkv_decode.cu: shared out over gridDim.x / batch CTAs) ----
+        if (ok && blockIdx.y == 0 && blockIdx.z == 0) {
+            const int parts = max(1, (int)gridDim.x / p.batch), part = parts > 1 ? (int)blockIdx.x / p.batch : 0;
+            for (int b = parts > 1 ? (int)blockIdx.x % p.batch : (int)blockIdx.x; b < p.batch && part < parts; b += gridDim.x) {
+                const int n = prefix[b + 1] - prefix[b];
+                const int used = n == 0 ? 0 : per_sequence ? 1 : (prefix[b + 1] - 1) / piece_len - prefix[b] / piece_len + 1;
+                const int sq = len_q(p, b);
+                const int64_t rows = p.seqstart_q ? p.total_q : p.seqlen_q, head = p.num_splits * rows;  // LSEs of a split, of a head
+                float* first = p.lse_acc + (p.seqstart_q ? p.seqstart_q[b] : (int64_t)b * p.hq * head) + used * rows;
+                for (int e = lane; e < (p.num_splits - used) * sq; e += 32) {
+                    const int s = e / sq;
+                    float* at = first + s * rows + (e - s * sq);
+                    for (int h = part; h < p.hq; h += parts) at[h * head] = -INFINITY;
+                }
+            }
+        }
+        // Copies of its own end before the warp does: of the small ones always, and after a wait that ran out, when no consumer may have
+        // waited for them, of the boxes too.
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+        if (*abort_flag) {
+            for (uint32_t u = it > (uint32_t)stages ? it - stages : 0; u < it; ++u)
+                for (int k = 0; k < 100000 && !mbar_try_wait_hint(&full[u % stages], (u / stages) & 1u, 2000u); ++k) {}
+        }
+        return;
+    }
+
+    // =============================== consumer warps =============================================
+    const int team = warp >> 3, wi = warp & 7;
+    const int hw = wi & (heads - 1), unit = wi >> p.heads_log2;  // head of the CTA; which 32 tokens of a tile
+    const int kh = head0 + hw;
+    const int g = lane >> 2, t4 = lane & 3;
+    // Keys are taken in an order in which neither the K reads (row kap(g)) nor the V reads (rows kap(2t), kap(2t + 1)) meet a bank twice.
+    auto kap = [](int i) { const int x = i & 3; return (i & 4) | (x == 0 ? 0 : x == 1 ? 3 : x == 2 ? 1 : 2); };
+    auto swizzle = [](int row) { return D == 128 ? (row >> 1) & 3 : (row >> 2) & 1; };  // of a row's 16-byte pieces, as the boxes have it
+    const int kkey = kap(g), vkey0 = kap(2 * t4), vkey1 = kap(2 * t4 + 1);
+    int koff[GR], voff0[GR], voff1[GR];
+#pragma unroll
+    for (int i = 0; i < GR; ++i) {
+        koff[i] = kkey * ROW + ((i ^ swizzle(kkey)) << 4) + t4 * 4;
+        voff0[i] = vkey0 * ROW + ((i ^ swizzle(vkey0)) << 4) + (g >> 1) * 4;
+        voff1[i] = vkey1 * ROW + ((i ^ swizzle(vkey1)) << 4) + (g >> 1) * 4;
+    }
+    const uint32_t pick = (g & 1) ? 0x7632u : 0x5410u;  // the 16-bit half of a word of V codes that is this lane's
+    bool failed = false;
+    uint32_t it = 0;
+
+    for (int piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+        int lo, hi, b = begin_piece(piece, lo, hi);
+        for (; b < p.batch && prefix[b] < hi; ++b) {
+            const int ta = max(lo, prefix[b]) - prefix[b], tb = min(hi, prefix[b + 1]) - prefix[b];
+            const int sq = len_q(p, b), rows = sq * G;
+            if (tb <= ta || row0 >= rows) continue;
+            const int len = len_k(p, b);
+            const int split = per_sequence ? 0 : piece - prefix[b] / piece_len;
+            const int64_t q0 = p.seqstart_q ? p.seqstart_q[b] : (int64_t)b * p.seqlen_q;
+
+            // ---- Q^T fragments: this lane has channels 32 i + 8 t .. + 7 of row g, as halves scaled by a power of two ----
+            uint32_t qf[NT][GR][4];
+            float ka[NT][2], kb[NT][NG][2];  // x = ka * (s . a) + kb . m for rows 2t and 2t + 1
+            int key_lo[NT][2], key_hi[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int r = row0 + 8 * n + g, i = r / G;
+                float x[GR][8], amax = 0.f;
+                const T* src = (const T*)p.q + ((q0 + i) * p.hq + kh * G + (r - i * G)) * D + 8 * t4;
+#pragma unroll
+                for (int c = 0; c < GR; ++c) {
+                    uint4 w = make_uint4(0, 0, 0, 0);
+                    if (r < rows) w = *reinterpret_cast<const uint4*>(src + 32 * c);
+                    const T* e = reinterpret_cast<const T*>(&w);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        x[c][k] = Elem<T>::to_f32(e[k]);
+                        amax = fmaxf(amax, fabsf(x[c][k]));
+                    }
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                // largest magnitude into [2^13, 2^14): with it the /16 of half of the channels and 2^-24 of the rest stay exact
+                const int ex = amax > 0.f ? max(-100, min(100, (int)((__float_as_uint(amax) >> 23) & 255) - 127)) : 13;
+                const float up = __uint_as_float((uint32_t)(127 + 13 - ex) << 23), down = __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
+                float sum[NG];
+#pragma unroll
+                for (int k = 0; k < NG; ++k) sum[k] = 0.f;
+#pragma unroll
+                for (int c = 0; c < GR; ++c) {
+                    __half h[8];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        h[k] = __float2half_rn(x[c][k] * up);
+                        sum[c / PER] += __half2float(h[k]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const __half2 two = __halves2half2(h[k], h[k + 4]);
+                        const __half2 v = (k & 1) ? __hmul2(two, __float2half2_rn(0.0625f)) : two;
+                        qf[n][c][k] = *reinterpret_cast<const uint32_t*>(&v);
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < NG; ++k) {
+                    sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+                    sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int from = (2 * t4 + e) * 4;  // a lane of row 2t + e
+                    const float scale = p.scale_log2 * __shfl_sync(0xffffffffu, down, from);
+                    ka[n][e] = scale * 16777216.f;
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) kb[n][k][e] = scale * __shfl_sync(0xffffffffu, sum[k], from);
+                    const int re = row0 + 8 * n + 2 * t4 + e;
+                    visible_range(re / G, sq, len, p.mask_type, p.wl, p.wr, key_lo[n][e], key_hi[n][e]);
+                    if (re >= rows) { key_lo[n][e] = 0; key_hi[n][e] = len - 1; }
+                }
+            }
+            int mask_from = len;  // first key that some row may not see
+            if (p.mask_type != 0) {
+                if (p.wr >= 0) mask_from = min(mask_from, (p.mask_type == 2 ? len - sq : 0) + p.wr + 1);
+                if (p.wl >= 0) mask_from = 0;
+            }
+
+            Sums<D, NG, NT> z;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int c = 0; c < GR; ++c)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z.o[n][c][e >> 2][e & 3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.ones[n][k][2] = z.ones[n][k][3] = z.mid[n][k][0] = z.mid[n][k][1] = 0.f;
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    z.l[n][e] = z.ref[n][e] = 0.f;
+                    z.m[n][e] = z.j[n][e] = -INFINITY;
+                }
+            }
+
+            // 8 times the weights' sum taken off the sums of codes.  Tensor cores cut the sums of their products off instead of rounding them;
+            // codes are never negative, so uncentred sums grow with the keys and lose on one side (4 x 524288 keys: O 0.9 % off), which
+            // centring every 128 keys prevents.
+            auto centre = [&]() {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                    for (int c = 0; c < GR; ++c)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            z.o[n][c][0][e] = fmaf(-8.f / 16777216.f, z.ones[n][c / PER][e & 1], z.o[n][c][0][e]);
+                            z.o[n][c][1][e] = fmaf(-8.f / 1048576.f, z.ones[n][c / PER][e & 1], z.o[n][c][1][e]);
+                        }
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.ones[n][k][2] = z.ones[n][k][3] = 0.f;
+                }
+            };
+            bool first = true;
+            int uncentred = 0;  // units
+            for (int t = ta; t < tb; ++t, ++it) {
+                if (TEAMS == 2 && (int)(it & 1u) != team) continue;
+                const int s = it % stages;
+                if (failed || !mbar_wait_bounded(&full[s], (it / stages) & 1u, abort_flag, p.status, 0x200)) { failed = true; continue; }
+                const int key0 = ((tile0[b] + t) << tok_log2) + unit * kUnit;
+                if (key0 < len) {
+                    const uint8_t* st = ring + (size_t)s * St::kBytes;
+                    const uint8_t* pk = st + 2 * St::kCodes + (hw * (toks + 1) + unit * kUnit) * (4 * NG);
+                    // 16-key blocks of this unit: chunks of 16 tokens or more, [chunk][head][token] rows
+                    const uint8_t* block[2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int k = unit * kUnit + 16 * u, c = k >> p.chunk_log2;
+                        block[u] = st + ((((c << p.heads_log2) + hw) << p.chunk_log2) + (k & ((1 << p.chunk_log2) - 1))) * ROW;
+                    }
+                    const bool masked = key0 + kUnit > mask_from;
+                    auto visible = [&](int n, int e, int key) { return key >= key_lo[n][e] && key <= key_hi[n][e]; };
+                    // scale and least value of the lane's key kkey + 8 i of the unit
+                    auto param = [&](const uint8_t* base, int i, int k, float& sc, float& least) {
+                        const uint32_t w = reinterpret_cast<const uint32_t*>(base)[(kkey + 8 * i) * NG + k];
+                        sc = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[0]);
+                        least = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[1]);
+                    };
+                    // ---- x = log2(e) scale q . k, [n][4 keys][2 rows] ----
+                    float x[NT][4][2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        float a[NT][NG][4];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int k = 0; k < NG; ++k) a[n][k][0] = a[n][k][1] = a[n][k][2] = a[n][k][3] = 0.f;
+#pragma unroll
+                        for (int c = 0; c < GR; ++c) {
+                            uint32_t w0 = *reinterpret_cast<const uint32_t*>(block[u] + koff[c]);
+                            uint32_t w1 = *reinterpret_cast<const uint32_t*>(block[u] + koff[c] + 8 * ROW);
+                            const uint32_t f0[4] = {w0 & kLowCodes, w1 & kLowCodes, w0 & kHighCodes, w1 & kHighCodes};
+                            w0 >>= 8;
+                            w1 >>= 8;
+                            const uint32_t f1[4] = {w0 & kLowCodes, w1 & kLowCodes, w0 & kHighCodes, w1 & kHighCodes};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                mma_16816<__half>(a[n][c / PER], f0, qf[n][c][0], qf[n][c][1]);
+                                mma_16816<__half>(a[n][c / PER], f1, qf[n][c][2], qf[n][c][3]);
+                            }
+                        }
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float sc[NG], least[NG];
+#pragma unroll
+                            for (int k = 0; k < NG; ++k) param(pk, 2 * u + i, k, sc[k], least[k]);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    float y = 0.f, v = 0.f;
+#pragma unroll
+                                    for (int k = 0; k < NG; ++k) {
+                                        y = fmaf(sc[k], a[n][k][2 * i + e], y);
+                                        v = fmaf(least[k], kb[n][k][e], v);
+                                    }
+                                    x[n][2 * u + i][e] = fmaf(y, ka[n][e], v);
+                                }
+                        }
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e)
+                                    if (!visible(n, e, key0 + kkey + 8 * i)) x[n][i][e] = -INFINITY;
+                    }
+                    // ---- weights, in the row's reference; the second round is the one after it has moved ----
+                    float vs[4][NG], vm[4][NG];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) param(pk + St::kParams, i, k, vs[i][k], vm[i][k]);
+                    float pr[NT][4][2];
+                    uint32_t wt[NT][NG][4];
+#pragma unroll 1
+                    for (int round = 0;; ++round) {
+                        bool moves = first;
+                        uint32_t most = 0;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            float sum = 0.f;
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    pr[n][i][e] = fast_exp2(x[n][i][e] - z.ref[n][e]);
+                                    sum += pr[n][i][e];
+                                }
+                            moves |= sum > 1e27f;
+#pragma unroll
+                            for (int k = 0; k < NG; ++k)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    float w0 = pr[n][i][0] * vs[i][k], w1 = pr[n][i][1] * vs[i][k];
+                                    if (masked) {  // (nothing of a hidden key counts, whatever its scale is)
+                                        if (x[n][i][0] == -INFINITY) w0 = 0.f;
+                                        if (x[n][i][1] == -INFINITY) w1 = 0.f;
+                                    }
+                                    wt[n][k][i] = halves(w0, w1);
+                                    most = max_halves(most, wt[n][k][i]);
+                                }
+                        }
+                        const __half2 mh = *reinterpret_cast<const __half2*>(&most);
+                        moves |= __high2float(mh) > 8192.f || __low2float(mh) > 8192.f;
+                        if (round == 1 || !__any_sync(0xffffffffu, moves)) break;
+                        first = false;
+                        float top[4];  // log2 of a key's largest scale
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            float sc = vs[i][0];
+#pragma unroll
+                            for (int k = 1; k < NG; ++k) sc = fmaxf(sc, vs[i][k]);
+                            top[i] = sc > 0.f ? __log2f(sc) : -INFINITY;
+                        }
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float mx = -INFINITY, jx = -INFINITY;
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) {
+                                    mx = fmaxf(mx, x[n][i][e]);
+                                    jx = fmaxf(jx, x[n][i][e] == -INFINITY ? -INFINITY : x[n][i][e] + top[i]);
+                                }
+#pragma unroll
+                                for (int off = 4; off < 32; off <<= 1) {
+                                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+                                    jx = fmaxf(jx, __shfl_xor_sync(0xffffffffu, jx, off));
+                                }
+                                mx = fmaxf(mx, z.m[n][e]);
+                                jx = fmaxf(jx, z.j[n][e]);
+                                // weights up to 2^4 at the move; p' within 2^+-96 of 1 at the largest x, whatever the scales are
+                                const float ref = mx == -INFINITY ? 0.f : fminf(fmaxf(jx - 4.f, mx - 60.f), mx + 96.f);
+                                const float f = z.m[n][e] == -INFINITY ? 0.f : fast_exp2(z.ref[n][e] - ref);  // (0: nothing summed yet)
+                                z.m[n][e] = mx;
+                                z.j[n][e] = jx;
+                                z.ref[n][e] = ref;
+                                z.l[n][e] *= f;
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) {
+                                    z.mid[n][k][e] *= f;
+                                    z.ones[n][k][e] *= f;
+                                    z.ones[n][k][2 + e] *= f;
+                                }
+#pragma unroll
+                                for (int c = 0; c < GR; ++c) {
+                                    z.o[n][c][0][e] *= f;
+                                    z.o[n][c][0][2 + e] *= f;
+                                    z.o[n][c][1][e] *= f;
+                                    z.o[n][c][1][2 + e] *= f;
+                                }
+                            }
+                    }
+                    // ---- what each weight adds ----
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) {
+                            const float mid = fmaf(8.f, vs[i][k], vm[i][k]);
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    if (k == 0) z.l[n][e] += pr[n][i][e];
+                                    if (!masked || x[n][i][e] != -INFINITY) z.mid[n][k][e] = fmaf(pr[n][i][e], mid, z.mid[n][k][e]);
+                                }
+                        }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int k = 0; k < NG; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) wt[n][k][i] = transpose8x8(wt[n][k][i]);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint8_t* vb = block[u] + St::kCodes;
+                        constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int k = 0; k < NG; ++k) mma_16816<__half>(z.ones[n][k], kOnes, wt[n][k][2 * u], wt[n][k][2 * u + 1]);
+#pragma unroll
+                        for (int c = 0; c < GR; ++c) {
+                            const uint32_t wa = *reinterpret_cast<const uint32_t*>(vb + voff0[c]), wb = *reinterpret_cast<const uint32_t*>(vb + voff1[c]);
+                            const uint32_t wc = *reinterpret_cast<const uint32_t*>(vb + voff0[c] + 8 * ROW),
+                                           wd = *reinterpret_cast<const uint32_t*>(vb + voff1[c] + 8 * ROW);
+                            uint32_t y0 = __byte_perm(wa, wb, pick), y1 = __byte_perm(wc, wd, pick);
+                            const uint32_t z0 = y0 >> 8, z1 = y1 >> 8;
+                            const uint32_t even_ch[4] = {y0 & kLowCodes, z0 & kLowCodes, y1 & kLowCodes, z1 & kLowCodes};      // channels 0, 2
+                            const uint32_t odd_ch[4] = {y0 & kHighCodes, z0 & kHighCodes, y1 & kHighCodes, z1 & kHighCodes};  // 1, 3: times 16
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                mma_16816<__half>(z.o[n][c][0], even_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
+                                mma_16816<__half>(z.o[n][c][1], odd_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
+                            }
+                        }
+                    }
+                    if (++uncentred == kCentre) {
+                        centre();
+                        uncentred = 0;
+                    }
+                }
+                // the last reads of the stage have to have come back before it is given back (see splitkv_decode.cu)
+                __threadfence_block();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[s]);
+            }
+
+            // ---- this warp's sums: O[n][e][c] = channels 32 c + 4 g .. + 3 of row 2t + e, in reference R ----
+            centre();
+            float4 o[NT][2][GR];
+            float l[NT][2];
+            bool has[NT][2];  // any key (a NaN among its scores does not show in the largest)
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float rest[NG];
+                    l[n][e] = z.l[n][e];
+#pragma unroll
+                    for (int k = 0; k < NG; ++k) rest[k] = z.mid[n][k][e];
+#pragma unroll
+                    for (int off = 4; off < 32; off <<= 1) {
+                        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], off);
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) rest[k] += __shfl_xor_sync(0xffffffffu, rest[k], off);
+                    }
+                    has[n][e] = z.m[n][e] != -INFINITY || l[n][e] != l[n][e];
+#pragma unroll
+                    for (int c = 0; c < GR; ++c) {
+                        const float add = rest[c / PER];
+                        o[n][e][c] = make_float4(fmaf(16777216.f, z.o[n][c][0][e], add), fmaf(1048576.f, z.o[n][c][1][e], add),
+                                                 fmaf(16777216.f, z.o[n][c][0][2 + e], add), fmaf(1048576.f, z.o[n][c][1][2 + e], add));
+                    }
+                }
+            // ---- the warps of a head meet: the upper half hands its sums to the lower one until one warp per head is left ----
+            for (int step = kConsumers / 2; step >= heads; step >>= 1) {
+                if (warp >= step && warp < 2 * step) {
+                    const int slot = warp - step;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                            for (int c = 0; c < GR; ++c) meet[(slot * kMeetFloat4 + (n * 2 + e) * GR + c) * 32 + lane] = o[n][e][c];
+                            if (g == 0) {
+                                meet_stats[((slot * NT + n) * 8 + 2 * t4 + e) * 2] = z.ref[n][e];
+                                meet_stats[((slot * NT + n) * 8 + 2 * t4 + e) * 2 + 1] = has[n][e] ? l[n][e] : -1.f;  // (-1: no key)
+                            }
+                        }
+                }
+                asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
+                if (warp < step) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float ref = meet_stats[((warp * NT + n) * 8 + 2 * t4 + e) * 2], lo_ = meet_stats[((warp * NT + n) * 8 + 2 * t4 + e) * 2 + 1];
+                            if (lo_ != -1.f) {
+                                const float both = has[n][e] ? fmaxf(ref, z.ref[n][e]) : ref;
+                                const float fa = has[n][e] ? fast_exp2(z.ref[n][e] - both) : 0.f, fb = fast_exp2(ref - both);
+                                z.ref[n][e] = both;
+                                has[n][e] = true;
+                                l[n][e] = l[n][e] * fa + lo_ * fb;
+#pragma unroll
+                                for (int c = 0; c < GR; ++c) {
+                                    const float4 y = meet[(warp * kMeetFloat4 + (n * 2 + e) * GR + c) * 32 + lane];
+                                    float4& v = o[n][e][c];
+                                    v = make_float4(v.x * fa + y.x * fb, v.y * fa + y.y * fb, v.z * fa + y.z * fb, v.w * fa + y.w * fb);
+                                }
+                            }
+                        }
+                }
+                asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
+            }
+            if (warp >= heads || failed) continue;
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = row0 + 8 * n + 2 * t4 + e, i = r / G, h = kh * G + (r - i * G);
+                    if (r >= rows) continue;
+                    const int64_t idx = p.seqstart_q ? ((int64_t)h * p.num_splits + split) * p.total_q + (q0 + i)
+                                                     : (((int64_t)b * p.hq + h) * p.num_splits + split) * p.seqlen_q + i;
+                    const float inv = has[n][e] ? 1.f / l[n][e] : 0.f;
+#pragma unroll
+                    for (int c = 0; c < GR; ++c) {
+                        const float4 v = o[n][e][c];
+                        *reinterpret_cast<float4*>(p.o_acc + idx * D + 32 * c + 4 * g) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                    }
+                    if (g == 0) p.lse_acc[idx] = !has[n][e] ? -INFINITY : l[n][e] != l[n][e] ? INFINITY  // (the merge makes NaN of it)
+                                                                   : (z.ref[n][e] + log2f(l[n][e])) * 0.6931471805599453f;
+                }
+        }
+    }
+}
+
+// Codes of a pool as (bytes of a row, token of the page, kv head, page); a box lands as [head][token][row].
+int make_codes_map(CUtensorMap* map, const void* base, int64_t pool, int64_t page, int64_t hkv, int D, int heads, int chunk) {
+    PFN_encodeTiled enc = get_encode_tiled();
+    FCK_REQUIRE(enc != nullptr, FLASHCK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    const cuuint64_t dims[4] = {(cuuint64_t)(D / 2), (cuuint64_t)page, (cuuint64_t)hkv, (cuuint64_t)pool};
+    const cuuint64_t strides[3] = {(cuuint64_t)(hkv * D / 2), (cuuint64_t)(D / 2), (cuuint64_t)(page * hkv * D / 2)};
+    const cuuint32_t box[4] = {(cuuint32_t)(D / 2), (cuuint32_t)chunk, (cuuint32_t)heads, 1};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    FCK_REQUIRE(r == CUDA_SUCCESS, FLASHCK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for pool pages=%lld page=%lld hkv=%lld hdim=%d", (int)r,
+                (long long)pool, (long long)page, (long long)hkv, D);
+    return FLASHCK_OK;
+}
+
+template <typename T, int D, int NG, int NT, int TEAMS>
+int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
+    using St = Stage<D, NG>;
+    const Int4Cache& c = p.cache;
+    while (dev.heads_log2 < 3 && c.hkv % (2ll << dev.heads_log2) == 0) ++dev.heads_log2;
+    const int heads = 1 << dev.heads_log2, toks = kPairs / heads;
+    int chunk = 16;
+    dev.chunk_log2 = 4;
+    while (2 * chunk <= toks && (!c.block_table || c.page % (2 * chunk) == 0)) { chunk *= 2; ++dev.chunk_log2; }
+    constexpr int kMeetWarps = TEAMS == 2 ? 8 : 4;
+    const size_t meet = (size_t)kMeetWarps * NT * (2 * (D / 32) * 32 * 16 + 64);
+    const size_t fixed = 1024 + meet + (size_t)(2 * c.batch + 4) * sizeof(int);
+    const size_t room = 227 * 1024;
+    FCK_REQUIRE(fixed + 2 * (St::kBytes + 16) <= room, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch %lld leaves no room for two stages",
+                (long long)c.batch);
+    dev.stages = (int)std::min<size_t>(8, (room - fixed) / (St::kBytes + 16));
+    const size_t smem = fixed + (size_t)dev.stages * (St::kBytes + 16);
+    CUtensorMap mk, mv;
+    if (int rc = make_codes_map(&mk, c.k_codes, c.pool, c.page, c.hkv, D, heads, chunk)) return rc;
+    if (int rc = make_codes_map(&mv, c.v_codes, c.pool, c.page, c.hkv, D, heads, chunk)) return rc;
+    auto kern = splitkv_int4_kernel<T, D, NG, NT, TEAMS>;
+    static thread_local int configured_device = -1;  // per instantiation
+    int devid = 0;
+    FCK_CUDA(cudaGetDevice(&devid));
+    if (configured_device != devid) {
+        FCK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room));
+        configured_device = devid;
+    }
+    const int64_t gy = (p.max_seqlen_q * (p.hq / c.hkv) + 8 * NT - 1) / (8 * NT), gz = c.hkv / heads;
+    FCK_REQUIRE(gy <= 65535, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: too many query rows per kv head");
+    const int64_t gx = std::max<int64_t>(1, sm_count() / (gy * gz));  // one wave, where the heads and rows leave one
+    FCK_CUDA(launch_dependent(kern, dim3((unsigned)gx, (unsigned)gy, (unsigned)gz), dim3((8 * TEAMS + 1) * 32), smem, stream, mk, mv, dev));
+    return FLASHCK_OK;
+}
+
+template <typename T, int D, int NG>
+int launch_rows(const SplitKVInt4Params& p, const Int4Dev& dev, cudaStream_t stream) {
+    // up to 8 rows: 16 consumer warps of one tile; more: 8 of two tiles each (the sums of two take 200 registers)
+    if (p.max_seqlen_q * (p.hq / p.cache.hkv) <= 8) return launch<T, D, NG, 1, 2>(p, dev, stream);
+    return launch<T, D, NG, 2, 1>(p, dev, stream);
+}
+
+template <typename T>
+int launch_type(const SplitKVInt4Params& p, const Int4Dev& dev, cudaStream_t stream) {
+    const int64_t groups = p.cache.d / p.cache.group;
+    if (p.cache.d == 128) {
+        if (groups == 1) return launch_rows<T, 128, 1>(p, dev, stream);
+        return groups == 2 ? launch_rows<T, 128, 2>(p, dev, stream) : launch_rows<T, 128, 4>(p, dev, stream);
+    }
+    return groups == 1 ? launch_rows<T, 64, 1>(p, dev, stream) : launch_rows<T, 64, 2>(p, dev, stream);
+}
+
+}  // namespace
+
+int launch_splitkv_int4(const SplitKVInt4Params& p, cudaStream_t stream) {
+    const Int4Cache& c = p.cache;
+    FCK_REQUIRE(c.d == 64 || c.d == 128, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: hdim 64 or 128 (got %lld)", (long long)c.d);
+    FCK_REQUIRE((c.group == 32 || c.group == 64 || c.group == 128) && c.group <= c.d, FLASHCK_ERR_UNSUPPORTED,
+                "FmhaFwdSplitKVInt4: groups of 32, 64 or 128 channels of a head (got %lld of %lld)", (long long)c.group, (long long)c.d);
+    FCK_REQUIRE(c.batch >= 1 && c.batch <= 8192, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch must be in [1,8192]");
+    FCK_REQUIRE(!c.block_table || c.page % 16 == 0, FLASHCK_ERR_UNSUPPORTED,
+                "FmhaFwdSplitKVInt4: page_block_size must be a positive multiple of 16 (got %lld)", (long long)c.page);
+    FCK_REQUIRE(c.page > 0 && c.page < (1ll << 31) && c.pool > 0 && c.pool < (1ll << 31) - 1, FLASHCK_ERR_INVALID_ARGUMENT,
+                "FmhaFwdSplitKVInt4: bad page or pool size");
+    FCK_REQUIRE(p.total_q < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: too many query rows");
+    Int4Dev dev{};
+    dev.status = device_status_ptr();
+    if (!dev.status) return FLASHCK_ERR_CUDA;
+    dev.q = p.q; dev.o_acc = p.o_acc; dev.lse_acc = p.lse_acc; dev.seqstart_q = p.seqstart_q;
+    dev.seqlen_k = c.seqlen; dev.block_table = c.block_table; dev.cache_batch_idx = c.cache_batch_idx;
+    dev.k_params = (const uint8_t*)c.k_params; dev.v_params = (const uint8_t*)c.v_params;
+    dev.batch = (int)c.batch; dev.seqlen_q = (int)p.seqlen_q; dev.hq = (int)p.hq; dev.hkv = (int)c.hkv;
+    dev.num_splits = (int)p.num_splits; dev.total_q = (int)p.total_q; dev.bt_stride = (int)c.bt_stride;
+    dev.page = (int)c.page; dev.pool = (int)c.pool;
+    dev.room = (int)std::min<int64_t>(c.block_table ? c.bt_stride * c.page : c.page, 0x7fffff00);
+    dev.mask_type = p.mask_type;
+    dev.wl = (int)(p.wl < 0 ? -1 : std::min<int64_t>(p.wl, 0x3fffffff));
+    dev.wr = (int)(p.wr < 0 ? -1 : std::min<int64_t>(p.wr, 0x3fffffff));
+    dev.scale_log2 = p.scale * 1.4426950408889634f;
+    return c.dtype == FLASHCK_DTYPE_BFLOAT16 ? launch_type<__nv_bfloat16>(p, dev, stream) : launch_type<__half>(p, dev, stream);
+}
+
+}  // namespace fck

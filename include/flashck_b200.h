@@ -352,6 +352,62 @@ FLASHCK_API int FmhaFwdAppendKV(void* q_buf_ptr, void* k_buf_ptr, void* knew_buf
                     int64_t paged_block_size, void* stream, int dtype);
 
 /*
+ * The 4-bit cache (no counterpart in the reference).  A group of `group` (32, 64 or 128) neighbouring channels of one token's head is
+ * held as lo + scale * code: lo its least value, scale = (greatest - lo) / 15 in the element type, code 0..15 the nearest, ties to even.
+ *   codes: uint8 [rows, hkv, d / 2], byte j with channel 2j in its low and 2j + 1 in its high four bits
+ *   params: element type [rows, hkv, d / group, 2] = (scale, lo)
+ * rows are pools [num_pool_pages, paged_block_size] behind block_table (int32 [.., block_table_stride]), or contiguous caches
+ * [num_pool_pages, kv_seq_len] without one (num_pool_pages: their rows, of which sequence b uses b or cache_batch_idx[b]; paged_block_size
+ * is kv_seq_len).  A page id or row outside the pools is never followed: reads give zeros, writes are skipped and reported.
+ * codes and params 16-byte aligned; hdim 64 or 128, dtype 3 or 4.  A group that holds a NaN or an infinity, or whose range leaves fp32,
+ * reads back as NaN.
+ *
+ * FmhaFwdAppendKVInt4 -- FmhaFwdAppendKV to such a cache: queries and new keys turned, the turned keys (rounded to the element type) and
+ * the new values quantised as they are written.
+ *   q -> q_out (another buffer; q NULL: none), k/v_held: element type, like knew: what the cache holds for the new tokens, or NULL
+ *   positions: int32 [axes, total_new] or NULL: new token j of sequence b is at seqlen_k[b] + j on every axis.  Queries are the last
+ *      new tokens of their sequence.  A position outside [0, rotary_rows) turns by NaN.
+ *   pair_axis: HOST memory, rotary_dim / 2 entries below axes (1 to 4): the axis whose position turns a pair; NULL: all the first
+ * Rows of q_out and k/v_held that belong to no sequence are zero.  A token that does not fit is skipped and reported, as there.
+ */
+FLASHCK_API int FmhaFwdAppendKVInt4(const void* q, void* q_out, void* k_codes, void* k_params, const void* knew, void* v_codes, void* v_params,
+                        const void* vnew, void* k_held, void* v_held, const void* k_seq_len_ptr, const int64_t* q_seq_start_ptr,
+                        const int64_t* knew_seq_start_ptr, const void* positions, const void* rotary_cos, const void* rotary_sin,
+                        const void* pair_axis, const void* block_table, const int64_t* cache_batch_idx, int64_t batch, int64_t q_seq_len,
+                        int64_t knew_seq_len, int64_t q_num_heads, int64_t kv_num_heads, int64_t head_dim, int64_t group, int64_t axes,
+                        int64_t rotary_dim, int64_t rotary_rows, int rope_type, int64_t block_table_stride, int64_t paged_block_size,
+                        int64_t num_pool_pages, void* stream, int dtype);
+
+/*
+ * FmhaFwdSplitKVInt4 -- FmhaFwdSplitKV over such a cache; lse_acc / o_acc as there (lse_acc is always needed), merged by
+ * FmhaFwdSplitKVCombine.  Pages of a multiple of 16 tokens.  Keys and values enter the products as the exact lo + scale * code.
+ */
+FLASHCK_API int FmhaFwdSplitKVInt4(const void* q, const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
+                       void* lse_acc, void* o_acc, const int64_t* q_seq_start_ptr, const void* k_seq_len_ptr, const void* block_table,
+                       const int64_t* cache_batch_idx, int64_t batch, int64_t q_seq_len, int64_t q_max_seq_len, int64_t q_num_heads,
+                       int64_t kv_num_heads, int64_t head_dim, int64_t group, int64_t num_splits, int64_t block_table_stride,
+                       int64_t paged_block_size, int64_t num_pool_pages, float scale, int64_t window_left, int64_t window_right,
+                       uint32_t mask_type, void* stream, int dtype);
+
+/*
+ * FmhaReadKVInt4 -- such a cache read back: k_out / v_out element type, packed [out_tokens, hkv, d] with out_seq_start (int64 [b+1]), or
+ * [b, out_tokens, hkv, d] without.  Rows that are no token of a sequence are zero.
+ */
+FLASHCK_API int FmhaReadKVInt4(const void* k_codes, const void* k_params, const void* v_codes, const void* v_params, void* k_out, void* v_out,
+                   const void* k_seq_len_ptr, const int64_t* out_seq_start_ptr, const void* block_table, const int64_t* cache_batch_idx,
+                   int64_t batch, int64_t out_tokens, int64_t kv_num_heads, int64_t head_dim, int64_t group, int64_t block_table_stride,
+                   int64_t paged_block_size, int64_t num_pool_pages, void* stream, int dtype);
+
+/*
+ * FmhaRotary -- rotary embedding by itself: q [tokens,hq,d] -> q_out, k [tokens,hkv,d] -> k_out (k NULL: none), by positions int32
+ * [axes, tokens]; tables, pair_axis, rotary_dim and rope_type (1 or 2) as in FmhaFwdAppendKVInt4.  inverse != 0 turns the other way,
+ * which is the gradient.  hdim a multiple of 8, rotary_dim at most 256; channels behind rotary_dim are copied.  In and out may not overlap.
+ */
+FLASHCK_API int FmhaRotary(const void* q, void* q_out, const void* k, void* k_out, const void* positions, const void* rotary_cos,
+               const void* rotary_sin, const void* pair_axis, int64_t axes, int64_t tokens, int64_t q_num_heads, int64_t kv_num_heads,
+               int64_t head_dim, int64_t rotary_dim, int64_t rotary_rows, int rope_type, int inverse, void* stream, int dtype);
+
+/*
  * FmhaFwdSplitKVStatic -- split-KV attention and combine in one call, for callers that cannot allocate.
  * This entry point has no counterpart in the reference.  It exists for callers that may not call cudaMalloc
  * (a serving loop with a fixed memory plan, code that must stay inside a framework allocator, threads barred
