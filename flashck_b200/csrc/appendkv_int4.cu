@@ -67,19 +67,50 @@ __device__ __forceinline__ int sequence_of(const int64_t* seqstart, int batch, i
     return __reduce_add_sync(0xffffffffu, n);
 }
 
-__device__ __forceinline__ float min_nan(float a, float b) {
-    float r;
-    asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+// Least of two pairs of T; NaN where either is.
+template <typename T>
+__device__ __forceinline__ uint32_t min2_nan(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t min2_nan<__half>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+template <>
+__device__ __forceinline__ uint32_t min2_nan<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
 
-// (x - lo) / scale to the nearest code, ties to even, without rounding the quotient: a multiple h of one half is compared with it by the
-// sign of r - h scale, which one FMA gives exactly.
+// What 8 codes stand for: lo + scale * code, one rounding.  A code set into the low mantissa bits of 128 (bf16) or 1024 (fp16) is that number
+// plus the code; two at a time are four channels apart in the word.
+template <typename T>
+__device__ __forceinline__ Vec8<T> values_of(uint32_t word, T scale, T lo) {
+    using T2 = typename Elem<T>::T2;
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    constexpr uint32_t kBase = kHalf ? 0x64006400u : 0x43004300u;
+    const T2 base = Elem<T>::bcast2(kHalf ? -1024.f : -128.f);
+    T2 s2, l2;
+    s2.x = s2.y = scale;
+    l2.x = l2.y = lo;
+    uint32_t f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t u = ((word >> (4 * i)) & 0x000f000fu) | kBase;
+        const T2 v = __hfma2(__hadd2(*reinterpret_cast<const T2*>(&u), base), s2, l2);
+        f[i] = *reinterpret_cast<const uint32_t*>(&v);  // channels i and i + 4
+    }
+    Vec8<T> x;
+    x.w[0] = __byte_perm(f[0], f[1], 0x5410);
+    x.w[1] = __byte_perm(f[2], f[3], 0x5410);
+    x.w[2] = __byte_perm(f[0], f[1], 0x7632);
+    x.w[3] = __byte_perm(f[2], f[3], 0x7632);
+    return x;
+}
+
+// r / scale to the nearest code, ties to even, without rounding a quotient: a multiple of one half, times the scale, is compared with r by the
+// sign of one FMA, which is exact.
 __device__ __noinline__ uint32_t exact_code(float r, float s) {
     uint32_t k = 0;
     if (!(s > 0.f)) return 0;
@@ -91,45 +122,42 @@ __device__ __noinline__ uint32_t exact_code(float r, float s) {
     return k;
 }
 
-// 8 channels of a group of `lanes` lanes: codes, scale and least value; `x` becomes what they stand for.
+// The codes of 8 channels, whose group has `lanes` lanes, and the group's scale and least value.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise(Vec8<T>& x, int lanes, T& scale_t, T& lo_t) {
-    float f[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f32(x.e[i]);
-    float lo = f[0], hi = f[0];
-#pragma unroll
-    for (int i = 1; i < 8; ++i) { lo = min_nan(lo, f[i]); hi = max_nan(hi, f[i]); }
-    for (int off = 1; off < lanes; off <<= 1) {
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, off));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, off));
-    }
-    lo_t = Elem<T>::from_f32(lo);
+__device__ __forceinline__ uint32_t quantise(const Vec8<T>& x, int lanes, T& scale_t, T& lo_t) {
+    // least and (negated) greatest value together, so that a level takes one shuffle
+    constexpr uint32_t kSigns = 0x80008000u;
+    const uint32_t least = min2_nan<T>(min2_nan<T>(x.w[0], x.w[1]), min2_nan<T>(x.w[2], x.w[3]));
+    const uint32_t most = min2_nan<T>(min2_nan<T>(x.w[0] ^ kSigns, x.w[1] ^ kSigns), min2_nan<T>(x.w[2] ^ kSigns, x.w[3] ^ kSigns));
+    uint32_t both = min2_nan<T>(__byte_perm(least, most, 0x5410), __byte_perm(least, most, 0x7632));
+    for (int off = 1; off < lanes; off <<= 1) both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, off));
+    lo_t = reinterpret_cast<const T*>(&both)[0];
+    const float lo = Elem<T>::to_f32(lo_t), hi = -Elem<T>::to_f32(reinterpret_cast<const T*>(&both)[1]);
     const float range = hi - lo;
     scale_t = Elem<T>::from_f32(range < INFINITY ? __fdiv_rn(range, 15.f) : NAN);  // (a group that is not finite is NaN as a whole)
     const float s = Elem<T>::to_f32(scale_t);
-    // quotients are off by a few 2^-22; where one is closer than 1e-4 to half way between two codes (0.2 in a thousand), or the
-    // reciprocal may overflow, the comparison above decides
+    // The quotient is rounded correctly (a product with the reciprocal, then once more with its exact remainder), and then to an integer by
+    // the addition of 1.5 * 2^23, ties to even.  Rounding twice does no harm: (k + 1/2) scale has at most 16 bits, so a difference x - lo that
+    // is not equal to it is at least a step of 32 bits away, relatively more than the half step at k + 1/2 to which its quotient is rounded.
+    // (Half way between two codes is common: a difference of two 8-bit significands meets a multiple of another one in a few per thousand.)
+    constexpr float kRound = 12582912.f;
     const float inv = __frcp_rn(s);
-    constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's low bits are the rounded integer
-    float away = 0.f;
-    uint32_t word = 0;
-    uint32_t code[8];
+    uint32_t u[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float quotient = fminf((f[i] - lo) * inv, 15.f), t = quotient + kRound;
-        away = fmaxf(away, fabsf(quotient - (t - kRound)));
-        code[i] = __float_as_uint(t) & 15u;
+        const float r = Elem<T>::to_f32(x.e[i]) - lo, q = r * inv;
+        u[i] = __float_as_uint(fmaf(fmaf(-q, s, r), inv, q) + kRound);
     }
-    if (away > 0.4999f || !(s > 1e-30f)) {
-        for (int i = 0; i < 8; ++i) code[i] = exact_code(f[i] - lo, s);
-    }
+    // scales that T holds with few digits (a code may pass 15), and those whose reciprocal or remainder fp32 may not hold
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    if (!(s >= (kHalf ? 6.103515625e-5f : 1e-25f) && s <= 1e25f)) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        word |= code[i] << (4 * i);
-        x.e[i] = Elem<T>::from_f32(fmaf(s, (float)code[i], lo));
+        for (int i = 0; i < 8; ++i) u[i] = exact_code(Elem<T>::to_f32(x.e[i]) - lo, s);
     }
-    return word;
+    // lowest bytes: even channels and odd ones
+    const uint32_t even = __byte_perm(__byte_perm(u[0], u[2], 0x0040), __byte_perm(u[4], u[6], 0x0040), 0x5410);
+    const uint32_t odd = __byte_perm(__byte_perm(u[1], u[3], 0x0040), __byte_perm(u[5], u[7], 0x0040), 0x5410);
+    return (even & 0x0f0f0f0fu) | ((odd & 0x0f0f0f0fu) << 4);
 }
 
 struct AppendInt4Dev {
@@ -170,8 +198,11 @@ __device__ __forceinline__ void store8(T* p, const Vec8<T>& x, bool vec) {
     }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(256) append_int4_kernel(const AppendInt4Dev a) {
+// ROPE: 0 none, 1 neighbouring pairs, 2 halves, in 16-byte pieces; 3 any of them channel by channel.
+template <typename T, int ROPE>
+__global__ void __launch_bounds__(256, 3) append_int4_kernel(const AppendInt4Dev a) {
+    constexpr bool kVec = ROPE != 3;
+    constexpr int kAhead = ROPE == 3 ? 1 : 2;  // heads in flight
     pdl_launch_dependents();
     pdl_wait();
     const CacheDev& c = a.cache;
@@ -206,52 +237,58 @@ __global__ void __launch_bounds__(256) append_int4_kernel(const AppendInt4Dev a)
         if (!a.positions) return at;
         return j >= 0 && token < a.total_new ? a.positions[axis * a.total_new + token] : -1;
     };
-    const int pieces = c.d >> 3, sub = lane / pieces, e0 = (lane - sub * pieces) << 3, heads_at_once = 32 / pieces;
-    const bool vec = a.rot.vec;
-    const int heads = queries ? a.hq : c.hkv, partner = partner_of(a.rot, e0);
+    const int pieces = c.d >> 3, sub = lane / pieces, e0 = (lane - sub * pieces) << 3, at_once = 32 / pieces;
+    const int heads = queries ? a.hq : c.hkv;
     const int64_t row = !queries && real ? cache_row(c, b, at) : -1;
     if (!queries && real && row < 0 && lane == 0 && part == 0) atomicOr(a.status, FLASHCK_STATUS_APPEND_OVERFLOW);
     const T* src = (const T*)(queries ? a.q : a.knew) + t * heads * c.d;
+    const T* vsrc = (const T*)a.vnew + t * heads * c.d;
     const int group_lanes = c.group >> 3;
-    for (int h0 = part * heads_at_once; h0 < heads; h0 += w * heads_at_once) {
-        const int h = h0 + sub;
-        const bool mine = h < heads;
-        Vec8<T> x, y;
-        x.v = make_uint4(0, 0, 0, 0);
-        if (real && mine) {
-            const T* p = src + (int64_t)h * c.d;
-            if (a.rot.type == 0) {
-                x = load8(p + e0, vec);
-            } else if (vec) {
-                const Vec8<T> own = load8(p + e0, true), other = load8(p + partner, true);
-                turn_piece<T>(a.rot, e0, pos, own, other, x);
-            } else {
-                turn_piece_any<T>(a.rot, e0, pos, p, x);
+    Turn<T, ROPE == 3 ? 0 : ROPE> turn(a.rot, e0);
+    if constexpr (ROPE == 1 || ROPE == 2) {
+        if (real) turn.load(a.rot, e0, pos);
+    }
+    for (int h0 = part * at_once; h0 < heads; h0 += w * at_once * kAhead) {
+        Vec8<T> x[kAhead], y[kAhead], v[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int h = h0 + i * w * at_once + sub;
+            x[i].v = v[i].v = y[i].v = make_uint4(0, 0, 0, 0);
+            if (real && h < heads) {
+                if constexpr (kVec) {
+                    x[i] = load8(src + h * c.d + e0, true);
+                    if (ROPE == 2) y[i] = load8(src + h * c.d + turn.partner, true);
+                } else {
+                    turn_piece_any<T>(a.rot, e0, pos, src + h * c.d, x[i]);
+                }
+                if (!queries) v[i] = load8(vsrc + h * c.d + e0, kVec);
             }
-        }
-        if (queries) {
-            if (mine) store8((T*)a.q_out + (t * heads + h) * c.d + e0, x, vec);
-            continue;
         }
 #pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            if (kv == 1) {
-                x.v = make_uint4(0, 0, 0, 0);
-                if (real && mine) x = load8((const T*)a.vnew + (t * heads + h) * c.d + e0, vec);
+        for (int i = 0; i < kAhead; ++i) {
+            const int h = h0 + i * w * at_once + sub;
+            if (kVec && real) x[i] = turn(x[i], y[i]);
+            if (queries) {
+                if (h < heads) store8((T*)a.q_out + (t * heads + h) * c.d + e0, x[i], kVec);
+                continue;
             }
-            T scale, lo;
-            const uint32_t word = quantise<T>(x, group_lanes, scale, lo);
-            if (!mine) continue;
-            if (row >= 0) {
-                const int64_t place = row * c.hkv + h;
-                reinterpret_cast<uint32_t*>(c.codes[kv])[(place * c.d + e0) >> 3] = word;
-                if ((e0 & (c.group - 1)) == 0) {
-                    T two[2] = {scale, lo};
-                    c.params[kv][(place * c.d + e0) / c.group] = *reinterpret_cast<const uint32_t*>(two);
+#pragma unroll
+            for (int kv = 0; kv < 2; ++kv) {
+                T scale, lo;
+                const uint32_t word = quantise<T>(kv ? v[i] : x[i], group_lanes, scale, lo);
+                if (h < heads) {
+                    if (row >= 0) {
+                        const int64_t place = row * c.hkv + h;
+                        reinterpret_cast<uint32_t*>(c.codes[kv])[(place * c.d + e0) >> 3] = word;
+                        if ((e0 & (c.group - 1)) == 0) {
+                            const T two[2] = {scale, lo};
+                            c.params[kv][place * (c.d / c.group) + e0 / c.group] = *reinterpret_cast<const uint32_t*>(two);
+                        }
+                    }
+                    void* held = kv ? a.v_held : a.k_held;
+                    if (held) store8((T*)held + (t * heads + h) * c.d + e0, values_of<T>(word, scale, lo), kVec);
                 }
             }
-            void* held = kv ? a.v_held : a.k_held;
-            if (held) store8((T*)held + (t * heads + h) * c.d + e0, x, vec);
         }
     }
 }
@@ -264,42 +301,57 @@ struct ReadInt4Dev {
     int warps_per_job;
 };
 
-template <typename T>
+// A job is R neighbouring tokens: a lane looks one of them up for all, and their loads are in flight together.
+template <typename T, int R>
 __global__ void __launch_bounds__(256) read_int4_kernel(const ReadInt4Dev a) {
     pdl_launch_dependents();
     pdl_wait();
     const CacheDev& c = a.cache;
     const int lane = threadIdx.x & 31, w = a.warps_per_job;
-    const int64_t t = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
+    const int64_t t0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w * R;
     const int part = (threadIdx.x >> 5) % w;
-    if (t >= a.total) return;
-    int b;
-    int64_t j, n;
-    if (a.seqstart) {
-        b = sequence_of(a.seqstart, c.batch, t, lane);
-        j = t - a.seqstart[b];
-        n = min((int64_t)c.seqlen[b], a.seqstart[b + 1] - a.seqstart[b]);
-    } else {
-        b = (int)(t / a.tokens);
-        j = t - b * a.tokens;
-        n = c.seqlen[b];
-    }
-    const int64_t row = j >= 0 && j < n ? cache_row(c, b, j) : -1;  // (no such token: zeros)
-    const int per_row = c.hkv * c.d >> 3;  // 8 channels each
-    for (int i = part * 32 + lane; i < per_row; i += w * 32) {
-#pragma unroll
-        for (int kv = 0; kv < 2; ++kv) {
-            Vec8<T> x;
-            x.v = make_uint4(0, 0, 0, 0);
-            if (row >= 0) {
-                const uint32_t word = reinterpret_cast<const uint32_t*>(c.codes[kv])[row * per_row + i];
-                const uint32_t two = c.params[kv][(row * per_row + i) / (c.group >> 3)];
-                const float s = Elem<T>::to_f32(reinterpret_cast<const T*>(&two)[0]), lo = Elem<T>::to_f32(reinterpret_cast<const T*>(&two)[1]);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) x.e[k] = Elem<T>::from_f32(fmaf(s, (float)((word >> (4 * k)) & 15u), lo));
-            }
-            *reinterpret_cast<uint4*>((T*)a.out[kv] + (t * per_row + i) * 8) = x.v;
+    if (t0 >= a.total) return;
+    int64_t row = -1;  // of token t0 + lane (no such token: zeros)
+    {
+        const int64_t t = t0 + lane;
+        int b;
+        int64_t j, n;
+        if (a.seqstart) {
+            b = sequence_of(a.seqstart, c.batch, t0, lane);
+            while (lane < R && b + 1 < c.batch && a.seqstart[b + 1] <= t) ++b;
+            j = t - a.seqstart[b];
+            n = min((int64_t)c.seqlen[b], a.seqstart[b + 1] - a.seqstart[b]);
+        } else {
+            b = (int)(t / a.tokens);
+            j = t - b * a.tokens;
+            n = b < c.batch ? c.seqlen[b] : 0;
         }
+        if (lane < R && t < a.total && j >= 0 && j < n) row = cache_row(c, b, j);
+    }
+    int64_t rows[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) rows[r] = __shfl_sync(0xffffffffu, row, r);
+    const int per_row = c.hkv * c.d >> 3, group_log2 = 31 - __clz(c.group >> 3);  // 8 channels each
+    for (int i = part * 32 + lane; i < per_row; i += w * 32) {
+        uint32_t word[2][R], two[2][R];
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                word[kv][r] = two[kv][r] = 0;
+                if (rows[r] >= 0) {
+                    word[kv][r] = reinterpret_cast<const uint32_t*>(c.codes[kv])[rows[r] * per_row + i];
+                    two[kv][r] = c.params[kv][rows[r] * (per_row >> group_log2) + (i >> group_log2)];
+                }
+            }
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const T* p = reinterpret_cast<const T*>(&two[kv][r]);
+                if (t0 + r < a.total)
+                    *reinterpret_cast<uint4*>((T*)a.out[kv] + ((t0 + r) * per_row + i) * 8) = values_of<T>(word[kv][r], p[0], p[1]).v;
+            }
     }
 }
 
@@ -316,6 +368,20 @@ int fill_cache(const char* fn, const Int4Cache& p, CacheDev& c) {
     c.batch = (int)p.batch; c.hkv = (int)p.hkv; c.d = (int)p.d; c.group = (int)p.group;
     c.bt_stride = (int)p.bt_stride; c.page = (int)p.page; c.pool = (int)p.pool;
     return FLASHCK_OK;
+}
+
+template <typename T>
+cudaError_t launch_append_type(const AppendInt4Dev& a, dim3 grid, dim3 block, cudaStream_t stream) {
+    if (!a.rot.vec) return launch_dependent(append_int4_kernel<T, 3>, grid, block, 0, stream, a);
+    if (a.rot.type == 0) return launch_dependent(append_int4_kernel<T, 0>, grid, block, 0, stream, a);
+    return a.rot.type == 1 ? launch_dependent(append_int4_kernel<T, 1>, grid, block, 0, stream, a)
+                           : launch_dependent(append_int4_kernel<T, 2>, grid, block, 0, stream, a);
+}
+
+template <typename T>
+cudaError_t launch_read_type(const ReadInt4Dev& a, bool runs, unsigned blocks, cudaStream_t stream) {
+    return runs ? launch_dependent(read_int4_kernel<T, 4>, dim3(blocks), dim3(256), 0, stream, a)
+                : launch_dependent(read_int4_kernel<T, 1>, dim3(blocks), dim3(256), 0, stream, a);
 }
 
 // Warps that share a job: enough to fill the SMs with few jobs, one with many (what they all work out is worked out fewer times).
@@ -347,8 +413,8 @@ int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream) {
     const int64_t blocks = (jobs * a.warps_per_job + 7) / 8;
     FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdAppendKVInt4: too many tokens");
     const dim3 grid((unsigned)blocks), block(256);
-    if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_dependent(append_int4_kernel<__nv_bfloat16>, grid, block, 0, stream, a));
-    else FCK_CUDA(launch_dependent(append_int4_kernel<__half>, grid, block, 0, stream, a));
+    if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_append_type<__nv_bfloat16>(a, grid, block, stream));
+    else FCK_CUDA(launch_append_type<__half>(a, grid, block, stream));
     return FLASHCK_OK;
 }
 
@@ -359,11 +425,11 @@ int launch_read_int4(const ReadInt4Params& p, cudaStream_t stream) {
     a.total = p.seqstart ? p.tokens : p.cache.batch * p.tokens;
     if (a.total == 0) return FLASHCK_OK;
     a.warps_per_job = warps_for(a.total, std::max<int64_t>(1, p.cache.hkv * p.cache.d / 256));
-    const int64_t blocks = (a.total * a.warps_per_job + 7) / 8;
+    const bool runs = a.total >= (int64_t)sm_count() * 256;  // enough tokens to fill the SMs by fours
+    const int64_t jobs = runs ? (a.total + 3) / 4 : a.total, blocks = (jobs * a.warps_per_job + 7) / 8;
     FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaReadKVInt4: too many tokens");
-    const dim3 grid((unsigned)blocks), block(256);
-    if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_dependent(read_int4_kernel<__nv_bfloat16>, grid, block, 0, stream, a));
-    else FCK_CUDA(launch_dependent(read_int4_kernel<__half>, grid, block, 0, stream, a));
+    if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_read_type<__nv_bfloat16>(a, runs, (unsigned)blocks, stream));
+    else FCK_CUDA(launch_read_type<__half>(a, runs, (unsigned)blocks, stream));
     return FLASHCK_OK;
 }
 

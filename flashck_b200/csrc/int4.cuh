@@ -31,15 +31,17 @@ __device__ __forceinline__ int axis_of(const RotaryDev& r, int pair) { return (r
 template <typename T>
 union Vec8 {
     uint4 v;
+    uint32_t w[4];
     T e[8];
 };
 
-// cos and sin of pairs [first, first + N) for positions pos[axis]; a position outside the tables turns by NaN.  The vector form is taken
+// cos and sin of pairs [first, first + N) for positions pos(axis); a position outside the tables turns by NaN.  The vector form is taken
 // where one axis turns all of them.
 template <typename T, int N, typename Pos>
 __device__ __forceinline__ void load_angles(const RotaryDev& r, int first, const Pos& pos, float (&c)[N], float (&s)[N]) {
-    const uint32_t axes = (r.axis[first >> 4] >> (2 * (first & 15))) & ((1u << (2 * N)) - 1u), a0 = axes & 3u;
-    if (axes == a0 * (0x5555u & ((1u << (2 * N)) - 1u))) {
+    constexpr uint32_t kAll = (1u << (2 * N)) - 1u;
+    const uint32_t axes = (r.axis[first >> 4] >> (2 * (first & 15))) & kAll, a0 = axes & 3u;
+    if (axes == a0 * (0x5555u & kAll)) {
         const int64_t p = pos(a0);
         if ((uint64_t)p < (uint64_t)r.rows) {
             using V = typename std::conditional<N == 8, uint4, uint2>::type;
@@ -62,44 +64,50 @@ __device__ __forceinline__ void load_angles(const RotaryDev& r, int first, const
             s[i] = in ? Elem<T>::to_f32(((const T*)r.sinr)[p * r.half + first + i]) : NAN;
         }
     }
-    if (r.back) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) s[i] = -s[i];
-    }
 }
 
-// Where piece `e0` of a head finds its partner channels in the 16-byte form (itself where it needs none).
-__device__ __forceinline__ int partner_of(const RotaryDev& r, int e0) {
-    return r.type != 2 || e0 >= 2 * r.half ? e0 : e0 < r.half ? e0 + r.half : e0 - r.half;
-}
+// The 16-byte form of the rotation: a lane's 8 channels [e0, e0 + 8) of every head of a token.  ROPE as RotaryDev::type.  The angles are
+// loaded once per token; each product and sum is rounded by itself, as in the append to a 16-bit cache.
+template <typename T, int ROPE>
+struct Turn {
+    static constexpr int N = ROPE == 1 ? 4 : 8;
+    float c[N], s[N];  // (half-rotated: s with the sign that the partner channel comes with)
+    int partner;       // where its partner channels are (itself where it needs none)
+    bool turns;
 
-// Channels [e0, e0 + 8) of a head, turned and rounded to T; x and y are its own and its partner's channels.  Each product and sum is
-// rounded by itself, as in the append to a 16-bit cache.
-template <typename T, typename Pos>
-__device__ __forceinline__ void turn_piece(const RotaryDev& r, int e0, const Pos& pos, const Vec8<T>& x, const Vec8<T>& y, Vec8<T>& out) {
-    if (e0 >= 2 * r.half) {
-        out.v = x.v;
-    } else if (r.type == 1) {
-        float c[4], s[4];
-        load_angles<T, 4>(r, e0 / 2, pos, c, s);
+    __device__ __forceinline__ Turn(const RotaryDev& r, int e0) {
+        turns = ROPE != 0 && e0 < 2 * r.half;
+        partner = ROPE != 2 || !turns ? e0 : e0 < r.half ? e0 + r.half : e0 - r.half;
+    }
+    template <typename Pos>
+    __device__ __forceinline__ void load(const RotaryDev& r, int e0, const Pos& pos) {
+        if (!turns) return;
+        const bool low = ROPE == 2 && e0 < r.half;
+        load_angles<T, N>(r, ROPE == 1 ? e0 / 2 : low ? e0 : e0 - r.half, pos, c, s);
+        if (low != r.back) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float a = Elem<T>::to_f32(x.e[2 * i]), b = Elem<T>::to_f32(x.e[2 * i + 1]);
-            out.e[2 * i] = Elem<T>::from_f32(__fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i])));
-            out.e[2 * i + 1] = Elem<T>::from_f32(__fadd_rn(__fmul_rn(a, s[i]), __fmul_rn(b, c[i])));
-        }
-    } else {
-        float c[8], s[8];
-        const bool low = e0 < r.half;
-        load_angles<T, 8>(r, low ? e0 : e0 - r.half, pos, c, s);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {  // low: a c - b s with b the partner; high: a s + b c with a the partner
-            const float own = Elem<T>::to_f32(x.e[i]), other = Elem<T>::to_f32(y.e[i]);
-            const float other_s = __fmul_rn(other, s[i]);
-            out.e[i] = Elem<T>::from_f32(__fadd_rn(__fmul_rn(own, c[i]), low ? -other_s : other_s));
+            for (int i = 0; i < N; ++i) s[i] = -s[i];
         }
     }
-}
+    __device__ __forceinline__ Vec8<T> operator()(const Vec8<T>& x, const Vec8<T>& y) const {
+        if (!turns) return x;
+        Vec8<T> out;
+        if constexpr (ROPE == 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float a = Elem<T>::to_f32(x.e[2 * i]), b = Elem<T>::to_f32(x.e[2 * i + 1]);
+                out.w[i] = Elem<T>::pack2(__fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i])), __fadd_rn(__fmul_rn(a, s[i]), __fmul_rn(b, c[i])));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                out.w[i] = Elem<T>::pack2(
+                    __fadd_rn(__fmul_rn(Elem<T>::to_f32(x.e[2 * i]), c[2 * i]), __fmul_rn(Elem<T>::to_f32(y.e[2 * i]), s[2 * i])),
+                    __fadd_rn(__fmul_rn(Elem<T>::to_f32(x.e[2 * i + 1]), c[2 * i + 1]), __fmul_rn(Elem<T>::to_f32(y.e[2 * i + 1]), s[2 * i + 1])));
+        }
+        return out;
+    }
+};
 
 // The same channel by channel, for widths, tables and rows that the 16-byte form does not take.
 template <typename T, typename Pos>

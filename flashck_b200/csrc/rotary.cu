@@ -20,8 +20,46 @@ struct RotaryCall {
     int heads[2], d, warps_per_job;
 };
 
-template <typename T>
+// Heads whose pieces divide a warp: a lane has the same channels of every head.
+template <typename T, int ROPE>
 __global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall a) {
+    constexpr int kAhead = 4;  // heads in flight
+    pdl_launch_dependents();
+    pdl_wait();
+    const int w = a.warps_per_job, lane = threadIdx.x & 31;
+    const int64_t t = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
+    const int part = (threadIdx.x >> 5) % w;
+    if (t >= a.tokens) return;
+    const int pieces = a.d >> 3, sub = lane / pieces, e0 = (lane - sub * pieces) << 3, at_once = 32 / pieces;
+    Turn<T, ROPE> turn(a.rot, e0);
+    turn.load(a.rot, e0, [&](int axis) -> int64_t { return a.positions[axis * a.tokens + t]; });
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int heads = a.heads[i];
+        const T* src = (const T*)a.src[i] + t * heads * a.d;
+        T* dst = (T*)a.dst[i] + t * heads * a.d;
+        for (int h0 = part * at_once + sub; h0 < heads; h0 += w * at_once * kAhead) {
+            Vec8<T> x[kAhead], y[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int h = h0 + u * w * at_once;
+                if (h < heads) {
+                    x[u].v = *reinterpret_cast<const uint4*>(src + h * a.d + e0);
+                    if (ROPE == 2) y[u].v = *reinterpret_cast<const uint4*>(src + h * a.d + turn.partner);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                const int h = h0 + u * w * at_once;
+                if (h < heads) *reinterpret_cast<uint4*>(dst + h * a.d + e0) = turn(x[u], y[u]).v;
+            }
+        }
+    }
+}
+
+// Any width, any alignment.
+template <typename T>
+__global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryCall a) {
     pdl_launch_dependents();
     pdl_wait();
     const int w = a.warps_per_job, lane = threadIdx.x & 31;
@@ -30,25 +68,26 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall a) {
     if (t >= a.tokens) return;
     auto pos = [&](int axis) -> int64_t { return a.positions[axis * a.tokens + t]; };
     const int pieces = a.d >> 3;
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
         const T* src = (const T*)a.src[i] + t * a.heads[i] * a.d;
         T* dst = (T*)a.dst[i] + t * a.heads[i] * a.d;
         for (int p = part * 32 + lane; p < a.heads[i] * pieces; p += w * 32) {
             const int h = p / pieces, e0 = (p - h * pieces) << 3;
-            const T* row = src + (int64_t)h * a.d;
-            Vec8<T> x, out;
-            if (a.rot.vec) {
-                Vec8<T> y;
-                x.v = *reinterpret_cast<const uint4*>(row + e0);
-                y.v = *reinterpret_cast<const uint4*>(row + partner_of(a.rot, e0));
-                turn_piece<T>(a.rot, e0, pos, x, y, out);
-                *reinterpret_cast<uint4*>(dst + (int64_t)h * a.d + e0) = out.v;
-            } else {
-                turn_piece_any<T>(a.rot, e0, pos, row, out);
-                for (int k = 0; k < 8; ++k) dst[(int64_t)h * a.d + e0 + k] = out.e[k];
-            }
+            Vec8<T> out;
+            turn_piece_any<T>(a.rot, e0, pos, src + (int64_t)h * a.d, out);
+            for (int k = 0; k < 8; ++k) dst[(int64_t)h * a.d + e0 + k] = out.e[k];
         }
     }
+}
+
+template <typename T>
+cudaError_t launch_type(const RotaryCall& a, unsigned blocks, cudaStream_t stream) {
+    const dim3 grid(blocks), block(256);
+    const int pieces = a.d / 8;
+    if (!a.rot.vec || pieces > 32 || 32 % pieces != 0) return launch_dependent(rotary_any_kernel<T>, grid, block, 0, stream, a);
+    return a.rot.type == 1 ? launch_dependent(rotary_kernel<T, 1>, grid, block, 0, stream, a)
+                           : launch_dependent(rotary_kernel<T, 2>, grid, block, 0, stream, a);
 }
 
 }  // namespace
@@ -57,7 +96,7 @@ int launch_rotary(const RotaryParams& p, cudaStream_t stream) {
     FCK_REQUIRE(p.d > 0 && p.d % 8 == 0 && p.d <= 1024, FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: hdim must be a multiple of 8, at most 1024 (got %lld)",
                 (long long)p.d);
     FCK_REQUIRE(p.rope_type != 0, FLASHCK_ERR_INVALID_ARGUMENT, "FmhaRotary: rope_type must be 1 or 2");
-    FCK_REQUIRE(p.hq <= 65536 && p.hkv <= 65536, FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: at most 65536 heads");
+    FCK_REQUIRE(p.hq <= 16384 && p.hkv <= 16384, FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: at most 16384 heads");
     RotaryCall a{};
     const auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
     if (int rc = fill_rotary("FmhaRotary", a.rot, p.rotary_cos, p.rotary_sin, p.rotary_rows, p.rotary_dim, p.d, p.rope_type, p.pair_axis, p.axes,
@@ -73,8 +112,8 @@ int launch_rotary(const RotaryParams& p, cudaStream_t stream) {
     a.warps_per_job = w;
     const int64_t blocks = (p.tokens * w + 7) / 8;
     FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: too many tokens");
-    if (p.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_dependent(rotary_kernel<__nv_bfloat16>, dim3((unsigned)blocks), dim3(256), 0, stream, a));
-    else FCK_CUDA(launch_dependent(rotary_kernel<__half>, dim3((unsigned)blocks), dim3(256), 0, stream, a));
+    if (p.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_type<__nv_bfloat16>(a, (unsigned)blocks, stream));
+    else FCK_CUDA(launch_type<__half>(a, (unsigned)blocks, stream));
     return FLASHCK_OK;
 }
 
