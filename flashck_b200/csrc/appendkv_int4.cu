@@ -122,15 +122,18 @@ __device__ __noinline__ uint32_t exact_code(float r, float s) {
     return k;
 }
 
-// The codes of 8 channels, whose group has `lanes` lanes, and the group's scale and least value.
+// Least and (negated) greatest of 8 values, together in a word, so that a level of a reduction takes one shuffle.
 template <typename T>
-__device__ __forceinline__ uint32_t quantise(const Vec8<T>& x, int lanes, T& scale_t, T& lo_t) {
-    // least and (negated) greatest value together, so that a level takes one shuffle
+__device__ __forceinline__ uint32_t range_of(const Vec8<T>& x) {
     constexpr uint32_t kSigns = 0x80008000u;
     const uint32_t least = min2_nan<T>(min2_nan<T>(x.w[0], x.w[1]), min2_nan<T>(x.w[2], x.w[3]));
     const uint32_t most = min2_nan<T>(min2_nan<T>(x.w[0] ^ kSigns, x.w[1] ^ kSigns), min2_nan<T>(x.w[2] ^ kSigns, x.w[3] ^ kSigns));
-    uint32_t both = min2_nan<T>(__byte_perm(least, most, 0x5410), __byte_perm(least, most, 0x7632));
-    for (int off = 1; off < lanes; off <<= 1) both = min2_nan<T>(both, __shfl_xor_sync(0xffffffffu, both, off));
+    return min2_nan<T>(__byte_perm(least, most, 0x5410), __byte_perm(least, most, 0x7632));
+}
+
+// The codes of 8 channels of a group with range `both`, and the group's scale and least value.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise(const Vec8<T>& x, uint32_t both, T& scale_t, T& lo_t) {
     lo_t = reinterpret_cast<const T*>(&both)[0];
     const float lo = Elem<T>::to_f32(lo_t), hi = -Elem<T>::to_f32(reinterpret_cast<const T*>(&both)[1]);
     const float range = hi - lo;
@@ -198,9 +201,33 @@ __device__ __forceinline__ void store8(T* p, const Vec8<T>& x, bool vec) {
     }
 }
 
-// ROPE: 0 none, 1 neighbouring pairs, 2 halves, in 16-byte pieces; 3 any of them channel by channel.
+// A token's place: its sequence b, and its place j among the rows of the sequence in its tensor, of which there are n.
+struct Token {
+    int b;
+    int64_t j, n, first;  // first: packed row of the sequence's first new token
+};
+__device__ __forceinline__ Token find_token(const AppendInt4Dev& a, bool queries, int64_t t, int lane) {
+    const int64_t* starts = queries ? a.seqstart_q : a.seqstart_knew;
+    const int64_t each = queries ? a.seqlen_q : a.seqlen_knew;
+    Token k;
+    if (starts) {
+        k.b = sequence_of(starts, a.cache.batch, t, lane);
+        const int64_t s0 = starts[k.b];
+        k.j = t - s0;
+        k.n = starts[k.b + 1] - s0;
+        k.first = queries ? a.seqstart_knew[k.b] : s0;
+    } else {
+        k.b = (int)((uint32_t)t / (uint32_t)each);
+        k.j = t - k.b * each;
+        k.n = each;
+        k.first = (int64_t)k.b * a.seqlen_knew;
+    }
+    return k;
+}
+
+// ROPE as in Turn; 3: channel by channel, any width and alignment.
 template <typename T, int ROPE>
-__global__ void __launch_bounds__(256, 3) append_int4_kernel(const AppendInt4Dev a) {
+__global__ void __launch_bounds__(256, ROPE == 4 ? 2 : 3) append_int4_kernel(const __grid_constant__ AppendInt4Dev a) {
     constexpr bool kVec = ROPE != 3;
     constexpr int kAhead = ROPE == 3 ? 1 : 2;  // heads in flight
     pdl_launch_dependents();
@@ -212,81 +239,102 @@ __global__ void __launch_bounds__(256, 3) append_int4_kernel(const AppendInt4Dev
     if (job >= a.total_new + a.total_q) return;  // (whole warps)
     const bool queries = job >= a.total_new;
     const int64_t t = queries ? job - a.total_new : job;
-    // ---- the token: its sequence b, its place j among the sequence's new tokens ----
-    const int64_t* starts = queries ? a.seqstart_q : a.seqstart_knew;
-    const int64_t each = queries ? a.seqlen_q : a.seqlen_knew;
-    int b;
-    int64_t j, n, first = 0;  // n: rows of the sequence in this tensor; first: packed row of its first new token
-    if (starts) {
-        b = sequence_of(starts, c.batch, t, lane);
-        const int64_t s0 = starts[b];
-        j = t - s0;
-        n = starts[b + 1] - s0;
-        first = queries ? a.seqstart_knew[b] : s0;
-    } else {
-        b = (int)(t / each);
-        j = t - b * each;
-        n = each;
-        first = (int64_t)b * a.seqlen_knew;
-    }
-    const bool real = j >= 0 && j < n;  // (a row that belongs to no sequence leaves as zeros)
-    if (queries) j += (a.seqstart_knew ? a.seqstart_knew[b + 1] - first : (int64_t)a.seqlen_knew) - n;  // the last new tokens are the queries'
-    const int64_t at = real ? c.seqlen[b] + j : -1;  // place in the cache
-    const int64_t token = first + j;
+    const int heads = queries ? a.hq : c.hkv;
+    const int lanes = c.d >> 4, at_once = 32 / lanes, sub = lane / lanes, e0 = (lane - sub * lanes) << 3, step = w * at_once;
+    if (part * at_once >= heads) return;
+    const T* src = (const T*)(queries ? a.q : a.knew) + t * heads * c.d;
+    const T* vsrc = (const T*)a.vnew + t * heads * c.d;
+    Turn<T, kVec ? ROPE : 0> turn(a.rot, e0, c.d);
+
+    Pieces<T> x[kAhead], y[kAhead], v[kAhead];
+    auto request = [&](int h0) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const int h = h0 + i * step + sub;
+            x[i].a.v = x[i].b.v = v[i].a.v = v[i].b.v = make_uint4(0, 0, 0, 0);
+            if (kVec && h < heads) {
+                x[i] = turn.own(src + h * c.d);
+                if (ROPE == 4) y[i] = turn.other(src + h * c.d);
+                if (!queries) v[i] = turn.own(vsrc + h * c.d);
+            }
+        }
+    };
+    request(part * at_once);  // (a row is there whether it belongs to a sequence or not: its loads do not wait for what follows)
+
+    const Token k = find_token(a, queries, t, lane);
+    const bool real = k.j >= 0 && k.j < k.n;  // (a row that belongs to no sequence leaves as zeros)
+    // the last new tokens are the queries'
+    const int64_t j = k.j + (queries ? (a.seqstart_knew ? a.seqstart_knew[k.b + 1] - k.first : (int64_t)a.seqlen_knew) - k.n : 0);
+    const int64_t at = real ? c.seqlen[k.b] + j : -1;  // place in the cache
+    const int64_t token = k.first + j;
     auto pos = [&](int axis) -> int64_t {
         if (!a.positions) return at;
         return j >= 0 && token < a.total_new ? a.positions[axis * a.total_new + token] : -1;
     };
-    const int pieces = c.d >> 3, sub = lane / pieces, e0 = (lane - sub * pieces) << 3, at_once = 32 / pieces;
-    const int heads = queries ? a.hq : c.hkv;
-    const int64_t row = !queries && real ? cache_row(c, b, at) : -1;
+    if (real) turn.load(a.rot, pos);
+    const int64_t row = !queries && real ? cache_row(c, k.b, at) : -1;
     if (!queries && real && row < 0 && lane == 0 && part == 0) atomicOr(a.status, FLASHCK_STATUS_APPEND_OVERFLOW);
-    const T* src = (const T*)(queries ? a.q : a.knew) + t * heads * c.d;
-    const T* vsrc = (const T*)a.vnew + t * heads * c.d;
-    const int group_lanes = c.group >> 3;
-    Turn<T, ROPE == 3 ? 0 : ROPE> turn(a.rot, e0);
-    if constexpr (ROPE == 1 || ROPE == 2) {
-        if (real) turn.load(a.rot, e0, pos);
-    }
-    for (int h0 = part * at_once; h0 < heads; h0 += w * at_once * kAhead) {
-        Vec8<T> x[kAhead], y[kAhead], v[kAhead];
+    const bool joint = c.group == c.d;  // one group: both pieces
+    const int group_lanes = joint ? lanes : c.group >> 3, groups = c.d / c.group;
+
+    for (int h0 = part * at_once; h0 < heads; h0 += step * kAhead) {
+        if (h0 != part * at_once) request(h0);
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
-            const int h = h0 + i * w * at_once + sub;
-            x[i].v = v[i].v = y[i].v = make_uint4(0, 0, 0, 0);
-            if (real && h < heads) {
-                if constexpr (kVec) {
-                    x[i] = load8(src + h * c.d + e0, true);
-                    if (ROPE == 2) y[i] = load8(src + h * c.d + turn.partner, true);
-                } else {
-                    turn_piece_any<T>(a.rot, e0, pos, src + h * c.d, x[i]);
+            const int h = h0 + i * step + sub;
+            const bool mine = h < heads;
+            if (h0 + i * step >= heads) break;  // (the whole warp)
+            if constexpr (!kVec) {
+                if (mine && real) {
+                    turn_piece_any<T>(a.rot, e0, pos, src + h * c.d, x[i].a);
+                    turn_piece_any<T>(a.rot, e0 + (c.d >> 1), pos, src + h * c.d, x[i].b);
+                    if (!queries) {
+                        v[i].a = load8(vsrc + h * c.d + e0, false);
+                        v[i].b = load8(vsrc + h * c.d + e0 + (c.d >> 1), false);
+                    }
                 }
-                if (!queries) v[i] = load8(vsrc + h * c.d + e0, kVec);
+            } else {
+                turn(x[i], y[i]);
+                if (!real) x[i].a.v = x[i].b.v = v[i].a.v = v[i].b.v = make_uint4(0, 0, 0, 0);
             }
-        }
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int h = h0 + i * w * at_once + sub;
-            if (kVec && real) x[i] = turn(x[i], y[i]);
             if (queries) {
-                if (h < heads) store8((T*)a.q_out + (t * heads + h) * c.d + e0, x[i], kVec);
+                if (mine) {
+                    T* dst = (T*)a.q_out + (t * heads + h) * c.d;
+                    store8(dst + e0, x[i].a, kVec);
+                    store8(dst + e0 + (c.d >> 1), x[i].b, kVec);
+                }
                 continue;
             }
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
-                T scale, lo;
-                const uint32_t word = quantise<T>(kv ? v[i] : x[i], group_lanes, scale, lo);
-                if (h < heads) {
-                    if (row >= 0) {
-                        const int64_t place = row * c.hkv + h;
-                        reinterpret_cast<uint32_t*>(c.codes[kv])[(place * c.d + e0) >> 3] = word;
-                        if ((e0 & (c.group - 1)) == 0) {
-                            const T two[2] = {scale, lo};
-                            c.params[kv][place * (c.d / c.group) + e0 / c.group] = *reinterpret_cast<const uint32_t*>(two);
-                        }
+                const Pieces<T>& z = kv ? v[i] : x[i];
+                uint32_t ra = range_of(z.a), rb = range_of(z.b);
+                if (joint) ra = rb = min2_nan<T>(ra, rb);
+                for (int off = 1; off < group_lanes; off <<= 1) {
+                    ra = min2_nan<T>(ra, __shfl_xor_sync(0xffffffffu, ra, off));
+                    if (!joint) rb = min2_nan<T>(rb, __shfl_xor_sync(0xffffffffu, rb, off));
+                }
+                if (joint) rb = ra;
+                T scale[2], lo[2];
+                const uint32_t wa = quantise<T>(z.a, ra, scale[0], lo[0]), wb = quantise<T>(z.b, rb, scale[1], lo[1]);
+                if (!mine) continue;
+                if (row >= 0) {
+                    const int64_t place = row * c.hkv + h;
+                    uint32_t* codes = reinterpret_cast<uint32_t*>(c.codes[kv]) + place * (c.d >> 3) + (e0 >> 3);
+                    codes[0] = wa;
+                    codes[lanes] = wb;
+                    if ((e0 & (c.group - 1)) == 0) {
+                        const T ta[2] = {scale[0], lo[0]}, tb[2] = {scale[1], lo[1]};
+                        uint32_t* params = c.params[kv] + place * groups + e0 / c.group;
+                        params[0] = *reinterpret_cast<const uint32_t*>(ta);
+                        if (!joint) params[groups >> 1] = *reinterpret_cast<const uint32_t*>(tb);
                     }
-                    void* held = kv ? a.v_held : a.k_held;
-                    if (held) store8((T*)held + (t * heads + h) * c.d + e0, values_of<T>(word, scale, lo), kVec);
+                }
+                T* held = (T*)(kv ? a.v_held : a.k_held);
+                if (held) {
+                    held += (t * heads + h) * c.d + e0;
+                    store8(held, values_of<T>(wa, scale[0], lo[0]), kVec);
+                    store8(held + (c.d >> 1), values_of<T>(wb, scale[1], lo[1]), kVec);
                 }
             }
         }
@@ -303,7 +351,7 @@ struct ReadInt4Dev {
 
 // A job is R neighbouring tokens: a lane looks one of them up for all, and their loads are in flight together.
 template <typename T, int R>
-__global__ void __launch_bounds__(256) read_int4_kernel(const ReadInt4Dev a) {
+__global__ void __launch_bounds__(256) read_int4_kernel(const __grid_constant__ ReadInt4Dev a) {
     pdl_launch_dependents();
     pdl_wait();
     const CacheDev& c = a.cache;
@@ -372,10 +420,13 @@ int fill_cache(const char* fn, const Int4Cache& p, CacheDev& c) {
 
 template <typename T>
 cudaError_t launch_append_type(const AppendInt4Dev& a, dim3 grid, dim3 block, cudaStream_t stream) {
-    if (!a.rot.vec) return launch_dependent(append_int4_kernel<T, 3>, grid, block, 0, stream, a);
-    if (a.rot.type == 0) return launch_dependent(append_int4_kernel<T, 0>, grid, block, 0, stream, a);
-    return a.rot.type == 1 ? launch_dependent(append_int4_kernel<T, 1>, grid, block, 0, stream, a)
-                           : launch_dependent(append_int4_kernel<T, 2>, grid, block, 0, stream, a);
+    switch (rope_form(a.rot, a.cache.d)) {
+        case 0: return launch_dependent(append_int4_kernel<T, 0>, grid, block, 0, stream, a);
+        case 1: return launch_dependent(append_int4_kernel<T, 1>, grid, block, 0, stream, a);
+        case 2: return launch_dependent(append_int4_kernel<T, 2>, grid, block, 0, stream, a);
+        case 4: return launch_dependent(append_int4_kernel<T, 4>, grid, block, 0, stream, a);
+        default: return launch_dependent(append_int4_kernel<T, 3>, grid, block, 0, stream, a);
+    }
 }
 
 template <typename T>
@@ -411,7 +462,7 @@ int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream) {
     if (jobs == 0) return FLASHCK_OK;
     a.warps_per_job = warps_for(jobs, std::max<int64_t>(1, std::max(p.hq, p.cache.hkv) * p.cache.d / 256));
     const int64_t blocks = (jobs * a.warps_per_job + 7) / 8;
-    FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdAppendKVInt4: too many tokens");
+    FCK_REQUIRE(jobs < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdAppendKVInt4: too many tokens");
     const dim3 grid((unsigned)blocks), block(256);
     if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_append_type<__nv_bfloat16>(a, grid, block, stream));
     else FCK_CUDA(launch_append_type<__half>(a, grid, block, stream));

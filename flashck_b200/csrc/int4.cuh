@@ -66,48 +66,94 @@ __device__ __forceinline__ void load_angles(const RotaryDev& r, int first, const
     }
 }
 
-// The 16-byte form of the rotation: a lane's 8 channels [e0, e0 + 8) of every head of a token.  ROPE as RotaryDev::type.  The angles are
-// loaded once per token; each product and sum is rounded by itself, as in the append to a 16-bit cache.
+// The 16-byte form of the rotation.  A lane has channels [e0, e0 + 8) and [e0 + d / 2, e0 + d / 2 + 8) of every head of a token, so that it holds
+// both halves of its half-rotated pairs where all of a head turns (ROPE 2); the angles are loaded once per token.  ROPE 1: neighbouring pairs;
+// 4: half-rotated pairs of which a head's front part consists, whose other half is read a second time (other()); 0: nothing turns.
+// Each product and sum is rounded by itself, as in the append to a 16-bit cache.
+template <typename T>
+struct Pieces {
+    Vec8<T> a, b;  // channels e0 .. and e0 + d / 2 ..
+};
+
 template <typename T, int ROPE>
 struct Turn {
-    static constexpr int N = ROPE == 1 ? 4 : 8;
-    float c[N], s[N];  // (half-rotated: s with the sign that the partner channel comes with)
-    int partner;       // where its partner channels are (itself where it needs none)
-    bool turns;
+    static constexpr int N = ROPE == 1 ? 4 : 8, SETS = ROPE == 0 ? 0 : ROPE == 2 ? 1 : 2;
+    float c[SETS ? SETS : 1][N], s[SETS ? SETS : 1][N];  // (ROPE 4: s with the sign that the partner channel comes with)
+    int e[2], partner[2];
+    bool turns[2];
 
-    __device__ __forceinline__ Turn(const RotaryDev& r, int e0) {
-        turns = ROPE != 0 && e0 < 2 * r.half;
-        partner = ROPE != 2 || !turns ? e0 : e0 < r.half ? e0 + r.half : e0 - r.half;
+    __device__ __forceinline__ Turn(const RotaryDev& r, int e0, int d) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            e[i] = e0 + i * (d >> 1);
+            turns[i] = ROPE != 0 && e[i] < 2 * r.half;
+            partner[i] = !turns[i] ? e[i] : e[i] < r.half ? e[i] + r.half : e[i] - r.half;
+        }
     }
     template <typename Pos>
-    __device__ __forceinline__ void load(const RotaryDev& r, int e0, const Pos& pos) {
-        if (!turns) return;
-        const bool low = ROPE == 2 && e0 < r.half;
-        load_angles<T, N>(r, ROPE == 1 ? e0 / 2 : low ? e0 : e0 - r.half, pos, c, s);
-        if (low != r.back) {
+    __device__ __forceinline__ void load(const RotaryDev& r, const Pos& pos) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) s[i] = -s[i];
+        for (int i = 0; i < SETS; ++i) {
+            if (!turns[i]) continue;
+            const bool low = ROPE == 4 && e[i] < r.half;
+            load_angles<T, N>(r, ROPE == 1 ? e[i] / 2 : ROPE == 2 || low ? e[i] : e[i] - r.half, pos, c[i], s[i]);
+            if (low != r.back) {
+#pragma unroll
+                for (int k = 0; k < N; ++k) s[i][k] = -s[i][k];
+            }
         }
     }
-    __device__ __forceinline__ Vec8<T> operator()(const Vec8<T>& x, const Vec8<T>& y) const {
-        if (!turns) return x;
+    static __device__ __forceinline__ Pieces<T> read(const T* head, const int (&at)[2]) {
+        Pieces<T> x;
+        x.a.v = *reinterpret_cast<const uint4*>(head + at[0]);
+        x.b.v = *reinterpret_cast<const uint4*>(head + at[1]);
+        return x;
+    }
+    __device__ __forceinline__ Pieces<T> own(const T* head) const { return read(head, e); }
+    __device__ __forceinline__ Pieces<T> other(const T* head) const { return read(head, partner); }
+    __device__ __forceinline__ void write(T* head, const Pieces<T>& x) const {
+        *reinterpret_cast<uint4*>(head + e[0]) = x.a.v;
+        *reinterpret_cast<uint4*>(head + e[1]) = x.b.v;
+    }
+
+    static __device__ __forceinline__ float f(T x) { return Elem<T>::to_f32(x); }
+    static __device__ __forceinline__ float turned(T x, float cx, T y, float sy) { return __fadd_rn(__fmul_rn(f(x), cx), __fmul_rn(f(y), sy)); }
+    __device__ __forceinline__ void one(Vec8<T>& x, const Vec8<T>& y, int i) const {
+        if (!turns[i]) return;
         Vec8<T> out;
-        if constexpr (ROPE == 1) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float a = Elem<T>::to_f32(x.e[2 * i]), b = Elem<T>::to_f32(x.e[2 * i + 1]);
-                out.w[i] = Elem<T>::pack2(__fsub_rn(__fmul_rn(a, c[i]), __fmul_rn(b, s[i])), __fadd_rn(__fmul_rn(a, s[i]), __fmul_rn(b, c[i])));
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                out.w[i] = Elem<T>::pack2(
-                    __fadd_rn(__fmul_rn(Elem<T>::to_f32(x.e[2 * i]), c[2 * i]), __fmul_rn(Elem<T>::to_f32(y.e[2 * i]), s[2 * i])),
-                    __fadd_rn(__fmul_rn(Elem<T>::to_f32(x.e[2 * i + 1]), c[2 * i + 1]), __fmul_rn(Elem<T>::to_f32(y.e[2 * i + 1]), s[2 * i + 1])));
+        for (int k = 0; k < 4; ++k) {
+            if constexpr (ROPE == 1)
+                out.w[k] = Elem<T>::pack2(turned(x.e[2 * k], c[i][k], x.e[2 * k + 1], -s[i][k]), turned(x.e[2 * k + 1], c[i][k], x.e[2 * k], s[i][k]));
+            else
+                out.w[k] = Elem<T>::pack2(turned(x.e[2 * k], c[i][2 * k], y.e[2 * k], s[i][2 * k]),
+                                          turned(x.e[2 * k + 1], c[i][2 * k + 1], y.e[2 * k + 1], s[i][2 * k + 1]));
         }
-        return out;
+        x = out;
+    }
+    __device__ __forceinline__ void operator()(Pieces<T>& x, const Pieces<T>& y) const {
+        if constexpr (ROPE == 2) {
+            Pieces<T> out;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                out.a.w[k] = Elem<T>::pack2(turned(x.a.e[2 * k], c[0][2 * k], x.b.e[2 * k], -s[0][2 * k]),
+                                            turned(x.a.e[2 * k + 1], c[0][2 * k + 1], x.b.e[2 * k + 1], -s[0][2 * k + 1]));
+                out.b.w[k] = Elem<T>::pack2(turned(x.b.e[2 * k], c[0][2 * k], x.a.e[2 * k], s[0][2 * k]),
+                                            turned(x.b.e[2 * k + 1], c[0][2 * k + 1], x.a.e[2 * k + 1], s[0][2 * k + 1]));
+            }
+            x = out;
+        } else if constexpr (ROPE != 0) {
+            one(x.a, y.a, 0);
+            one(x.b, y.b, 1);
+        }
     }
 };
+
+// The form that a call takes: 3 is channel by channel.
+inline int rope_form(const RotaryDev& r, int d) {
+    if (!r.vec || d % 16 != 0 || d > 512 || 32 % (d / 16) != 0) return 3;
+    return r.type != 2 ? r.type : 2 * r.half == d ? 2 : 4;
+}
 
 // The same channel by channel, for widths, tables and rows that the 16-byte form does not take.
 template <typename T, typename Pos>

@@ -1,7 +1,7 @@
 // Rotation of queries and keys by the positions of their tokens, along one or several axes (int4.cuh has the arithmetic).
 //
-// Bound by its traffic: each row read and written once.  A lane holds 8 channels of a head and keeps its cosines and sines for all heads
-// of the token; a half-rotated pair's other half is read a second time, from L1.
+// Bound by its traffic: each row read and written once.  A warp turns a token (a few warps, where tokens are few); a lane keeps the cosines
+// and sines of its 16 channels for all heads.
 #include <algorithm>
 #include <type_traits>
 
@@ -20,38 +20,40 @@ struct RotaryCall {
     int heads[2], d, warps_per_job;
 };
 
-// Heads whose pieces divide a warp: a lane has the same channels of every head.
 template <typename T, int ROPE>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall a) {
-    constexpr int kAhead = 4;  // heads in flight
+__global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ RotaryCall a) {
+    constexpr int kAhead = ROPE == 4 ? 2 : 4;  // heads in flight
     pdl_launch_dependents();
     pdl_wait();
     const int w = a.warps_per_job, lane = threadIdx.x & 31;
     const int64_t t = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
     const int part = (threadIdx.x >> 5) % w;
     if (t >= a.tokens) return;
-    const int pieces = a.d >> 3, sub = lane / pieces, e0 = (lane - sub * pieces) << 3, at_once = 32 / pieces;
-    Turn<T, ROPE> turn(a.rot, e0);
-    turn.load(a.rot, e0, [&](int axis) -> int64_t { return a.positions[axis * a.tokens + t]; });
+    const int lanes = a.d >> 4, sub = lane / lanes, e0 = (lane - sub * lanes) << 3, step = 32 / lanes * w;
+    Turn<T, ROPE> turn(a.rot, e0, a.d);
+    turn.load(a.rot, [&](int axis) -> int64_t { return a.positions[axis * a.tokens + t]; });
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const int heads = a.heads[i];
         const T* src = (const T*)a.src[i] + t * heads * a.d;
         T* dst = (T*)a.dst[i] + t * heads * a.d;
-        for (int h0 = part * at_once + sub; h0 < heads; h0 += w * at_once * kAhead) {
-            Vec8<T> x[kAhead], y[kAhead];
+        for (int h0 = part * (32 / lanes) + sub; h0 < heads; h0 += step * kAhead) {
+            Pieces<T> x[kAhead], y[kAhead];
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int h = h0 + u * w * at_once;
+                const int h = h0 + u * step;
                 if (h < heads) {
-                    x[u].v = *reinterpret_cast<const uint4*>(src + h * a.d + e0);
-                    if (ROPE == 2) y[u].v = *reinterpret_cast<const uint4*>(src + h * a.d + turn.partner);
+                    x[u] = turn.own(src + h * a.d);
+                    if (ROPE == 4) y[u] = turn.other(src + h * a.d);
                 }
             }
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                const int h = h0 + u * w * at_once;
-                if (h < heads) *reinterpret_cast<uint4*>(dst + h * a.d + e0) = turn(x[u], y[u]).v;
+                const int h = h0 + u * step;
+                if (h < heads) {
+                    turn(x[u], y[u]);
+                    turn.write(dst + h * a.d, x[u]);
+                }
             }
         }
     }
@@ -59,7 +61,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryCall a) {
 
 // Any width, any alignment.
 template <typename T>
-__global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryCall a) {
+__global__ void __launch_bounds__(256) rotary_any_kernel(const __grid_constant__ RotaryCall a) {
     pdl_launch_dependents();
     pdl_wait();
     const int w = a.warps_per_job, lane = threadIdx.x & 31;
@@ -84,10 +86,12 @@ __global__ void __launch_bounds__(256) rotary_any_kernel(const RotaryCall a) {
 template <typename T>
 cudaError_t launch_type(const RotaryCall& a, unsigned blocks, cudaStream_t stream) {
     const dim3 grid(blocks), block(256);
-    const int pieces = a.d / 8;
-    if (!a.rot.vec || pieces > 32 || 32 % pieces != 0) return launch_dependent(rotary_any_kernel<T>, grid, block, 0, stream, a);
-    return a.rot.type == 1 ? launch_dependent(rotary_kernel<T, 1>, grid, block, 0, stream, a)
-                           : launch_dependent(rotary_kernel<T, 2>, grid, block, 0, stream, a);
+    switch (rope_form(a.rot, a.d)) {
+        case 1: return launch_dependent(rotary_kernel<T, 1>, grid, block, 0, stream, a);
+        case 2: return launch_dependent(rotary_kernel<T, 2>, grid, block, 0, stream, a);
+        case 4: return launch_dependent(rotary_kernel<T, 4>, grid, block, 0, stream, a);
+        default: return launch_dependent(rotary_any_kernel<T>, grid, block, 0, stream, a);
+    }
 }
 
 }  // namespace
