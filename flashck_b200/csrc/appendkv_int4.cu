@@ -27,7 +27,7 @@ int fill_rotary(const char* fn, RotaryDev& r, const void* cosr, const void* sinr
     FCK_REQUIRE(rows >= 0 && rows < (1ll << 31), FLASHCK_ERR_INVALID_ARGUMENT, "%s: bad number of rows of the rotary tables", fn);
     FCK_REQUIRE(axes >= 1 && axes <= kMaxAxes, FLASHCK_ERR_UNSUPPORTED, "%s: 1 to %d axes of positions (got %lld)", fn, kMaxAxes, (long long)axes);
     r.cosr = cosr; r.sinr = sinr;
-    r.rows = (int)rows; r.half = (int)(rotary_dim / 2);
+    r.rows = (int)rows; r.half = (int)(rotary_dim / 2); r.axes = (int)axes;
     const auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
     r.vec = rows_aligned && aligned(cosr) && aligned(sinr) && rotary_dim % (rope_type == 1 ? 8 : 16) == 0;
     for (int i = 0; pair_axis && i < r.half; ++i) {
@@ -54,10 +54,11 @@ __device__ __forceinline__ int64_t cache_row(const CacheDev& c, int b, int64_t p
     const int64_t bphys = c.cache_batch_idx ? c.cache_batch_idx[b] : b;
     if (pos < 0) return -1;
     if (!c.block_table) return pos < c.page && (uint64_t)bphys < (uint64_t)c.pool ? bphys * c.page + pos : -1;
-    const int64_t slot = pos / c.page;
-    if (slot >= c.bt_stride) return -1;
+    if (pos > 0x7fffffff) return -1;
+    const uint32_t slot = (uint32_t)pos / (uint32_t)c.page;
+    if (slot >= (uint32_t)c.bt_stride) return -1;
     const int32_t pg = c.block_table[bphys * c.bt_stride + slot];
-    return (uint32_t)pg < (uint32_t)c.pool ? (int64_t)pg * c.page + (pos - slot * c.page) : -1;
+    return (uint32_t)pg < (uint32_t)c.pool ? (int64_t)pg * c.page + ((uint32_t)pos - slot * c.page) : -1;
 }
 
 // The sequence of packed row t, by the whole warp: the number of starts 1 .. batch - 1 at or below t.
@@ -136,26 +137,36 @@ template <typename T>
 __device__ __forceinline__ uint32_t quantise(const Vec8<T>& x, uint32_t both, T& scale_t, T& lo_t) {
     lo_t = reinterpret_cast<const T*>(&both)[0];
     const float lo = Elem<T>::to_f32(lo_t), hi = -Elem<T>::to_f32(reinterpret_cast<const T*>(&both)[1]);
+    // A quotient is rounded correctly by a product with the reciprocal, and once more with its exact remainder.
     const float range = hi - lo;
-    scale_t = Elem<T>::from_f32(range < INFINITY ? __fdiv_rn(range, 15.f) : NAN);  // (a group that is not finite is NaN as a whole)
+    constexpr float kFifteenth = 1.f / 15.f;
+    float step = range * kFifteenth;
+    step = fmaf(fmaf(-step, 15.f, range), kFifteenth, step);
+    scale_t = Elem<T>::from_f32(range < INFINITY ? step : NAN);  // (a group that is not finite is NaN as a whole)
     const float s = Elem<T>::to_f32(scale_t);
-    // The quotient is rounded correctly (a product with the reciprocal, then once more with its exact remainder), and then to an integer by
-    // the addition of 1.5 * 2^23, ties to even.  Rounding twice does no harm: (k + 1/2) scale has at most 16 bits, so a difference x - lo that
-    // is not equal to it is at least a step of 32 bits away, relatively more than the half step at k + 1/2 to which its quotient is rounded.
-    // (Half way between two codes is common: a difference of two 8-bit significands meets a multiple of another one in a few per thousand.)
-    constexpr float kRound = 12582912.f;
-    const float inv = __frcp_rn(s);
+    // The codes: such a quotient, to an integer by the addition of 1.5 * 2^23, ties to even.  Rounding twice does no harm: (k + 1/2) scale
+    // has at most 16 bits, so a difference x - lo that is not equal to it is at least a step of 32 bits away, relatively more than the half
+    // step at k + 1/2 to which its quotient is rounded.  (Half way between two codes is common: a difference of two 8-bit significands meets
+    // a multiple of another one in a few per thousand.)
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    const uint64_t inv2 = two(inv, inv), minus_s = two(-s, -s), minus_lo = two(-lo, -lo), round2 = two(12582912.f, 12582912.f);
     uint32_t u[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float r = Elem<T>::to_f32(x.e[i]) - lo, q = r * inv;
-        u[i] = __float_as_uint(fmaf(fmaf(-q, s, r), inv, q) + kRound);
+    for (int i = 0; i < 4; ++i) {
+        const uint64_t r = add2(widen<T>(x.w[i]), minus_lo), q = mul2(r, inv2);
+        float k0, k1;
+        apart(add2(fma2(fma2(q, minus_s, r), inv2, q), round2), k0, k1);
+        u[2 * i] = __float_as_uint(k0);
+        u[2 * i + 1] = __float_as_uint(k1);
     }
     // scales that T holds with few digits (a code may pass 15), and those whose reciprocal or remainder fp32 may not hold
     constexpr bool kHalf = std::is_same<T, __half>::value;
     if (!(s >= (kHalf ? 6.103515625e-5f : 1e-25f) && s <= 1e25f)) {
+        scale_t = Elem<T>::from_f32(range < INFINITY ? __fdiv_rn(range, 15.f) : NAN);
+        const float exact = Elem<T>::to_f32(scale_t);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[i] = exact_code(Elem<T>::to_f32(x.e[i]) - lo, s);
+        for (int i = 0; i < 8; ++i) u[i] = exact_code(Elem<T>::to_f32(x.e[i]) - lo, exact);
     }
     // lowest bytes: even channels and odd ones
     const uint32_t even = __byte_perm(__byte_perm(u[0], u[2], 0x0040), __byte_perm(u[4], u[6], 0x0040), 0x5410);
@@ -176,7 +187,7 @@ struct AppendInt4Dev {
     const int64_t* seqstart_knew;
     const int32_t* positions;
     int* status;
-    int seqlen_q, seqlen_knew, hq, warps_per_job;
+    int seqlen_q, seqlen_knew, hq, warps_log2;  // warps of a job
     int64_t total_new, total_q;
 };
 
@@ -227,20 +238,21 @@ __device__ __forceinline__ Token find_token(const AppendInt4Dev& a, bool queries
 
 // ROPE as in Turn; 3: channel by channel, any width and alignment.
 template <typename T, int ROPE>
-__global__ void __launch_bounds__(256, ROPE == 4 ? 2 : 3) append_int4_kernel(const __grid_constant__ AppendInt4Dev a) {
+__global__ void __launch_bounds__(256, 4) append_int4_kernel(const __grid_constant__ AppendInt4Dev a) {
     constexpr bool kVec = ROPE != 3;
-    constexpr int kAhead = ROPE == 3 ? 1 : 2;  // heads in flight
+    constexpr int kAhead = 1;  // heads in flight
     pdl_launch_dependents();
     pdl_wait();
     const CacheDev& c = a.cache;
-    const int lane = threadIdx.x & 31, w = a.warps_per_job;
-    const int64_t job = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
-    const int part = (threadIdx.x >> 5) % w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t job = (int64_t)blockIdx.x << (3 - a.warps_log2) | (warp >> a.warps_log2);
+    const int part = warp & ((1 << a.warps_log2) - 1);
     if (job >= a.total_new + a.total_q) return;  // (whole warps)
     const bool queries = job >= a.total_new;
     const int64_t t = queries ? job - a.total_new : job;
     const int heads = queries ? a.hq : c.hkv;
-    const int lanes = c.d >> 4, at_once = 32 / lanes, sub = lane / lanes, e0 = (lane - sub * lanes) << 3, step = w * at_once;
+    const int lanes_log2 = c.d == 64 ? 2 : 3, lanes = 1 << lanes_log2, at_once = 32 >> lanes_log2;
+    const int sub = lane >> lanes_log2, e0 = (lane & (lanes - 1)) << 3, step = at_once << a.warps_log2;
     if (part * at_once >= heads) return;
     const T* src = (const T*)(queries ? a.q : a.knew) + t * heads * c.d;
     const T* vsrc = (const T*)a.vnew + t * heads * c.d;
@@ -267,15 +279,14 @@ __global__ void __launch_bounds__(256, ROPE == 4 ? 2 : 3) append_int4_kernel(con
     const int64_t j = k.j + (queries ? (a.seqstart_knew ? a.seqstart_knew[k.b + 1] - k.first : (int64_t)a.seqlen_knew) - k.n : 0);
     const int64_t at = real ? c.seqlen[k.b] + j : -1;  // place in the cache
     const int64_t token = k.first + j;
-    auto pos = [&](int axis) -> int64_t {
-        if (!a.positions) return at;
-        return j >= 0 && token < a.total_new ? a.positions[axis * a.total_new + token] : -1;
-    };
+    Positions pos;
+    if (ROPE != 0 && a.positions && j >= 0 && token < a.total_new) pos.load(a.positions, a.rot.axes, a.total_new, token);
+    else pos.fill(a.positions ? -1 : at);
     if (real) turn.load(a.rot, pos);
     const int64_t row = !queries && real ? cache_row(c, k.b, at) : -1;
     if (!queries && real && row < 0 && lane == 0 && part == 0) atomicOr(a.status, FLASHCK_STATUS_APPEND_OVERFLOW);
     const bool joint = c.group == c.d;  // one group: both pieces
-    const int group_lanes = joint ? lanes : c.group >> 3, groups = c.d / c.group;
+    const int group_lanes = joint ? lanes : c.group >> 3, group_log2 = 31 - __clz(c.group), groups = c.d >> group_log2;
 
     for (int h0 = part * at_once; h0 < heads; h0 += step * kAhead) {
         if (h0 != part * at_once) request(h0);
@@ -325,7 +336,7 @@ __global__ void __launch_bounds__(256, ROPE == 4 ? 2 : 3) append_int4_kernel(con
                     codes[lanes] = wb;
                     if ((e0 & (c.group - 1)) == 0) {
                         const T ta[2] = {scale[0], lo[0]}, tb[2] = {scale[1], lo[1]};
-                        uint32_t* params = c.params[kv] + place * groups + e0 / c.group;
+                        uint32_t* params = c.params[kv] + place * groups + (e0 >> group_log2);
                         params[0] = *reinterpret_cast<const uint32_t*>(ta);
                         if (!joint) params[groups >> 1] = *reinterpret_cast<const uint32_t*>(tb);
                     }
@@ -346,7 +357,7 @@ struct ReadInt4Dev {
     void* out[2];
     const int64_t* seqstart;
     int64_t tokens, total;
-    int warps_per_job;
+    int warps_log2;
 };
 
 // A job is R neighbouring tokens: a lane looks one of them up for all, and their loads are in flight together.
@@ -355,9 +366,9 @@ __global__ void __launch_bounds__(256) read_int4_kernel(const __grid_constant__ 
     pdl_launch_dependents();
     pdl_wait();
     const CacheDev& c = a.cache;
-    const int lane = threadIdx.x & 31, w = a.warps_per_job;
-    const int64_t t0 = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w * R;
-    const int part = (threadIdx.x >> 5) % w;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t t0 = ((int64_t)blockIdx.x << (3 - a.warps_log2) | (warp >> a.warps_log2)) * R;
+    const int part = warp & ((1 << a.warps_log2) - 1), w = 1 << a.warps_log2;
     if (t0 >= a.total) return;
     int64_t row = -1;  // of token t0 + lane (no such token: zeros)
     {
@@ -436,9 +447,9 @@ cudaError_t launch_read_type(const ReadInt4Dev& a, bool runs, unsigned blocks, c
 }
 
 // Warps that share a job: enough to fill the SMs with few jobs, one with many (what they all work out is worked out fewer times).
-int warps_for(int64_t jobs, int64_t most) {
-    int w = 8;
-    while (w > 1 && (w > most || jobs * w > (int64_t)sm_count() * 32)) w >>= 1;
+int warps_log2_for(int64_t jobs, int64_t most) {
+    int w = 3;
+    while (w > 0 && ((1 << w) > most || jobs << w > (int64_t)sm_count() * 32)) --w;
     return w;
 }
 
@@ -460,8 +471,8 @@ int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream) {
     a.total_q = !p.q ? 0 : p.seqstart_q ? p.seqlen_q : p.cache.batch * p.seqlen_q;
     const int64_t jobs = a.total_new + a.total_q;
     if (jobs == 0) return FLASHCK_OK;
-    a.warps_per_job = warps_for(jobs, std::max<int64_t>(1, std::max(p.hq, p.cache.hkv) * p.cache.d / 256));
-    const int64_t blocks = (jobs * a.warps_per_job + 7) / 8;
+    a.warps_log2 = warps_log2_for(jobs, std::max<int64_t>(1, std::max(p.hq, p.cache.hkv) * p.cache.d / 256));
+    const int64_t blocks = ((jobs << a.warps_log2) + 7) / 8;
     FCK_REQUIRE(jobs < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaFwdAppendKVInt4: too many tokens");
     const dim3 grid((unsigned)blocks), block(256);
     if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_append_type<__nv_bfloat16>(a, grid, block, stream));
@@ -475,9 +486,9 @@ int launch_read_int4(const ReadInt4Params& p, cudaStream_t stream) {
     a.out[0] = p.k; a.out[1] = p.v; a.seqstart = p.seqstart; a.tokens = p.tokens;
     a.total = p.seqstart ? p.tokens : p.cache.batch * p.tokens;
     if (a.total == 0) return FLASHCK_OK;
-    a.warps_per_job = warps_for(a.total, std::max<int64_t>(1, p.cache.hkv * p.cache.d / 256));
+    a.warps_log2 = warps_log2_for(a.total, std::max<int64_t>(1, p.cache.hkv * p.cache.d / 256));
     const bool runs = a.total >= (int64_t)sm_count() * 256;  // enough tokens to fill the SMs by fours
-    const int64_t jobs = runs ? (a.total + 3) / 4 : a.total, blocks = (jobs * a.warps_per_job + 7) / 8;
+    const int64_t jobs = runs ? (a.total + 3) / 4 : a.total, blocks = ((jobs << a.warps_log2) + 7) / 8;
     FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaReadKVInt4: too many tokens");
     if (p.cache.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_read_type<__nv_bfloat16>(a, runs, (unsigned)blocks, stream));
     else FCK_CUDA(launch_read_type<__half>(a, runs, (unsigned)blocks, stream));

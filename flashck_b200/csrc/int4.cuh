@@ -7,6 +7,8 @@
 // (scale, lo).  A group with a NaN or an infinity, or one whose range leaves fp32, reads back as NaN.
 #pragma once
 
+#include <type_traits>
+
 #include "kernels.h"
 
 namespace fck {
@@ -18,7 +20,7 @@ constexpr int kMaxPairs = 128, kMaxAxes = 4;
 struct RotaryDev {
     const void* cosr;
     const void* sinr;
-    int rows, half, type;  // type: 0 none, 1 neighbouring pairs (2i, 2i + 1), 2 (i, i + half)
+    int rows, half, axes, type;  // type: 0 none, 1 neighbouring pairs (2i, 2i + 1), 2 (i, i + half)
     bool vec;              // 16-byte form: tables and rows aligned, a piece of 8 channels holds whole runs of pairs
     bool back;             // turned the other way: the gradient of the rotation
     uint32_t axis[kMaxPairs / 16];
@@ -35,18 +37,33 @@ union Vec8 {
     T e[8];
 };
 
-// cos and sin of pairs [first, first + N) for positions pos(axis); a position outside the tables turns by NaN.  The vector form is taken
-// where one axis turns all of them.
-template <typename T, int N, typename Pos>
-__device__ __forceinline__ void load_angles(const RotaryDev& r, int first, const Pos& pos, float (&c)[N], float (&s)[N]) {
+// A token's position along each axis, loaded together; -1 (outside the tables) for the axes that there are not.
+struct Positions {
+    int p[kMaxAxes];
+
+    __device__ __forceinline__ void load(const int32_t* positions, int axes, int64_t tokens, int64_t t) {
+#pragma unroll
+        for (int i = 0; i < kMaxAxes; ++i) p[i] = i < axes ? positions[i * tokens + t] : -1;
+    }
+    __device__ __forceinline__ void fill(int64_t at) {
+#pragma unroll
+        for (int i = 0; i < kMaxAxes; ++i) p[i] = at < 0 || at > 0x7fffffff ? -1 : (int)at;
+    }
+    __device__ __forceinline__ int operator()(int axis) const { return axis < 2 ? (axis == 0 ? p[0] : p[1]) : (axis == 2 ? p[2] : p[3]); }
+};
+
+// cos and sin of pairs [first, first + N); a position outside the tables turns by NaN.  The vector form is taken where one axis turns all of
+// them; in the other form too the loads do not wait for one another.
+template <typename T, int N>
+__device__ __forceinline__ void load_angles(const RotaryDev& r, int first, const Positions& pos, float (&c)[N], float (&s)[N]) {
     constexpr uint32_t kAll = (1u << (2 * N)) - 1u;
     const uint32_t axes = (r.axis[first >> 4] >> (2 * (first & 15))) & kAll, a0 = axes & 3u;
     if (axes == a0 * (0x5555u & kAll)) {
-        const int64_t p = pos(a0);
-        if ((uint64_t)p < (uint64_t)r.rows) {
+        const int p = pos(a0);
+        if ((uint32_t)p < (uint32_t)r.rows) {
             using V = typename std::conditional<N == 8, uint4, uint2>::type;
-            const V cv = *reinterpret_cast<const V*>((const T*)r.cosr + p * r.half + first);
-            const V sv = *reinterpret_cast<const V*>((const T*)r.sinr + p * r.half + first);
+            const V cv = *reinterpret_cast<const V*>((const T*)r.cosr + (int64_t)p * r.half + first);
+            const V sv = *reinterpret_cast<const V*>((const T*)r.sinr + (int64_t)p * r.half + first);
             const T* ce = reinterpret_cast<const T*>(&cv);
             const T* se = reinterpret_cast<const T*>(&sv);
 #pragma unroll
@@ -55,14 +72,24 @@ __device__ __forceinline__ void load_angles(const RotaryDev& r, int first, const
 #pragma unroll
             for (int i = 0; i < N; ++i) c[i] = s[i] = NAN;
         }
-    } else {
+    } else if (r.rows > 0) {
+        T ce[N], se[N];
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-            const int64_t p = pos(axis_of(r, first + i));
-            const bool in = (uint64_t)p < (uint64_t)r.rows;
-            c[i] = in ? Elem<T>::to_f32(((const T*)r.cosr)[p * r.half + first + i]) : NAN;
-            s[i] = in ? Elem<T>::to_f32(((const T*)r.sinr)[p * r.half + first + i]) : NAN;
+            const int p = pos((axes >> (2 * i)) & 3);
+            const int64_t at = (int64_t)((uint32_t)p < (uint32_t)r.rows ? p : 0) * r.half + first + i;
+            ce[i] = ((const T*)r.cosr)[at];
+            se[i] = ((const T*)r.sinr)[at];
         }
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool in = (uint32_t)pos((axes >> (2 * i)) & 3) < (uint32_t)r.rows;
+            c[i] = in ? Elem<T>::to_f32(ce[i]) : NAN;
+            s[i] = in ? Elem<T>::to_f32(se[i]) : NAN;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) c[i] = s[i] = NAN;
     }
 }
 
@@ -75,10 +102,49 @@ struct Pieces {
     Vec8<T> a, b;  // channels e0 .. and e0 + d / 2 ..
 };
 
+// two fp32 operations an instruction
+__device__ __forceinline__ uint64_t two(float lo, float hi) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void apart(uint64_t x, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(x)); }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ uint64_t widen(uint32_t w) {
+    if constexpr (std::is_same<T, __half>::value) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+        return two(f.x, f.y);
+    } else {
+        return two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint32_t narrow(uint64_t x) {
+    float lo, hi;
+    apart(x, lo, hi);
+    return Elem<T>::pack2(lo, hi);
+}
+
 template <typename T, int ROPE>
 struct Turn {
     static constexpr int N = ROPE == 1 ? 4 : 8, SETS = ROPE == 0 ? 0 : ROPE == 2 ? 1 : 2;
-    float c[SETS ? SETS : 1][N], s[SETS ? SETS : 1][N];  // (ROPE 4: s with the sign that the partner channel comes with)
+    // for each word (two channels) of a piece what its own channels and their partners are multiplied by
+    uint64_t c[SETS ? SETS : 1][4], s[SETS ? SETS : 1][4];
     int e[2], partner[2];
     bool turns[2];
 
@@ -90,16 +156,21 @@ struct Turn {
             partner[i] = !turns[i] ? e[i] : e[i] < r.half ? e[i] + r.half : e[i] - r.half;
         }
     }
-    template <typename Pos>
-    __device__ __forceinline__ void load(const RotaryDev& r, const Pos& pos) {
+    __device__ __forceinline__ void load(const RotaryDev& r, const Positions& pos) {
 #pragma unroll
         for (int i = 0; i < SETS; ++i) {
             if (!turns[i]) continue;
+            float ca[N], sa[N];
             const bool low = ROPE == 4 && e[i] < r.half;
-            load_angles<T, N>(r, ROPE == 1 ? e[i] / 2 : ROPE == 2 || low ? e[i] : e[i] - r.half, pos, c[i], s[i]);
+            load_angles<T, N>(r, ROPE == 1 ? e[i] / 2 : ROPE == 2 || low ? e[i] : e[i] - r.half, pos, ca, sa);
             if (low != r.back) {
 #pragma unroll
-                for (int k = 0; k < N; ++k) s[i][k] = -s[i][k];
+                for (int k = 0; k < N; ++k) sa[k] = -sa[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                c[i][k] = ROPE == 1 ? two(ca[k], ca[k]) : two(ca[2 * k % N], ca[(2 * k + 1) % N]);
+                s[i][k] = ROPE == 1 ? two(-sa[k], sa[k]) : two(sa[2 * k % N], sa[(2 * k + 1) % N]);
             }
         }
     }
@@ -115,33 +186,31 @@ struct Turn {
         *reinterpret_cast<uint4*>(head + e[0]) = x.a.v;
         *reinterpret_cast<uint4*>(head + e[1]) = x.b.v;
     }
-
-    static __device__ __forceinline__ float f(T x) { return Elem<T>::to_f32(x); }
-    static __device__ __forceinline__ float turned(T x, float cx, T y, float sy) { return __fadd_rn(__fmul_rn(f(x), cx), __fmul_rn(f(y), sy)); }
     __device__ __forceinline__ void one(Vec8<T>& x, const Vec8<T>& y, int i) const {
         if (!turns[i]) return;
-        Vec8<T> out;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            if constexpr (ROPE == 1)
-                out.w[k] = Elem<T>::pack2(turned(x.e[2 * k], c[i][k], x.e[2 * k + 1], -s[i][k]), turned(x.e[2 * k + 1], c[i][k], x.e[2 * k], s[i][k]));
-            else
-                out.w[k] = Elem<T>::pack2(turned(x.e[2 * k], c[i][2 * k], y.e[2 * k], s[i][2 * k]),
-                                          turned(x.e[2 * k + 1], c[i][2 * k + 1], y.e[2 * k + 1], s[i][2 * k + 1]));
+            const uint64_t own = widen<T>(x.w[k]);
+            uint64_t partners = own;
+            if constexpr (ROPE == 1) {
+                float lo, hi;
+                apart(own, lo, hi);
+                partners = two(hi, lo);
+            } else {
+                partners = widen<T>(y.w[k]);
+            }
+            x.w[k] = narrow<T>(add2(mul2(own, c[i][k]), mul2(partners, s[i][k])));
         }
-        x = out;
     }
     __device__ __forceinline__ void operator()(Pieces<T>& x, const Pieces<T>& y) const {
         if constexpr (ROPE == 2) {
-            Pieces<T> out;
+            const uint64_t minus = two(-1.f, -1.f);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                out.a.w[k] = Elem<T>::pack2(turned(x.a.e[2 * k], c[0][2 * k], x.b.e[2 * k], -s[0][2 * k]),
-                                            turned(x.a.e[2 * k + 1], c[0][2 * k + 1], x.b.e[2 * k + 1], -s[0][2 * k + 1]));
-                out.b.w[k] = Elem<T>::pack2(turned(x.b.e[2 * k], c[0][2 * k], x.a.e[2 * k], s[0][2 * k]),
-                                            turned(x.b.e[2 * k + 1], c[0][2 * k + 1], x.a.e[2 * k + 1], s[0][2 * k + 1]));
+                const uint64_t a = widen<T>(x.a.w[k]), b = widen<T>(x.b.w[k]);
+                x.a.w[k] = narrow<T>(fma2(mul2(b, s[0][k]), minus, mul2(a, c[0][k])));
+                x.b.w[k] = narrow<T>(add2(mul2(b, c[0][k]), mul2(a, s[0][k])));
             }
-            x = out;
         } else if constexpr (ROPE != 0) {
             one(x.a, y.a, 0);
             one(x.b, y.b, 1);
@@ -156,8 +225,8 @@ inline int rope_form(const RotaryDev& r, int d) {
 }
 
 // The same channel by channel, for widths, tables and rows that the 16-byte form does not take.
-template <typename T, typename Pos>
-__device__ __forceinline__ void turn_piece_any(const RotaryDev& r, int e0, const Pos& pos, const T* row, Vec8<T>& out) {
+template <typename T>
+__device__ __forceinline__ void turn_piece_any(const RotaryDev& r, int e0, const Positions& pos, const T* row, Vec8<T>& out) {
     for (int i = 0; i < 8; ++i) {
         const int e = e0 + i;
         T y = row[e];
@@ -165,10 +234,10 @@ __device__ __forceinline__ void turn_piece_any(const RotaryDev& r, int e0, const
             const int pair = r.type == 1 ? e >> 1 : e < r.half ? e : e - r.half;
             const bool low = r.type == 1 ? !(e & 1) : e < r.half;
             const T other = row[r.type == 1 ? e ^ 1 : low ? e + r.half : e - r.half];
-            const int64_t p = pos(axis_of(r, pair));
-            const bool in = (uint64_t)p < (uint64_t)r.rows;
-            const float c = in ? Elem<T>::to_f32(((const T*)r.cosr)[p * r.half + pair]) : NAN;
-            float s = in ? Elem<T>::to_f32(((const T*)r.sinr)[p * r.half + pair]) : NAN;
+            const int p = pos(axis_of(r, pair));
+            const bool in = (uint32_t)p < (uint32_t)r.rows;
+            const float c = in ? Elem<T>::to_f32(((const T*)r.cosr)[(int64_t)p * r.half + pair]) : NAN;
+            float s = in ? Elem<T>::to_f32(((const T*)r.sinr)[(int64_t)p * r.half + pair]) : NAN;
             if (r.back) s = -s;
             const float other_s = __fmul_rn(Elem<T>::to_f32(other), s);
             y = Elem<T>::from_f32(__fadd_rn(__fmul_rn(Elem<T>::to_f32(y), c), low ? -other_s : other_s));

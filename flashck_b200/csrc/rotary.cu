@@ -17,7 +17,7 @@ struct RotaryCall {
     void* dst[2];
     const int32_t* positions;
     int64_t tokens;
-    int heads[2], d, warps_per_job;
+    int heads[2], d, warps_log2;  // warps of a token
 };
 
 template <typename T, int ROPE>
@@ -25,35 +25,39 @@ __global__ void __launch_bounds__(256) rotary_kernel(const __grid_constant__ Rot
     constexpr int kAhead = ROPE == 4 ? 2 : 4;  // heads in flight
     pdl_launch_dependents();
     pdl_wait();
-    const int w = a.warps_per_job, lane = threadIdx.x & 31;
-    const int64_t t = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
-    const int part = (threadIdx.x >> 5) % w;
+    const int w = 1 << a.warps_log2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t t = (int64_t)blockIdx.x << (3 - a.warps_log2) | (warp >> a.warps_log2);
+    const int part = warp & (w - 1);
     if (t >= a.tokens) return;
     const int lanes = a.d >> 4, sub = lane / lanes, e0 = (lane - sub * lanes) << 3, step = 32 / lanes * w;
+    const int both = a.heads[0] + a.heads[1];  // the queries' heads, then the keys'
+    auto src = [&](int h) { return h < a.heads[0] ? (const T*)a.src[0] + (t * a.heads[0] + h) * a.d : (const T*)a.src[1] + (t * a.heads[1] + h - a.heads[0]) * a.d; };
+    auto dst = [&](int h) { return h < a.heads[0] ? (T*)a.dst[0] + (t * a.heads[0] + h) * a.d : (T*)a.dst[1] + (t * a.heads[1] + h - a.heads[0]) * a.d; };
+    Positions pos;
+    pos.load(a.positions, a.rot.axes, a.tokens, t);
     Turn<T, ROPE> turn(a.rot, e0, a.d);
-    turn.load(a.rot, [&](int axis) -> int64_t { return a.positions[axis * a.tokens + t]; });
+    Pieces<T> x[kAhead], y[kAhead];
+    auto request = [&](int h0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int heads = a.heads[i];
-        const T* src = (const T*)a.src[i] + t * heads * a.d;
-        T* dst = (T*)a.dst[i] + t * heads * a.d;
-        for (int h0 = part * (32 / lanes) + sub; h0 < heads; h0 += step * kAhead) {
-            Pieces<T> x[kAhead], y[kAhead];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int h = h0 + u * step;
-                if (h < heads) {
-                    x[u] = turn.own(src + h * a.d);
-                    if (ROPE == 4) y[u] = turn.other(src + h * a.d);
-                }
+        for (int u = 0; u < kAhead; ++u) {
+            const int h = h0 + u * step;
+            if (h < both) {
+                x[u] = turn.own(src(h));
+                if (ROPE == 4) y[u] = turn.other(src(h));
             }
+        }
+    };
+    int h0 = part * (32 / lanes) + sub;
+    request(h0);  // (in flight while positions and angles come)
+    turn.load(a.rot, pos);
+    for (; h0 < both; h0 += step * kAhead) {
+        if (h0 >= step * kAhead) request(h0);
 #pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                const int h = h0 + u * step;
-                if (h < heads) {
-                    turn(x[u], y[u]);
-                    turn.write(dst + h * a.d, x[u]);
-                }
+        for (int u = 0; u < kAhead; ++u) {
+            const int h = h0 + u * step;
+            if (h < both) {
+                turn(x[u], y[u]);
+                turn.write(dst(h), x[u]);
             }
         }
     }
@@ -64,11 +68,12 @@ template <typename T>
 __global__ void __launch_bounds__(256) rotary_any_kernel(const __grid_constant__ RotaryCall a) {
     pdl_launch_dependents();
     pdl_wait();
-    const int w = a.warps_per_job, lane = threadIdx.x & 31;
-    const int64_t t = ((int64_t)blockIdx.x * 8 + (threadIdx.x >> 5)) / w;
-    const int part = (threadIdx.x >> 5) % w;
+    const int w = 1 << a.warps_log2, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t t = (int64_t)blockIdx.x << (3 - a.warps_log2) | (warp >> a.warps_log2);
+    const int part = warp & (w - 1);
     if (t >= a.tokens) return;
-    auto pos = [&](int axis) -> int64_t { return a.positions[axis * a.tokens + t]; };
+    Positions pos;
+    pos.load(a.positions, a.rot.axes, a.tokens, t);
     const int pieces = a.d >> 3;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -111,10 +116,10 @@ int launch_rotary(const RotaryParams& p, cudaStream_t stream) {
     a.heads[0] = (int)p.hq; a.heads[1] = p.k ? (int)p.hkv : 0;
     if (p.tokens == 0 || a.heads[0] + a.heads[1] == 0) return FLASHCK_OK;
     const int64_t most = std::max<int64_t>(1, (p.hq + a.heads[1]) * p.d / 256);
-    int w = 8;
-    while (w > 1 && (w > most || p.tokens * w > (int64_t)sm_count() * 32)) w >>= 1;
-    a.warps_per_job = w;
-    const int64_t blocks = (p.tokens * w + 7) / 8;
+    int w = 3;
+    while (w > 0 && ((1 << w) > most || p.tokens << w > (int64_t)sm_count() * 32)) --w;
+    a.warps_log2 = w;
+    const int64_t blocks = ((p.tokens << w) + 7) / 8;
     FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: too many tokens");
     if (p.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_type<__nv_bfloat16>(a, (unsigned)blocks, stream));
     else FCK_CUDA(launch_type<__half>(a, (unsigned)blocks, stream));
