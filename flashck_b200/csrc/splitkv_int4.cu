@@ -34,7 +34,7 @@ namespace {
 constexpr int kPairs = 256;  // (head, token) pairs of a stage
 constexpr int kUnit = 32;    // tokens a warp takes of it
 constexpr int kCentre = 4;   // units between two centrings
-constexpr uint32_t kLowCodes = 0x000f000fu, kHighCodes = 0x00f000f0u;
+constexpr uint32_t kCode = 0x000f000fu;
 
 struct Int4Dev {
     const void* q;
@@ -50,6 +50,7 @@ struct Int4Dev {
     int batch, seqlen_q, hq, hkv, num_splits, total_q, bt_stride, page, pool, room;  // room: tokens that a sequence's part of the cache has
     int mask_type, wl, wr;
     int heads_log2, chunk_log2, stages;  // kv heads of a CTA; tokens of a box
+    int line_log2;                       // bytes of a box's innermost rows: 128, or what the CTA's heads have
     float scale_log2;
 };
 
@@ -61,6 +62,23 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
+}
+template <int N>
+__device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void registers_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N)); }
+// The four fields of a word whose halves hold four codes each, as halves over 2^24: first the lowest, then 16 times the next one (from the
+// byte that both make up, less the lowest: that subtraction runs beside the masks, which have half of its rate), the same of the upper bytes.
+__device__ __forceinline__ uint32_t less(uint32_t a, uint32_t b) {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+__device__ __forceinline__ void fields(uint32_t w, uint32_t (&f)[4]) {
+    const uint32_t lower = w & 0x00ff00ffu, upper = __byte_perm(w, 0, 0x4341);
+    f[0] = w & kCode;
+    f[1] = less(lower, f[0]);
+    f[2] = upper & kCode;
+    f[3] = less(upper, f[2]);
 }
 __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -79,13 +97,22 @@ __device__ __forceinline__ uint32_t halves(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Shared memory of a stage: K codes, V codes, K params, V params [heads][tokens + 1][NG] (the extra entry keeps the producer's lanes, which
-// walk the heads, off one bank).
+// Shared memory of a stage: K codes, V codes [chunk][128-byte column][token] rows, K params, V params [token] rows of the CTA's heads with 16
+// bytes between two where they are 32 bytes and longer (a warp's reads, of 8 tokens, then meet no bank twice).
 template <int D, int NG>
 struct Stage {
     static constexpr int kCodes = kPairs * (D / 2);
-    static constexpr int kParams = (kPairs + 8) * NG * 4;
+    static constexpr int kParams = kPairs * NG * 4 + 512 * NG;
     static constexpr int kBytes = (2 * kCodes + 2 * kParams + 1023) / 1024 * 1024;
+};
+
+// Registers of the warpgroups: 8 TEAMS warps with kConsumer and 4 with kProducer share what the block is launched with, kLaunch a thread (what
+// its launch bounds leave: 65536 / threads, down to a multiple of 8).
+template <int TEAMS>
+struct Split {
+    static constexpr int kThreads = (8 * TEAMS + 4) * 32, kLaunch = 65536 / kThreads / 8 * 8;
+    static constexpr int kProducer = TEAMS == 2 ? 32 : 40, kConsumer = TEAMS == 2 ? 112 : 232;
+    static_assert((8 * TEAMS * kConsumer + 4 * kProducer) * 32 <= kThreads * kLaunch, "an increase would wait for good");
 };
 
 // What one warp has summed over its keys, for rows 2t and 2t + 1 (t = lane % 4) of each of NT tiles of 8 rows.
@@ -99,7 +126,7 @@ struct Sums {
 };
 
 template <typename T, int D, int NG, int NT, int TEAMS>
-__global__ void __launch_bounds__((8 * TEAMS + 1) * 32, 1)
+__global__ void __launch_bounds__((8 * TEAMS + 4) * 32, 1)
 splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Int4Dev p) {
     constexpr int ROW = D / 2, GR = D / 32, PER = GR / NG;  // bytes of a row; 16-byte pieces (32 channels) of it; of them per group
     constexpr int kConsumers = 8 * TEAMS;
@@ -188,13 +215,19 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int head0 = blockIdx.z << p.heads_log2;
     const int row0 = blockIdx.y * 8 * NT;  // first (token, group head) row of this CTA's tiles
 
-    if (warp == kConsumers) {
-        // =========================== producer warp ===========================================
+    if (warp >= kConsumers) {
+        // =========================== producer warp (of a warpgroup that gives its registers away) ===========================
+        registers_down<Split<TEAMS>::kProducer>();
+        if (warp > kConsumers) return;
         if (lane == 0) {
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
         }
-        const int chunk = 1 << p.chunk_log2, box = heads * chunk * ROW;
+        const int chunk = 1 << p.chunk_log2, box = heads * chunk * ROW, column0 = (head0 * ROW) >> p.line_log2;
+        // scales and least values: a lane copies a piece of 4 to 16 bytes of a token's, for K and V
+        const int width = heads * NG * 4, pitch = width + (width >= 32 ? 16 : 0);
+        const int piece_log2 = min(4, 31 - __clz(width)), pieces_log2 = 31 - __clz(width) - piece_log2;
+        const int copies = toks << pieces_log2;
         uint32_t it = 0;
         bool ok = true;
         for (int piece = blockIdx.x; piece < pieces && ok; piece += gridDim.x) {
@@ -232,20 +265,27 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     if (lane == 0) mbar_expect_tx(&full[s], 2 * chunks * box);
                     __syncwarp();
                     if (lane < chunks) {
-                        tma_load_4d(st + lane * box, &map_k, &full[s], 0, tok, head0, pg);
-                        tma_load_4d(st + St::kCodes + lane * box, &map_v, &full[s], 0, tok, head0, pg);
+                        tma_load_4d(st + lane * box, &map_k, &full[s], 0, tok, column0, pg);
+                        tma_load_4d(st + St::kCodes + lane * box, &map_v, &full[s], 0, tok, column0, pg);
                     }
-                    const int64_t at = pg < p.pool ? (int64_t)pg * p.page + tok : -1;  // row of the chunk's first token
+                    const int64_t at = pg < p.pool ? ((int64_t)pg * p.page + tok) * p.hkv + head0 : -1;  // the chunk's first (token, head)
                     const uint32_t dst = smem_u32(st + 2 * St::kCodes);
-#pragma unroll
-                    for (int i = 0; i < kPairs / 32; ++i) {
-                        const int e = i * 32 + lane, k = e >> p.heads_log2, h = e & (heads - 1);  // token of the tile, head of the CTA
-                        const int64_t row = __shfl_sync(0xffffffffu, at, k >> p.chunk_log2);
-                        const bool there = row >= 0 && token0 + k < len;  // (the rest of a tile has scales of zero)
-                        const int64_t off = there ? ((row + (k & (chunk - 1))) * p.hkv + head0 + h) * (4 * NG) : 0;
-                        const uint32_t to = dst + (h * (toks + 1) + k) * (4 * NG);
-                        copy_async<4 * NG>(to, p.k_params + off, there);
-                        copy_async<4 * NG>(to + St::kParams, p.v_params + off, there);
+                    for (int e = lane; e < copies; e += 32) {
+                        const int k = e >> pieces_log2, part = (e & ((1 << pieces_log2) - 1)) << piece_log2;  // token of the tile, byte of its row
+                        const int64_t first = __shfl_sync(0xffffffffu, at, k >> p.chunk_log2);
+                        const bool there = first >= 0 && token0 + k < len;  // (the rest of a tile has scales of zero)
+                        const int64_t off = there ? (first + (int64_t)(k & (chunk - 1)) * p.hkv) * (4 * NG) + part : 0;
+                        const uint32_t to = dst + k * pitch + part;
+                        if (piece_log2 == 4) {
+                            copy_async<16>(to, p.k_params + off, there);
+                            copy_async<16>(to + St::kParams, p.v_params + off, there);
+                        } else if (piece_log2 == 3) {
+                            copy_async<8>(to, p.k_params + off, there);
+                            copy_async<8>(to + St::kParams, p.v_params + off, there);
+                        } else {
+                            copy_async<4>(to, p.k_params + off, there);
+                            copy_async<4>(to + St::kParams, p.v_params + off, there);
+                        }
                     }
                     arrive_after_copies(&full[s]);
                 }
@@ -278,24 +318,32 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
 
     // =============================== consumer warps =============================================
+    registers_up<Split<TEAMS>::kConsumer>();
     const int team = warp >> 3, wi = warp & 7;
     const int hw = wi & (heads - 1), unit = wi >> p.heads_log2;  // head of the CTA; which 32 tokens of a tile
     const int kh = head0 + hw;
     const int g = lane >> 2, t4 = lane & 3;
-    // Keys are taken in an order in which neither the K reads (row kap(g)) nor the V reads (rows kap(2t), kap(2t + 1)) meet a bank twice.
-    auto kap = [](int i) { const int x = i & 3; return (i & 4) | (x == 0 ? 0 : x == 1 ? 3 : x == 2 ? 1 : 2); };
-    auto swizzle = [](int row) { return D == 128 ? (row >> 1) & 3 : (row >> 2) & 1; };  // of a row's 16-byte pieces, as the boxes have it
-    const int kkey = kap(g), vkey0 = kap(2 * t4), vkey1 = kap(2 * t4 + 1);
-    int koff[GR], voff0[GR], voff1[GR];
+    // ldmatrix: this lane's row of the four 8 x 16-byte matrices of 16 keys and two 16-byte pieces (32 channels each): matrix m holds keys
+    // 8 (m & 1) .. + 7 and piece m >> 1.  Swizzled as the boxes are, the 8 rows of a matrix lie in different banks.
+    const int mrow = (lane & 7) + 8 * ((lane >> 3) & 1);
+    const int mswz = p.line_log2 == 7 ? lane & 7 : p.line_log2 == 6 ? (lane >> 1) & 3 : (lane >> 2) & 1;
+    const int per_line_log2 = p.line_log2 - (D == 128 ? 6 : 5);  // heads of a line
+    uint32_t off[2][GR / 2];  // of the warp's two blocks of 16 keys in a stage
 #pragma unroll
-    for (int i = 0; i < GR; ++i) {
-        koff[i] = kkey * ROW + ((i ^ swizzle(kkey)) << 4) + t4 * 4;
-        voff0[i] = vkey0 * ROW + ((i ^ swizzle(vkey0)) << 4) + (g >> 1) * 4;
-        voff1[i] = vkey1 * ROW + ((i ^ swizzle(vkey1)) << 4) + (g >> 1) * 4;
+    for (int u = 0; u < 2; ++u) {
+        const int k = unit * kUnit + 16 * u, c = k >> p.chunk_log2;  // (chunks of 16 tokens or more)
+        const int column = (c << (p.heads_log2 - per_line_log2)) + (hw >> per_line_log2);
+        const int row = (column << p.chunk_log2) + (k & ((1 << p.chunk_log2) - 1)) + mrow;
+        const int first = (hw & ((1 << per_line_log2) - 1)) * GR;
+#pragma unroll
+        for (int i = 0; i < GR / 2; ++i) off[u][i] = (row << p.line_log2) + (((first + 2 * i + (lane >> 4)) ^ mswz) << 4);
     }
-    const uint32_t pick = (g & 1) ? 0x7632u : 0x5410u;  // the 16-bit half of a word of V codes that is this lane's
+    const int width = heads * NG * 4, pitch = width + (width >= 32 ? 16 : 0);
+    const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * pitch + hw * (4 * NG);
+    const uint32_t ring_at = smem_u32(ring);
     bool failed = false;
-    uint32_t it = 0;
+    int stage = 0, turn = 0;  // the ring's next stage, the parity of its use; whose turn it is
+    uint32_t phase = 0;
 
     for (int piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
         int lo, hi, b = begin_piece(piece, lo, hi);
@@ -310,7 +358,6 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             // ---- Q^T fragments: this lane has channels 32 i + 8 t .. + 7 of row g, as halves scaled by a power of two ----
             uint32_t qf[NT][GR][4];
             float ka[NT][2], kb[NT][NG][2];  // x = ka * (s . a) + kb . m for rows 2t and 2t + 1
-            int key_lo[NT][2], key_hi[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int r = row0 + 8 * n + g, i = r / G;
@@ -362,15 +409,14 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     ka[n][e] = scale * 16777216.f;
 #pragma unroll
                     for (int k = 0; k < NG; ++k) kb[n][k][e] = scale * __shfl_sync(0xffffffffu, sum[k], from);
-                    const int re = row0 + 8 * n + 2 * t4 + e;
-                    visible_range(re / G, sq, len, p.mask_type, p.wl, p.wr, key_lo[n][e], key_hi[n][e]);
-                    if (re >= rows) { key_lo[n][e] = 0; key_hi[n][e] = len - 1; }
                 }
             }
             int mask_from = len;  // first key that some row may not see
+            int mask_below = 0;     // and the first one that no row's left bound hides
             if (p.mask_type != 0) {
-                if (p.wr >= 0) mask_from = min(mask_from, (p.mask_type == 2 ? len - sq : 0) + p.wr + 1);
-                if (p.wl >= 0) mask_from = 0;
+                const int shift = p.mask_type == 2 ? len - sq : 0;
+                if (p.wr >= 0) mask_from = min(mask_from, shift + p.wr + 1);
+                if (p.wl >= 0) mask_below = shift + sq - 1 - p.wl;
             }
 
             Sums<D, NG, NT> z;
@@ -408,26 +454,24 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             };
             bool first = true;
             int uncentred = 0;  // units
-            for (int t = ta; t < tb; ++t, ++it) {
-                if (TEAMS == 2 && (int)(it & 1u) != team) continue;
-                const int s = it % stages;
-                if (failed || !mbar_wait_bounded(&full[s], (it / stages) & 1u, abort_flag, p.status, 0x200)) { failed = true; continue; }
+            for (int t = ta; t < tb; ++t) {
+                const int now = stage, mine = TEAMS == 1 || turn == team;
+                const uint32_t parity = phase;
+                turn ^= 1;
+                if (++stage == stages) {
+                    stage = 0;
+                    phase ^= 1u;
+                }
+                if (!mine) continue;
+                if (failed || !mbar_wait_bounded(&full[now], parity, abort_flag, p.status, 0x200)) { failed = true; continue; }
                 const int key0 = ((tile0[b] + t) << tok_log2) + unit * kUnit;
                 if (key0 < len) {
-                    const uint8_t* st = ring + (size_t)s * St::kBytes;
-                    const uint8_t* pk = st + 2 * St::kCodes + (hw * (toks + 1) + unit * kUnit) * (4 * NG);
-                    // 16-key blocks of this unit: chunks of 16 tokens or more, [chunk][head][token] rows
-                    const uint8_t* block[2];
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int k = unit * kUnit + 16 * u, c = k >> p.chunk_log2;
-                        block[u] = st + ((((c << p.heads_log2) + hw) << p.chunk_log2) + (k & ((1 << p.chunk_log2) - 1))) * ROW;
-                    }
-                    const bool masked = key0 + kUnit > mask_from;
-                    auto visible = [&](int n, int e, int key) { return key >= key_lo[n][e] && key <= key_hi[n][e]; };
-                    // scale and least value of the lane's key kkey + 8 i of the unit
+                    const uint32_t st = ring_at + now * St::kBytes;
+                    const uint8_t* pk = ring + now * St::kBytes + param_off;
+                    const bool masked = key0 + kUnit > mask_from || key0 < mask_below;
+                    // scale and least value of the lane's key g + 8 i of the unit
                     auto param = [&](const uint8_t* base, int i, int k, float& sc, float& least) {
-                        const uint32_t w = reinterpret_cast<const uint32_t*>(base)[(kkey + 8 * i) * NG + k];
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + 8 * i * pitch + 4 * k);
                         sc = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[0]);
                         least = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[1]);
                     };
@@ -441,17 +485,21 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                             for (int k = 0; k < NG; ++k) a[n][k][0] = a[n][k][1] = a[n][k][2] = a[n][k][3] = 0.f;
 #pragma unroll
-                        for (int c = 0; c < GR; ++c) {
-                            uint32_t w0 = *reinterpret_cast<const uint32_t*>(block[u] + koff[c]);
-                            uint32_t w1 = *reinterpret_cast<const uint32_t*>(block[u] + koff[c] + 8 * ROW);
-                            const uint32_t f0[4] = {w0 & kLowCodes, w1 & kLowCodes, w0 & kHighCodes, w1 & kHighCodes};
-                            w0 >>= 8;
-                            w1 >>= 8;
-                            const uint32_t f1[4] = {w0 & kLowCodes, w1 & kLowCodes, w0 & kHighCodes, w1 & kHighCodes};
+                        for (int i = 0; i < GR / 2; ++i) {
+                            uint32_t w[4];  // keys g, g + 8 of piece 2 i, of piece 2 i + 1: the lane's 8 channels
+                            ldmatrix_x4(w, st + off[u][i]);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                mma_16816<__half>(a[n][c / PER], f0, qf[n][c][0], qf[n][c][1]);
-                                mma_16816<__half>(a[n][c / PER], f1, qf[n][c][2], qf[n][c][3]);
+                            for (int h = 0; h < 2; ++h) {
+                                const int c = 2 * i + h;
+                                uint32_t f0[4], f1[4];
+                                fields(w[2 * h], f0);
+                                fields(w[2 * h + 1], f1);
+                                const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    mma_16816<__half>(a[n][c / PER], a0, qf[n][c][0], qf[n][c][1]);
+                                    mma_16816<__half>(a[n][c / PER], a1, qf[n][c][2], qf[n][c][3]);
+                                }
                             }
                         }
 #pragma unroll
@@ -477,10 +525,16 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
+                            for (int e = 0; e < 2; ++e) {
+                                const int r = row0 + 8 * n + 2 * t4 + e;
+                                int first_key = 0, last_key = len - 1;
+                                if (r < rows) visible_range(r / G, sq, len, p.mask_type, p.wl, p.wr, first_key, last_key);
 #pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                    if (!visible(n, e, key0 + kkey + 8 * i)) x[n][i][e] = -INFINITY;
+                                for (int i = 0; i < 4; ++i) {
+                                    const int key = key0 + g + 8 * i;
+                                    if (key < first_key || key > last_key) x[n][i][e] = -INFINITY;
+                                }
+                            }
                     }
                     // ---- weights, in the row's reference; the second round is the one after it has moved ----
                     float vs[4][NG], vm[4][NG];
@@ -591,25 +645,27 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             for (int i = 0; i < 4; ++i) wt[n][k][i] = transpose8x8(wt[n][k][i]);
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        const uint8_t* vb = block[u] + St::kCodes;
                         constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
                             for (int k = 0; k < NG; ++k) mma_16816<__half>(z.ones[n][k], kOnes, wt[n][k][2 * u], wt[n][k][2 * u + 1]);
 #pragma unroll
-                        for (int c = 0; c < GR; ++c) {
-                            const uint32_t wa = *reinterpret_cast<const uint32_t*>(vb + voff0[c]), wb = *reinterpret_cast<const uint32_t*>(vb + voff1[c]);
-                            const uint32_t wc = *reinterpret_cast<const uint32_t*>(vb + voff0[c] + 8 * ROW),
-                                           wd = *reinterpret_cast<const uint32_t*>(vb + voff1[c] + 8 * ROW);
-                            uint32_t y0 = __byte_perm(wa, wb, pick), y1 = __byte_perm(wc, wd, pick);
-                            const uint32_t z0 = y0 >> 8, z1 = y1 >> 8;
-                            const uint32_t even_ch[4] = {y0 & kLowCodes, z0 & kLowCodes, y1 & kLowCodes, z1 & kLowCodes};      // channels 0, 2
-                            const uint32_t odd_ch[4] = {y0 & kHighCodes, z0 & kHighCodes, y1 & kHighCodes, z1 & kHighCodes};  // 1, 3: times 16
+                        for (int i = 0; i < GR / 2; ++i) {
+                            uint32_t y[4];  // transposed: codes 4 g .. + 3 of piece 2 i, keys 2 t, 2 t + 1 and the same + 8; of piece 2 i + 1
+                            ldmatrix_x4_trans(y, st + St::kCodes + off[u][i]);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                mma_16816<__half>(z.o[n][c][0], even_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
-                                mma_16816<__half>(z.o[n][c][1], odd_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
+                            for (int h = 0; h < 2; ++h) {
+                                const int c = 2 * i + h;
+                                uint32_t f0[4], f1[4];
+                                fields(y[2 * h], f0);
+                                fields(y[2 * h + 1], f1);
+                                const uint32_t even_ch[4] = {f0[0], f0[2], f1[0], f1[2]}, odd_ch[4] = {f0[1], f0[3], f1[1], f1[3]};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    mma_16816<__half>(z.o[n][c][0], even_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
+                                    mma_16816<__half>(z.o[n][c][1], odd_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
+                                }
                             }
                         }
                     }
@@ -621,7 +677,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 // the last reads of the stage have to have come back before it is given back (see splitkv_decode.cu)
                 __threadfence_block();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[s]);
+                if (lane == 0) mbar_arrive(&empty[now]);
             }
 
             // ---- this warp's sums: O[n][e][c] = channels 32 c + 4 g .. + 3 of row 2t + e, in reference R ----
@@ -713,19 +769,20 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
 }
 
-// Codes of a pool as (bytes of a row, token of the page, kv head, page); a box lands as [head][token][row].
-int make_codes_map(CUtensorMap* map, const void* base, int64_t pool, int64_t page, int64_t hkv, int D, int heads, int chunk) {
+// Codes of a pool as (bytes of a line, token of the page, line of the token, page); a box lands as [line][token][bytes].  (TMA takes a few
+// cycles for an innermost row: with 64-byte rows, a head each, it fetched 4.0 TB/s.)
+int make_codes_map(CUtensorMap* map, const void* base, int64_t pool, int64_t page, int64_t token_bytes, int line, int box_lines, int chunk) {
     PFN_encodeTiled enc = get_encode_tiled();
     FCK_REQUIRE(enc != nullptr, FLASHCK_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
-    const cuuint64_t dims[4] = {(cuuint64_t)(D / 2), (cuuint64_t)page, (cuuint64_t)hkv, (cuuint64_t)pool};
-    const cuuint64_t strides[3] = {(cuuint64_t)(hkv * D / 2), (cuuint64_t)(D / 2), (cuuint64_t)(page * hkv * D / 2)};
-    const cuuint32_t box[4] = {(cuuint32_t)(D / 2), (cuuint32_t)chunk, (cuuint32_t)heads, 1};
+    const cuuint64_t dims[4] = {(cuuint64_t)line, (cuuint64_t)page, (cuuint64_t)(token_bytes / line), (cuuint64_t)pool};
+    const cuuint64_t strides[3] = {(cuuint64_t)token_bytes, (cuuint64_t)line, (cuuint64_t)(page * token_bytes)};
+    const cuuint32_t box[4] = {(cuuint32_t)line, (cuuint32_t)chunk, (cuuint32_t)box_lines, 1};
     const cuuint32_t estr[4] = {1, 1, 1, 1};
+    const CUtensorMapSwizzle swizzle = line == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : line == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B;
     const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           D == 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_32B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    FCK_REQUIRE(r == CUDA_SUCCESS, FLASHCK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for pool pages=%lld page=%lld hkv=%lld hdim=%d", (int)r,
-                (long long)pool, (long long)page, (long long)hkv, D);
+                           swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    FCK_REQUIRE(r == CUDA_SUCCESS, FLASHCK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for pool pages=%lld page=%lld bytes of a token=%lld", (int)r,
+                (long long)pool, (long long)page, (long long)token_bytes);
     return FLASHCK_OK;
 }
 
@@ -747,20 +804,26 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     dev.stages = (int)std::min<size_t>(8, (room - fixed) / (St::kBytes + 16));
     const size_t smem = fixed + (size_t)dev.stages * (St::kBytes + 16);
     CUtensorMap mk, mv;
-    if (int rc = make_codes_map(&mk, c.k_codes, c.pool, c.page, c.hkv, D, heads, chunk)) return rc;
-    if (int rc = make_codes_map(&mv, c.v_codes, c.pool, c.page, c.hkv, D, heads, chunk)) return rc;
+    const int line = std::min(128, heads * (D / 2)), lines = heads * (D / 2) / line;
+    dev.line_log2 = line == 128 ? 7 : line == 64 ? 6 : 5;
+    if (int rc = make_codes_map(&mk, c.k_codes, c.pool, c.page, c.hkv * (D / 2), line, lines, chunk)) return rc;
+    if (int rc = make_codes_map(&mv, c.v_codes, c.pool, c.page, c.hkv * (D / 2), line, lines, chunk)) return rc;
     auto kern = splitkv_int4_kernel<T, D, NG, NT, TEAMS>;
     static thread_local int configured_device = -1;  // per instantiation
     int devid = 0;
     FCK_CUDA(cudaGetDevice(&devid));
     if (configured_device != devid) {
         FCK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room));
+        cudaFuncAttributes attr;
+        FCK_CUDA(cudaFuncGetAttributes(&attr, kern));
+        FCK_REQUIRE(attr.numRegs == Split<TEAMS>::kLaunch, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: built with %d registers a thread instead of %d",
+                    attr.numRegs, Split<TEAMS>::kLaunch);  // (the warpgroups' shares would not add up)
         configured_device = devid;
     }
     const int64_t gy = (p.max_seqlen_q * (p.hq / c.hkv) + 8 * NT - 1) / (8 * NT), gz = c.hkv / heads;
     FCK_REQUIRE(gy <= 65535, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: too many query rows per kv head");
     const int64_t gx = std::max<int64_t>(1, sm_count() / (gy * gz));  // one wave, where the heads and rows leave one
-    FCK_CUDA(launch_dependent(kern, dim3((unsigned)gx, (unsigned)gy, (unsigned)gz), dim3((8 * TEAMS + 1) * 32), smem, stream, mk, mv, dev));
+    FCK_CUDA(launch_dependent(kern, dim3((unsigned)gx, (unsigned)gy, (unsigned)gz), dim3(Split<TEAMS>::kThreads), smem, stream, mk, mv, dev));
     return FLASHCK_OK;
 }
 
