@@ -34,6 +34,7 @@ namespace {
 constexpr int kPairs = 256;  // (head, token) pairs of a stage
 constexpr int kUnit = 32;    // tokens a warp takes of it
 constexpr int kCentre = 4;   // units between two centrings
+constexpr int kMeetWarps = 4;  // warps that hand their sums over at a time
 constexpr uint32_t kCode = 0x000f000fu;
 
 struct Int4Dev {
@@ -97,12 +98,11 @@ __device__ __forceinline__ uint32_t halves(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Shared memory of a stage: K codes, V codes [chunk][128-byte column][token] rows, K params, V params [token] rows of the CTA's heads with 16
-// bytes between two where they are 32 bytes and longer (a warp's reads, of 8 tokens, then meet no bank twice).
+// Shared memory of a stage: K codes, V codes [chunk][128-byte column][token] rows, K params, V params [token] rows of the CTA's heads.
 template <int D, int NG>
 struct Stage {
     static constexpr int kCodes = kPairs * (D / 2);
-    static constexpr int kParams = kPairs * NG * 4 + 512 * NG;
+    static constexpr int kParams = kPairs * NG * 4;
     static constexpr int kBytes = (2 * kCodes + 2 * kParams + 1023) / 1024 * 1024;
 };
 
@@ -137,8 +137,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int heads = 1 << p.heads_log2, tok_log2 = 8 - p.heads_log2, toks = 1 << tok_log2;
 
     uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-    float4* meet = reinterpret_cast<float4*>(ring + (size_t)stages * St::kBytes);  // [4 TEAMS or 8][row pair floats]: the warps' sums
-    constexpr int kMeetWarps = TEAMS == 2 ? 8 : 4, kMeetFloat4 = NT * 2 * GR;      // float4 per lane
+    float4* meet = reinterpret_cast<float4*>(ring + (size_t)stages * St::kBytes);  // [kMeetWarps][rows and columns of a lane][lane]: warps' sums
+    constexpr int kMeetFloat4 = NT * 2 * GR;  // float4 per lane
     float* meet_stats = reinterpret_cast<float*>(meet + kMeetWarps * kMeetFloat4 * 32);  // [warp][NT][2][8 rows: ref, l]
     uint64_t* bars = reinterpret_cast<uint64_t*>(meet_stats + kMeetWarps * NT * 16);
     uint64_t* full = bars;
@@ -225,7 +225,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         const int chunk = 1 << p.chunk_log2, box = heads * chunk * ROW, column0 = (head0 * ROW) >> p.line_log2;
         // scales and least values: a lane copies a piece of 4 to 16 bytes of a token's, for K and V
-        const int width = heads * NG * 4, pitch = width + (width >= 32 ? 16 : 0);
+        const int width = heads * NG * 4;
         const int piece_log2 = min(4, 31 - __clz(width)), pieces_log2 = 31 - __clz(width) - piece_log2;
         const int copies = toks << pieces_log2;
         uint32_t it = 0;
@@ -237,27 +237,34 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 if (tb <= ta || row0 >= len_q(p, b) * G) continue;  // (the consumers skip the same segments)
                 const int len = len_k(p, b);
                 const int64_t bphys = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
-                // lane c looks after chunk c of a tile (at most 16), one tile ahead: its page, or one that is not there
-                auto entry = [&](int t, int& pg, int& tok) {
-                    const int token = ((tile0[b] + t) << tok_log2) + (lane << p.chunk_log2);
+                // pages of 32 chunks (a few tiles) per round, a lane each, loaded one round ahead; a page that is not there is one behind the pool
+                const int per_tile_log2 = tok_log2 - p.chunk_log2, first_chunk = (tile0[b] + ta) << per_tile_log2;
+                auto entry = [&](int c, int& pg, int& tok) {
+                    const int64_t token = (int64_t)(first_chunk + c) << p.chunk_log2;
                     pg = p.pool;
                     tok = 0;
-                    if (t >= tb || token >= len || lane >= (toks >> p.chunk_log2)) return;
+                    if (token >= len || c >= (tb - ta) << per_tile_log2) return;
                     if (p.block_table) {
-                        const int slot = token / p.page;
-                        tok = token - slot * p.page;
+                        const int slot = (int)token / p.page;
+                        tok = (int)token - slot * p.page;
                         const int id = slot < p.bt_stride ? p.block_table[bphys * p.bt_stride + slot] : -1;
                         if ((uint32_t)id < (uint32_t)p.pool) pg = id;
                     } else {
-                        tok = token;
+                        tok = (int)token;
                         if ((uint64_t)bphys < (uint64_t)p.pool) pg = (int)bphys;
                     }
                 };
-                int pg_next, tok_next;
-                entry(ta, pg_next, tok_next);
+                int pg_cur, tok_cur, pg_next, tok_next;
+                entry(lane, pg_next, tok_next);
                 for (int t = ta; t < tb; ++t, ++it) {
-                    const int pg = pg_next, tok = tok_next, s = it % stages;
-                    entry(t + 1, pg_next, tok_next);
+                    const int s = it % stages, c0 = (t - ta) << per_tile_log2;  // the tile's first chunk
+                    if ((c0 & 31) == 0) {
+                        pg_cur = pg_next;
+                        tok_cur = tok_next;
+                        entry(c0 + 32 + lane, pg_next, tok_next);
+                    }
+                    const int from = (c0 & 31) + (lane & ((1 << per_tile_log2) - 1));
+                    const int pg = __shfl_sync(0xffffffffu, pg_cur, from), tok = __shfl_sync(0xffffffffu, tok_cur, from);
                     const int token0 = (tile0[b] + t) << tok_log2;
                     const int chunks = min(toks >> p.chunk_log2, (len - token0 + chunk - 1) >> p.chunk_log2);
                     if (!mbar_wait_bounded(&empty[s], ((it / stages) & 1u) ^ 1u, abort_flag, p.status, 0x100)) { ok = false; break; }
@@ -275,7 +282,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         const int64_t first = __shfl_sync(0xffffffffu, at, k >> p.chunk_log2);
                         const bool there = first >= 0 && token0 + k < len;  // (the rest of a tile has scales of zero)
                         const int64_t off = there ? (first + (int64_t)(k & (chunk - 1)) * p.hkv) * (4 * NG) + part : 0;
-                        const uint32_t to = dst + k * pitch + part;
+                        const uint32_t to = dst + k * width + part;
                         if (piece_log2 == 4) {
                             copy_async<16>(to, p.k_params + off, there);
                             copy_async<16>(to + St::kParams, p.v_params + off, there);
@@ -338,8 +345,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
         for (int i = 0; i < GR / 2; ++i) off[u][i] = (row << p.line_log2) + (((first + 2 * i + (lane >> 4)) ^ mswz) << 4);
     }
-    const int width = heads * NG * 4, pitch = width + (width >= 32 ? 16 : 0);
-    const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * pitch + hw * (4 * NG);
+    const int width = heads * NG * 4;
+    const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * width + hw * (4 * NG);
     const uint32_t ring_at = smem_u32(ring);
     bool failed = false;
     int stage = 0, turn = 0;  // the ring's next stage, the parity of its use; whose turn it is
@@ -471,7 +478,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     const bool masked = key0 + kUnit > mask_from || key0 < mask_below;
                     // scale and least value of the lane's key g + 8 i of the unit
                     auto param = [&](const uint8_t* base, int i, int k, float& sc, float& least) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + 8 * i * pitch + 4 * k);
+                        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + 8 * i * width + 4 * k);
                         sc = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[0]);
                         least = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[1]);
                     };
@@ -707,10 +714,11 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                                  fmaf(16777216.f, z.o[n][c][0][2 + e], add), fmaf(1048576.f, z.o[n][c][1][2 + e], add));
                     }
                 }
-            // ---- the warps of a head meet: the upper half hands its sums to the lower one until one warp per head is left ----
-            for (int step = kConsumers / 2; step >= heads; step >>= 1) {
-                if (warp >= step && warp < 2 * step) {
-                    const int slot = warp - step;
+            // ---- the warps of a head meet: the upper half hands its sums to the lower one until one warp per head is left,
+            // kMeetWarps at a time ----
+            for (int from = kConsumers / 2, step = from; step >= heads; from = from + kMeetWarps < 2 * step ? from + kMeetWarps : (step >>= 1)) {
+                const int slot = warp - from, to = warp - (from - step);  // of the one that hands over, and of the one that takes
+                if (slot >= 0 && slot < min(kMeetWarps, step)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -724,12 +732,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         }
                 }
                 asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
-                if (warp < step) {
+                if (to >= 0 && to < min(kMeetWarps, step)) {
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int e = 0; e < 2; ++e) {
-                            const float ref = meet_stats[((warp * NT + n) * 8 + 2 * t4 + e) * 2], lo_ = meet_stats[((warp * NT + n) * 8 + 2 * t4 + e) * 2 + 1];
+                            const float ref = meet_stats[((to * NT + n) * 8 + 2 * t4 + e) * 2], lo_ = meet_stats[((to * NT + n) * 8 + 2 * t4 + e) * 2 + 1];
                             if (lo_ != -1.f) {
                                 const float both = has[n][e] ? fmaxf(ref, z.ref[n][e]) : ref;
                                 const float fa = has[n][e] ? fast_exp2(z.ref[n][e] - both) : 0.f, fb = fast_exp2(ref - both);
@@ -738,7 +746,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 l[n][e] = l[n][e] * fa + lo_ * fb;
 #pragma unroll
                                 for (int c = 0; c < GR; ++c) {
-                                    const float4 y = meet[(warp * kMeetFloat4 + (n * 2 + e) * GR + c) * 32 + lane];
+                                    const float4 y = meet[(to * kMeetFloat4 + (n * 2 + e) * GR + c) * 32 + lane];
                                     float4& v = o[n][e][c];
                                     v = make_float4(v.x * fa + y.x * fb, v.y * fa + y.y * fb, v.z * fa + y.z * fb, v.w * fa + y.w * fb);
                                 }
@@ -795,13 +803,14 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     int chunk = 16;
     dev.chunk_log2 = 4;
     while (2 * chunk <= toks && (!c.block_table || c.page % (2 * chunk) == 0)) { chunk *= 2; ++dev.chunk_log2; }
-    constexpr int kMeetWarps = TEAMS == 2 ? 8 : 4;
     const size_t meet = (size_t)kMeetWarps * NT * (2 * (D / 32) * 32 * 16 + 64);
     const size_t fixed = 1024 + meet + (size_t)(2 * c.batch + 4) * sizeof(int);
     const size_t room = 227 * 1024;
     FCK_REQUIRE(fixed + 2 * (St::kBytes + 16) <= room, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch %lld leaves no room for two stages",
                 (long long)c.batch);
-    dev.stages = (int)std::min<size_t>(8, (room - fixed) / (St::kBytes + 16));
+    // Two teams: an even number, so that a stage always falls to the same team.  (A parity tells two neighbouring uses apart: a team that came to a
+    // stage for every other use could take the other team's, not yet filled, for the one before its own.)
+    dev.stages = (int)std::min<size_t>(8, (room - fixed) / (St::kBytes + 16)) & ~(TEAMS - 1);
     const size_t smem = fixed + (size_t)dev.stages * (St::kBytes + 16);
     CUtensorMap mk, mv;
     const int line = std::min(128, heads * (D / 2)), lines = heads * (D / 2) / line;
