@@ -36,6 +36,7 @@ constexpr int kUnit = 32;    // tokens a warp takes of it
 constexpr int kCentre = 4;   // units between two centrings
 constexpr int kMeetWarps = 4;  // warps that hand their sums over at a time
 constexpr uint32_t kCode = 0x000f000fu;
+constexpr float kNoKey = -1e30f;  // (any score is so far above it that the reference moves)
 
 struct Int4Dev {
     const void* q;
@@ -122,13 +123,14 @@ struct Sums {
     float ones[NT][NG][4];      // sum w since the last centring (entries 0 and 1; the fragment's lower rows repeat them)
     float mid[NT][NG][2];       // sum p' (m + 8 s) over the lane's keys
     float l[NT][2];             // sum p' over the lane's keys
-    float m[NT][2], j[NT][2], ref[NT][2];  // largest x, largest x + log2 s, and R at its last move
+    float ref[NT][2];           // R; kNoKey before the first key
 };
 
 template <typename T, int D, int NG, int NT, int TEAMS>
 __global__ void __launch_bounds__((8 * TEAMS + 4) * 32, 1)
 splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Int4Dev p) {
     constexpr int ROW = D / 2, GR = D / 32, PER = GR / NG;  // bytes of a row; 16-byte pieces (32 channels) of it; of them per group
+    constexpr int ACCS = GR / NG >= 4 ? 2 : 1;
     constexpr int kConsumers = 8 * TEAMS;
     using St = Stage<D, NG>;
     extern __shared__ uint8_t smem_raw[];
@@ -335,21 +337,21 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int mrow = (lane & 7) + 8 * ((lane >> 3) & 1);
     const int mswz = p.line_log2 == 7 ? lane & 7 : p.line_log2 == 6 ? (lane >> 1) & 3 : (lane >> 2) & 1;
     const int per_line_log2 = p.line_log2 - (D == 128 ? 6 : 5);  // heads of a line
-    uint32_t off[2][GR / 2];  // of the warp's two blocks of 16 keys in a stage
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int k = unit * kUnit + 16 * u, c = k >> p.chunk_log2;  // (chunks of 16 tokens or more)
+    uint32_t off;  // of the warp's first 16 keys in a stage (piece 2 i: exclusive or with 32 i); the next 16 are block_step behind
+    {
+        const int k = unit * kUnit, c = k >> p.chunk_log2;
         const int column = (c << (p.heads_log2 - per_line_log2)) + (hw >> per_line_log2);
         const int row = (column << p.chunk_log2) + (k & ((1 << p.chunk_log2) - 1)) + mrow;
-        const int first = (hw & ((1 << per_line_log2) - 1)) * GR;
-#pragma unroll
-        for (int i = 0; i < GR / 2; ++i) off[u][i] = (row << p.line_log2) + (((first + 2 * i + (lane >> 4)) ^ mswz) << 4);
+        off = (row << p.line_log2) + ((((hw & ((1 << per_line_log2) - 1)) * GR + (lane >> 4)) ^ mswz) << 4);
     }
+    const uint32_t block_step = p.chunk_log2 == 4 ? heads * 16 * ROW : 16u << p.line_log2;  // (the next chunk, or further down this one)
     const int width = heads * NG * 4;
     const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * width + hw * (4 * NG);
     const uint32_t ring_at = smem_u32(ring);
     bool failed = false;
-    int stage = 0, turn = 0;  // the ring's next stage, the parity of its use; whose turn it is
+    // Tiles are counted over all segments; a team takes every TEAMS-th.  tile_count: before this segment; next: this team's next one, its stage and
+    // the parity of its use.
+    int tile_count = 0, next = TEAMS == 2 ? team : 0, stage = next;
     uint32_t phase = 0;
 
     for (int piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
@@ -437,8 +439,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.ones[n][k][2] = z.ones[n][k][3] = z.mid[n][k][0] = z.mid[n][k][1] = 0.f;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    z.l[n][e] = z.ref[n][e] = 0.f;
-                    z.m[n][e] = z.j[n][e] = -INFINITY;
+                    z.l[n][e] = 0.f;
+                    z.ref[n][e] = kNoKey;
                 }
             }
 
@@ -459,21 +461,20 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.ones[n][k][2] = z.ones[n][k][3] = 0.f;
                 }
             };
-            bool first = true;
             int uncentred = 0;  // units
-            for (int t = ta; t < tb; ++t) {
-                const int now = stage, mine = TEAMS == 1 || turn == team;
+            for (int t = ta + next - tile_count; t < tb; t += TEAMS) {
+                const int now = stage;
                 const uint32_t parity = phase;
-                turn ^= 1;
-                if (++stage == stages) {
-                    stage = 0;
+                next += TEAMS;
+                stage += TEAMS;
+                if (stage >= stages) {
+                    stage -= stages;
                     phase ^= 1u;
                 }
-                if (!mine) continue;
                 if (failed || !mbar_wait_bounded(&full[now], parity, abort_flag, p.status, 0x200)) { failed = true; continue; }
                 const int key0 = ((tile0[b] + t) << tok_log2) + unit * kUnit;
                 if (key0 < len) {
-                    const uint32_t st = ring_at + now * St::kBytes;
+                    const uint32_t at = ring_at + now * St::kBytes + off;
                     const uint8_t* pk = ring + now * St::kBytes + param_off;
                     const bool masked = key0 + kUnit > mask_from || key0 < mask_below;
                     // scale and least value of the lane's key g + 8 i of the unit
@@ -482,167 +483,197 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         sc = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[0]);
                         least = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[1]);
                     };
-                    // ---- x = log2(e) scale q . k, [n][4 keys][2 rows] ----
-                    float x[NT][4][2];
+                    float x[NT][4][2];       // scores of the lane's 4 keys and 2 rows, then weights p'
+                    uint32_t wt[NT][NG][4];  // p' s as halves
+                    bool careful = false;    // a hidden key's scale or least value is not finite: its weight of 0 must not meet it
+                    // Usually one round.  A second one (that starts from the scores again) moves the reference of rows that need it.
+#pragma unroll 1
+                    for (int round = 0;; ++round) {
+                        // ---- x = log2(e) scale q . k - R ----
+                        {
+                            float a[2][NT][NG * ACCS][4];  // (ACCS: chains of products that do not wait for one another)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        float a[NT][NG][4];
+                            for (int u = 0; u < 2; ++u)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
+                                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int k = 0; k < NG; ++k) a[n][k][0] = a[n][k][1] = a[n][k][2] = a[n][k][3] = 0.f;
+                                    for (int k = 0; k < NG * ACCS; ++k) a[u][n][k][0] = a[u][n][k][1] = a[u][n][k][2] = a[u][n][k][3] = 0.f;
 #pragma unroll
-                        for (int i = 0; i < GR / 2; ++i) {
-                            uint32_t w[4];  // keys g, g + 8 of piece 2 i, of piece 2 i + 1: the lane's 8 channels
-                            ldmatrix_x4(w, st + off[u][i]);
+                            for (int i = 0; i < GR / 2; ++i)
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                const int c = 2 * i + h;
-                                uint32_t f0[4], f1[4];
-                                fields(w[2 * h], f0);
-                                fields(w[2 * h + 1], f1);
-                                const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
+                                for (int u = 0; u < 2; ++u) {
+                                    uint32_t w[4];  // keys g, g + 8 of piece 2 i, of piece 2 i + 1: the lane's 8 channels
+                                    ldmatrix_x4(w, (at ^ (i << 5)) + u * block_step);
 #pragma unroll
-                                for (int n = 0; n < NT; ++n) {
-                                    mma_16816<__half>(a[n][c / PER], a0, qf[n][c][0], qf[n][c][1]);
-                                    mma_16816<__half>(a[n][c / PER], a1, qf[n][c][2], qf[n][c][3]);
+                                    for (int h = 0; h < 2; ++h) {
+                                        const int c = 2 * i + h;
+                                        uint32_t f0[4], f1[4];
+                                        fields(w[2 * h], f0);
+                                        fields(w[2 * h + 1], f1);
+                                        const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
+#pragma unroll
+                                        for (int n = 0; n < NT; ++n) {
+                                            mma_16816<__half>(a[u][n][c / PER * ACCS], a0, qf[n][c][0], qf[n][c][1]);
+                                            mma_16816<__half>(a[u][n][c / PER * ACCS + ACCS - 1], a1, qf[n][c][2], qf[n][c][3]);
+                                        }
+                                    }
                                 }
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float sc[NG], least[NG];
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) param(pk, i, k, sc[k], least[k]);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) {
+                                        float y = 0.f, v = round ? 0.f : -z.ref[n][e];
+#pragma unroll
+                                        for (int k = 0; k < NG; ++k) {
+                                            const int j = 2 * (i & 1) + e;
+                                            float dot = a[i >> 1][n][k * ACCS][j];
+                                            if (ACCS == 2) dot += a[i >> 1][n][k * ACCS + 1][j];
+                                            y = k == 0 ? sc[k] * dot : fmaf(sc[k], dot, y);
+                                            v = fmaf(least[k], kb[n][k][e], v);
+                                        }
+                                        x[n][i][e] = fmaf(y, ka[n][e], v);
+                                    }
                             }
                         }
+                        float vs[4][NG];
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            float sc[NG], least[NG];
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                            for (int k = 0; k < NG; ++k) param(pk, 2 * u + i, k, sc[k], least[k]);
+                            for (int k = 0; k < NG; ++k) {
+                                float unused;
+                                param(pk + St::kParams, i, k, vs[i][k], unused);
+                            }
+                        if (masked) {
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
-                                    float y = 0.f, v = 0.f;
+                                    const int r = row0 + 8 * n + 2 * t4 + e;
+                                    int first_key = 0, last_key = len - 1;
+                                    if (r < rows) visible_range(r / G, sq, len, p.mask_type, p.wl, p.wr, first_key, last_key);
 #pragma unroll
-                                    for (int k = 0; k < NG; ++k) {
-                                        y = fmaf(sc[k], a[n][k][2 * i + e], y);
-                                        v = fmaf(least[k], kb[n][k][e], v);
+                                    for (int i = 0; i < 4; ++i) {
+                                        const int key = key0 + g + 8 * i;
+                                        if (key < first_key || key > last_key) x[n][i][e] = -INFINITY;
                                     }
-                                    x[n][2 * u + i][e] = fmaf(y, ka[n][e], v);
                                 }
-                        }
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const int r = row0 + 8 * n + 2 * t4 + e;
-                                int first_key = 0, last_key = len - 1;
-                                if (r < rows) visible_range(r / G, sq, len, p.mask_type, p.wl, p.wr, first_key, last_key);
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    const int key = key0 + g + 8 * i;
-                                    if (key < first_key || key > last_key) x[n][i][e] = -INFINITY;
-                                }
-                            }
-                    }
-                    // ---- weights, in the row's reference; the second round is the one after it has moved ----
-                    float vs[4][NG], vm[4][NG];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int k = 0; k < NG; ++k) param(pk + St::kParams, i, k, vs[i][k], vm[i][k]);
-                    float pr[NT][4][2];
-                    uint32_t wt[NT][NG][4];
-#pragma unroll 1
-                    for (int round = 0;; ++round) {
-                        bool moves = first;
-                        uint32_t most = 0;
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            float sum = 0.f;
+                            bool finite = true;
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    pr[n][i][e] = fast_exp2(x[n][i][e] - z.ref[n][e]);
-                                    sum += pr[n][i][e];
+                                for (int k = 0; k < NG; ++k) {
+                                    float sc, least;
+                                    param(pk + St::kParams, i, k, sc, least);
+                                    finite &= fabsf(sc) < INFINITY && fabsf(least) < INFINITY;
                                 }
-                            moves |= sum > 1e27f;
+                            careful = __any_sync(0xffffffffu, !finite);
+                        }
+                        if (round == 1) {
+                            float top[4];  // log2 of a key's largest scale
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                float sc = vs[i][0];
+#pragma unroll
+                                for (int k = 1; k < NG; ++k) sc = fmaxf(sc, vs[i][k]);
+                                top[i] = sc > 0.f ? __log2f(sc) : -INFINITY;
+                            }
+#pragma unroll
+                            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    float mx = -INFINITY, jx = -INFINITY;
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) {
+                                        mx = fmaxf(mx, x[n][i][e]);
+                                        jx = fmaxf(jx, x[n][i][e] == -INFINITY ? -INFINITY : x[n][i][e] + top[i]);
+                                    }
+#pragma unroll
+                                    for (int d = 4; d < 32; d <<= 1) {
+                                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                                        jx = fmaxf(jx, __shfl_xor_sync(0xffffffffu, jx, d));
+                                    }
+                                    // weights up to 2^4 after a move; p' of the largest x within 2^-96 and 2^60, whatever the scales are
+                                    const float ref = fmaxf(z.ref[n][e], fminf(fmaxf(jx - 4.f, mx - 60.f), mx + 96.f));
+                                    const float f = fast_exp2(z.ref[n][e] - ref);  // (0 where nothing is summed yet)
+                                    z.ref[n][e] = ref;
+                                    z.l[n][e] *= f;
+#pragma unroll
+                                    for (int k = 0; k < NG; ++k) {
+                                        z.mid[n][k][e] *= f;
+                                        z.ones[n][k][e] *= f;
+                                        z.ones[n][k][2 + e] *= f;
+                                    }
+#pragma unroll
+                                    for (int c = 0; c < GR; ++c) {
+                                        z.o[n][c][0][e] *= f;
+                                        z.o[n][c][0][2 + e] *= f;
+                                        z.o[n][c][1][e] *= f;
+                                        z.o[n][c][1][2 + e] *= f;
+                                    }
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) x[n][i][e] -= ref;
+                                }
+                        }
+                        // ---- weights ----
+                        bool moves = false;
+                        uint32_t most = 0;
+                        float sum[NT][2];
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) x[n][i][e] = fast_exp2(x[n][i][e]);
+                                sum[n][e] = (x[n][0][e] + x[n][1][e]) + (x[n][2][e] + x[n][3][e]);
+                            }
+                            moves |= fmaxf(sum[n][0], sum[n][1]) > 1e27f;
 #pragma unroll
                             for (int k = 0; k < NG; ++k)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    float w0 = pr[n][i][0] * vs[i][k], w1 = pr[n][i][1] * vs[i][k];
-                                    if (masked) {  // (nothing of a hidden key counts, whatever its scale is)
-                                        if (x[n][i][0] == -INFINITY) w0 = 0.f;
-                                        if (x[n][i][1] == -INFINITY) w1 = 0.f;
-                                    }
-                                    wt[n][k][i] = halves(w0, w1);
-                                    most = max_halves(most, wt[n][k][i]);
-                                }
+                                for (int i = 0; i < 4; ++i) wt[n][k][i] = halves(x[n][i][0] * vs[i][k], x[n][i][1] * vs[i][k]);
                         }
-                        const __half2 mh = *reinterpret_cast<const __half2*>(&most);
-                        moves |= __high2float(mh) > 8192.f || __low2float(mh) > 8192.f;
-                        if (round == 1 || !__any_sync(0xffffffffu, moves)) break;
-                        first = false;
-                        float top[4];  // log2 of a key's largest scale
+                        if (careful) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float sc = vs[i][0];
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int k = 1; k < NG; ++k) sc = fmaxf(sc, vs[i][k]);
-                            top[i] = sc > 0.f ? __log2f(sc) : -INFINITY;
+                                for (int k = 0; k < NG; ++k)
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i)
+                                        wt[n][k][i] = halves(x[n][i][0] == 0.f ? 0.f : x[n][i][0] * vs[i][k], x[n][i][1] == 0.f ? 0.f : x[n][i][1] * vs[i][k]);
                         }
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                float mx = -INFINITY, jx = -INFINITY;
+                            for (int k = 0; k < NG; ++k)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    mx = fmaxf(mx, x[n][i][e]);
-                                    jx = fmaxf(jx, x[n][i][e] == -INFINITY ? -INFINITY : x[n][i][e] + top[i]);
-                                }
+                                for (int i = 0; i < 4; ++i) most = max_halves(most, wt[n][k][i]);
+                        moves |= ((most + 0x10001000u) & 0x80008000u) != 0u;  // 2^13 and more
+                        if (round == 1 || !__any_sync(0xffffffffu, moves)) {
 #pragma unroll
-                                for (int off = 4; off < 32; off <<= 1) {
-                                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-                                    jx = fmaxf(jx, __shfl_xor_sync(0xffffffffu, jx, off));
-                                }
-                                mx = fmaxf(mx, z.m[n][e]);
-                                jx = fmaxf(jx, z.j[n][e]);
-                                // weights up to 2^4 at the move; p' within 2^+-96 of 1 at the largest x, whatever the scales are
-                                const float ref = mx == -INFINITY ? 0.f : fminf(fmaxf(jx - 4.f, mx - 60.f), mx + 96.f);
-                                const float f = z.m[n][e] == -INFINITY ? 0.f : fast_exp2(z.ref[n][e] - ref);  // (0: nothing summed yet)
-                                z.m[n][e] = mx;
-                                z.j[n][e] = jx;
-                                z.ref[n][e] = ref;
-                                z.l[n][e] *= f;
+                            for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int k = 0; k < NG; ++k) {
-                                    z.mid[n][k][e] *= f;
-                                    z.ones[n][k][e] *= f;
-                                    z.ones[n][k][2 + e] *= f;
-                                }
-#pragma unroll
-                                for (int c = 0; c < GR; ++c) {
-                                    z.o[n][c][0][e] *= f;
-                                    z.o[n][c][0][2 + e] *= f;
-                                    z.o[n][c][1][e] *= f;
-                                    z.o[n][c][1][2 + e] *= f;
-                                }
-                            }
+                                for (int e = 0; e < 2; ++e) z.l[n][e] += sum[n][e];
+                            break;
+                        }
                     }
                     // ---- what each weight adds ----
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
 #pragma unroll
                         for (int k = 0; k < NG; ++k) {
-                            const float mid = fmaf(8.f, vs[i][k], vm[i][k]);
+                            float sc, least;
+                            param(pk + St::kParams, i, k, sc, least);
+                            const float mid = fmaf(8.f, sc, least);
 #pragma unroll
                             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    if (k == 0) z.l[n][e] += pr[n][i][e];
-                                    if (!masked || x[n][i][e] != -INFINITY) z.mid[n][k][e] = fmaf(pr[n][i][e], mid, z.mid[n][k][e]);
-                                }
+                                for (int e = 0; e < 2; ++e)
+                                    if (!careful || x[n][i][e] != 0.f) z.mid[n][k][e] = fmaf(x[n][i][e], mid, z.mid[n][k][e]);
                         }
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
@@ -657,10 +688,13 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         for (int n = 0; n < NT; ++n)
 #pragma unroll
                             for (int k = 0; k < NG; ++k) mma_16816<__half>(z.ones[n][k], kOnes, wt[n][k][2 * u], wt[n][k][2 * u + 1]);
+                    }
 #pragma unroll
-                        for (int i = 0; i < GR / 2; ++i) {
+                    for (int i = 0; i < GR / 2; ++i)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
                             uint32_t y[4];  // transposed: codes 4 g .. + 3 of piece 2 i, keys 2 t, 2 t + 1 and the same + 8; of piece 2 i + 1
-                            ldmatrix_x4_trans(y, st + St::kCodes + off[u][i]);
+                            ldmatrix_x4_trans(y, (at ^ (i << 5)) + St::kCodes + u * block_step);
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const int c = 2 * i + h;
@@ -675,7 +709,6 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 }
                             }
                         }
-                    }
                     if (++uncentred == kCentre) {
                         centre();
                         uncentred = 0;
@@ -686,12 +719,13 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&empty[now]);
             }
+            tile_count += tb - ta;
 
             // ---- this warp's sums: O[n][e][c] = channels 32 c + 4 g .. + 3 of row 2t + e, in reference R ----
             centre();
             float4 o[NT][2][GR];
             float l[NT][2];
-            bool has[NT][2];  // any key (a NaN among its scores does not show in the largest)
+            bool has[NT][2];  // any key (the largest score's p' is at least 2^-96; a NaN counts)
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -706,7 +740,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                         for (int k = 0; k < NG; ++k) rest[k] += __shfl_xor_sync(0xffffffffu, rest[k], off);
                     }
-                    has[n][e] = z.m[n][e] != -INFINITY || l[n][e] != l[n][e];
+                    has[n][e] = !(l[n][e] <= 0.f);
 #pragma unroll
                     for (int c = 0; c < GR; ++c) {
                         const float add = rest[c / PER];
