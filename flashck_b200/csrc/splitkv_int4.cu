@@ -82,6 +82,13 @@ __device__ __forceinline__ void fields(uint32_t w, uint32_t (&f)[4]) {
     f[2] = upper & kCode;
     f[3] = less(upper, f[2]);
 }
+// For values: the lowest field, and the byte, 16 times the next one plus the lowest, which the sums are freed from at the end.
+__device__ __forceinline__ void bytes(uint32_t w, uint32_t (&f)[4]) {
+    f[1] = w & 0x00ff00ffu;
+    f[3] = __byte_perm(w, 0, 0x4341);
+    f[0] = w & kCode;
+    f[2] = f[3] & kCode;
+}
 __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
@@ -119,7 +126,7 @@ struct Split {
 // What one warp has summed over its keys, for rows 2t and 2t + 1 (t = lane % 4) of each of NT tiles of 8 rows.
 template <int D, int NG, int NT>
 struct Sums {
-    float o[NT][D / 32][2][4];  // sum w u, w = p' s, over 2^24 ([0]: channels 4g, 4g + 2) or 2^20 ([1]: 4g + 1, 4g + 3 of 32)
+    float o[NT][D / 32][2][4];  // sum w u over 2^24, w = p' s ([0]: channels 4g, 4g + 2 of 32; [1]: 16 times 4g + 1, 4g + 3 plus those)
     float ones[NT][NG][4];      // sum w since the last centring (entries 0 and 1; the fragment's lower rows repeat them)
     float mid[NT][NG][2];       // sum p' (m + 8 s) over the lane's keys
     float l[NT][2];             // sum p' over the lane's keys
@@ -455,7 +462,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             z.o[n][c][0][e] = fmaf(-8.f / 16777216.f, z.ones[n][c / PER][e & 1], z.o[n][c][0][e]);
-                            z.o[n][c][1][e] = fmaf(-8.f / 1048576.f, z.ones[n][c / PER][e & 1], z.o[n][c][1][e]);
+                            z.o[n][c][1][e] = fmaf(-136.f / 16777216.f, z.ones[n][c / PER][e & 1], z.o[n][c][1][e]);
                         }
 #pragma unroll
                     for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.ones[n][k][2] = z.ones[n][k][3] = 0.f;
@@ -662,19 +669,33 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         }
                     }
                     // ---- what each weight adds ----
+                    if (careful) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
+                        for (int i = 0; i < 4; ++i)
 #pragma unroll
-                        for (int k = 0; k < NG; ++k) {
-                            float sc, least;
-                            param(pk + St::kParams, i, k, sc, least);
-                            const float mid = fmaf(8.f, sc, least);
+                            for (int k = 0; k < NG; ++k) {
+                                float sc, least;
+                                param(pk + St::kParams, i, k, sc, least);
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
+                                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                for (int e = 0; e < 2; ++e)
-                                    if (!careful || x[n][i][e] != 0.f) z.mid[n][k][e] = fmaf(x[n][i][e], mid, z.mid[n][k][e]);
-                        }
+                                    for (int e = 0; e < 2; ++e)
+                                        if (x[n][i][e] != 0.f) z.mid[n][k][e] = fmaf(x[n][i][e], fmaf(8.f, sc, least), z.mid[n][k][e]);
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int k = 0; k < NG; ++k) {
+                                float sc, least;
+                                param(pk + St::kParams, i, k, sc, least);
+                                const float mid = fmaf(8.f, sc, least);
+#pragma unroll
+                                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                                    for (int e = 0; e < 2; ++e) z.mid[n][k][e] = fmaf(x[n][i][e], mid, z.mid[n][k][e]);
+                            }
+                    }
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -699,8 +720,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             for (int h = 0; h < 2; ++h) {
                                 const int c = 2 * i + h;
                                 uint32_t f0[4], f1[4];
-                                fields(y[2 * h], f0);
-                                fields(y[2 * h + 1], f1);
+                                bytes(y[2 * h], f0);
+                                bytes(y[2 * h + 1], f1);
                                 const uint32_t even_ch[4] = {f0[0], f0[2], f1[0], f1[2]}, odd_ch[4] = {f0[1], f0[3], f1[1], f1[3]};
 #pragma unroll
                                 for (int n = 0; n < NT; ++n) {
@@ -744,8 +765,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                     for (int c = 0; c < GR; ++c) {
                         const float add = rest[c / PER];
-                        o[n][e][c] = make_float4(fmaf(16777216.f, z.o[n][c][0][e], add), fmaf(1048576.f, z.o[n][c][1][e], add),
-                                                 fmaf(16777216.f, z.o[n][c][0][2 + e], add), fmaf(1048576.f, z.o[n][c][1][2 + e], add));
+                        const float even0 = z.o[n][c][0][e], even2 = z.o[n][c][0][2 + e];
+                        o[n][e][c] = make_float4(fmaf(16777216.f, even0, add), fmaf(1048576.f, z.o[n][c][1][e] - even0, add),
+                                                 fmaf(16777216.f, even2, add), fmaf(1048576.f, z.o[n][c][1][2 + e] - even2, add));
                     }
                 }
             // ---- the warps of a head meet: the upper half hands its sums to the lower one until one warp per head is left,
