@@ -18,7 +18,7 @@
 // has summed is rescaled.  Moves are rare, and what decides one is a maximum over packed halves and a vote, without a shuffle.
 //
 // Bound by the cache's bytes in HBM: 136 a token and head at hdim 128 with one group, for 370 issue slots of an SM's four schedulers per 16
-// keys, of which about half are used.  A CTA per SM: a producer warp and 8 or 16 consumer warps.  A stage is 256 (head, token) pairs --
+// keys, of which about half are used.  A CTA per SM: four producer warps and 8 or 16 consumer warps.  A stage is 256 (head, token) pairs --
 // 32 tokens of 8 heads, 256 of one -- of K and V codes, by TMA (boxes of up to 256 tokens of a page, 64- or 32-byte swizzle: a warp's reads
 // meet no bank twice), and their scales, by 4- to 16-byte asynchronous copies.  8 consumer warps take 32 tokens of one head each; with 16,
 // two teams take stages in turn.  The warps of a head meet once per segment, in shared memory.  The work is cut as in splitkv_decode.cu.
@@ -225,10 +225,11 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int row0 = blockIdx.y * 8 * NT;  // first (token, group head) row of this CTA's tiles
 
     if (warp >= kConsumers) {
-        // =========================== producer warp (of a warpgroup that gives its registers away) ===========================
+        // ============ producer warps: two fetch codes and two scales, each pair every other stage (their number is even, so a stage always falls
+        // to the same two; one warp for all of it was what bound the kernel, at 1700 cycles a stage) ============
         registers_down<Split<TEAMS>::kProducer>();
-        if (warp > kConsumers) return;
-        if (lane == 0) {
+        const int mine = warp & 1, kind = (warp >> 1) & 1;  // stages mine, mine + 2, ..; 0: codes, 1: scales and least values
+        if (kind == 0 && lane == 0) {
             tma_prefetch_desc(&map_k);
             tma_prefetch_desc(&map_v);
         }
@@ -237,7 +238,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const int width = heads * NG * 4;
         const int piece_log2 = min(4, 31 - __clz(width)), pieces_log2 = 31 - __clz(width) - piece_log2;
         const int copies = toks << pieces_log2;
-        uint32_t it = 0;
+        const int per_tile_log2 = tok_log2 - p.chunk_log2;
+        int tile_count = 0, next = mine, stage = mine;  // (as the consumers count them)
+        uint32_t phase = 0;
         bool ok = true;
         for (int piece = blockIdx.x; piece < pieces && ok; piece += gridDim.x) {
             int lo, hi, b = begin_piece(piece, lo, hi);
@@ -247,12 +250,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 const int len = len_k(p, b);
                 const int64_t bphys = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
                 // pages of 32 chunks (a few tiles) per round, a lane each, loaded one round ahead; a page that is not there is one behind the pool
-                const int per_tile_log2 = tok_log2 - p.chunk_log2, first_chunk = (tile0[b] + ta) << per_tile_log2;
+                const int first_chunk = (tile0[b] + ta) << per_tile_log2, all_chunks = (tb - ta) << per_tile_log2;
                 auto entry = [&](int c, int& pg, int& tok) {
                     const int64_t token = (int64_t)(first_chunk + c) << p.chunk_log2;
                     pg = p.pool;
                     tok = 0;
-                    if (token >= len || c >= (tb - ta) << per_tile_log2) return;
+                    if (token >= len || c >= all_chunks) return;
                     if (p.block_table) {
                         const int slot = (int)token / p.page;
                         tok = (int)token - slot * p.page;
@@ -263,26 +266,37 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         if ((uint64_t)bphys < (uint64_t)p.pool) pg = (int)bphys;
                     }
                 };
-                int pg_cur, tok_cur, pg_next, tok_next;
+                int pg_cur = 0, tok_cur = 0, pg_next, tok_next, round = -1;
                 entry(lane, pg_next, tok_next);
-                for (int t = ta; t < tb; ++t, ++it) {
-                    const int s = it % stages, c0 = (t - ta) << per_tile_log2;  // the tile's first chunk
-                    if ((c0 & 31) == 0) {
+                for (int t = ta + next - tile_count; t < tb; t += 2) {
+                    const int s = stage, c0 = (t - ta) << per_tile_log2;  // the tile's first chunk
+                    const uint32_t parity = phase ^ 1u;
+                    next += 2;
+                    stage += 2;
+                    if (stage >= stages) {
+                        stage -= stages;
+                        phase ^= 1u;
+                    }
+                    if ((c0 >> 5) != round) {  // (a round has 2 tiles or more, so none is passed over)
+                        round = c0 >> 5;
                         pg_cur = pg_next;
                         tok_cur = tok_next;
-                        entry(c0 + 32 + lane, pg_next, tok_next);
+                        entry((round + 1) * 32 + lane, pg_next, tok_next);
                     }
                     const int from = (c0 & 31) + (lane & ((1 << per_tile_log2) - 1));
                     const int pg = __shfl_sync(0xffffffffu, pg_cur, from), tok = __shfl_sync(0xffffffffu, tok_cur, from);
                     const int token0 = (tile0[b] + t) << tok_log2;
-                    const int chunks = min(toks >> p.chunk_log2, (len - token0 + chunk - 1) >> p.chunk_log2);
-                    if (!mbar_wait_bounded(&empty[s], ((it / stages) & 1u) ^ 1u, abort_flag, p.status, 0x100)) { ok = false; break; }
+                    if (!mbar_wait_bounded(&empty[s], parity, abort_flag, p.status, 0x100)) { ok = false; break; }
                     uint8_t* st = ring + (size_t)s * St::kBytes;
-                    if (lane == 0) mbar_expect_tx(&full[s], 2 * chunks * box);
-                    __syncwarp();
-                    if (lane < chunks) {
-                        tma_load_4d(st + lane * box, &map_k, &full[s], 0, tok, column0, pg);
-                        tma_load_4d(st + St::kCodes + lane * box, &map_v, &full[s], 0, tok, column0, pg);
+                    if (kind == 0) {
+                        const int chunks = min(1 << per_tile_log2, (len - token0 + chunk - 1) >> p.chunk_log2);
+                        if (lane == 0) mbar_expect_tx(&full[s], 2 * chunks * box);
+                        __syncwarp();
+                        if (lane < chunks) {
+                            tma_load_4d(st + lane * box, &map_k, &full[s], 0, tok, column0, pg);
+                            tma_load_4d(st + St::kCodes + lane * box, &map_v, &full[s], 0, tok, column0, pg);
+                        }
+                        continue;
                     }
                     const int64_t at = pg < p.pool ? ((int64_t)pg * p.page + tok) * p.hkv + head0 : -1;  // the chunk's first (token, head)
                     const uint32_t dst = smem_u32(st + 2 * St::kCodes);
@@ -305,10 +319,11 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     }
                     arrive_after_copies(&full[s]);
                 }
+                tile_count += tb - ta;
             }
         }
         // ---- unused splits get LSE = -inf (see splitkv_decode.cu: shared out over gridDim.x / batch CTAs) ----
-        if (ok && blockIdx.y == 0 && blockIdx.z == 0) {
+        if (ok && warp == kConsumers && blockIdx.y == 0 && blockIdx.z == 0) {
             const int parts = max(1, (int)gridDim.x / p.batch), part = parts > 1 ? (int)blockIdx.x / p.batch : 0;
             for (int b = parts > 1 ? (int)blockIdx.x % p.batch : (int)blockIdx.x; b < p.batch && part < parts; b += gridDim.x) {
                 const int n = prefix[b + 1] - prefix[b];
@@ -327,8 +342,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         // waited for them, of the boxes too.
         asm volatile("cp.async.wait_all;\n" ::: "memory");
         if (*abort_flag) {
-            for (uint32_t u = it > (uint32_t)stages ? it - stages : 0; u < it; ++u)
-                for (int k = 0; k < 100000 && !mbar_try_wait_hint(&full[u % stages], (u / stages) & 1u, 2000u); ++k) {}
+            // (the last use of each of this warp's stages; one that it did not fill, or not wholly, costs the limit)
+            for (int u = next - 2; u >= 0 && u >= next - stages; u -= 2)
+                for (int k = 0; k < 10000 && !mbar_try_wait_hint(&full[u % stages], (uint32_t)(u / stages) & 1u, 2000u); ++k) {}
         }
         return;
     }
@@ -864,9 +880,9 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     const size_t room = 227 * 1024;
     FCK_REQUIRE(fixed + 2 * (St::kBytes + 16) <= room, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch %lld leaves no room for two stages",
                 (long long)c.batch);
-    // Two teams: an even number, so that a stage always falls to the same team.  (A parity tells two neighbouring uses apart: a team that came to a
-    // stage for every other use could take the other team's, not yet filled, for the one before its own.)
-    dev.stages = (int)std::min<size_t>(8, (room - fixed) / (St::kBytes + 16)) & ~(TEAMS - 1);
+    // An even number, so that a stage always falls to the same team and the same producers.  (A parity tells two neighbouring uses apart: a warp that
+    // came to a stage for every other use could take another's, not yet filled, for the one before its own.)
+    dev.stages = (int)std::min<size_t>(8, (room - fixed) / (St::kBytes + 16)) & ~1;
     const size_t smem = fixed + (size_t)dev.stages * (St::kBytes + 16);
     CUtensorMap mk, mv;
     const int line = std::min(128, heads * (D / 2)), lines = heads * (D / 2) / line;
