@@ -33,7 +33,7 @@ namespace {
 
 constexpr int kPairs = 256;  // (head, token) pairs of a stage
 constexpr int kUnit = 32;    // tokens a warp takes of it
-constexpr int kCentre = 4;   // units between two centrings
+constexpr int kCentre = 8;   // units between two centrings
 constexpr int kMeetWarps = 4;  // warps that hand their sums over at a time
 constexpr uint32_t kCode = 0x000f000fu;
 constexpr float kNoKey = -1e30f;  // (any score is so far above it that the reference moves)
@@ -64,6 +64,26 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
     return y;
+}
+template <bool TRANS, int OFFSET>
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t addr) {
+    if constexpr (TRANS)
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4+%5];\n"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr), "n"(OFFSET));
+    else
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4+%5];\n"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr), "n"(OFFSET));
+}
+// c = a b, or with SUM c += a b
+template <bool SUM>
+__device__ __forceinline__ void product(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (SUM) {
+        mma_16816<__half>(c, a, b0, b1);
+    } else {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+                     : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
+    }
 }
 template <int N>
 __device__ __forceinline__ void registers_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N)); }
@@ -360,17 +380,20 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int mrow = (lane & 7) + 8 * ((lane >> 3) & 1);
     const int mswz = p.line_log2 == 7 ? lane & 7 : p.line_log2 == 6 ? (lane >> 1) & 3 : (lane >> 2) & 1;
     const int per_line_log2 = p.line_log2 - (D == 128 ? 6 : 5);  // heads of a line
-    uint32_t off;  // of the warp's first 16 keys in a stage (piece 2 i: exclusive or with 32 i); the next 16 are block_step behind
+    uint32_t off[2][GR / 2];  // in the ring: of the warp's two blocks of 16 keys and two pairs of pieces of a stage
     {
         const int k = unit * kUnit, c = k >> p.chunk_log2;
         const int column = (c << (p.heads_log2 - per_line_log2)) + (hw >> per_line_log2);
         const int row = (column << p.chunk_log2) + (k & ((1 << p.chunk_log2) - 1)) + mrow;
-        off = (row << p.line_log2) + ((((hw & ((1 << per_line_log2) - 1)) * GR + (lane >> 4)) ^ mswz) << 4);
+        const int piece = (hw & ((1 << per_line_log2) - 1)) * GR + (lane >> 4);
+        const int block_step = p.chunk_log2 == 4 ? heads * 16 * ROW : 16 << p.line_log2;  // (the next chunk, or further down this one)
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < GR / 2; ++i) off[u][i] = smem_u32(ring) + u * block_step + (row << p.line_log2) + (((piece + 2 * i) ^ mswz) << 4);
     }
-    const uint32_t block_step = p.chunk_log2 == 4 ? heads * 16 * ROW : 16u << p.line_log2;  // (the next chunk, or further down this one)
     const int width = heads * NG * 4;
     const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * width + hw * (4 * NG);
-    const uint32_t ring_at = smem_u32(ring);
     bool failed = false;
     // Tiles are counted over all segments; a team takes every TEAMS-th.  tile_count: before this segment; next: this team's next one, its stage and
     // the parity of its use.
@@ -469,7 +492,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
             // 8 times the weights' sum taken off the sums of codes.  Tensor cores cut the sums of their products off instead of rounding them;
             // codes are never negative, so uncentred sums grow with the keys and lose on one side (4 x 524288 keys: O 0.9 % off), which
-            // centring every 128 keys prevents.
+            // centring every 256 keys prevents.
             auto centre = [&]() {
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -485,7 +508,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 }
             };
             int uncentred = 0;  // units
+            int key0 = ((tile0[b] + ta + next - tile_count) << tok_log2) + unit * kUnit - TEAMS * toks;
             for (int t = ta + next - tile_count; t < tb; t += TEAMS) {
+                key0 += TEAMS * toks;
                 const int now = stage;
                 const uint32_t parity = phase;
                 next += TEAMS;
@@ -495,9 +520,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     phase ^= 1u;
                 }
                 if (failed || !mbar_wait_bounded(&full[now], parity, abort_flag, p.status, 0x200)) { failed = true; continue; }
-                const int key0 = ((tile0[b] + t) << tok_log2) + unit * kUnit;
                 if (key0 < len) {
-                    const uint32_t at = ring_at + now * St::kBytes + off;
+                    uint32_t at[2][GR / 2];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u)
+#pragma unroll
+                        for (int i = 0; i < GR / 2; ++i) at[u][i] = off[u][i] + now * St::kBytes;
                     const uint8_t* pk = ring + now * St::kBytes + param_off;
                     const bool masked = key0 + kUnit > mask_from || key0 < mask_below;
                     // scale and least value of the lane's key g + 8 i of the unit
@@ -508,6 +536,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     };
                     float x[NT][4][2];       // scores of the lane's 4 keys and 2 rows, then weights p'
                     uint32_t wt[NT][NG][4];  // p' s as halves
+                    float mid[4];            // m + 8 s of the keys (of one group; with more it would take too many registers, and is worked out again)
                     bool careful = false;    // a hidden key's scale or least value is not finite: its weight of 0 must not meet it
                     // Usually one round.  A second one (that starts from the scores again) moves the reference of rows that need it.
 #pragma unroll 1
@@ -516,17 +545,11 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         {
                             float a[2][NT][NG * ACCS][4];  // (ACCS: chains of products that do not wait for one another)
 #pragma unroll
-                            for (int u = 0; u < 2; ++u)
-#pragma unroll
-                                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                    for (int k = 0; k < NG * ACCS; ++k) a[u][n][k][0] = a[u][n][k][1] = a[u][n][k][2] = a[u][n][k][3] = 0.f;
-#pragma unroll
                             for (int i = 0; i < GR / 2; ++i)
 #pragma unroll
                                 for (int u = 0; u < 2; ++u) {
                                     uint32_t w[4];  // keys g, g + 8 of piece 2 i, of piece 2 i + 1: the lane's 8 channels
-                                    ldmatrix_x4(w, (at ^ (i << 5)) + u * block_step);
+                                    load_matrices<false, 0>(w, at[u][i]);
 #pragma unroll
                                     for (int h = 0; h < 2; ++h) {
                                         const int c = 2 * i + h;
@@ -536,8 +559,15 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                         const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
 #pragma unroll
                                         for (int n = 0; n < NT; ++n) {
-                                            mma_16816<__half>(a[u][n][c / PER * ACCS], a0, qf[n][c][0], qf[n][c][1]);
-                                            mma_16816<__half>(a[u][n][c / PER * ACCS + ACCS - 1], a1, qf[n][c][2], qf[n][c][3]);
+                                            float(&s0)[4] = a[u][n][c / PER * ACCS];
+                                            float(&s1)[4] = a[u][n][c / PER * ACCS + ACCS - 1];
+                                            if (c % PER == 0) {
+                                                product<false>(s0, a0, qf[n][c][0], qf[n][c][1]);
+                                                product<ACCS == 1>(s1, a1, qf[n][c][2], qf[n][c][3]);
+                                            } else {
+                                                product<true>(s0, a0, qf[n][c][0], qf[n][c][1]);
+                                                product<true>(s1, a1, qf[n][c][2], qf[n][c][3]);
+                                            }
                                         }
                                     }
                                 }
@@ -568,8 +598,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
                             for (int k = 0; k < NG; ++k) {
-                                float unused;
-                                param(pk + St::kParams, i, k, vs[i][k], unused);
+                                float least;
+                                param(pk + St::kParams, i, k, vs[i][k], least);
+                                if (NG == 1) mid[i] = fmaf(8.f, vs[i][k], least);
                             }
                         if (masked) {
 #pragma unroll
@@ -703,13 +734,16 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
                             for (int k = 0; k < NG; ++k) {
-                                float sc, least;
-                                param(pk + St::kParams, i, k, sc, least);
-                                const float mid = fmaf(8.f, sc, least);
+                                float centre_of = mid[i];
+                                if (NG > 1) {
+                                    float sc, least;
+                                    param(pk + St::kParams, i, k, sc, least);
+                                    centre_of = fmaf(8.f, sc, least);
+                                }
 #pragma unroll
                                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                                    for (int e = 0; e < 2; ++e) z.mid[n][k][e] = fmaf(x[n][i][e], mid, z.mid[n][k][e]);
+                                    for (int e = 0; e < 2; ++e) z.mid[n][k][e] = fmaf(x[n][i][e], centre_of, z.mid[n][k][e]);
                             }
                     }
 #pragma unroll
@@ -731,7 +765,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             uint32_t y[4];  // transposed: codes 4 g .. + 3 of piece 2 i, keys 2 t, 2 t + 1 and the same + 8; of piece 2 i + 1
-                            ldmatrix_x4_trans(y, (at ^ (i << 5)) + St::kCodes + u * block_step);
+                            load_matrices<true, St::kCodes>(y, at[u][i]);
 #pragma unroll
                             for (int h = 0; h < 2; ++h) {
                                 const int c = 2 * i + h;
