@@ -114,6 +114,15 @@ __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
     asm("max.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// s[0] and s[1] plus the halves of a word
+__device__ __forceinline__ void add_halves(float (&s)[2], uint32_t w) {
+    asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\nadd.f32.f16 %0, lo, %0;\nadd.f32.f16 %1, hi, %1;\n}\n" : "+f"(s[0]), "+f"(s[1]) : "r"(w));
+}
+__device__ __forceinline__ bool elected() {
+    uint32_t yes;
+    asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
+    return yes != 0;
+}
 template <int BYTES>
 __device__ __forceinline__ void copy_async(uint32_t dst, const void* src, bool there) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;\n" ::"r"(dst), "l"(src), "n"(BYTES), "r"(there ? BYTES : 0) : "memory");
@@ -147,7 +156,7 @@ struct Split {
 template <int D, int NG, int NT>
 struct Sums {
     float o[NT][D / 32][2][4];  // sum w u over 2^24, w = p' s ([0]: channels 4g, 4g + 2 of 32; [1]: 16 times 4g + 1, 4g + 3 plus those)
-    float ones[NT][NG][4];      // sum w since the last centring (entries 0 and 1; the fragment's lower rows repeat them)
+    float ones[NT][NG][2];      // sum w (as rounded) over the lane's keys since the last centring
     float mid[NT][NG][2];       // sum p' (m + 8 s) over the lane's keys
     float l[NT][2];             // sum p' over the lane's keys
     float ref[NT][2];           // R; kNoKey before the first key
@@ -157,7 +166,6 @@ template <typename T, int D, int NG, int NT, int TEAMS>
 __global__ void __launch_bounds__((8 * TEAMS + 4) * 32, 1)
 splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Int4Dev p) {
     constexpr int ROW = D / 2, GR = D / 32, PER = GR / NG;  // bytes of a row; 16-byte pieces (32 channels) of it; of them per group
-    constexpr int ACCS = GR / NG >= 4 ? 2 : 1;
     constexpr int kConsumers = 8 * TEAMS;
     using St = Stage<D, NG>;
     extern __shared__ uint8_t smem_raw[];
@@ -306,6 +314,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     const int from = (c0 & 31) + (lane & ((1 << per_tile_log2) - 1));
                     const int pg = __shfl_sync(0xffffffffu, pg_cur, from), tok = __shfl_sync(0xffffffffu, tok_cur, from);
                     const int token0 = (tile0[b] + t) << tok_log2;
+                    // (stages ahead of the consumers there is no hurry: looking seldom leaves them the issue slots)
+                    for (int k = 0; k < 64 && !mbar_try_wait(&empty[s], parity); ++k) __nanosleep(200);
                     if (!mbar_wait_bounded(&empty[s], parity, abort_flag, p.status, 0x100)) { ok = false; break; }
                     uint8_t* st = ring + (size_t)s * St::kBytes;
                     if (kind == 0) {
@@ -482,7 +492,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                     for (int e = 0; e < 8; ++e) z.o[n][c][e >> 2][e & 3] = 0.f;
 #pragma unroll
-                for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.ones[n][k][2] = z.ones[n][k][3] = z.mid[n][k][0] = z.mid[n][k][1] = 0.f;
+                for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.mid[n][k][0] = z.mid[n][k][1] = 0.f;
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     z.l[n][e] = 0.f;
@@ -497,6 +507,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
 #pragma unroll
+                    for (int k = 0; k < NG; ++k)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int d = 4; d < 32; d <<= 1) z.ones[n][k][e] += __shfl_xor_sync(0xffffffffu, z.ones[n][k][e], d);
+#pragma unroll
                     for (int c = 0; c < GR; ++c)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
@@ -504,10 +520,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             z.o[n][c][1][e] = fmaf(-136.f / 16777216.f, z.ones[n][c / PER][e & 1], z.o[n][c][1][e]);
                         }
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.ones[n][k][2] = z.ones[n][k][3] = 0.f;
+                    for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = 0.f;
                 }
             };
-            int uncentred = 0;  // units
             int key0 = ((tile0[b] + ta + next - tile_count) << tok_log2) + unit * kUnit - TEAMS * toks;
             for (int t = ta + next - tile_count; t < tb; t += TEAMS) {
                 key0 += TEAMS * toks;
@@ -543,7 +558,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     for (int round = 0;; ++round) {
                         // ---- x = log2(e) scale q . k - R ----
                         {
-                            float a[2][NT][NG * ACCS][4];  // (ACCS: chains of products that do not wait for one another)
+                            float a[2][NT][NG][4];
 #pragma unroll
                             for (int i = 0; i < GR / 2; ++i)
 #pragma unroll
@@ -559,15 +574,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                         const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
 #pragma unroll
                                         for (int n = 0; n < NT; ++n) {
-                                            float(&s0)[4] = a[u][n][c / PER * ACCS];
-                                            float(&s1)[4] = a[u][n][c / PER * ACCS + ACCS - 1];
-                                            if (c % PER == 0) {
-                                                product<false>(s0, a0, qf[n][c][0], qf[n][c][1]);
-                                                product<ACCS == 1>(s1, a1, qf[n][c][2], qf[n][c][3]);
-                                            } else {
-                                                product<true>(s0, a0, qf[n][c][0], qf[n][c][1]);
-                                                product<true>(s1, a1, qf[n][c][2], qf[n][c][3]);
-                                            }
+                                            if (c % PER == 0) product<false>(a[u][n][c / PER], a0, qf[n][c][0], qf[n][c][1]);
+                                            else product<true>(a[u][n][c / PER], a0, qf[n][c][0], qf[n][c][1]);
+                                            product<true>(a[u][n][c / PER], a1, qf[n][c][2], qf[n][c][3]);
                                         }
                                     }
                                 }
@@ -584,9 +593,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                                         for (int k = 0; k < NG; ++k) {
                                             const int j = 2 * (i & 1) + e;
-                                            float dot = a[i >> 1][n][k * ACCS][j];
-                                            if (ACCS == 2) dot += a[i >> 1][n][k * ACCS + 1][j];
-                                            y = k == 0 ? sc[k] * dot : fmaf(sc[k], dot, y);
+                                            y = k == 0 ? sc[k] * a[i >> 1][n][k][j] : fmaf(sc[k], a[i >> 1][n][k][j], y);
                                             v = fmaf(least[k], kb[n][k][e], v);
                                         }
                                         x[n][i][e] = fmaf(y, ka[n][e], v);
@@ -660,7 +667,6 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                     for (int k = 0; k < NG; ++k) {
                                         z.mid[n][k][e] *= f;
                                         z.ones[n][k][e] *= f;
-                                        z.ones[n][k][2 + e] *= f;
                                     }
 #pragma unroll
                                     for (int c = 0; c < GR; ++c) {
@@ -751,15 +757,10 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                         for (int k = 0; k < NG; ++k)
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) wt[n][k][i] = transpose8x8(wt[n][k][i]);
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        constexpr uint32_t kOnes[4] = {0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u};
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
-                            for (int k = 0; k < NG; ++k) mma_16816<__half>(z.ones[n][k], kOnes, wt[n][k][2 * u], wt[n][k][2 * u + 1]);
-                    }
+                            for (int i = 0; i < 4; ++i) {
+                                add_halves(z.ones[n][k], wt[n][k][i]);
+                                wt[n][k][i] = transpose8x8(wt[n][k][i]);
+                            }
 #pragma unroll
                     for (int i = 0; i < GR / 2; ++i)
 #pragma unroll
@@ -780,15 +781,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 }
                             }
                         }
-                    if (++uncentred == kCentre) {
-                        centre();
-                        uncentred = 0;
-                    }
+                    if (((key0 >> (tok_log2 + TEAMS - 1)) & (kCentre - 1)) == 0) centre();
                 }
                 // the last reads of the stage have to have come back before it is given back (see splitkv_decode.cu)
                 __threadfence_block();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[now]);
+                if (elected()) mbar_arrive(&empty[now]);
             }
             tile_count += tb - ta;
 
