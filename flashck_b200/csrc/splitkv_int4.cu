@@ -52,6 +52,7 @@ struct Int4Dev {
     int batch, seqlen_q, hq, hkv, num_splits, total_q, bt_stride, page, pool, room;  // room: tokens that a sequence's part of the cache has
     int mask_type, wl, wr;
     int heads_log2, chunk_log2, stages;  // kv heads of a CTA; tokens of a box
+    int dual;                            // the teams of 8 warps take a tile of 8 rows each and all stages, instead of every other stage
     int line_log2;                       // bytes of a box's innermost rows: 128, or what the CTA's heads have
     float scale_log2;
 };
@@ -118,6 +119,9 @@ __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
 __device__ __forceinline__ void add_halves(float (&s)[2], uint32_t w) {
     asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %2;\nadd.f32.f16 %0, lo, %0;\nadd.f32.f16 %1, hi, %1;\n}\n" : "+f"(s[0]), "+f"(s[1]) : "r"(w));
 }
+__device__ __forceinline__ void add_halves(float (&s)[1], uint32_t w) {
+    asm("{\n.reg .b16 lo, hi;\nmov.b32 {lo, hi}, %1;\nadd.f32.f16 %0, lo, %0;\n}\n" : "+f"(s[0]) : "r"(w));
+}
 __device__ __forceinline__ bool elected() {
     uint32_t yes;
     asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}\n" : "=r"(yes));
@@ -143,30 +147,26 @@ struct Stage {
     static constexpr int kBytes = (2 * kCodes + 2 * kParams + 1023) / 1024 * 1024;
 };
 
-// Registers of the warpgroups: 8 TEAMS warps with kConsumer and 4 with kProducer share what the block is launched with, kLaunch a thread (what
-// its launch bounds leave: 65536 / threads, down to a multiple of 8).
-template <int TEAMS>
-struct Split {
-    static constexpr int kThreads = (8 * TEAMS + 4) * 32, kLaunch = 65536 / kThreads / 8 * 8;
-    static constexpr int kProducer = TEAMS == 2 ? 32 : 40, kConsumer = TEAMS == 2 ? 112 : 232;
-    static_assert((8 * TEAMS * kConsumer + 4 * kProducer) * 32 <= kThreads * kLaunch, "an increase would wait for good");
-};
+// 16 consumer warps and 4 producer warps share the registers that the block is launched with: kLaunch a thread (what the launch bounds leave:
+// 65536 / threads, down to a multiple of 8).
+constexpr int kConsumers = 16, kThreads = (kConsumers + 4) * 32, kLaunch = 65536 / kThreads / 8 * 8, kProducerRegs = 32, kConsumerRegs = 112;
+static_assert((kConsumers * kConsumerRegs + 4 * kProducerRegs) * 32 <= kThreads * kLaunch, "an increase would wait for good");
 
-// What one warp has summed over its keys, for rows 2t and 2t + 1 (t = lane % 4) of each of NT tiles of 8 rows.
-template <int D, int NG, int NT>
+// What one warp has summed over its keys, for the lane's E rows: 2t and 2t + 1 of 8 (E = 2, t = lane % 4), or t of 4 (E = 1; what belongs to odd
+// columns then stays zero).
+template <int D, int NG, int E>
 struct Sums {
-    float o[NT][D / 32][2][4];  // sum w u over 2^24, w = p' s ([0]: channels 4g, 4g + 2 of 32; [1]: 16 times 4g + 1, 4g + 3 plus those)
-    float ones[NT][NG][2];      // sum w (as rounded) over the lane's keys since the last centring
-    float mid[NT][NG][2];       // sum p' (m + 8 s) over the lane's keys
-    float l[NT][2];             // sum p' over the lane's keys
-    float ref[NT][2];           // R; kNoKey before the first key
+    float o[D / 32][2][4];  // sum w u over 2^24, w = p' s ([0]: channels 4g, 4g + 2 of 32; [1]: 16 times 4g + 1, 4g + 3 plus those)
+    float ones[NG][E];      // sum w (as rounded) over the lane's keys since the last centring
+    float mid[NG][E];       // sum p' (m + 8 s) over the lane's keys
+    float l[E];             // sum p' over the lane's keys
+    float ref[E];           // R; kNoKey before the first key
 };
 
-template <typename T, int D, int NG, int NT, int TEAMS>
-__global__ void __launch_bounds__((8 * TEAMS + 4) * 32, 1)
+template <typename T, int D, int NG, int E>
+__global__ void __launch_bounds__(kThreads, 1)
 splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Int4Dev p) {
     constexpr int ROW = D / 2, GR = D / 32, PER = GR / NG;  // bytes of a row; 16-byte pieces (32 channels) of it; of them per group
-    constexpr int kConsumers = 8 * TEAMS;
     using St = Stage<D, NG>;
     extern __shared__ uint8_t smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -175,9 +175,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
     uint8_t* ring = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
     float4* meet = reinterpret_cast<float4*>(ring + (size_t)stages * St::kBytes);  // [kMeetWarps][rows and columns of a lane][lane]: warps' sums
-    constexpr int kMeetFloat4 = NT * 2 * GR;  // float4 per lane
-    float* meet_stats = reinterpret_cast<float*>(meet + kMeetWarps * kMeetFloat4 * 32);  // [warp][NT][2][8 rows: ref, l]
-    uint64_t* bars = reinterpret_cast<uint64_t*>(meet_stats + kMeetWarps * NT * 16);
+    constexpr int kMeetFloat4 = E * GR;  // float4 per lane
+    float* meet_stats = reinterpret_cast<float*>(meet + kMeetWarps * kMeetFloat4 * 32);  // [warp][4 E rows][ref, l]
+    uint64_t* bars = reinterpret_cast<uint64_t*>(meet_stats + kMeetWarps * 4 * E * 2);
     uint64_t* full = bars;
     uint64_t* empty = bars + stages;
     int* prefix = reinterpret_cast<int*>(bars + 2 * stages);  // [batch + 1] tiles before each sequence
@@ -188,7 +188,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             mbar_init(&full[s], 33);  // the lanes' copies of scales, and the byte count of the boxes
-            mbar_init(&empty[s], 8);
+            mbar_init(&empty[s], p.dual ? 16 : 8);
         }
         *abort_flag = 0;
         mbar_fence_init();
@@ -250,12 +250,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         return a;
     };
     const int head0 = blockIdx.z << p.heads_log2;
-    const int row0 = blockIdx.y * 8 * NT;  // first (token, group head) row of this CTA's tiles
+    const int row0 = blockIdx.y * (p.dual ? 16 : 4 * E);  // first (token, group head) row of this CTA
 
     if (warp >= kConsumers) {
         // ============ producer warps: two fetch codes and two scales, each pair every other stage (their number is even, so a stage always falls
         // to the same two; one warp for all of it was what bound the kernel, at 1700 cycles a stage) ============
-        registers_down<Split<TEAMS>::kProducer>();
+        registers_down<kProducerRegs>();
         const int mine = warp & 1, kind = (warp >> 1) & 1;  // stages mine, mine + 2, ..; 0: codes, 1: scales and least values
         if (kind == 0 && lane == 0) {
             tma_prefetch_desc(&map_k);
@@ -380,7 +380,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
 
     // =============================== consumer warps =============================================
-    registers_up<Split<TEAMS>::kConsumer>();
+    registers_up<kConsumerRegs>();
     const int team = warp >> 3, wi = warp & 7;
     const int hw = wi & (heads - 1), unit = wi >> p.heads_log2;  // head of the CTA; which 32 tokens of a tile
     const int kh = head0 + hw;
@@ -405,9 +405,10 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int width = heads * NG * 4;
     const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * width + hw * (4 * NG);
     bool failed = false;
-    // Tiles are counted over all segments; a team takes every TEAMS-th.  tile_count: before this segment; next: this team's next one, its stage and
-    // the parity of its use.
-    int tile_count = 0, next = TEAMS == 2 ? team : 0, stage = next;
+    // Tiles are counted over all segments; a team takes every other one, or (dual) every one.  tile_count: before this segment; next: this team's next
+    // one, its stage and the parity of its use.
+    const int step = p.dual ? 1 : 2, first_row = row0 + (p.dual ? 8 * team : 0);
+    int tile_count = 0, next = p.dual ? 0 : team, stage = next;
     uint32_t phase = 0;
 
     for (int piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
@@ -420,12 +421,14 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const int split = per_sequence ? 0 : piece - prefix[b] / piece_len;
             const int64_t q0 = p.seqstart_q ? p.seqstart_q[b] : (int64_t)b * p.seqlen_q;
 
-            // ---- Q^T fragments: this lane has channels 32 i + 8 t .. + 7 of row g, as halves scaled by a power of two ----
-            uint32_t qf[NT][GR][4];
-            float ka[NT][2], kb[NT][NG][2];  // x = ka * (s . a) + kb . m for rows 2t and 2t + 1
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const int r = row0 + 8 * n + g, i = r / G;
+            // ---- Q^T fragments: this lane has channels 32 i + 8 t .. + 7 of a row, as halves scaled by a power of two.  E = 2: of row g.  K's
+            // operands are fields (channels 0, 4 of 8), and 16 times the next ones (1, 5), and so on.  E = 1: columns 2r and 2r + 1 belong to row r,
+            // whose score is the sum of both.  K's operands are fields n0 and whole bytes n0 + 16 n1; q0 n0 + q1 n1 = q0 n0 + q1/16 (n0 + 16 n1) -
+            // q1/16 n0, of which the odd column holds the last term: no subtraction to free the bytes of their lower fields. ----
+            uint32_t qf[GR][4];
+            float ka[E], kb[NG][E];  // x = ka * (s . a) + kb . m
+            {
+                const int r = first_row + (E == 2 ? g : g >> 1), i = r / G;
                 float x[GR][8], amax = 0.f;
                 const T* src = (const T*)p.q + ((q0 + i) * p.hq + kh * G + (r - i * G)) * D + 8 * t4;
 #pragma unroll
@@ -456,10 +459,15 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         sum[c / PER] += __half2float(h[k]);
                     }
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const __half2 two = __halves2half2(h[k], h[k + 4]);
-                        const __half2 v = (k & 1) ? __hmul2(two, __float2half2_rn(0.0625f)) : two;
-                        qf[n][c][k] = *reinterpret_cast<const uint32_t*>(&v);
+                    for (int k = 0; k < 4; k += 2) {
+                        const __half2 own = __halves2half2(h[k], h[k + 4]);
+                        const __half2 odd = __hmul2(__halves2half2(h[k + 1], h[k + 5]), __float2half2_rn(0.0625f)), minus = __hneg2(odd);
+                        qf[c][k] = *reinterpret_cast<const uint32_t*>(&own);
+                        qf[c][k + 1] = *reinterpret_cast<const uint32_t*>(&odd);
+                        if (E == 1 && (g & 1)) {
+                            qf[c][k] = *reinterpret_cast<const uint32_t*>(&minus);
+                            qf[c][k + 1] = 0u;
+                        }
                     }
                 }
 #pragma unroll
@@ -468,12 +476,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
                 }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int from = (2 * t4 + e) * 4;  // a lane of row 2t + e
+                for (int e = 0; e < E; ++e) {
+                    const int from = (2 * t4 + e) * 4;  // a lane of the row
                     const float scale = p.scale_log2 * __shfl_sync(0xffffffffu, down, from);
-                    ka[n][e] = scale * 16777216.f;
+                    ka[e] = scale * 16777216.f;
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) kb[n][k][e] = scale * __shfl_sync(0xffffffffu, sum[k], from);
+                    for (int k = 0; k < NG; ++k) kb[k][e] = scale * __shfl_sync(0xffffffffu, sum[k], from);
                 }
             }
             int mask_from = len;  // first key that some row may not see
@@ -484,20 +492,17 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 if (p.wl >= 0) mask_below = shift + sq - 1 - p.wl;
             }
 
-            Sums<D, NG, NT> z;
+            Sums<D, NG, E> z;
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
+            for (int c = 0; c < GR; ++c)
 #pragma unroll
-                for (int c = 0; c < GR; ++c)
+                for (int j = 0; j < 8; ++j) z.o[c][j >> 2][j & 3] = 0.f;
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z.o[n][c][e >> 2][e & 3] = 0.f;
+            for (int e = 0; e < E; ++e) {
 #pragma unroll
-                for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = z.mid[n][k][0] = z.mid[n][k][1] = 0.f;
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    z.l[n][e] = 0.f;
-                    z.ref[n][e] = kNoKey;
-                }
+                for (int k = 0; k < NG; ++k) z.ones[k][e] = z.mid[k][e] = 0.f;
+                z.l[e] = 0.f;
+                z.ref[e] = kNoKey;
             }
 
             // 8 times the weights' sum taken off the sums of codes.  Tensor cores cut the sums of their products off instead of rounding them;
@@ -505,37 +510,38 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             // centring every 256 keys prevents.
             auto centre = [&]() {
 #pragma unroll
-                for (int n = 0; n < NT; ++n) {
+                for (int k = 0; k < NG; ++k)
 #pragma unroll
-                    for (int k = 0; k < NG; ++k)
+                    for (int e = 0; e < E; ++e)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
+                        for (int d = 4; d < 32; d <<= 1) z.ones[k][e] += __shfl_xor_sync(0xffffffffu, z.ones[k][e], d);
 #pragma unroll
-                            for (int d = 4; d < 32; d <<= 1) z.ones[n][k][e] += __shfl_xor_sync(0xffffffffu, z.ones[n][k][e], d);
+                for (int c = 0; c < GR; ++c)
 #pragma unroll
-                    for (int c = 0; c < GR; ++c)
+                    for (int j = 0; j < 4; ++j) {
+                        if ((j & 1) >= E) continue;
+                        z.o[c][0][j] = fmaf(-8.f / 16777216.f, z.ones[c / PER][j & (E - 1)], z.o[c][0][j]);
+                        z.o[c][1][j] = fmaf(-136.f / 16777216.f, z.ones[c / PER][j & (E - 1)], z.o[c][1][j]);
+                    }
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            z.o[n][c][0][e] = fmaf(-8.f / 16777216.f, z.ones[n][c / PER][e & 1], z.o[n][c][0][e]);
-                            z.o[n][c][1][e] = fmaf(-136.f / 16777216.f, z.ones[n][c / PER][e & 1], z.o[n][c][1][e]);
-                        }
+                for (int k = 0; k < NG; ++k)
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) z.ones[n][k][0] = z.ones[n][k][1] = 0.f;
-                }
+                    for (int e = 0; e < E; ++e) z.ones[k][e] = 0.f;
             };
-            int key0 = ((tile0[b] + ta + next - tile_count) << tok_log2) + unit * kUnit - TEAMS * toks;
-            for (int t = ta + next - tile_count; t < tb; t += TEAMS) {
-                key0 += TEAMS * toks;
+            const int rows_here = rows - first_row;  // (none, where a second tile of rows is not there: the team only gives its stages back)
+            int key0 = ((tile0[b] + ta + next - tile_count) << tok_log2) + unit * kUnit - step * toks;
+            for (int t = ta + next - tile_count; t < tb; t += step) {
+                key0 += step * toks;
                 const int now = stage;
                 const uint32_t parity = phase;
-                next += TEAMS;
-                stage += TEAMS;
+                next += step;
+                stage += step;
                 if (stage >= stages) {
                     stage -= stages;
                     phase ^= 1u;
                 }
                 if (failed || !mbar_wait_bounded(&full[now], parity, abort_flag, p.status, 0x200)) { failed = true; continue; }
-                if (key0 < len) {
+                if (key0 < len && rows_here > 0) {
                     uint32_t at[2][GR / 2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
@@ -549,16 +555,16 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         sc = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[0]);
                         least = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[1]);
                     };
-                    float x[NT][4][2];       // scores of the lane's 4 keys and 2 rows, then weights p'
-                    uint32_t wt[NT][NG][4];  // p' s as halves
-                    float mid[4];            // m + 8 s of the keys (of one group; with more it would take too many registers, and is worked out again)
-                    bool careful = false;    // a hidden key's scale or least value is not finite: its weight of 0 must not meet it
+                    float x[4][E];       // scores of the lane's 4 keys, then weights p'
+                    uint32_t wt[NG][4];  // p' s as halves
+                    float mid[4];        // m + 8 s of the keys (of one group; with more it would take too many registers, and is worked out again)
+                    bool careful = false;  // a hidden key's scale or least value is not finite: its weight of 0 must not meet it
                     // Usually one round.  A second one (that starts from the scores again) moves the reference of rows that need it.
 #pragma unroll 1
                     for (int round = 0;; ++round) {
                         // ---- x = log2(e) scale q . k - R ----
                         {
-                            float a[2][NT][NG][4];
+                            float a[2][NG][4];
 #pragma unroll
                             for (int i = 0; i < GR / 2; ++i)
 #pragma unroll
@@ -569,15 +575,17 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                     for (int h = 0; h < 2; ++h) {
                                         const int c = 2 * i + h;
                                         uint32_t f0[4], f1[4];
-                                        fields(w[2 * h], f0);
-                                        fields(w[2 * h + 1], f1);
-                                        const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
-#pragma unroll
-                                        for (int n = 0; n < NT; ++n) {
-                                            if (c % PER == 0) product<false>(a[u][n][c / PER], a0, qf[n][c][0], qf[n][c][1]);
-                                            else product<true>(a[u][n][c / PER], a0, qf[n][c][0], qf[n][c][1]);
-                                            product<true>(a[u][n][c / PER], a1, qf[n][c][2], qf[n][c][3]);
+                                        if constexpr (E == 2) {
+                                            fields(w[2 * h], f0);
+                                            fields(w[2 * h + 1], f1);
+                                        } else {
+                                            bytes(w[2 * h], f0);
+                                            bytes(w[2 * h + 1], f1);
                                         }
+                                        const uint32_t a0[4] = {f0[0], f1[0], f0[1], f1[1]}, a1[4] = {f0[2], f1[2], f0[3], f1[3]};
+                                        if (c % PER == 0) product<false>(a[u][c / PER], a0, qf[c][0], qf[c][1]);
+                                        else product<true>(a[u][c / PER], a0, qf[c][0], qf[c][1]);
+                                        product<true>(a[u][c / PER], a1, qf[c][2], qf[c][3]);
                                     }
                                 }
 #pragma unroll
@@ -586,18 +594,17 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                                 for (int k = 0; k < NG; ++k) param(pk, i, k, sc[k], least[k]);
 #pragma unroll
-                                for (int n = 0; n < NT; ++n)
+                                for (int e = 0; e < E; ++e) {
+                                    float y = 0.f, v = round ? 0.f : -z.ref[e];
 #pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        float y = 0.f, v = round ? 0.f : -z.ref[n][e];
-#pragma unroll
-                                        for (int k = 0; k < NG; ++k) {
-                                            const int j = 2 * (i & 1) + e;
-                                            y = k == 0 ? sc[k] * a[i >> 1][n][k][j] : fmaf(sc[k], a[i >> 1][n][k][j], y);
-                                            v = fmaf(least[k], kb[n][k][e], v);
-                                        }
-                                        x[n][i][e] = fmaf(y, ka[n][e], v);
+                                    for (int k = 0; k < NG; ++k) {
+                                        const float(&both)[4] = a[i >> 1][k];
+                                        const float dot = E == 2 ? both[2 * (i & 1) + e] : both[2 * (i & 1)] + both[2 * (i & 1) + 1];
+                                        y = k == 0 ? sc[k] * dot : fmaf(sc[k], dot, y);
+                                        v = fmaf(least[k], kb[k][e], v);
                                     }
+                                    x[i][e] = fmaf(y, ka[e], v);
+                                }
                             }
                         }
                         float vs[4][NG];
@@ -611,18 +618,16 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             }
                         if (masked) {
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
+                            for (int e = 0; e < E; ++e) {
+                                const int r = first_row + E * t4 + e;
+                                int first_key = 0, last_key = len - 1;
+                                if (r < rows) visible_range(r / G, sq, len, p.mask_type, p.wl, p.wr, first_key, last_key);
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    const int r = row0 + 8 * n + 2 * t4 + e;
-                                    int first_key = 0, last_key = len - 1;
-                                    if (r < rows) visible_range(r / G, sq, len, p.mask_type, p.wl, p.wr, first_key, last_key);
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        const int key = key0 + g + 8 * i;
-                                        if (key < first_key || key > last_key) x[n][i][e] = -INFINITY;
-                                    }
+                                for (int i = 0; i < 4; ++i) {
+                                    const int key = key0 + g + 8 * i;
+                                    if (key < first_key || key > last_key) x[i][e] = -INFINITY;
                                 }
+                            }
                             bool finite = true;
 #pragma unroll
                             for (int i = 0; i < 4; ++i)
@@ -644,80 +649,67 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 top[i] = sc > 0.f ? __log2f(sc) : -INFINITY;
                             }
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
+                            for (int e = 0; e < E; ++e) {
+                                float mx = -INFINITY, jx = -INFINITY;
 #pragma unroll
-                                for (int e = 0; e < 2; ++e) {
-                                    float mx = -INFINITY, jx = -INFINITY;
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) {
-                                        mx = fmaxf(mx, x[n][i][e]);
-                                        jx = fmaxf(jx, x[n][i][e] == -INFINITY ? -INFINITY : x[n][i][e] + top[i]);
-                                    }
-#pragma unroll
-                                    for (int d = 4; d < 32; d <<= 1) {
-                                        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                                        jx = fmaxf(jx, __shfl_xor_sync(0xffffffffu, jx, d));
-                                    }
-                                    // weights up to 2^4 after a move; p' of the largest x within 2^-96 and 2^60, whatever the scales are
-                                    const float ref = fmaxf(z.ref[n][e], fminf(fmaxf(jx - 4.f, mx - 60.f), mx + 96.f));
-                                    const float f = fast_exp2(z.ref[n][e] - ref);  // (0 where nothing is summed yet)
-                                    z.ref[n][e] = ref;
-                                    z.l[n][e] *= f;
-#pragma unroll
-                                    for (int k = 0; k < NG; ++k) {
-                                        z.mid[n][k][e] *= f;
-                                        z.ones[n][k][e] *= f;
-                                    }
-#pragma unroll
-                                    for (int c = 0; c < GR; ++c) {
-                                        z.o[n][c][0][e] *= f;
-                                        z.o[n][c][0][2 + e] *= f;
-                                        z.o[n][c][1][e] *= f;
-                                        z.o[n][c][1][2 + e] *= f;
-                                    }
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i) x[n][i][e] -= ref;
+                                for (int i = 0; i < 4; ++i) {
+                                    mx = fmaxf(mx, x[i][e]);
+                                    jx = fmaxf(jx, x[i][e] == -INFINITY ? -INFINITY : x[i][e] + top[i]);
                                 }
+#pragma unroll
+                                for (int d = 4; d < 32; d <<= 1) {
+                                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+                                    jx = fmaxf(jx, __shfl_xor_sync(0xffffffffu, jx, d));
+                                }
+                                // weights up to 2^4 after a move; p' of the largest x within 2^-96 and 2^60, whatever the scales are
+                                const float ref = fmaxf(z.ref[e], fminf(fmaxf(jx - 4.f, mx - 60.f), mx + 96.f));
+                                const float f = fast_exp2(z.ref[e] - ref);  // (0 where nothing is summed yet)
+                                z.ref[e] = ref;
+                                z.l[e] *= f;
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) {
+                                    z.mid[k][e] *= f;
+                                    z.ones[k][e] *= f;
+                                }
+#pragma unroll
+                                for (int c = 0; c < GR; ++c) {
+                                    z.o[c][0][e] *= f;
+                                    z.o[c][0][2 + e] *= f;
+                                    z.o[c][1][e] *= f;
+                                    z.o[c][1][2 + e] *= f;
+                                }
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) x[i][e] -= ref;
+                            }
                         }
                         // ---- weights ----
-                        bool moves = false;
-                        uint32_t most = 0;
-                        float sum[NT][2];
+                        float sum[E];
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
+                        for (int e = 0; e < E; ++e) {
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) x[n][i][e] = fast_exp2(x[n][i][e]);
-                                sum[n][e] = (x[n][0][e] + x[n][1][e]) + (x[n][2][e] + x[n][3][e]);
-                            }
-                            moves |= fmaxf(sum[n][0], sum[n][1]) > 1e27f;
-#pragma unroll
-                            for (int k = 0; k < NG; ++k)
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) wt[n][k][i] = halves(x[n][i][0] * vs[i][k], x[n][i][1] * vs[i][k]);
+                            for (int i = 0; i < 4; ++i) x[i][e] = fast_exp2(x[i][e]);
+                            sum[e] = (x[0][e] + x[1][e]) + (x[2][e] + x[3][e]);
                         }
+#pragma unroll
+                        for (int k = 0; k < NG; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) wt[k][i] = halves(x[i][0] * vs[i][k], E == 2 ? x[i][E - 1] * vs[i][k] : 0.f);
                         if (careful) {
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int k = 0; k < NG; ++k)
-#pragma unroll
-                                    for (int i = 0; i < 4; ++i)
-                                        wt[n][k][i] = halves(x[n][i][0] == 0.f ? 0.f : x[n][i][0] * vs[i][k], x[n][i][1] == 0.f ? 0.f : x[n][i][1] * vs[i][k]);
-                        }
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-#pragma unroll
                             for (int k = 0; k < NG; ++k)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) most = max_halves(most, wt[n][k][i]);
-                        moves |= ((most + 0x10001000u) & 0x80008000u) != 0u;  // 2^13 and more
+                                for (int i = 0; i < 4; ++i)
+                                    wt[k][i] = halves(x[i][0] == 0.f ? 0.f : x[i][0] * vs[i][k], E == 1 || x[i][E - 1] == 0.f ? 0.f : x[i][E - 1] * vs[i][k]);
+                        }
+                        uint32_t most = 0;
+#pragma unroll
+                        for (int k = 0; k < NG; ++k)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) most = max_halves(most, wt[k][i]);
+                        const bool moves = fmaxf(sum[0], sum[E - 1]) > 1e27f || ((most + 0x10001000u) & 0x80008000u) != 0u;  // (2^13 and more)
                         if (round == 1 || !__any_sync(0xffffffffu, moves)) {
 #pragma unroll
-                            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                for (int e = 0; e < 2; ++e) z.l[n][e] += sum[n][e];
+                            for (int e = 0; e < E; ++e) z.l[e] += sum[e];
                             break;
                         }
                     }
@@ -730,10 +722,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 float sc, least;
                                 param(pk + St::kParams, i, k, sc, least);
 #pragma unroll
-                                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e)
-                                        if (x[n][i][e] != 0.f) z.mid[n][k][e] = fmaf(x[n][i][e], fmaf(8.f, sc, least), z.mid[n][k][e]);
+                                for (int e = 0; e < E; ++e)
+                                    if (x[i][e] != 0.f) z.mid[k][e] = fmaf(x[i][e], fmaf(8.f, sc, least), z.mid[k][e]);
                             }
                     } else {
 #pragma unroll
@@ -747,20 +737,16 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                     centre_of = fmaf(8.f, sc, least);
                                 }
 #pragma unroll
-                                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e) z.mid[n][k][e] = fmaf(x[n][i][e], centre_of, z.mid[n][k][e]);
+                                for (int e = 0; e < E; ++e) z.mid[k][e] = fmaf(x[i][e], centre_of, z.mid[k][e]);
                             }
                     }
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int k = 0; k < NG; ++k)
 #pragma unroll
-                        for (int k = 0; k < NG; ++k)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                add_halves(z.ones[n][k], wt[n][k][i]);
-                                wt[n][k][i] = transpose8x8(wt[n][k][i]);
-                            }
+                        for (int i = 0; i < 4; ++i) {
+                            add_halves(z.ones[k], wt[k][i]);
+                            wt[k][i] = transpose8x8(wt[k][i]);
+                        }
 #pragma unroll
                     for (int i = 0; i < GR / 2; ++i)
 #pragma unroll
@@ -774,14 +760,11 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 bytes(y[2 * h], f0);
                                 bytes(y[2 * h + 1], f1);
                                 const uint32_t even_ch[4] = {f0[0], f0[2], f1[0], f1[2]}, odd_ch[4] = {f0[1], f0[3], f1[1], f1[3]};
-#pragma unroll
-                                for (int n = 0; n < NT; ++n) {
-                                    mma_16816<__half>(z.o[n][c][0], even_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
-                                    mma_16816<__half>(z.o[n][c][1], odd_ch, wt[n][c / PER][2 * u], wt[n][c / PER][2 * u + 1]);
-                                }
+                                mma_16816<__half>(z.o[c][0], even_ch, wt[c / PER][2 * u], wt[c / PER][2 * u + 1]);
+                                mma_16816<__half>(z.o[c][1], odd_ch, wt[c / PER][2 * u], wt[c / PER][2 * u + 1]);
                             }
                         }
-                    if (((key0 >> (tok_log2 + TEAMS - 1)) & (kCentre - 1)) == 0) centre();
+                    if (((key0 >> (tok_log2 + step - 1)) & (kCentre - 1)) == 0) centre();
                 }
                 // the last reads of the stage have to have come back before it is given back (see splitkv_decode.cu)
                 __threadfence_block();
@@ -790,93 +773,90 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             tile_count += tb - ta;
 
-            // ---- this warp's sums: O[n][e][c] = channels 32 c + 4 g .. + 3 of row 2t + e, in reference R ----
+            // ---- this warp's sums: o[e][c] = channels 32 c + 4 g .. + 3 of the lane's row e, in its reference ----
             centre();
-            float4 o[NT][2][GR];
-            float l[NT][2];
-            bool has[NT][2];  // any key (the largest score's p' is at least 2^-96; a NaN counts)
+            float4 o[E][GR];
+            float l[E];
+            bool has[E];  // any key (the largest score's p' is at least 2^-96; a NaN counts)
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int e = 0; e < E; ++e) {
+                float rest[NG];
+                l[e] = z.l[e];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float rest[NG];
-                    l[n][e] = z.l[n][e];
+                for (int k = 0; k < NG; ++k) rest[k] = z.mid[k][e];
 #pragma unroll
-                    for (int k = 0; k < NG; ++k) rest[k] = z.mid[n][k][e];
+                for (int d = 4; d < 32; d <<= 1) {
+                    l[e] += __shfl_xor_sync(0xffffffffu, l[e], d);
 #pragma unroll
-                    for (int off = 4; off < 32; off <<= 1) {
-                        l[n][e] += __shfl_xor_sync(0xffffffffu, l[n][e], off);
-#pragma unroll
-                        for (int k = 0; k < NG; ++k) rest[k] += __shfl_xor_sync(0xffffffffu, rest[k], off);
-                    }
-                    has[n][e] = !(l[n][e] <= 0.f);
-#pragma unroll
-                    for (int c = 0; c < GR; ++c) {
-                        const float add = rest[c / PER];
-                        const float even0 = z.o[n][c][0][e], even2 = z.o[n][c][0][2 + e];
-                        o[n][e][c] = make_float4(fmaf(16777216.f, even0, add), fmaf(1048576.f, z.o[n][c][1][e] - even0, add),
-                                                 fmaf(16777216.f, even2, add), fmaf(1048576.f, z.o[n][c][1][2 + e] - even2, add));
-                    }
+                    for (int k = 0; k < NG; ++k) rest[k] += __shfl_xor_sync(0xffffffffu, rest[k], d);
                 }
-            // ---- the warps of a head meet: the upper half hands its sums to the lower one until one warp per head is left,
-            // kMeetWarps at a time ----
-            for (int from = kConsumers / 2, step = from; step >= heads; from = from + kMeetWarps < 2 * step ? from + kMeetWarps : (step >>= 1)) {
-                const int slot = warp - from, to = warp - (from - step);  // of the one that hands over, and of the one that takes
-                if (slot >= 0 && slot < min(kMeetWarps, step)) {
+                has[e] = !(l[e] <= 0.f);
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                for (int c = 0; c < GR; ++c) {
+                    const float add = rest[c / PER], even0 = z.o[c][0][e], even2 = z.o[c][0][2 + e];
+                    o[e][c] = make_float4(fmaf(16777216.f, even0, add), fmaf(1048576.f, z.o[c][1][e] - even0, add), fmaf(16777216.f, even2, add),
+                                          fmaf(1048576.f, z.o[c][1][2 + e] - even2, add));
+                }
+            }
+            // ---- the warps of a head (and team, if these have rows of their own) meet: the upper half hands its sums to the lower one until one
+            // warp is left, kMeetWarps at a time ----
+            for (int half = p.dual ? 4 : 8; half >= heads; half >>= 1) {
+                const int parts = p.dual ? 2 : max(1, half / kMeetWarps), many = min(kMeetWarps, half);
+                for (int part = 0; part < parts; ++part) {
+                    const int gives = (p.dual ? (team == part ? wi : -1) : warp - kMeetWarps * part) - half;
+                    const int takes = p.dual ? (team == part ? wi : -1) : warp - kMeetWarps * part;
+                    if (gives >= 0 && gives < many) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
+                        for (int e = 0; e < E; ++e) {
 #pragma unroll
-                            for (int c = 0; c < GR; ++c) meet[(slot * kMeetFloat4 + (n * 2 + e) * GR + c) * 32 + lane] = o[n][e][c];
+                            for (int c = 0; c < GR; ++c) meet[(gives * kMeetFloat4 + e * GR + c) * 32 + lane] = o[e][c];
                             if (g == 0) {
-                                meet_stats[((slot * NT + n) * 8 + 2 * t4 + e) * 2] = z.ref[n][e];
-                                meet_stats[((slot * NT + n) * 8 + 2 * t4 + e) * 2 + 1] = has[n][e] ? l[n][e] : -1.f;  // (-1: no key)
+                                float* stats = meet_stats + (gives * 4 * E + E * t4 + e) * 2;
+                                stats[0] = z.ref[e];
+                                stats[1] = has[e] ? l[e] : -1.f;  // (-1: no key)
                             }
                         }
-                }
-                asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
-                if (to >= 0 && to < min(kMeetWarps, step)) {
+                    }
+                    asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
+                    if (takes >= 0 && takes < many) {
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float ref = meet_stats[((to * NT + n) * 8 + 2 * t4 + e) * 2], lo_ = meet_stats[((to * NT + n) * 8 + 2 * t4 + e) * 2 + 1];
-                            if (lo_ != -1.f) {
-                                const float both = has[n][e] ? fmaxf(ref, z.ref[n][e]) : ref;
-                                const float fa = has[n][e] ? fast_exp2(z.ref[n][e] - both) : 0.f, fb = fast_exp2(ref - both);
-                                z.ref[n][e] = both;
-                                has[n][e] = true;
-                                l[n][e] = l[n][e] * fa + lo_ * fb;
+                        for (int e = 0; e < E; ++e) {
+                            const float* stats = meet_stats + (takes * 4 * E + E * t4 + e) * 2;
+                            const float ref = stats[0], other = stats[1];
+                            if (other != -1.f) {
+                                const float both = has[e] ? fmaxf(ref, z.ref[e]) : ref;
+                                const float fa = has[e] ? fast_exp2(z.ref[e] - both) : 0.f, fb = fast_exp2(ref - both);
+                                z.ref[e] = both;
+                                has[e] = true;
+                                l[e] = l[e] * fa + other * fb;
 #pragma unroll
                                 for (int c = 0; c < GR; ++c) {
-                                    const float4 y = meet[(to * kMeetFloat4 + (n * 2 + e) * GR + c) * 32 + lane];
-                                    float4& v = o[n][e][c];
+                                    const float4 y = meet[(takes * kMeetFloat4 + e * GR + c) * 32 + lane];
+                                    float4& v = o[e][c];
                                     v = make_float4(v.x * fa + y.x * fb, v.y * fa + y.y * fb, v.z * fa + y.z * fb, v.w * fa + y.w * fb);
                                 }
                             }
                         }
-                }
-                asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
-            }
-            if (warp >= heads || failed) continue;
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int r = row0 + 8 * n + 2 * t4 + e, i = r / G, h = kh * G + (r - i * G);
-                    if (r >= rows) continue;
-                    const int64_t idx = p.seqstart_q ? ((int64_t)h * p.num_splits + split) * p.total_q + (q0 + i)
-                                                     : (((int64_t)b * p.hq + h) * p.num_splits + split) * p.seqlen_q + i;
-                    const float inv = has[n][e] ? 1.f / l[n][e] : 0.f;
-#pragma unroll
-                    for (int c = 0; c < GR; ++c) {
-                        const float4 v = o[n][e][c];
-                        *reinterpret_cast<float4*>(p.o_acc + idx * D + 32 * c + 4 * g) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
                     }
-                    if (g == 0) p.lse_acc[idx] = !has[n][e] ? -INFINITY : l[n][e] != l[n][e] ? INFINITY  // (the merge makes NaN of it)
-                                                                   : (z.ref[n][e] + log2f(l[n][e])) * 0.6931471805599453f;
+                    asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
                 }
+            }
+            if ((p.dual ? wi : warp) >= heads || failed) continue;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int r = first_row + E * t4 + e, i = r / G, h = kh * G + (r - i * G);
+                if (r >= rows) continue;
+                const int64_t idx = p.seqstart_q ? ((int64_t)h * p.num_splits + split) * p.total_q + (q0 + i)
+                                                 : (((int64_t)b * p.hq + h) * p.num_splits + split) * p.seqlen_q + i;
+                const float inv = has[e] ? 1.f / l[e] : 0.f;
+#pragma unroll
+                for (int c = 0; c < GR; ++c) {
+                    const float4 v = o[e][c];
+                    *reinterpret_cast<float4*>(p.o_acc + idx * D + 32 * c + 4 * g) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                }
+                if (g == 0) p.lse_acc[idx] = !has[e] ? -INFINITY : l[e] != l[e] ? INFINITY  // (the merge makes NaN of it)
+                                                                 : (z.ref[e] + log2f(l[e])) * 0.6931471805599453f;
+            }
         }
     }
 }
@@ -898,7 +878,7 @@ int make_codes_map(CUtensorMap* map, const void* base, int64_t pool, int64_t pag
     return FLASHCK_OK;
 }
 
-template <typename T, int D, int NG, int NT, int TEAMS>
+template <typename T, int D, int NG, int E>
 int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     using St = Stage<D, NG>;
     const Int4Cache& c = p.cache;
@@ -907,7 +887,7 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     int chunk = 16;
     dev.chunk_log2 = 4;
     while (2 * chunk <= toks && (!c.block_table || c.page % (2 * chunk) == 0)) { chunk *= 2; ++dev.chunk_log2; }
-    const size_t meet = (size_t)kMeetWarps * NT * (2 * (D / 32) * 32 * 16 + 64);
+    const size_t meet = (size_t)kMeetWarps * E * ((D / 32) * 32 * 16 + 32);
     const size_t fixed = 1024 + meet + (size_t)(2 * c.batch + 4) * sizeof(int);
     const size_t room = 227 * 1024;
     FCK_REQUIRE(fixed + 2 * (St::kBytes + 16) <= room, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch %lld leaves no room for two stages",
@@ -921,7 +901,7 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     dev.line_log2 = line == 128 ? 7 : line == 64 ? 6 : 5;
     if (int rc = make_codes_map(&mk, c.k_codes, c.pool, c.page, c.hkv * (D / 2), line, lines, chunk)) return rc;
     if (int rc = make_codes_map(&mv, c.v_codes, c.pool, c.page, c.hkv * (D / 2), line, lines, chunk)) return rc;
-    auto kern = splitkv_int4_kernel<T, D, NG, NT, TEAMS>;
+    auto kern = splitkv_int4_kernel<T, D, NG, E>;
     static thread_local int configured_device = -1;  // per instantiation
     int devid = 0;
     FCK_CUDA(cudaGetDevice(&devid));
@@ -929,22 +909,25 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
         FCK_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room));
         cudaFuncAttributes attr;
         FCK_CUDA(cudaFuncGetAttributes(&attr, kern));
-        FCK_REQUIRE(attr.numRegs == Split<TEAMS>::kLaunch, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: built with %d registers a thread instead of %d",
-                    attr.numRegs, Split<TEAMS>::kLaunch);  // (the warpgroups' shares would not add up)
+        FCK_REQUIRE(attr.numRegs == kLaunch, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: built with %d registers a thread instead of %d",
+                    attr.numRegs, kLaunch);  // (the warpgroups' shares would not add up)
         configured_device = devid;
     }
-    const int64_t gy = (p.max_seqlen_q * (p.hq / c.hkv) + 8 * NT - 1) / (8 * NT), gz = c.hkv / heads;
+    const int64_t rows = p.max_seqlen_q * (p.hq / c.hkv), rows_per_cta = dev.dual ? 16 : 4 * E;
+    const int64_t gy = (rows + rows_per_cta - 1) / rows_per_cta, gz = c.hkv / heads;
     FCK_REQUIRE(gy <= 65535, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: too many query rows per kv head");
     const int64_t gx = std::max<int64_t>(1, sm_count() / (gy * gz));  // one wave, where the heads and rows leave one
-    FCK_CUDA(launch_dependent(kern, dim3((unsigned)gx, (unsigned)gy, (unsigned)gz), dim3(Split<TEAMS>::kThreads), smem, stream, mk, mv, dev));
+    FCK_CUDA(launch_dependent(kern, dim3((unsigned)gx, (unsigned)gy, (unsigned)gz), dim3(kThreads), smem, stream, mk, mv, dev));
     return FLASHCK_OK;
 }
 
 template <typename T, int D, int NG>
 int launch_rows(const SplitKVInt4Params& p, const Int4Dev& dev, cudaStream_t stream) {
-    // up to 8 rows: 16 consumer warps of one tile; more: 8 of two tiles each (the sums of two take 200 registers)
-    if (p.max_seqlen_q * (p.hq / p.cache.hkv) <= 8) return launch<T, D, NG, 1, 2>(p, dev, stream);
-    return launch<T, D, NG, 2, 1>(p, dev, stream);
+    // Rows per kv head.  Up to 4: two columns a row.  Up to 8: one tile.  More: two tiles, a team of 8 warps each, per pass over the cache.
+    Int4Dev d = dev;
+    const int64_t rows = p.max_seqlen_q * (p.hq / p.cache.hkv);
+    d.dual = rows > 8;
+    return rows <= 4 ? launch<T, D, NG, 1>(p, d, stream) : launch<T, D, NG, 2>(p, d, stream);
 }
 
 template <typename T>
