@@ -52,7 +52,7 @@ struct Int4Dev {
     int batch, seqlen_q, hq, hkv, num_splits, total_q, bt_stride, page, pool, room;  // room: tokens that a sequence's part of the cache has
     int mask_type, wl, wr;
     int heads_log2, chunk_log2, stages;  // kv heads of a CTA; tokens of a box
-    int dual;                            // the teams of 8 warps take a tile of 8 rows each and all stages, instead of every other stage
+    int dual;                            // sequences may have a second tile of 8 rows, which the second team of warps takes: both go through all stages
     int line_log2;                       // bytes of a box's innermost rows: 128, or what the CTA's heads have
     float scale_log2;
 };
@@ -405,9 +405,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const int width = heads * NG * 4;
     const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * width + hw * (4 * NG);
     bool failed = false;
-    // Tiles are counted over all segments; a team takes every other one, or (dual) every one.  tile_count: before this segment; next: this team's next
+    // Tiles are counted over all segments; a team takes every other one, or (dual) goes through all.  tile_count: before this segment; next: this team's next
     // one, its stage and the parity of its use.
-    const int step = p.dual ? 1 : 2, first_row = row0 + (p.dual ? 8 * team : 0);
+    const int step = p.dual ? 1 : 2;
     int tile_count = 0, next = p.dual ? 0 : team, stage = next;
     uint32_t phase = 0;
 
@@ -420,6 +420,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const int len = len_k(p, b);
             const int split = per_sequence ? 0 : piece - prefix[b] / piece_len;
             const int64_t q0 = p.seqstart_q ? p.seqstart_q[b] : (int64_t)b * p.seqlen_q;
+            const bool two_tiles = p.dual && rows - row0 > 8;  // a team's own rows; else the teams share one tile, and take stages in turn
+            const int first_row = row0 + (two_tiles ? 8 * team : 0);
 
             // ---- Q^T fragments: this lane has channels 32 i + 8 t .. + 7 of a row, as halves scaled by a power of two.  E = 2: of row g.  K's
             // operands are fields (channels 0, 4 of 8), and 16 times the next ones (1, 5), and so on.  E = 1: columns 2r and 2r + 1 belong to row r,
@@ -528,7 +530,6 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                     for (int e = 0; e < E; ++e) z.ones[k][e] = 0.f;
             };
-            const int rows_here = rows - first_row;  // (none, where a second tile of rows is not there: the team only gives its stages back)
             int key0 = ((tile0[b] + ta + next - tile_count) << tok_log2) + unit * kUnit - step * toks;
             for (int t = ta + next - tile_count; t < tb; t += step) {
                 key0 += step * toks;
@@ -541,7 +542,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     phase ^= 1u;
                 }
                 if (failed || !mbar_wait_bounded(&full[now], parity, abort_flag, p.status, 0x200)) { failed = true; continue; }
-                if (key0 < len && rows_here > 0) {
+                // (dual, one tile: the other team's stages are only given back)
+                if (key0 < len && (!p.dual || two_tiles || ((next ^ team) & 1))) {
                     uint32_t at[2][GR / 2];
 #pragma unroll
                     for (int u = 0; u < 2; ++u)
@@ -800,11 +802,11 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             // ---- the warps of a head (and team, if these have rows of their own) meet: the upper half hands its sums to the lower one until one
             // warp is left, kMeetWarps at a time ----
-            for (int half = p.dual ? 4 : 8; half >= heads; half >>= 1) {
-                const int parts = p.dual ? 2 : max(1, half / kMeetWarps), many = min(kMeetWarps, half);
+            for (int half = two_tiles ? 4 : 8; half >= heads; half >>= 1) {
+                const int parts = two_tiles ? 2 : max(1, half / kMeetWarps), many = min(kMeetWarps, half);
                 for (int part = 0; part < parts; ++part) {
-                    const int gives = (p.dual ? (team == part ? wi : -1) : warp - kMeetWarps * part) - half;
-                    const int takes = p.dual ? (team == part ? wi : -1) : warp - kMeetWarps * part;
+                    const int gives = (two_tiles ? (team == part ? wi : -1) : warp - kMeetWarps * part) - half;
+                    const int takes = two_tiles ? (team == part ? wi : -1) : warp - kMeetWarps * part;
                     if (gives >= 0 && gives < many) {
 #pragma unroll
                         for (int e = 0; e < E; ++e) {
@@ -841,7 +843,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     asm volatile("bar.sync 1, %0;\n" ::"n"(kConsumers * 32) : "memory");
                 }
             }
-            if ((p.dual ? wi : warp) >= heads || failed) continue;
+            if ((two_tiles ? wi : warp) >= heads || failed) continue;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int r = first_row + E * t4 + e, i = r / G, h = kh * G + (r - i * G);
