@@ -549,17 +549,19 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     for (int u = 0; u < 2; ++u)
 #pragma unroll
                         for (int i = 0; i < GR / 2; ++i) at[u][i] = off[u][i] + now * St::kBytes;
-                    const uint8_t* pk = ring + now * St::kBytes + param_off;
+                    const uint32_t pk = smem_u32(ring) + now * St::kBytes + param_off;
                     const bool masked = key0 + kUnit > mask_from || key0 < mask_below;
                     // scale and least value of the lane's key g + 8 i of the unit
-                    auto param = [&](const uint8_t* base, int i, int k, float& sc, float& least) {
-                        const uint32_t w = *reinterpret_cast<const uint32_t*>(base + 8 * i * width + 4 * k);
+                    auto param = [&](uint32_t base, int i, int k, float& sc, float& least) {
+                        uint32_t w;
+                        asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w) : "r"(base + 8 * i * width + 4 * k));
                         sc = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[0]);
                         least = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[1]);
                     };
                     float x[4][E];       // scores of the lane's 4 keys, then weights p'
                     uint32_t wt[NG][4];  // p' s as halves
-                    float mid[4];        // m + 8 s of the keys (of one group; with more it would take too many registers, and is worked out again)
+                    constexpr bool kKeepMids = NG == 1 || D == 64;  // (else they would take too many registers, and are worked out again)
+                    float mid[4][NG];    // m + 8 s of the keys
                     bool careful = false;  // a hidden key's scale or least value is not finite: its weight of 0 must not meet it
                     // Usually one round.  A second one (that starts from the scores again) moves the reference of rows that need it.
 #pragma unroll 1
@@ -616,7 +618,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             for (int k = 0; k < NG; ++k) {
                                 float least;
                                 param(pk + St::kParams, i, k, vs[i][k], least);
-                                if (NG == 1) mid[i] = fmaf(8.f, vs[i][k], least);
+                                if (kKeepMids) mid[i][k] = fmaf(8.f, vs[i][k], least);
                             }
                         if (masked) {
 #pragma unroll
@@ -732,8 +734,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         for (int i = 0; i < 4; ++i)
 #pragma unroll
                             for (int k = 0; k < NG; ++k) {
-                                float centre_of = mid[i];
-                                if (NG > 1) {
+                                float centre_of = mid[i][k];
+                                if (!kKeepMids) {
                                     float sc, least;
                                     param(pk + St::kParams, i, k, sc, least);
                                     centre_of = fmaf(8.f, sc, least);
