@@ -188,6 +188,7 @@ struct AppendInt4Dev {
     const int32_t* positions;
     int* status;
     int seqlen_q, seqlen_knew, hq, warps_log2;  // warps of a job
+    bool joined;  // the queries are the new tokens: one job for both
     int64_t total_new, total_q;
 };
 
@@ -240,7 +241,6 @@ __device__ __forceinline__ Token find_token(const AppendInt4Dev& a, bool queries
 template <typename T, int ROPE>
 __global__ void __launch_bounds__(256, 4) append_int4_kernel(const __grid_constant__ AppendInt4Dev a) {
     constexpr bool kVec = ROPE != 3;
-    constexpr int kAhead = 1;  // heads in flight
     pdl_launch_dependents();
     pdl_wait();
     const CacheDev& c = a.cache;
@@ -248,77 +248,69 @@ __global__ void __launch_bounds__(256, 4) append_int4_kernel(const __grid_consta
     const int64_t job = (int64_t)blockIdx.x << (3 - a.warps_log2) | (warp >> a.warps_log2);
     const int part = warp & ((1 << a.warps_log2) - 1);
     if (job >= a.total_new + a.total_q) return;  // (whole warps)
-    const bool queries = job >= a.total_new;
-    const int64_t t = queries ? job - a.total_new : job;
-    const int heads = queries ? a.hq : c.hkv;
+    // a job of queries, of keys and values, or (joined: the queries are the new tokens) of both
+    const bool only_queries = job >= a.total_new;
+    const int64_t t = only_queries ? job - a.total_new : job;
     const int lanes_log2 = c.d == 64 ? 2 : 3, lanes = 1 << lanes_log2, at_once = 32 >> lanes_log2;
     const int sub = lane >> lanes_log2, e0 = (lane & (lanes - 1)) << 3, step = at_once << a.warps_log2;
-    if (part * at_once >= heads) return;
-    const T* src = (const T*)(queries ? a.q : a.knew) + t * heads * c.d;
-    const T* vsrc = (const T*)a.vnew + t * heads * c.d;
+    if (part * at_once >= (only_queries || a.joined ? max(a.hq, only_queries ? 0 : c.hkv) : c.hkv)) return;
     Turn<T, kVec ? ROPE : 0> turn(a.rot, e0, c.d);
 
-    Pieces<T> x[kAhead], y[kAhead], v[kAhead];
-    auto request = [&](int h0) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int h = h0 + i * step + sub;
-            x[i].a.v = x[i].b.v = v[i].a.v = v[i].b.v = make_uint4(0, 0, 0, 0);
-            if (kVec && h < heads) {
-                x[i] = turn.own(src + h * c.d);
-                if (ROPE == 4) y[i] = turn.other(src + h * c.d);
-                if (!queries) v[i] = turn.own(vsrc + h * c.d);
-            }
+    Pieces<T> x, y, v;
+    auto request = [&](bool queries, int h0) {
+        const int heads = queries ? a.hq : c.hkv, h = h0 + sub;
+        const T* src = (const T*)(queries ? a.q : a.knew) + (t * heads + h) * c.d;
+        x.a.v = x.b.v = v.a.v = v.b.v = make_uint4(0, 0, 0, 0);
+        if (kVec && h < heads) {
+            x = turn.own(src);
+            if (ROPE == 4) y = turn.other(src);
+            if (!queries) v = turn.own((const T*)a.vnew + (t * heads + h) * c.d);
         }
     };
-    request(part * at_once);  // (a row is there whether it belongs to a sequence or not: its loads do not wait for what follows)
+    request(only_queries, part * at_once);  // (a row is there whether it belongs to a sequence or not: its loads do not wait for what follows)
 
-    const Token k = find_token(a, queries, t, lane);
+    const Token k = find_token(a, only_queries, t, lane);
     const bool real = k.j >= 0 && k.j < k.n;  // (a row that belongs to no sequence leaves as zeros)
     // the last new tokens are the queries'
-    const int64_t j = k.j + (queries ? (a.seqstart_knew ? a.seqstart_knew[k.b + 1] - k.first : (int64_t)a.seqlen_knew) - k.n : 0);
+    const int64_t j = k.j + (only_queries ? (a.seqstart_knew ? a.seqstart_knew[k.b + 1] - k.first : (int64_t)a.seqlen_knew) - k.n : 0);
     const int64_t at = real ? c.seqlen[k.b] + j : -1;  // place in the cache
     const int64_t token = k.first + j;
     Positions pos;
     if (ROPE != 0 && a.positions && j >= 0 && token < a.total_new) pos.load(a.positions, a.rot.axes, a.total_new, token);
     else pos.fill(a.positions ? -1 : at);
     if (real) turn.load(a.rot, pos);
-    const int64_t row = !queries && real ? cache_row(c, k.b, at) : -1;
-    if (!queries && real && row < 0 && lane == 0 && part == 0) atomicOr(a.status, FLASHCK_STATUS_APPEND_OVERFLOW);
+    const int64_t row = !only_queries && real ? cache_row(c, k.b, at) : -1;
+    if (!only_queries && real && row < 0 && lane == 0 && part == 0) atomicOr(a.status, FLASHCK_STATUS_APPEND_OVERFLOW);
     const bool joint = c.group == c.d;  // one group: both pieces
     const int group_lanes = joint ? lanes : c.group >> 3, group_log2 = 31 - __clz(c.group), groups = c.d >> group_log2;
 
-    for (int h0 = part * at_once; h0 < heads; h0 += step * kAhead) {
-        if (h0 != part * at_once) request(h0);
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
-            const int h = h0 + i * step + sub;
-            const bool mine = h < heads;
-            if (h0 + i * step >= heads) break;  // (the whole warp)
-            if constexpr (!kVec) {
-                if (mine && real) {
-                    turn_piece_any<T>(a.rot, e0, pos, src + h * c.d, x[i].a);
-                    turn_piece_any<T>(a.rot, e0 + (c.d >> 1), pos, src + h * c.d, x[i].b);
-                    if (!queries) {
-                        v[i].a = load8(vsrc + h * c.d + e0, false);
-                        v[i].b = load8(vsrc + h * c.d + e0 + (c.d >> 1), false);
-                    }
+    auto turned = [&](bool queries, int h) {
+        const int heads = queries ? a.hq : c.hkv;
+        if constexpr (!kVec) {
+            if (h < heads && real) {
+                const T* src = (const T*)(queries ? a.q : a.knew) + (t * heads + h) * c.d;
+                turn_piece_any<T>(a.rot, e0, pos, src, x.a);
+                turn_piece_any<T>(a.rot, e0 + (c.d >> 1), pos, src, x.b);
+                if (!queries) {
+                    const T* vsrc = (const T*)a.vnew + (t * heads + h) * c.d;
+                    v.a = load8(vsrc + e0, false);
+                    v.b = load8(vsrc + e0 + (c.d >> 1), false);
                 }
-            } else {
-                turn(x[i], y[i]);
-                if (!real) x[i].a.v = x[i].b.v = v[i].a.v = v[i].b.v = make_uint4(0, 0, 0, 0);
             }
-            if (queries) {
-                if (mine) {
-                    T* dst = (T*)a.q_out + (t * heads + h) * c.d;
-                    store8(dst + e0, x[i].a, kVec);
-                    store8(dst + e0 + (c.d >> 1), x[i].b, kVec);
-                }
-                continue;
-            }
+        } else {
+            turn(x, y);
+            if (!real) x.a.v = x.b.v = v.a.v = v.b.v = make_uint4(0, 0, 0, 0);
+        }
+    };
+    if (!only_queries) {
+        for (int h0 = part * at_once; h0 < c.hkv; h0 += step) {
+            const int h = h0 + sub;
+            const bool mine = h < c.hkv;
+            if (h0 != part * at_once) request(false, h0);
+            turned(false, h);
 #pragma unroll
             for (int kv = 0; kv < 2; ++kv) {
-                const Pieces<T>& z = kv ? v[i] : x[i];
+                const Pieces<T>& z = kv ? v : x;
                 uint32_t ra = range_of(z.a), rb = range_of(z.b);
                 if (joint) ra = rb = min2_nan<T>(ra, rb);
                 for (int off = 1; off < group_lanes; off <<= 1) {
@@ -343,10 +335,22 @@ __global__ void __launch_bounds__(256, 4) append_int4_kernel(const __grid_consta
                 }
                 T* held = (T*)(kv ? a.v_held : a.k_held);
                 if (held) {
-                    held += (t * heads + h) * c.d + e0;
+                    held += (t * c.hkv + h) * c.d + e0;
                     store8(held, values_of<T>(wa, scale[0], lo[0]), kVec);
                     store8(held + (c.d >> 1), values_of<T>(wb, scale[1], lo[1]), kVec);
                 }
+            }
+        }
+    }
+    if (only_queries || a.joined) {
+        for (int h0 = part * at_once; h0 < a.hq; h0 += step) {
+            const int h = h0 + sub;
+            if (!only_queries || h0 != part * at_once) request(true, h0);
+            turned(true, h);
+            if (h < a.hq) {
+                T* dst = (T*)a.q_out + (t * a.hq + h) * c.d + e0;
+                store8(dst, x.a, kVec);
+                store8(dst + (c.d >> 1), x.b, kVec);
             }
         }
     }
@@ -469,6 +473,8 @@ int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream) {
     a.seqlen_q = (int)p.seqlen_q; a.seqlen_knew = (int)p.seqlen_knew; a.hq = (int)p.hq;
     a.total_new = p.seqstart_knew ? p.seqlen_knew : p.cache.batch * p.seqlen_knew;
     a.total_q = !p.q ? 0 : p.seqstart_q ? p.seqlen_q : p.cache.batch * p.seqlen_q;
+    a.joined = p.q && p.seqstart_q == p.seqstart_knew && p.seqlen_q == p.seqlen_knew;
+    if (a.joined) a.total_q = 0;
     const int64_t jobs = a.total_new + a.total_q;
     if (jobs == 0) return FLASHCK_OK;
     a.warps_log2 = warps_log2_for(jobs, std::max<int64_t>(1, std::max(p.hq, p.cache.hkv) * p.cache.d / 256));
