@@ -150,6 +150,7 @@ __device__ __forceinline__ uint32_t quantise(const Vec8<T>& x, uint32_t both, T&
     // a multiple of another one in a few per thousand.)
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    if (s == 0.f) inv = 0.f;  // (all codes 0; a lane without a head comes here too)
     const uint64_t inv2 = two(inv, inv), minus_s = two(-s, -s), minus_lo = two(-lo, -lo), round2 = two(12582912.f, 12582912.f);
     uint32_t u[8];
 #pragma unroll
@@ -162,7 +163,7 @@ __device__ __forceinline__ uint32_t quantise(const Vec8<T>& x, uint32_t both, T&
     }
     // scales that T holds with few digits (a code may pass 15), and those whose reciprocal or remainder fp32 may not hold
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    if (!(s >= (kHalf ? 6.103515625e-5f : 1e-25f) && s <= 1e25f)) {
+    if (!(s == 0.f || (s >= (kHalf ? 6.103515625e-5f : 1e-25f) && s <= 1e25f))) {
         scale_t = Elem<T>::from_f32(range < INFINITY ? __fdiv_rn(range, 15.f) : NAN);
         const float exact = Elem<T>::to_f32(scale_t);
 #pragma unroll
