@@ -139,11 +139,14 @@ __device__ __forceinline__ uint32_t halves(float lo, float hi) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Shared memory of a stage: K codes, V codes [chunk][128-byte column][token] rows, K params, V params [token] rows of the CTA's heads.
-template <int D, int NG>
+// Shared memory of a stage: K codes, V codes [chunk][128-byte column][token] rows, K params, V params [token] rows of the CTA's heads, with
+// 16 bytes between two where they are 64 bytes and more: a warp reads one of 8 tokens at a time, which then lie in different banks.  (With E = 2,
+// whose sums leave no register for another stride, that costs more than it gives: 32 sequences of 64 / 8 heads, groups of 64, 167 -> 175 us; with
+// E = 1 and 32 / 8 heads 159 -> 136, groups of 32 275 -> 210.)
+template <int D, int NG, int E>
 struct Stage {
     static constexpr int kCodes = kPairs * (D / 2);
-    static constexpr int kParams = kPairs * NG * 4;
+    static constexpr int kParams = kPairs * NG * 4 + (E == 2 || NG == 1 ? 0 : 256 * NG);
     static constexpr int kBytes = (2 * kCodes + 2 * kParams + 1023) / 1024 * 1024;
 };
 
@@ -167,7 +170,7 @@ template <typename T, int D, int NG, int E>
 __global__ void __launch_bounds__(kThreads, 1)
 splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Int4Dev p) {
     constexpr int ROW = D / 2, GR = D / 32, PER = GR / NG;  // bytes of a row; 16-byte pieces (32 channels) of it; of them per group
-    using St = Stage<D, NG>;
+    using St = Stage<D, NG, E>;
     extern __shared__ uint8_t smem_raw[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int G = p.hq / p.hkv, stages = p.stages;
@@ -263,7 +266,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
         const int chunk = 1 << p.chunk_log2, box = heads * chunk * ROW, column0 = (head0 * ROW) >> p.line_log2;
         // scales and least values: a lane copies a piece of 4 to 16 bytes of a token's, for K and V
-        const int width = heads * NG * 4;
+        const int width = heads * NG * 4, pitch = width + (E == 1 && width >= 64 ? 16 : 0);
         const int piece_log2 = min(4, 31 - __clz(width)), pieces_log2 = 31 - __clz(width) - piece_log2;
         const int copies = toks << pieces_log2;
         const int per_tile_log2 = tok_log2 - p.chunk_log2;
@@ -335,7 +338,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         const int64_t first = __shfl_sync(0xffffffffu, at, k >> p.chunk_log2);
                         const bool there = first >= 0 && token0 + k < len;  // (the rest of a tile has scales of zero)
                         const int64_t off = there ? (first + (int64_t)(k & (chunk - 1)) * p.hkv) * (4 * NG) + part : 0;
-                        const uint32_t to = dst + k * width + part;
+                        const uint32_t to = dst + k * pitch + part;
                         if (piece_log2 == 4) {
                             copy_async<16>(to, p.k_params + off, there);
                             copy_async<16>(to + St::kParams, p.v_params + off, there);
@@ -402,8 +405,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
             for (int i = 0; i < GR / 2; ++i) off[u][i] = smem_u32(ring) + u * block_step + (row << p.line_log2) + (((piece + 2 * i) ^ mswz) << 4);
     }
-    const int width = heads * NG * 4;
-    const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * width + hw * (4 * NG);
+    const int width = heads * NG * 4, pitch = width + (E == 1 && width >= 64 ? 16 : 0);
+    const uint32_t param_off = 2 * St::kCodes + (unit * kUnit + g) * pitch + hw * (4 * NG);
     bool failed = false;
     // Tiles are counted over all segments; a team takes every other one, or (dual) goes through all.  tile_count: before this segment; next: this team's next
     // one, its stage and the parity of its use.
@@ -554,7 +557,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     // scale and least value of the lane's key g + 8 i of the unit
                     auto param = [&](uint32_t base, int i, int k, float& sc, float& least) {
                         uint32_t w;
-                        asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w) : "r"(base + 8 * i * width + 4 * k));
+                        asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w) : "r"(base + 8 * i * pitch + 4 * k));
                         sc = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[0]);
                         least = Elem<T>::to_f32(reinterpret_cast<const T*>(&w)[1]);
                     };
@@ -884,7 +887,7 @@ int make_codes_map(CUtensorMap* map, const void* base, int64_t pool, int64_t pag
 
 template <typename T, int D, int NG, int E>
 int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
-    using St = Stage<D, NG>;
+    using St = Stage<D, NG, E>;
     const Int4Cache& c = p.cache;
     while (dev.heads_log2 < 3 && c.hkv % (2ll << dev.heads_log2) == 0) ++dev.heads_log2;
     const int heads = 1 << dev.heads_log2, toks = kPairs / heads;
