@@ -122,6 +122,21 @@ class FlashAttention(torch.nn.Module):
         return self._fn("append_kv")(q, k_cache, v_cache, knew, vnew, seqlen_k, cos, sin,
                                      rope=rope if rotary is not None else RopeEnum.NONE, **kwargs)
 
+    def forward_int4(self, q: torch.Tensor, k_cache: torch.Tensor, k_params: torch.Tensor, v_cache: torch.Tensor, v_params: torch.Tensor,
+                     seqlen_k: torch.Tensor, **kwargs):
+        """Attention of one or a few new tokens over a 4-bit cache (:func:`fmha_fwd_splitkv_int4`)."""
+        self._check_heads(q, k_params[..., 0])
+        return self._fn("forward_splitkv_int4")(q, k_cache, k_params, v_cache, v_params, seqlen_k=seqlen_k, scale=self.scale,
+                                                causal=self.causal, window_size=self.window_size, **kwargs)
+
+    def append_kv_int4(self, q: Optional[torch.Tensor], k_cache: torch.Tensor, k_params: torch.Tensor, v_cache: torch.Tensor,
+                       v_params: torch.Tensor, knew: torch.Tensor, vnew: torch.Tensor, seqlen_k: torch.Tensor,
+                       rotary: Optional[Tuple[torch.Tensor, torch.Tensor]] = None, rope: int = RopeEnum.INTERLEAVED, **kwargs):
+        """Turns the queries and the new keys and writes the new K/V in 4 bits (:func:`fmha_fwd_append_kv_int4`)."""
+        cos, sin = rotary if rotary is not None else (None, None)
+        return self._fn("append_kv_int4")(q, k_cache, k_params, v_cache, v_params, knew, vnew, seqlen_k, cos, sin,
+                                          rope=rope if rotary is not None else RopeEnum.NONE, **kwargs)
+
     def extra_repr(self) -> str:
         return (f"num_heads={self.num_heads}, num_kv_heads={self.num_kv_heads}, head_dim={self.head_dim}, "
                 f"head_dim_v={self.head_dim_v}, causal={self.causal}, window_size={self.window_size}, scale={self.scale}")

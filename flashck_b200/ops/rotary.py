@@ -62,7 +62,8 @@ def _as_positions(positions: torch.Tensor, tokens: int) -> Tuple[torch.Tensor, i
         raise TypeError("positions must be a torch.Tensor")
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"positions must have dtype torch.int32 or torch.int64, got {positions.dtype}")
-    p = _f._as_i32("positions", positions)
+    # (the kernels hold 32 bits: what lies behind them is outside every table, and must not come back to it)
+    p = _f._as_i32("positions", positions.clamp(-1, 2 ** 31 - 1) if positions.dtype == torch.int64 and positions.is_cuda else positions)
     axes = p.numel() // tokens if tokens else 1
     if p.numel() != axes * tokens or axes < 1 or (axes > 1 and p.shape[0] != axes):
         _f._refuse("positions", positions, f"{tokens} positions, or [axes, ...] of them")

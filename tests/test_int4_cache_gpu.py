@@ -490,3 +490,98 @@ def test_the_binding_and_python_agree(monkeypatch):
     a = all_calls()
     monkeypatch.setattr(fmha, "_NATIVE", False)
     assert all(torch.equal(x, y) for x, y in zip(a, all_calls()))
+
+
+def test_equal_calls_give_equal_bits():
+    """Many short segments and both ways in which the teams of warps share the rows; a read of a stage too early shows as a difference."""
+    for tokens, hq, group in (([1] * 40, 32, 128), ([1] * 40, 64, 64), ([1, 4] * 20, 32, 64), ([4] * 40, 32, 32)):
+        c = Cache([1 + 131 * i % 700 for i in range(40)], 8, 128, group, torch.bfloat16, 16)
+        c.seqlen = torch.maximum(c.seqlen, _i32(tokens))
+        q = _normal(_g(3), sum(tokens), hq, 128, dtype=torch.bfloat16)
+        call = lambda: ops.fmha_fwd_splitkv_int4(q, *c.parts, seqlen_k=c.seqlen, block_table=c.table, cu_seqlens_q=_starts(tokens),  # noqa: E731
+                                                 max_seqlen_q=max(tokens), causal=True, return_lse=True)
+        first = call()
+        for _ in range(60):
+            again = call()
+            assert all(torch.equal(torch.nan_to_num(a), torch.nan_to_num(b)) for a, b in zip(first, again))
+    assert _lib.device_status() == 0
+
+
+def test_pools_of_more_than_4_gigabytes():
+    """The pages in use lie at the end of pools whose offsets pass 32 bits."""
+    pages, page, hkv, d = 600000, 128, 1, 128  # 4.9e9 bytes of codes, each
+    parts = []
+    for _ in range(2):
+        parts += [torch.empty(pages, page, hkv, d // 2, dtype=torch.uint8, device="cuda"), torch.empty(pages, page, hkv, 1, 2, dtype=torch.bfloat16, device="cuda")]
+    table = _i32([[pages - 1, pages - 7, pages - 3]])
+    g = _g(0)
+    k, v, q = (_normal(g, 1, 300, h, d, dtype=torch.bfloat16) for h in (1, 1, 8))
+    held = ops.fmha_fwd_append_kv_int4(q, *parts, k, v, _i32([0]), rope=RopeEnum.NONE, block_table=table, return_kv=True)[1:]
+    assert all(torch.equal(a, b) for a, b in zip(held, ops.fmha_read_kv_int4(*parts, _i32([300]), block_table=table, max_seqlen_k=300)))
+    o = ops.fmha_fwd_splitkv_int4(q[:, :1].contiguous(), *parts, seqlen_k=_i32([300]), block_table=table)
+    rows = (table[0].long()[torch.arange(300, device="cuda") // page] * page + torch.arange(300, device="cuda") % page)
+    want, _, bound, _ = ref.attend(q[0, :1], *(x.flatten(0, 1)[rows] for x in parts), d ** -0.5, (0, -1, -1))
+    ref.assert_within("o", o[0], want, bound)
+
+
+def test_the_module():
+    from flashck_b200.nn import FlashAttention
+    layer = FlashAttention(8, 64, 2, causal=True)
+    c = Cache([40, 9], 2, 64, 32, torch.float16, 16, room=64)
+    q, new = _normal(_g(1), 2, 1, 8, 64, dtype=torch.float16), _normal(_g(2), 2, 1, 2, 64, dtype=torch.float16)
+    cos, sin = (t.to(torch.float16) for t in _angles(100, 32))
+    turned = layer.append_kv_int4(q, *c.parts, new, new, c.seqlen, (cos, sin), block_table=c.table)
+    assert torch.equal(turned, ops.fmha_fwd_append_kv_int4(q, *c.parts, new, new, c.seqlen, cos, sin, block_table=c.table))
+    o = layer.forward_int4(turned, *c.parts, c.seqlen + 1, block_table=c.table)
+    assert torch.equal(o, ops.fmha_fwd_splitkv_int4(turned, *c.parts, seqlen_k=c.seqlen + 1, block_table=c.table, causal=True))
+    with pytest.raises(ValueError, match="must end in"):
+        layer.forward_int4(q[..., :4, :].contiguous(), *c.parts, c.seqlen, block_table=c.table)
+
+
+def test_calls_that_do_not_fit_are_refused():
+    c = Cache([40, 9], 2, 64, 32, torch.float16, 16, room=64)
+    q, new = _normal(_g(1), 2, 1, 8, 64, dtype=torch.float16), _normal(_g(2), 2, 1, 2, 64, dtype=torch.float16)
+    attend = lambda q=q, parts=c.parts, **kw: ops.fmha_fwd_splitkv_int4(q, *parts, **{**dict(seqlen_k=c.seqlen, block_table=c.table), **kw})  # noqa: E731
+    append = lambda k=new, v=new, q=q, **kw: ops.fmha_fwd_append_kv_int4(q, *c.parts, k, v, c.seqlen, **{**dict(rope=0, block_table=c.table), **kw})  # noqa: E731
+    kc, kp, vc, vp = c.parts
+    cos = torch.ones(70, 32, device="cuda", dtype=torch.float16)
+    cases = [
+        (lambda: attend(q.bfloat16()), TypeError), (lambda: attend(q[:1]), ValueError), (lambda: attend(q[..., :32].contiguous()), ValueError),
+        (lambda: attend(q[:, :, :3].contiguous()), ValueError), (lambda: attend(seqlen_k=c.seqlen[:1]), ValueError),
+        (lambda: attend(block_table=c.table[:1]), ValueError), (lambda: attend(block_table=None, parts=[x[:1] for x in c.parts]), ValueError),
+        (lambda: attend(parts=[kc, kp, vc[:1], vp]), ValueError), (lambda: attend(parts=[kc, kp[:, :8].contiguous(), vc, vp]), ValueError),
+        (lambda: attend(parts=[kc, kp.bfloat16(), vc, vp]), TypeError), (lambda: attend(parts=[kc.int(), kp, vc, vp]), TypeError),
+        (lambda: attend(parts=[kc[..., :16].contiguous(), kp, vc[..., :16].contiguous(), vp]), ValueError),
+        (lambda: attend(parts=[kc, kp.transpose(0, 1), vc, vp]), ValueError), (lambda: attend(cu_seqlens_q=_starts([1, 1])), ValueError),
+        (lambda: attend(q.flatten(0, 1), cu_seqlens_q=_starts([2])), ValueError), (lambda: attend(seqlen_k=None), TypeError),
+        (lambda: attend(parts=[x.view(-1, 8, *x.shape[2:]) for x in c.parts]), ValueError), (lambda: attend(num_splits=5000), RuntimeError),
+        (lambda: attend(torch.cat([q.flatten(), q.flatten()])[4: 4 + q.numel()].view(q.shape)), ValueError),
+        (lambda: append(k=new[..., :32].contiguous()), ValueError), (lambda: append(v=new[:, :, :1].contiguous()), ValueError),
+        (lambda: append(q=q[:1]), ValueError), (lambda: append(cu_seqlens_knew=_starts([1, 1])), ValueError), (lambda: append(rope=1), ValueError),
+        (lambda: append(rope=1, rotary_cos=cos, rotary_sin=cos[:, :8].contiguous()), ValueError),
+        (lambda: append(rope=1, rotary_cos=cos, rotary_sin=cos, rotary_dim=32), ValueError),
+        (lambda: append(rope=1, rotary_cos=cos.bfloat16(), rotary_sin=cos.bfloat16()), TypeError),
+        (lambda: append(rope=1, rotary_cos=cos, rotary_sin=cos, positions=_i32([1, 2, 3])), ValueError),
+        (lambda: append(rope=1, rotary_cos=cos, rotary_sin=cos, positions=_i32([[1, 2], [3, 4]])), ValueError),
+        (lambda: append(rope=1, rotary_cos=cos, rotary_sin=cos, positions=_i32([[1, 2], [3, 4]]), sections=(16, 17)), ValueError),
+        (lambda: append(rope=1, rotary_cos=cos, rotary_sin=cos, positions=torch.ones(2, device="cuda")), TypeError),
+        (lambda: append(positions=_i32([1, 2])), ValueError), (lambda: append(rope=5, rotary_cos=cos, rotary_sin=cos), RuntimeError),
+        (lambda: ops.fmha_read_kv_int4(*c.parts, c.seqlen, block_table=c.table), ValueError),
+        (lambda: ops.fmha_read_kv_int4(*c.parts, c.seqlen, block_table=c.table, max_seqlen_k=-1), ValueError),
+        (lambda: ops.fmha_read_kv_int4(*c.parts, c.seqlen, block_table=c.table, total_k=5), ValueError),
+        (lambda: ops.fmha_read_kv_int4(*c.parts, c.seqlen, block_table=c.table, cu_seqlens_k=_starts([5]), total_k=5), ValueError),
+        (lambda: ops.apply_rotary(q, None, _i32([0, 1, 2]), cos, cos), ValueError), (lambda: ops.apply_rotary(q, new.bfloat16(), _i32([0, 1]), cos, cos), TypeError),
+        (lambda: ops.apply_rotary(q, None, _i32([0, 1]), cos, cos, rope=0), ValueError),
+        (lambda: ops.apply_rotary(q[..., :32].contiguous(), None, _i32([0, 1]), cos, cos), ValueError),
+        (lambda: ops.apply_rotary(q[..., :60].contiguous(), None, _i32([0, 1]), cos[:, :30].contiguous(), cos[:, :30].contiguous()), RuntimeError),
+        (lambda: ops.apply_rotary(q.transpose(1, 2), None, _i32([0, 1]), cos, cos), ValueError),
+    ]
+    for i, (call, error) in enumerate(cases):
+        with pytest.raises(error):
+            call()
+            pytest.fail(f"case {i} was taken")
+    # nothing to do is no error
+    assert attend(q[:, :0]).shape == (2, 0, 8, 64)
+    k, v = ops.fmha_read_kv_int4(*c.parts, c.seqlen, block_table=c.table, max_seqlen_k=0)
+    assert k.shape == (2, 0, 2, 64)
+    assert append(k=new[:, :0].contiguous(), v=new[:, :0].contiguous(), q=None) is None

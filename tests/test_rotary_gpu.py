@@ -77,6 +77,13 @@ def test_positions_outside_the_tables_turn_by_nan():
     assert torch.isfinite(y[..., :8]).all() and torch.isnan(y[2:, :, 8:16]).all()
 
 
+def test_positions_of_64_bits():
+    q = torch.ones(4, 1, 64, device="cuda", dtype=torch.bfloat16)
+    t = torch.ones(7, 32, device="cuda", dtype=torch.bfloat16)
+    y, _ = ops.apply_rotary(q, None, torch.tensor([3, 2 ** 32 + 3, -2 ** 32 + 3, 2 ** 31], device="cuda"), t, t)
+    assert torch.isfinite(y[0]).all() and torch.isnan(y[1:]).all()
+
+
 def test_empty():
     t = torch.ones(7, 16, device="cuda", dtype=torch.bfloat16)
     q = torch.ones(0, 2, 64, device="cuda", dtype=torch.bfloat16)
