@@ -1,7 +1,7 @@
 // Rotation of queries and keys by the positions of their tokens, along one or several axes (int4.cuh has the arithmetic).
 //
 // Bound by its traffic: each row read and written once.  A warp turns a token (a few warps, where tokens are few); a lane keeps the cosines
-// and sines of its 16 channels for all heads.
+// and sines of its 16 channels for all heads.  16384 tokens of 32 + 8 heads of 128: 57 us, floor 52 at 6.46 TB/s (the copy rate).
 #include <algorithm>
 #include <type_traits>
 

@@ -5,23 +5,30 @@
 //     O_c   = sum_j p_j (m_j + s_j u_jc) = sum_j (p_j s_j) (u_jc - 8)  +  sum_j p_j (m_j + 8 s_j),
 // and no key or value is ever written out: the products run over the codes themselves, scales and least values come in once per key.
 // The second sum of O is one number per row and group; with 8 taken off, what the rounding of p s to 16 bits costs is in proportion to
-// the values' spread, not to their distance from the least one (the rounded weights are summed by an MMA against ones for it).
+// the values' spread, not to their distance from the least one.
 //
-// Codes become MMA operands in 0.6 (K) and 0.75 (V) instructions each: a 4-bit field in the low mantissa bits of a half IS u * 2^-24 (a
-// subnormal, which the tensor cores multiply exactly), one four bits higher u * 2^-20; so a mask gives two operands, a shift by 8 the next
-// two, and the powers of two go to Q, or to O at the end.  Two keys' codes of one channel are put side by side by one byte permutation.
-// Both products are taken transposed (S^T = K Q^T, O^T = V^T P^T): m16n8k16 then has 16 keys or channels against 8 query rows, which a
-// group of 4 or 8 heads fills, instead of 16 rows half empty.  P^T's fragments come from S^T's by movmatrix.
+// Codes become MMA operands in a few instructions: a 4-bit field in the low mantissa bits of a half IS u * 2^-24 (a subnormal, which the tensor
+// cores multiply exactly), a byte of two fields u0 + 16 u1.  ldmatrix hands a warp the K rows as they lie, and, transposed, the 16-bit pieces (4
+// channels) of the V rows of two keys side by side.  A mask or a byte permutation makes each operand; the powers of two go to Q, or to O at the
+// end, and so does the lower field that a byte brings along: V's bytes are freed of it by one subtraction of sums, K's by a subtraction of halves
+// (8 rows) or by a second column of Q (4 rows).
+// Both products are taken transposed (S^T = K Q^T, O^T = V^T P^T): m16n8k16 then has 16 keys or channels against 8 query columns, which a group of
+// 8 heads fills (or 4 with two columns each), instead of 16 rows half empty.  P^T's fragments come from S^T's by movmatrix.
 //
 // Halves have no range for arbitrary Q and scales.  A row of Q is scaled by a power of two.  The weights p s are kept in range by the row's
 // reference R (p' = exp2(x - R)): it follows the largest x + log2 s seen, moves when a weight passes 2^13, and then everything the row
 // has summed is rescaled.  Moves are rare, and what decides one is a maximum over packed halves and a vote, without a shuffle.
 //
-// Bound by the cache's bytes in HBM: 136 a token and head at hdim 128 with one group, for 370 issue slots of an SM's four schedulers per 16
-// keys, of which about half are used.  A CTA per SM: four producer warps and 8 or 16 consumer warps.  A stage is 256 (head, token) pairs --
-// 32 tokens of 8 heads, 256 of one -- of K and V codes, by TMA (boxes of up to 256 tokens of a page, 64- or 32-byte swizzle: a warp's reads
-// meet no bank twice), and their scales, by 4- to 16-byte asynchronous copies.  8 consumer warps take 32 tokens of one head each; with 16,
-// two teams take stages in turn.  The warps of a head meet once per segment, in shared memory.  The work is cut as in splitkv_decode.cu.
+// A CTA per SM: four producer warps and 16 consumer warps.  A stage is 256 (head, token) pairs -- 32 tokens of 8 heads, 256 of one -- of K and V
+// codes, by TMA (boxes of up to 256 tokens of a page, rows of 128 bytes, swizzled: a warp's reads meet no bank twice), and their scales, by 4- to
+// 16-byte asynchronous copies.  A consumer warp takes 32 tokens of one head; the warps form two teams of 8, which take stages in turn (up to 8
+// rows per kv head), or all stages with a tile of 8 rows each (more).  The warps of a head meet once per segment, in shared memory.  The work is
+// cut as in splitkv_decode.cu.
+//
+// What bounds it (B200, bf16, hdim 128, 8 kv heads): the floor is the cache's bytes in HBM, 136 a token and head with one group.  64 sequences of
+// 1-32k keys under 32 heads: 208 us and 5 for the merge, floor 173 at 6.46 TB/s; with the arithmetic left out of a copy the loads alone take 192.
+// About 380 instructions a warp and 32 keys, at 0.62 a cycle and scheduler, are what the rest is.  4 x 524288 keys under 64 heads with two groups:
+// 555 us, floor 374: eight rows and two groups have more sums than registers, and 40 loads and stores of spilled ones per 32 keys.
 #include <algorithm>
 #include <type_traits>
 
@@ -140,9 +147,9 @@ __device__ __forceinline__ uint32_t halves(float lo, float hi) {
 }
 
 // Shared memory of a stage: K codes, V codes [chunk][128-byte column][token] rows, K params, V params [token] rows of the CTA's heads, with
-// 16 bytes between two where they are 64 bytes and more: a warp reads one of 8 tokens at a time, which then lie in different banks.  (With E = 2,
-// whose sums leave no register for another stride, that costs more than it gives: 32 sequences of 64 / 8 heads, groups of 64, 167 -> 175 us; with
-// E = 1 and 32 / 8 heads 159 -> 136, groups of 32 275 -> 210.)
+// 16 bytes between two where they are 64 bytes and more: a warp reads one of 8 tokens at a time, which then lie in different banks.  (With E = 2 it
+// costs more than it gives: 32 sequences of 64 / 8 heads, groups of 64, 167 -> 185 us; with E = 1 and 32 / 8 heads 159 -> 135, groups of 32
+// 275 -> 209.)
 template <int D, int NG, int E>
 struct Stage {
     static constexpr int kCodes = kPairs * (D / 2);
