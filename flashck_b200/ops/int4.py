@@ -167,7 +167,7 @@ def fmha_fwd_splitkv_int4(q: torch.Tensor, k_cache: torch.Tensor, k_params: torc
     read once per 16 rows of a kv head (``sq * hq / hkv``): a chunk of a prompt goes through :func:`fmha_read_kv_int4` and
     :func:`fmha_fwd_var_len`.
 
-    Returns o like q (and LSE fp32 ``[b, hq, sq]`` / ``[hq, total_q]``); packed rows that belong to no sequence are not written."""
+    Returns o like q (and LSE fp32 ``[b, hq, sq]`` / ``[hq, total_q]``); packed rows that belong to no sequence hold nothing of meaning."""
     native = _f._native()
     if native and cache_batch_idx is None:
         r = native._call_splitkv_int4(q, k_cache, k_params, v_cache, v_params, seqlen_k, block_table, cu_seqlens_q, max_seqlen_q, num_splits, scale,

@@ -585,3 +585,28 @@ def test_calls_that_do_not_fit_are_refused():
     k, v = ops.fmha_read_kv_int4(*c.parts, c.seqlen, block_table=c.table, max_seqlen_k=0)
     assert k.shape == (2, 0, 2, 64)
     assert append(k=new[:, :0].contiguous(), v=new[:, :0].contiguous(), q=None) is None
+
+
+@pytest.mark.parametrize("mask", [(0, -1, -1), (1, -1, 0), (2, -1, 0), (2, 30, 0), (2, 5, 3), (3, 100, 10)])
+@pytest.mark.parametrize("tokens,hq,hkv", [(2, 4, 2), (4, 3, 3), (3, 1, 1), (5, 1, 1), (8, 2, 2)])
+def test_masks_of_few_rows(mask, tokens, hq, hkv):
+    """Several tokens and up to 4, and up to 8 rows per kv head."""
+    _attend(Cache([200, 77, 3], hkv, 128, 64, torch.bfloat16, 16), [tokens] * 3, hq, mask)
+
+
+def test_as_many_sequences_as_are_taken():
+    """The schedule of 8192 sequences leaves room for few stages.  A split per sequence makes a sequence's bits its own."""
+    lens = [1 + 53 * i % 70 for i in range(8192)]
+    c = Cache([4096 * 16], 2, 128, 32, torch.bfloat16, 0)  # (values only: the pools are laid out below)
+    parts = [x.view(4096, 16, *x.shape[2:]) for x in c.parts]
+    table = torch.randint(0, 4096, (8192, 5), generator=_g(0), device="cuda", dtype=torch.int32)
+    for hq in (2, 16):
+        q = _normal(_g(1), 8192, 1, hq, 128, dtype=torch.bfloat16)
+        call = lambda s: ops.fmha_fwd_splitkv_int4(q[s], *parts, seqlen_k=_i32(lens[s]), block_table=table[s], num_splits=1)  # noqa: E731
+        whole = call(slice(0, 8192))
+        assert torch.isfinite(whole).all()
+        for i in range(0, 8192, 1024):
+            assert torch.equal(whole[i: i + 1024], call(slice(i, i + 1024)))
+    with pytest.raises(RuntimeError, match="8192"):
+        ops.fmha_fwd_splitkv_int4(torch.cat([q, q[:1]]), *parts, seqlen_k=_i32(lens + [1]), block_table=torch.cat([table, table[:1]]))
+    assert _lib.device_status() == 0
