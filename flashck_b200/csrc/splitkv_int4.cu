@@ -68,6 +68,10 @@ __device__ __forceinline__ int len_q(const Int4Dev& p, int b) {
     return p.seqstart_q ? (int)(p.seqstart_q[b + 1] - p.seqstart_q[b]) : p.seqlen_q;
 }
 __device__ __forceinline__ int len_k(const Int4Dev& p, int b) { return min(p.seqlen_k[b], p.room); }
+// What a tile of a sequence costs, in units of the schedule: with more than 8 rows both teams go through all tiles, else each through every other one.  (A CTA
+// alone took 3200 and 2000 cycles a tile at hdim 64; 32 sequences of 1-4 tokens, 32 / 8 heads, hdim 128, with one cost for both: groups of 128 210 -> 191 us,
+// of 64 282 -> 251, of 32 486 -> 433.  2 : 1 was worse than one cost: 48 short ones at hdim 64 85 -> 97.)
+__device__ __forceinline__ int cost(const Int4Dev& p, int b) { return !p.dual ? 1 : len_q(p, b) * (p.hq / p.hkv) > 8 ? 3 : 2; }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
@@ -190,7 +194,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint64_t* bars = reinterpret_cast<uint64_t*>(meet_stats + kMeetWarps * 4 * E * 2);
     uint64_t* full = bars;
     uint64_t* empty = bars + stages;
-    int* prefix = reinterpret_cast<int*>(bars + 2 * stages);  // [batch + 1] tiles before each sequence
+    int* prefix = reinterpret_cast<int*>(bars + 2 * stages);  // [batch + 1] cost of the tiles before each sequence
     int* tile0 = prefix + p.batch + 1;
     volatile int* abort_flag = tile0 + p.batch;
     int* longest = const_cast<int*>(abort_flag) + 1;
@@ -205,7 +209,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     pdl_launch_dependents();
     pdl_wait();
-    // ---- schedule: tiles (stages) per sequence and their prefix sums ----
+    // ---- schedule: what the tiles (stages) of each sequence cost, and the prefix sums ----
     if (warp == 0) {
         int run = 0, mx = 0;
         for (int base = 0; base < p.batch; base += 32) {
@@ -217,7 +221,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     int first = 0;
                     if (p.mask_type != 0 && p.wl >= 0) first = max(0, min(len - 1, (p.mask_type == 2 ? len - len_q(p, b) : 0) - p.wl));
                     t0 = first >> tok_log2;
-                    n = ((len - 1) >> tok_log2) + 1 - t0;
+                    n = (((len - 1) >> tok_log2) + 1 - t0) * cost(p, b);
                 }
                 tile0[b] = t0;
             }
@@ -242,9 +246,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const bool per_sequence = p.num_splits <= 1;
     const int even = (total + (int)gridDim.x - 1) / (int)gridDim.x;
     const int cap = per_sequence ? 0 : (*longest + p.num_splits - 2) / (p.num_splits - 1);
-    const int piece_len = max(1, max(even, cap));
+    const int piece_len = max(p.dual ? 3 : 1, max(even, cap));  // (a piece amid a sequence has a tile of it)
     const int pieces = per_sequence ? p.batch : (total + piece_len - 1) / piece_len;
-    auto begin_piece = [&](int piece, int& lo, int& hi) {  // its tiles, and the sequence it starts in
+    auto begin_piece = [&](int piece, int& lo, int& hi) {  // its units, and the sequence it starts in
         if (per_sequence) {
             lo = prefix[piece];
             hi = prefix[piece + 1];
@@ -258,6 +262,14 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if (prefix[mid] <= lo) a = mid; else z = mid - 1;
         }
         return a;
+    };
+    auto tiles = [&](int b, int lo, int hi, int& ta, int& tb) {  // a piece's tiles of a sequence: those whose first unit it has
+        ta = max(lo, prefix[b]) - prefix[b];
+        tb = min(hi, prefix[b + 1]) - prefix[b];
+        if (!p.dual) return;
+        const bool three = cost(p, b) == 3;
+        ta = three ? (ta + 2) / 3 : (ta + 1) / 2;
+        tb = three ? (tb + 2) / 3 : (tb + 1) / 2;
     };
     const int head0 = blockIdx.z << p.heads_log2;
     const int row0 = blockIdx.y * (p.dual ? 16 : 4 * E);  // first (token, group head) row of this CTA
@@ -283,7 +295,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int piece = blockIdx.x; piece < pieces && ok; piece += gridDim.x) {
             int lo, hi, b = begin_piece(piece, lo, hi);
             for (; b < p.batch && prefix[b] < hi && ok; ++b) {
-                const int ta = max(lo, prefix[b]) - prefix[b], tb = min(hi, prefix[b + 1]) - prefix[b];
+                int ta, tb;
+                tiles(b, lo, hi, ta, tb);
                 if (tb <= ta || row0 >= len_q(p, b) * G) continue;  // (the consumers skip the same segments)
                 const int len = len_k(p, b);
                 const int64_t bphys = p.cache_batch_idx ? p.cache_batch_idx[b] : b;
@@ -367,7 +380,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const int parts = max(1, (int)gridDim.x / p.batch), part = parts > 1 ? (int)blockIdx.x / p.batch : 0;
             for (int b = parts > 1 ? (int)blockIdx.x % p.batch : (int)blockIdx.x; b < p.batch && part < parts; b += gridDim.x) {
                 const int n = prefix[b + 1] - prefix[b];
-                const int used = n == 0 ? 0 : per_sequence ? 1 : (prefix[b + 1] - 1) / piece_len - prefix[b] / piece_len + 1;
+                const int used = n == 0 ? 0 : per_sequence ? 1 : (prefix[b + 1] - cost(p, b)) / piece_len - prefix[b] / piece_len + 1;
                 const int sq = len_q(p, b);
                 const int64_t rows = p.seqstart_q ? p.total_q : p.seqlen_q, head = p.num_splits * rows;  // LSEs of a split, of a head
                 float* first = p.lse_acc + (p.seqstart_q ? p.seqstart_q[b] : (int64_t)b * p.hq * head) + used * rows;
@@ -424,7 +437,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     for (int piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
         int lo, hi, b = begin_piece(piece, lo, hi);
         for (; b < p.batch && prefix[b] < hi; ++b) {
-            const int ta = max(lo, prefix[b]) - prefix[b], tb = min(hi, prefix[b + 1]) - prefix[b];
+            int ta, tb;
+            tiles(b, lo, hi, ta, tb);
             const int sq = len_q(p, b), rows = sq * G;
             if (tb <= ta || row0 >= rows) continue;
             const int len = len_k(p, b);
@@ -898,6 +912,8 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     const Int4Cache& c = p.cache;
     while (dev.heads_log2 < 3 && c.hkv % (2ll << dev.heads_log2) == 0) ++dev.heads_log2;
     const int heads = 1 << dev.heads_log2, toks = kPairs / heads;
+    FCK_REQUIRE((int64_t)c.batch * (dev.room / toks + 4) * (dev.dual ? 3 : 1) < (1ll << 30), FLASHCK_ERR_UNSUPPORTED,
+                "FmhaFwdSplitKVInt4: %lld sequences of up to %d keys are more than the schedule counts", (long long)c.batch, dev.room);
     int chunk = 16;
     dev.chunk_log2 = 4;
     while (2 * chunk <= toks && (!c.block_table || c.page % (2 * chunk) == 0)) { chunk *= 2; ++dev.chunk_log2; }

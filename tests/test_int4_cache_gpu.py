@@ -610,3 +610,23 @@ def test_as_many_sequences_as_are_taken():
     with pytest.raises(RuntimeError, match="8192"):
         ops.fmha_fwd_splitkv_int4(torch.cat([q, q[:1]]), *parts, seqlen_k=_i32(lens + [1]), block_table=torch.cat([table, table[:1]]))
     assert _lib.device_status() == 0
+
+
+@pytest.mark.parametrize("splits", [0, 1, 2, 3, 40, 128])
+@pytest.mark.parametrize("d,group", [(64, 32), (128, 128)])
+def test_batches_of_few_and_many_rows(d, group, splits):
+    """Sequences of up to 8 rows per kv head beside ones of more, whose tiles cost more: pieces that begin and end at any unit of a tile."""
+    lens = [3000, 1, 0, 33, 700, 31, 32, 2000, 64, 5, 257, 1500]
+    tokens = [1, 4, 3, 3, 2, 4, 1, 4, 0, 3, 2, 3]
+    _attend(Cache(lens, 2, d, group, torch.float16, 16), tokens, 8, num_splits=splits)
+    _attend(Cache([40 + 29 * i for i in range(70)], 8, d, group, torch.bfloat16, 0), [1 + i * i % 4 for i in range(70)], 32, num_splits=splits)
+
+
+def test_a_schedule_past_32_bits_is_refused():
+    parts = [torch.zeros(1, 1 << 16, 1, n, dtype=t, device="cuda") for n, t in ((32, torch.uint8), (2, torch.float16)) * 2]
+    parts = [x if x.dtype == torch.uint8 else x.view(1, 1 << 16, 1, 1, 2) for x in parts]
+    table = torch.zeros(1024, 1 << 12, dtype=torch.int32, device="cuda")
+    q = torch.zeros(1024, 1, 1, 64, dtype=torch.float16, device="cuda")
+    with pytest.raises(RuntimeError, match="schedule"):
+        ops.fmha_fwd_splitkv_int4(q, *parts, seqlen_k=_i32([1] * 1024), block_table=table)
+    assert _lib.device_status() == 0
