@@ -42,6 +42,9 @@ constexpr int kPairs = 256;  // (head, token) pairs of a stage
 constexpr int kUnit = 32;    // tokens a warp takes of it
 constexpr int kCentre = 8;   // units between two centrings
 constexpr int kMeetWarps = 4;  // warps that hand their sums over at a time
+// Units of the schedule that a sequence costs beside its tiles, for its queries and the meeting of the warps: 4 x 524288 keys 560 -> 550 us, 32 sequences
+// of 1-32k keys and 64 / 8 heads 165 -> 159; 3 and 10 gave about the same.
+constexpr int kBegin = 6;
 constexpr uint32_t kCode = 0x000f000fu;
 constexpr float kNoKey = -1e30f;  // (any score is so far above it that the reference moves)
 
@@ -198,6 +201,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     int* tile0 = prefix + p.batch + 1;
     volatile int* abort_flag = tile0 + p.batch;
     int* longest = const_cast<int*>(abort_flag) + 1;
+    int* begin = longest + 1;  // what the first tile of a sequence costs more
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
@@ -207,11 +211,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         *abort_flag = 0;
         mbar_fence_init();
     }
+    const bool per_sequence = p.num_splits <= 1;
     pdl_launch_dependents();
     pdl_wait();
     // ---- schedule: what the tiles (stages) of each sequence cost, and the prefix sums ----
     if (warp == 0) {
-        int run = 0, mx = 0;
+        int run = 0, mx = 0, sequences = 0;
         for (int base = 0; base < p.batch; base += 32) {
             const int b = base + lane;
             int n = 0, t0 = 0;
@@ -233,20 +238,34 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             }
             if (b < p.batch) prefix[b] = run + incl - n;
             run += __shfl_sync(0xffffffffu, incl, 31);
+            sequences += __popc(__ballot_sync(0xffffffffu, n > 0));
             mx = max(mx, __reduce_max_sync(0xffffffffu, n));
+        }
+        // (only where a piece has many tiles anyway: it must not pass over a sequence without having a tile of it)
+        const int extra = !per_sequence && run / 4 >= kBegin * (int)gridDim.x ? kBegin : 0;
+        if (extra) {
+            __syncwarp();
+            int before = 0;  // sequences with tiles
+            for (int base = 0; base < p.batch; base += 32) {
+                const int b = base + lane, from = b < p.batch ? prefix[b] : run, to = b + 1 < p.batch ? prefix[b + 1] : run;
+                const uint32_t have = __ballot_sync(0xffffffffu, to > from);  // (and all have read)
+                if (b < p.batch) prefix[b] = from + extra * (before + __popc(have & ((1u << lane) - 1u)));
+                before += __popc(have);
+            }
+            run += extra * sequences;
         }
         if (lane == 0) {
             prefix[p.batch] = run;
-            *longest = mx;
+            *longest = mx + extra;
+            *begin = extra;
         }
     }
     __syncthreads();
 
     const int total = prefix[p.batch];
-    const bool per_sequence = p.num_splits <= 1;
     const int even = (total + (int)gridDim.x - 1) / (int)gridDim.x;
     const int cap = per_sequence ? 0 : (*longest + p.num_splits - 2) / (p.num_splits - 1);
-    const int piece_len = max(p.dual ? 3 : 1, max(even, cap));  // (a piece amid a sequence has a tile of it)
+    const int piece_len = max((p.dual ? 3 : 1) + *begin, max(even, cap));  // (a piece amid a sequence has a tile of it)
     const int pieces = per_sequence ? p.batch : (total + piece_len - 1) / piece_len;
     auto begin_piece = [&](int piece, int& lo, int& hi) {  // its units, and the sequence it starts in
         if (per_sequence) {
@@ -264,12 +283,14 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         return a;
     };
     auto tiles = [&](int b, int lo, int hi, int& ta, int& tb) {  // a piece's tiles of a sequence: those whose first unit it has
-        ta = max(lo, prefix[b]) - prefix[b];
-        tb = min(hi, prefix[b + 1]) - prefix[b];
-        if (!p.dual) return;
-        const bool three = cost(p, b) == 3;
-        ta = three ? (ta + 2) / 3 : (ta + 1) / 2;
-        tb = three ? (tb + 2) / 3 : (tb + 1) / 2;
+        const int w = cost(p, b), from = max(lo, prefix[b]) - prefix[b], to = min(hi, prefix[b + 1]) - prefix[b];
+        const auto before = [&](int x) {  // tiles whose first unit is below x: the first one's is 0, the others' begin + w, begin + 2 w, ..
+            if (x <= *begin) return x > 0 ? 1 : 0;
+            x += w - 1 - *begin;
+            return w == 1 ? x : w == 2 ? x / 2 : x / 3;
+        };
+        ta = before(from);
+        tb = before(to);
     };
     const int head0 = blockIdx.z << p.heads_log2;
     const int row0 = blockIdx.y * (p.dual ? 16 : 4 * E);  // first (token, group head) row of this CTA
@@ -380,7 +401,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             const int parts = max(1, (int)gridDim.x / p.batch), part = parts > 1 ? (int)blockIdx.x / p.batch : 0;
             for (int b = parts > 1 ? (int)blockIdx.x % p.batch : (int)blockIdx.x; b < p.batch && part < parts; b += gridDim.x) {
                 const int n = prefix[b + 1] - prefix[b];
-                const int used = n == 0 ? 0 : per_sequence ? 1 : (prefix[b + 1] - cost(p, b)) / piece_len - prefix[b] / piece_len + 1;
+                const int w = cost(p, b), last = n == *begin + w ? prefix[b] : prefix[b + 1] - w;  // the last tile's first unit
+                const int used = n == 0 ? 0 : per_sequence ? 1 : last / piece_len - prefix[b] / piece_len + 1;
                 const int sq = len_q(p, b);
                 const int64_t rows = p.seqstart_q ? p.total_q : p.seqlen_q, head = p.num_splits * rows;  // LSEs of a split, of a head
                 float* first = p.lse_acc + (p.seqstart_q ? p.seqstart_q[b] : (int64_t)b * p.hq * head) + used * rows;
@@ -912,13 +934,13 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     const Int4Cache& c = p.cache;
     while (dev.heads_log2 < 3 && c.hkv % (2ll << dev.heads_log2) == 0) ++dev.heads_log2;
     const int heads = 1 << dev.heads_log2, toks = kPairs / heads;
-    FCK_REQUIRE((int64_t)c.batch * (dev.room / toks + 4) * (dev.dual ? 3 : 1) < (1ll << 30), FLASHCK_ERR_UNSUPPORTED,
+    FCK_REQUIRE((int64_t)c.batch * (dev.room / toks + 8) * (dev.dual ? 3 : 1) < (1ll << 30), FLASHCK_ERR_UNSUPPORTED,
                 "FmhaFwdSplitKVInt4: %lld sequences of up to %d keys are more than the schedule counts", (long long)c.batch, dev.room);
     int chunk = 16;
     dev.chunk_log2 = 4;
     while (2 * chunk <= toks && (!c.block_table || c.page % (2 * chunk) == 0)) { chunk *= 2; ++dev.chunk_log2; }
     const size_t meet = (size_t)kMeetWarps * E * ((D / 32) * 32 * 16 + 32);
-    const size_t fixed = 1024 + meet + (size_t)(2 * c.batch + 4) * sizeof(int);
+    const size_t fixed = 1024 + meet + (size_t)(2 * c.batch + 6) * sizeof(int);
     const size_t room = 227 * 1024;
     FCK_REQUIRE(fixed + 2 * (St::kBytes + 16) <= room, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch %lld leaves no room for two stages",
                 (long long)c.batch);

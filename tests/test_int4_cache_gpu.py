@@ -622,6 +622,14 @@ def test_batches_of_few_and_many_rows(d, group, splits):
     _attend(Cache([40 + 29 * i for i in range(70)], 8, d, group, torch.bfloat16, 0), [1 + i * i % 4 for i in range(70)], 32, num_splits=splits)
 
 
+@pytest.mark.parametrize("splits", [0, 2, 30, 128])
+@pytest.mark.parametrize("tokens,hq", [([1] * 14, 16), ([1, 4, 3, 3, 2, 4, 1, 4, 1, 3, 2, 3, 1, 4], 64)])
+def test_long_and_short_sequences_together(tokens, hq, splits):
+    """Enough work that a sequence's beginning counts in the split of the work: ones of one tile, of none and of hundreds next to one another."""
+    lens = [9000, 1, 0, 32, 11000, 33, 12001, 2, 20000, 31, 64, 15000, 700, 6]
+    _attend(Cache(lens, 16, 64, 64, torch.bfloat16, 16), tokens, hq, num_splits=splits)
+
+
 def test_a_schedule_past_32_bits_is_refused():
     parts = [torch.zeros(1, 1 << 16, 1, n, dtype=t, device="cuda") for n, t in ((32, torch.uint8), (2, torch.float16)) * 2]
     parts = [x if x.dtype == torch.uint8 else x.view(1, 1 << 16, 1, 1, 2) for x in parts]
