@@ -22,13 +22,14 @@
 // A CTA per SM: four producer warps and 16 consumer warps.  A stage is 256 (head, token) pairs -- 32 tokens of 8 heads, 256 of one -- of K and V
 // codes, by TMA (boxes of up to 256 tokens of a page, rows of 128 bytes, swizzled: a warp's reads meet no bank twice), and their scales, by 4- to
 // 16-byte asynchronous copies.  A consumer warp takes 32 tokens of one head; the warps form two teams of 8, which take stages in turn (up to 8
-// rows per kv head), or all stages with a tile of 8 rows each (more).  The warps of a head meet once per segment, in shared memory.  The work is
-// cut as in splitkv_decode.cu.
+// rows per kv head), or all stages with a tile of 8 rows each (more).  The warps of a head meet once per segment, in shared memory.  The work
+// is cut as in splitkv_decode.cu, by what it costs: a tile of more than 8 rows is 3 units where one of fewer is 2 (see cost()), a sequence's
+// beginning kBegin units.
 //
 // What bounds it (B200, bf16, hdim 128, 8 kv heads): the floor is the cache's bytes in HBM, 136 a token and head with one group.  64 sequences of
-// 1-32k keys under 32 heads: 208 us and 5 for the merge, floor 173 at 6.46 TB/s; with the arithmetic left out of a copy the loads alone take 192.
+// 1-32k keys under 32 heads: 198 us and 5 for the merge, floor 173 at 6.46 TB/s; with the arithmetic left out of a copy the loads alone take 192.
 // About 380 instructions a warp and 32 keys, at 0.62 a cycle and scheduler, are what the rest is.  4 x 524288 keys under 64 heads with two groups:
-// 555 us, floor 374: eight rows and two groups have more sums than registers, and 40 loads and stores of spilled ones per 32 keys.
+// 545-558 us, floor 374: eight rows and two groups have more sums than registers, and 40 loads and stores of spilled ones per 32 keys.
 #include <algorithm>
 #include <type_traits>
 
