@@ -556,7 +556,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 
             // 8 times the weights' sum taken off the sums of codes.  Tensor cores cut the sums of their products off instead of rounding them;
             // codes are never negative, so uncentred sums grow with the keys and lose on one side (4 x 524288 keys: O 0.9 % off), which
-            // centring every 256 keys prevents.
+            // centring every 256 keys of the warp's own prevents.
             auto centre = [&]() {
 #pragma unroll
                 for (int k = 0; k < NG; ++k)
@@ -577,6 +577,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                     for (int e = 0; e < E; ++e) z.ones[k][e] = 0.f;
             };
+            // a team that takes every other tile has those of one parity: its own count is half of the tile's number
+            const int own_log2 = tok_log2 + (two_tiles ? 0 : 1);
             int key0 = ((tile0[b] + ta + next - tile_count) << tok_log2) + unit * kUnit - step * toks;
             for (int t = ta + next - tile_count; t < tb; t += step) {
                 key0 += step * toks;
@@ -815,7 +817,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 mma_16816<__half>(z.o[c][1], odd_ch, wt[c / PER][2 * u], wt[c / PER][2 * u + 1]);
                             }
                         }
-                    if (((key0 >> (tok_log2 + step - 1)) & (kCentre - 1)) == 0) centre();
+                    if (((key0 >> own_log2) & (kCentre - 1)) == 0) centre();
                 }
                 // the last reads of the stage have to have come back before it is given back (see splitkv_decode.cu)
                 __threadfence_block();
