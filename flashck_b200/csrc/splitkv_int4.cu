@@ -361,7 +361,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     const int token0 = (tile0[b] + t) << tok_log2;
                     // (stages ahead of the consumers there is no hurry: looking seldom leaves them the issue slots)
                     for (int k = 0; k < 64 && !mbar_try_wait(&empty[s], parity); ++k) __nanosleep(200);
-                    if (!mbar_wait_bounded(&empty[s], parity, abort_flag, p.status, 0x100)) { ok = false; break; }
+                    // (all lanes leave a wait with one outcome, here and in the consumers: shuffles and arrivals of whole warps follow)
+                    if (!(ok = __all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], parity, abort_flag, p.status, 0x100)))) break;
                     uint8_t* st = ring + (size_t)s * St::kBytes;
                     if (kind == 0) {
                         const int chunks = min(1 << per_tile_log2, (len - token0 + chunk - 1) >> p.chunk_log2);
@@ -590,7 +591,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                     stage -= stages;
                     phase ^= 1u;
                 }
-                if (failed || !mbar_wait_bounded(&full[now], parity, abort_flag, p.status, 0x200)) { failed = true; continue; }
+                if (failed || !__all_sync(0xffffffffu, mbar_wait_bounded(&full[now], parity, abort_flag, p.status, 0x200))) { failed = true; continue; }
                 // (dual, one tile: the other team's stages are only given back)
                 if (key0 < len && (!p.dual || two_tiles || ((next ^ team) & 1))) {
                     uint32_t at[2][GR / 2];
