@@ -306,8 +306,9 @@ splitkv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 for (int t = ta; t < tb; ++t, ++it) {
                     const int s = it % stages;
                     const uint32_t ph = (it / stages) & 1u;
-                    if (!mbar_wait_bounded(&full_k[s], ph, abort_flag, p.status, 2)) return;
-                    if (!mbar_wait_bounded(&full_v[s], ph, abort_flag, p.status, 4)) return;
+                    // (a warp's lanes leave a wait with one outcome, here and below: what follows takes all of them)
+                    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_k[s], ph, abort_flag, p.status, 2))) return;
+                    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_v[s], ph, abort_flag, p.status, 4))) return;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&empty[s]);
                 }
@@ -382,7 +383,7 @@ splitkv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 for (int n = 0; n < 2 * NT; ++n) sacc[n][0] = sacc[n][1] = sacc[n][2] = sacc[n][3] = 0.f;
 #pragma unroll
                 for (int u = 0; u < NT; ++u) {
-                    if (!mbar_wait_bounded(&full_k[st[u]], ph[u], abort_flag, p.status, 2)) { failed = true; return; }
+                    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_k[st[u]], ph[u], abort_flag, p.status, 2))) { failed = true; return; }
                 }
                 {
                     const int key = (lm >> 1) * 8 + lr;  // token row this lane addresses
@@ -474,7 +475,7 @@ splitkv_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     pa[1] = Elem<T>::pack2(sacc[2 * u][2], sacc[2 * u][3]);
                     pa[2] = Elem<T>::pack2(sacc[2 * u + 1][0], sacc[2 * u + 1][1]);
                     pa[3] = Elem<T>::pack2(sacc[2 * u + 1][2], sacc[2 * u + 1][3]);
-                    if (!mbar_wait_bounded(&full_v[st[u]], ph[u], abort_flag, p.status, 4)) { failed = true; return; }
+                    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&full_v[st[u]], ph[u], abort_flag, p.status, 4))) { failed = true; return; }
                     const int key = (lm & 1) * 8 + lr;
 #pragma unroll
                     for (int j = 0; j < D / 16; ++j) {

@@ -25,7 +25,7 @@ def _unvoted(text):
     return bad
 
 
-@pytest.mark.parametrize("name", ["splitkv_int4.cu"])
+@pytest.mark.parametrize("name", ["splitkv_int4.cu", "splitkv_decode.cu"])
 def test_warps_leave_a_wait_together(name):
     with open(os.path.join(CSRC, name)) as f:
         text = f.read()
