@@ -18,6 +18,8 @@
 // Halves have no range for arbitrary Q and scales.  A row of Q is scaled by a power of two.  The weights p s are kept in range by the row's
 // reference R (p' = exp2(x - R)): it follows the largest x + log2 s seen, moves when a weight passes 2^13, and then everything the row
 // has summed is rescaled.  Moves are rare, and what decides one is a maximum over packed halves and a vote, without a shuffle.
+// Of several groups each follows its own largest x + log2 s, by a power of two (its lift) that its weights are multiplied by on top: with R
+// alone a group whose scales are 2^-20 of another's would keep 9 of its weights' 11 bits, and none at 2^-30.
 //
 // A CTA per SM: four producer warps and 16 consumer warps.  A stage is 256 (head, token) pairs -- 32 tokens of 8 heads, 256 of one -- of K and V
 // codes, by TMA (boxes of up to 256 tokens of a page, rows of 128 bytes, swizzled: a warp's reads meet no bank twice), and their scales, by 4- to
@@ -47,6 +49,9 @@ constexpr int kMeetWarps = 4;  // warps that hand their sums over at a time
 // of 1-32k keys and 64 / 8 heads 165 -> 159; 3 and 10 gave about the same.
 constexpr int kBegin = 6;
 constexpr uint32_t kCode = 0x000f000fu;
+// Least lift of a group, as a power of two.  (Below it the largest weights are 2^-2 and more, and a half's numbers are normal down to 2^-14; groups whose
+// scales are of a kind, the usual ones, then take no lift at all.)
+constexpr float kLeastLift = 6.f;
 constexpr float kNoKey = -1e30f;  // (any score is so far above it that the reference moves)
 
 struct Int4Dev {
@@ -170,11 +175,11 @@ struct Stage {
 constexpr int kConsumers = 16, kThreads = (kConsumers + 4) * 32, kLaunch = 65536 / kThreads / 8 * 8, kProducerRegs = 32, kConsumerRegs = 112;
 static_assert((kConsumers * kConsumerRegs + 4 * kProducerRegs) * 32 <= kThreads * kLaunch, "an increase would wait for good");
 
-// What one warp has summed over its keys, for the lane's E rows: 2t and 2t + 1 of 8 (E = 2, t = lane % 4), or t of 4 (E = 1; what belongs to odd
+// What one warp has summed over its keys (weights w = p' s, of several groups times the group's lift, a power of two in shared memory), for the lane's E rows: 2t and 2t + 1 of 8 (E = 2, t = lane % 4), or t of 4 (E = 1; what belongs to odd
 // columns then stays zero).
 template <int D, int NG, int E>
 struct Sums {
-    float o[D / 32][2][4];  // sum w u over 2^24, w = p' s ([0]: channels 4g, 4g + 2 of 32; [1]: 16 times 4g + 1, 4g + 3 plus those)
+    float o[D / 32][2][4];  // sum w u over 2^24 ([0]: channels 4g, 4g + 2 of 32; [1]: 16 times 4g + 1, 4g + 3 plus those)
     float ones[NG][E];      // sum w (as rounded) over the lane's keys since the last centring
     float mid[NG][E];       // sum p' (m + 8 s) over the lane's keys
     float l[E];             // sum p' over the lane's keys
@@ -203,6 +208,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     volatile int* abort_flag = tile0 + p.batch;
     int* longest = const_cast<int*>(abort_flag) + 1;
     int* begin = longest + 1;  // what the first tile of a sequence costs more
+    float* lifts = reinterpret_cast<float*>(begin + 1) + ((warp & (kConsumers - 1)) * NG * 4 + (lane & 3)) * E;  // [warp][NG][rows]: see Sums; of this lane's first row
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
@@ -555,6 +561,8 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 z.ref[e] = kNoKey;
             }
 
+            bool lifted = false;  // some lift is not 1
+
             // 8 times the weights' sum taken off the sums of codes.  Tensor cores cut the sums of their products off instead of rounding them;
             // codes are never negative, so uncentred sums grow with the keys and lose on one side (4 x 524288 keys: O 0.9 % off), which
             // centring every 256 keys of the warp's own prevents.
@@ -694,46 +702,68 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                             careful = __any_sync(0xffffffffu, !finite);
                         }
                         if (round == 1) {
-                            float top[4];  // log2 of a key's largest scale
+                            float lift[NG][E];
+                            float top[4][NG];  // log2 of a key's scales
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                float sc = vs[i][0];
+                            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                                for (int k = 1; k < NG; ++k) sc = fmaxf(sc, vs[i][k]);
-                                top[i] = sc > 0.f ? __log2f(sc) : -INFINITY;
-                            }
+                                for (int k = 0; k < NG; ++k) top[i][k] = vs[i][k] > 0.f ? __log2f(vs[i][k]) : -INFINITY;
 #pragma unroll
                             for (int e = 0; e < E; ++e) {
-                                float mx = -INFINITY, jx = -INFINITY;
+                                float mx = -INFINITY, jx = -INFINITY, jk[NG];  // jk: of a group, jx: of all
 #pragma unroll
-                                for (int i = 0; i < 4; ++i) {
-                                    mx = fmaxf(mx, x[i][e]);
-                                    jx = fmaxf(jx, x[i][e] == -INFINITY ? -INFINITY : x[i][e] + top[i]);
-                                }
+                                for (int i = 0; i < 4; ++i) mx = fmaxf(mx, x[i][e]);
 #pragma unroll
-                                for (int d = 4; d < 32; d <<= 1) {
-                                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
-                                    jx = fmaxf(jx, __shfl_xor_sync(0xffffffffu, jx, d));
+                                for (int d = 4; d < 32; d <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, d));
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) {
+                                    jk[k] = -INFINITY;
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) jk[k] = fmaxf(jk[k], x[i][e] == -INFINITY ? -INFINITY : x[i][e] + top[i][k]);
+#pragma unroll
+                                    for (int d = 4; d < 32; d <<= 1) jk[k] = fmaxf(jk[k], __shfl_xor_sync(0xffffffffu, jk[k], d));
+                                    jx = fmaxf(jx, jk[k]);
                                 }
                                 // weights up to 2^4 after a move; p' of the largest x within 2^-96 and 2^60, whatever the scales are
                                 const float ref = fmaxf(z.ref[e], fminf(fmaxf(jx - 4.f, mx - 60.f), mx + 96.f));
                                 const float f = fast_exp2(z.ref[e] - ref);  // (0 where nothing is summed yet)
-                                z.ref[e] = ref;
                                 z.l[e] *= f;
 #pragma unroll
                                 for (int k = 0; k < NG; ++k) {
+                                    float fo = f;  // for sums of weights
+                                    if constexpr (NG > 1) {
+                                        // weights up to 2^4 in each group, and no more against what the group has summed than the new reference takes off
+                                        const int was = lifted ? (int)(__float_as_uint(lifts[k * 4 * E + e]) >> 23) : 127;
+                                        const float most = floorf(fminf((float)(was - 127) + (ref - z.ref[e]), 4.f - (jk[k] - ref)));
+                                        const int is = most < kLeastLift ? 127 : 127 + (int)fminf(most, 100.f);
+                                        lift[k][e] = __uint_as_float((uint32_t)is << 23);
+                                        fo *= __uint_as_float((uint32_t)max(0, 127 + is - was) << 23);
+                                    }
                                     z.mid[k][e] *= f;
-                                    z.ones[k][e] *= f;
-                                }
+                                    z.ones[k][e] *= fo;
 #pragma unroll
-                                for (int c = 0; c < GR; ++c) {
-                                    z.o[c][0][e] *= f;
-                                    z.o[c][0][2 + e] *= f;
-                                    z.o[c][1][e] *= f;
-                                    z.o[c][1][2 + e] *= f;
+                                    for (int c = k * PER; c < (k + 1) * PER; ++c) {
+                                        z.o[c][0][e] *= fo;
+                                        z.o[c][0][2 + e] *= fo;
+                                        z.o[c][1][e] *= fo;
+                                        z.o[c][1][2 + e] *= fo;
+                                    }
                                 }
+                                z.ref[e] = ref;
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) x[i][e] -= ref;
+                            }
+                            if constexpr (NG > 1) {
+                                bool any = false;
+                                __syncwarp();  // (8 lanes have a row: all have read what it was lifted by)
+#pragma unroll
+                                for (int k = 0; k < NG; ++k)
+#pragma unroll
+                                    for (int e = 0; e < E; ++e) {
+                                        lifts[k * 4 * E + e] = lift[k][e];
+                                        any |= lift[k][e] != 1.f;
+                                    }
+                                lifted = __any_sync(0xffffffffu, any);
                             }
                         }
                         // ---- weights ----
@@ -748,12 +778,16 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                         for (int k = 0; k < NG; ++k)
 #pragma unroll
                             for (int i = 0; i < 4; ++i) wt[k][i] = halves(x[i][0] * vs[i][k], E == 2 ? x[i][E - 1] * vs[i][k] : 0.f);
-                        if (careful) {
+                        // (the weights again: a lift multiplied into every weight took 8 rows and two groups 551 -> 585 us)
+                        if (careful || lifted) {
+                            auto weight = [&](int i, int k, int e) {
+                                const float w = x[i][e] == 0.f ? 0.f : x[i][e] * vs[i][k];
+                                return lifted ? w * lifts[k * 4 * E + e] : w;
+                            };
 #pragma unroll
                             for (int k = 0; k < NG; ++k)
 #pragma unroll
-                                for (int i = 0; i < 4; ++i)
-                                    wt[k][i] = halves(x[i][0] == 0.f ? 0.f : x[i][0] * vs[i][k], E == 1 || x[i][E - 1] == 0.f ? 0.f : x[i][E - 1] * vs[i][k]);
+                                for (int i = 0; i < 4; ++i) wt[k][i] = halves(weight(i, k, 0), E == 2 ? weight(i, k, E - 1) : 0.f);
                         }
                         uint32_t most = 0;
 #pragma unroll
@@ -848,8 +882,11 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                 for (int c = 0; c < GR; ++c) {
                     const float add = rest[c / PER], even0 = z.o[c][0][e], even2 = z.o[c][0][2 + e];
-                    o[e][c] = make_float4(fmaf(16777216.f, even0, add), fmaf(1048576.f, z.o[c][1][e] - even0, add), fmaf(16777216.f, even2, add),
-                                          fmaf(1048576.f, z.o[c][1][2 + e] - even2, add));
+                    // 2^24 and 2^20 over the group's lift
+                    const float whole = NG == 1 || !lifted ? 16777216.f : __uint_as_float((278u << 23) - __float_as_uint(lifts[(c / PER) * 4 * E + e]));
+                    const float byte = whole * 0.0625f;
+                    o[e][c] = make_float4(fmaf(whole, even0, add), fmaf(byte, z.o[c][1][e] - even0, add), fmaf(whole, even2, add),
+                                          fmaf(byte, z.o[c][1][2 + e] - even2, add));
                 }
             }
             // ---- the warps of a head (and team, if these have rows of their own) meet: the upper half hands its sums to the lower one until one
@@ -944,7 +981,8 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     dev.chunk_log2 = 4;
     while (2 * chunk <= toks && (!c.block_table || c.page % (2 * chunk) == 0)) { chunk *= 2; ++dev.chunk_log2; }
     const size_t meet = (size_t)kMeetWarps * E * ((D / 32) * 32 * 16 + 32);
-    const size_t fixed = 1024 + meet + (size_t)(2 * c.batch + 6) * sizeof(int);
+    const size_t lifts = NG > 1 ? (size_t)kConsumers * NG * 4 * E * sizeof(float) : 0;
+    const size_t fixed = 1024 + meet + lifts + (size_t)(2 * c.batch + 6) * sizeof(int);
     const size_t room = 227 * 1024;
     FCK_REQUIRE(fixed + 2 * (St::kBytes + 16) <= room, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch %lld leaves no room for two stages",
                 (long long)c.batch);
