@@ -468,7 +468,7 @@ int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream) {
     const auto aligned = [](const void* x) { return (reinterpret_cast<uintptr_t>(x) & 15u) == 0; };
     const bool rows = aligned(p.q) && aligned(p.q_out) && aligned(p.knew) && aligned(p.vnew) && aligned(p.k_held) && aligned(p.v_held);
     if (int rc = fill_rotary("FmhaFwdAppendKVInt4", a.rot, p.rotary_cos, p.rotary_sin, p.rotary_rows, p.rotary_dim, p.cache.d, p.rope_type,
-                             p.pair_axis, p.positions ? p.axes : 1, rows)) return rc;
+                             p.pair_axis, p.positions || p.pair_axis ? p.axes : 1, rows)) return rc;
     a.status = device_status_ptr();
     if (!a.status) return FLASHCK_ERR_CUDA;
     a.q = p.q; a.q_out = p.q_out; a.knew = p.knew; a.vnew = p.vnew; a.k_held = p.k_held; a.v_held = p.v_held;

@@ -478,7 +478,7 @@ struct Axes {
     }
     bool fill(Reader& r, PyObject* sections, bool dealt, const at::Tensor* positions, int64_t tokens, int64_t half) {
         if (positions) {
-            axes = tokens > 0 ? positions->numel() / tokens : 1;
+            axes = tokens > 0 ? positions->numel() / tokens : PyTuple_CheckExact(sections) ? PyTuple_GET_SIZE(sections) : 1;
             if (positions->numel() != axes * tokens || axes < 1 || axes > 4 || (axes > 1 && positions->size(0) != axes)) return false;
         }
         if (sections == Py_None) return axes == 1;

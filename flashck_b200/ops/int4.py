@@ -136,7 +136,7 @@ def fmha_fwd_append_kv_int4(q: Optional[torch.Tensor], k_cache: torch.Tensor, k_
             raise ValueError("rotary_cos / rotary_sin are required unless rope == RopeEnum.NONE")
         rotary_dim, rows = _tables(rotary_cos, rotary_sin, knew.dtype, rotary_dim)
         if positions is not None:
-            pos, axes = _as_positions(positions, tokens)
+            pos, axes = _as_positions(positions, tokens, sections)
         pairs = _pair_axes(None if sections is None else tuple(int(n) for n in sections), bool(interleaved_sections), rotary_dim // 2, axes)
     elif positions is not None or sections is not None:
         raise ValueError("positions and sections need a rotation (rope)")

@@ -56,15 +56,15 @@ def _tables(cos: torch.Tensor, sin: torch.Tensor, dtype: torch.dtype, rotary_dim
     return 2 * cos.shape[1], cos.shape[0]
 
 
-def _as_positions(positions: torch.Tensor, tokens: int) -> Tuple[torch.Tensor, int]:
-    """(positions int32 [axes, tokens], axes)."""
+def _as_positions(positions: torch.Tensor, tokens: int, sections: Optional[Sequence[int]] = None) -> Tuple[torch.Tensor, int]:
+    """(positions int32 [axes, tokens], axes).  Positions of no token have as many axes as there are sections."""
     if positions is None or not isinstance(positions, torch.Tensor):
         raise TypeError("positions must be a torch.Tensor")
     if positions.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"positions must have dtype torch.int32 or torch.int64, got {positions.dtype}")
     # (the kernels hold 32 bits: what lies behind them is outside every table, and must not come back to it)
     p = _f._as_i32("positions", positions.clamp(-1, 2 ** 31 - 1) if positions.dtype == torch.int64 and positions.is_cuda else positions)
-    axes = p.numel() // tokens if tokens else 1
+    axes = p.numel() // tokens if tokens else 1 if sections is None else len(sections)
     if p.numel() != axes * tokens or axes < 1 or (axes > 1 and p.shape[0] != axes):
         _f._refuse("positions", positions, f"{tokens} positions, or [axes, ...] of them")
     return p, axes
@@ -92,7 +92,7 @@ def _rotary(q, k, positions, cos, sin, sections, interleaved_sections, rope, inv
         tokens *= n
     if rope not in (int(RopeEnum.INTERLEAVED), int(RopeEnum.HALF_ROTATED)):
         raise ValueError("rope must be RopeEnum.INTERLEAVED or RopeEnum.HALF_ROTATED")
-    pos, axes = _as_positions(positions, tokens)
+    pos, axes = _as_positions(positions, tokens, sections)
     rotary_dim, rows = _tables(cos, sin, q.dtype, None)
     if rotary_dim > d:
         raise ValueError(f"the rotary tables turn {rotary_dim} columns of heads of {d}")
