@@ -6,7 +6,8 @@ codes uint8 ``[pages, page, hkv, d / 2]``, byte j with channel 2j in its low and
 ``[pages, page, hkv, d / group, 2]`` = (scale, lo) in the model's dtype; or ``[b_cache, capacity, ...]`` of both without a block table.
 Against a 16-bit cache it takes 17 / 64 (group 128) to 5 / 16 (group 32) of the bytes, which is what decode is bound by.
 
-A page id outside the pools is not followed: reads take zeros there, writes are skipped and reported (:func:`_lib.device_status`).
+A page id outside the pools is not followed, nor a ``cache_batch_idx`` outside the block table or the contiguous rows: reads take zeros there,
+writes are skipped and reported (:func:`_lib.device_status`).
 """
 from __future__ import annotations
 
@@ -81,6 +82,12 @@ class _Cache:
             _f._refuse("cache_batch_idx", self.index, f"{self.batch} entries")
         _same_device(device, k_cache=k_cache, k_params=k_params, v_cache=v_cache, v_params=v_params, seqlen_k=self.seqlen,
                      block_table=self.table, cache_batch_idx=self.index)
+        if self.table is not None and self.index is not None:
+            # The kernels do not know how many rows the table has: the rows are picked here, and one that is not there has no page.
+            table, index = self.table, self.index.flatten()[:self.batch]
+            there = (index >= 0) & (index < table.shape[0])
+            picked = table[index.clamp(0, table.shape[0] - 1)] if table.shape[0] else table.new_empty(self.batch, self.bt_stride)
+            self.table, self.index = torch.where(there[:, None], picked, -1), None
 
 
 def fmha_fwd_append_kv_int4(q: Optional[torch.Tensor], k_cache: torch.Tensor, k_params: torch.Tensor, v_cache: torch.Tensor,

@@ -358,7 +358,8 @@ FLASHCK_API int FmhaFwdAppendKV(void* q_buf_ptr, void* k_buf_ptr, void* knew_buf
  *   params: element type [rows, hkv, d / group, 2] = (scale, lo)
  * rows are pools [num_pool_pages, paged_block_size] behind block_table (int32 [.., block_table_stride]), or contiguous caches
  * [num_pool_pages, kv_seq_len] without one (num_pool_pages: their rows, of which sequence b uses b or cache_batch_idx[b]; paged_block_size
- * is kv_seq_len).  A page id or row outside the pools is never followed: reads give zeros, writes are skipped and reported.
+ * is kv_seq_len).  A page id or row outside the pools is never followed: reads give zeros, writes are skipped and reported.  With a block
+ * table cache_batch_idx[b] names the table's row, whose number is not an argument: the caller answers for it.
  * codes and params 16-byte aligned; hdim 64 or 128, dtype 3 or 4.  A group that holds a NaN or an infinity, or whose range leaves fp32,
  * reads back as NaN.
  *
