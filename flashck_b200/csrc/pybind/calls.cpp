@@ -461,7 +461,7 @@ struct Int4Args {
         group = d / groups;
         for (const at::Tensor* t : {k, kp, v, vp})
             if ((uintptr_t)t->data_ptr() % 16) return false;
-        return bt ? bt->size(0) >= batch && k->size(1) % unit == 0 : k->size(0) >= batch;
+        return bt ? bt->size(0) >= batch && bt->size(1) > 0 && k->size(1) % unit == 0 : k->size(0) >= batch;
     }
     int64_t stride() const { return bt ? bt->size(1) : 0; }
 };

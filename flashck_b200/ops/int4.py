@@ -71,8 +71,8 @@ class _Cache:
         self.index = _f._as_i64("cache_batch_idx", cache_batch_idx) if cache_batch_idx is not None else None
         self.bt_stride = 0
         if self.table is not None:
-            if self.table.dim() != 2 or (self.index is None and self.table.shape[0] < self.batch):
-                _f._refuse("block_table", self.table, f"a row for each of the {self.batch} sequences")
+            if self.table.dim() != 2 or self.table.shape[1] < 1 or (self.index is None and self.table.shape[0] < self.batch):
+                _f._refuse("block_table", self.table, f"a row for each of the {self.batch} sequences and a column for their pages")
             self.bt_stride = self.table.shape[1]
             if self.page % paged_unit:
                 raise ValueError(f"pages must have a multiple of {paged_unit} tokens, got {self.page}")
