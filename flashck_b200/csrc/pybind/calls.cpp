@@ -583,6 +583,14 @@ PyObject* call_append_kv_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs
     END_HANDLE_TH_ERRORS
 }
 
+// ops.int4._split_depth
+int64_t split_depth_int4(int64_t batch, int64_t rows, int64_t hkv) {
+    int64_t heads = 8;
+    while (hkv % heads != 0) heads /= 2;
+    const int64_t ctas = 148 / ((rows + 15) / 16 * (hkv / heads));
+    return ctas <= 1 ? 1 : std::min(num_splits_for(batch, 1), ctas + 1);
+}
+
 // (q, k_cache, k_params, v_cache, v_params, seqlen_k, block_table | None, cu_seqlens_q | None, max_seqlen_q, num_splits, scale, causal,
 //  window_size, mask_type, return_lse)
 PyObject* call_splitkv_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
@@ -609,7 +617,7 @@ PyObject* call_splitkv_int4(PyObject*, PyObject* const* args, Py_ssize_t nargs) 
     const int64_t hq = q->size(-2), sq = q->size(-3), bs = group ? 1 : c.batch;
     if (q->numel() == 0 || hq % c.hkv != 0 || c.k->numel() == 0 || (uintptr_t)q->data_ptr() % 16) Py_RETURN_NONE;
     max_q = group && max_q > 0 ? std::min(max_q, sq) : sq;
-    if (splits <= 0) splits = num_splits_for(c.batch, 1);
+    if (splits <= 0) splits = split_depth_int4(c.batch, max_q * (hq / c.hkv), c.hkv);
     at::Tensor o, lse, work;
     int rc;
     {
@@ -724,6 +732,12 @@ PyObject* num_splits(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     if (!r.ok) Py_RETURN_NONE;
     return PyLong_FromLongLong(num_splits_for(b, rows));
 }
+PyObject* split_depth(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+    Reader r{args, nargs};
+    const int64_t b = r.integer(), rows = r.integer(), hkv = r.integer();
+    if (!r.ok || rows < 1 || hkv < 1) Py_RETURN_NONE;
+    return PyLong_FromLongLong(split_depth_int4(b, rows, hkv));
+}
 
 PyMethodDef methods[] = {
     {"_call_forward", (PyCFunction)(void (*)(void))call_forward, METH_FASTCALL, nullptr},
@@ -738,6 +752,7 @@ PyMethodDef methods[] = {
     {"_call_rotary", (PyCFunction)(void (*)(void))call_rotary, METH_FASTCALL, nullptr},
     {"_accumulates_on_default_stream", (PyCFunction)accumulates_on_default_stream, METH_O, nullptr},
     {"_num_splits", (PyCFunction)(void (*)(void))num_splits, METH_FASTCALL, nullptr},
+    {"_split_depth", (PyCFunction)(void (*)(void))split_depth, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 

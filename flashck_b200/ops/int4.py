@@ -161,6 +161,17 @@ def fmha_fwd_append_kv_int4(q: Optional[torch.Tensor], k_cache: torch.Tensor, k_
     return (q_out, *held) if return_kv else q_out
 
 
+def _split_depth(batch: int, rows: int, hkv: int, sm_count: int = 148) -> int:
+    """Workspace depth for :func:`fmha_fwd_splitkv_int4` where the caller leaves it open, for ``rows`` query rows per kv head (``seqlen_q * hq / hkv``).
+
+    As :func:`default_num_splits`, but no more than the grid can use: its CTAs are shared out over the groups of kv heads (up to 8 together) and the
+    tiles of 16 rows, and a sequence cut among those that remain touches one piece more than there are.  (One sequence of 2048 queries of 32 / 8
+    heads: 34 MB of workspace where 128 splits take 4.3 GB.)"""
+    heads = next(n for n in (8, 4, 2, 1) if hkv % n == 0)
+    ctas = sm_count // (-(-rows // 16) * (hkv // heads))
+    return 1 if ctas <= 1 else min(_f.default_num_splits(batch, sm_count), ctas + 1)
+
+
 def fmha_fwd_splitkv_int4(q: torch.Tensor, k_cache: torch.Tensor, k_params: torch.Tensor, v_cache: torch.Tensor, v_params: torch.Tensor, *,
                           seqlen_k: torch.Tensor, block_table: Optional[torch.Tensor] = None, cache_batch_idx: Optional[torch.Tensor] = None,
                           cu_seqlens_q: Optional[torch.Tensor] = None, max_seqlen_q: int = 0, num_splits: int = 0,
@@ -206,7 +217,7 @@ def fmha_fwd_splitkv_int4(q: torch.Tensor, k_cache: torch.Tensor, k_params: torc
         return (o, lse) if return_lse else o
     if c.pool == 0 or c.page == 0:
         raise ValueError("the cache has no room")
-    splits = int(num_splits) if num_splits and num_splits > 0 else _f.default_num_splits(c.batch)
+    splits = int(num_splits) if num_splits and num_splits > 0 else _split_depth(c.batch, max_sq * (hq // c.hkv), c.hkv)
     lse_acc, o_acc = _f.splitkv_workspace(q, c.d, splits, cu_q)
     lib = _lib.lib()
     with _f._on(q.device):
