@@ -8,6 +8,7 @@ from __future__ import annotations
 import concurrent.futures
 import glob
 import os
+import re
 import shutil
 import subprocess
 import sys
@@ -22,6 +23,21 @@ NVCC_FLAGS = [
     "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
     "--expt-relaxed-constexpr", "-diag-suppress", "177",
 ]
+
+# Kernels that hand registers from some warps to others, and the registers a thread that they count on being launched with (kLaunch in the source):
+# an increase waits until the block's pool can serve it, which it never can if a compiler gave the kernel fewer.
+_REGISTERS = {"splitkv_int4.cu": ("splitkv_int4_kernel", 96)}
+
+
+def check_registers(source: str, log: str) -> None:
+    """Raises RuntimeError where ptxas' log of ``source`` shows such a kernel with another number of registers."""
+    kernel, want = _REGISTERS.get(source, (None, 0))
+    if kernel is None:
+        return
+    used = [int(n) for n in re.findall(r"entry function '[^']*" + kernel + r"[^']*'(?:(?!entry function).)*?Used (\d+) registers", log, re.S)]
+    if not used or any(n != want for n in used):
+        raise RuntimeError(f"{source}: {kernel} needs {want} registers a thread, this compiler gave {sorted(set(used)) or 'no count'}; its split of the "
+                           "registers among its warps has to be adapted")
 
 
 def _nvcc() -> str:
@@ -52,6 +68,11 @@ def build(force: bool = False, verbose: bool = False) -> str:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"nvcc failed for {src}:\n{r.stdout}\n{r.stderr}")
+        try:
+            check_registers(os.path.basename(src), r.stderr)
+        except RuntimeError:
+            os.remove(obj)
+            raise
         return obj, r.stderr
 
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources))) as ex:

@@ -1004,7 +1004,7 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
         cudaFuncAttributes attr;
         FCK_CUDA(cudaFuncGetAttributes(&attr, kern));
         FCK_REQUIRE(attr.numRegs == kLaunch, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: built with %d registers a thread instead of %d",
-                    attr.numRegs, kLaunch);  // (the warpgroups' shares would not add up)
+                    attr.numRegs, kLaunch);  // (the warps' shares would not add up; the package's build checks it, so this is for other builds)
         configured_device = devid;
     }
     const int64_t rows = p.max_seqlen_q * (p.hq / c.hkv), rows_per_cta = dev.dual ? 16 : 4 * E;
