@@ -501,7 +501,9 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 // largest magnitude into [2^13, 2^14): with it the /16 of half of the channels and 2^-24 of the rest stay exact
-                const int ex = amax > 0.f ? max(-100, min(100, (int)((__float_as_uint(amax) >> 23) & 255) - 127)) : 13;
+                // (as far as 32 bits hold ka = scale 2^(ex + 11): ex up to 118 for scales of 2^-3, and halves up to 2^16 take rows up to 2^121)
+                const int most = min(120, 115 - ((int)((__float_as_uint(p.scale_log2) >> 23) & 255) - 127));
+                const int ex = amax > 0.f ? max(-100, min(most, (int)((__float_as_uint(amax) >> 23) & 255) - 127)) : 13;
                 const float up = __uint_as_float((uint32_t)(127 + 13 - ex) << 23), down = __uint_as_float((uint32_t)(127 - 13 + ex) << 23);
                 float sum[NG];
 #pragma unroll

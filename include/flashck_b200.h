@@ -381,7 +381,8 @@ FLASHCK_API int FmhaFwdAppendKVInt4(const void* q, void* q_out, void* k_codes, v
 
 /*
  * FmhaFwdSplitKVInt4 -- FmhaFwdSplitKV over such a cache; lse_acc / o_acc as there (lse_acc is always needed), merged by
- * FmhaFwdSplitKVCombine.  Pages of a multiple of 16 tokens.  Keys and values enter the products as the exact lo + scale * code.
+ * FmhaFwdSplitKVCombine.  Pages of a multiple of 16 tokens.  Keys and values enter the products as the exact lo + scale * code.  Of a query row
+ * what is below 2^-34 of its largest magnitude is dropped, and rows whose largest passes 2^120 (over 8 scale, where that is less) may give NaN.
  */
 FLASHCK_API int FmhaFwdSplitKVInt4(const void* q, const void* k_codes, const void* k_params, const void* v_codes, const void* v_params,
                        void* lse_acc, void* o_acc, const int64_t* q_seq_start_ptr, const void* k_seq_len_ptr, const void* block_table,
