@@ -453,13 +453,6 @@ cudaError_t launch_read_type(const ReadInt4Dev& a, bool runs, unsigned blocks, c
                 : launch_dependent(read_int4_kernel<T, 1>, dim3(blocks), dim3(256), 0, stream, a);
 }
 
-// Warps that share a job: enough to fill the SMs with few jobs, one with many (what they all work out is worked out fewer times).
-int warps_log2_for(int64_t jobs, int64_t most) {
-    int w = 3;
-    while (w > 0 && ((1 << w) > most || jobs << w > (int64_t)sm_count() * 32)) --w;
-    return w;
-}
-
 }  // namespace
 
 int launch_append_int4(const AppendInt4Params& p, cudaStream_t stream) {

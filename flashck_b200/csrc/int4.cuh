@@ -248,6 +248,14 @@ __device__ __forceinline__ void turn_piece_any(const RotaryDev& r, int e0, const
 
 #endif  // __CUDACC__
 
+// Host side: the warps (log2) that share a token's work: enough to fill the SMs with few tokens, one with many (what they all work out is worked out
+// fewer times).
+inline int warps_log2_for(int64_t jobs, int64_t most) {
+    int w = 3;
+    while (w > 0 && ((1 << w) > most || jobs << w > (int64_t)sm_count() * 32)) --w;
+    return w;
+}
+
 // Host side: `pair_axis` (one entry per pair, or nullptr: all turn with the first axis) into the bits of RotaryDev.
 int fill_rotary(const char* fn, RotaryDev& r, const void* cosr, const void* sinr, int64_t rows, int64_t rotary_dim, int64_t d, int rope_type,
                 const uint8_t* pair_axis, int64_t axes, bool rows_aligned);

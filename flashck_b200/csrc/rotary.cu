@@ -116,10 +116,8 @@ int launch_rotary(const RotaryParams& p, cudaStream_t stream) {
     a.heads[0] = (int)p.hq; a.heads[1] = p.k ? (int)p.hkv : 0;
     if (p.tokens == 0 || a.heads[0] + a.heads[1] == 0) return FLASHCK_OK;
     const int64_t most = std::max<int64_t>(1, (p.hq + a.heads[1]) * p.d / 256);
-    int w = 3;
-    while (w > 0 && ((1 << w) > most || p.tokens << w > (int64_t)sm_count() * 32)) --w;
-    a.warps_log2 = w;
-    const int64_t blocks = ((p.tokens << w) + 7) / 8;
+    a.warps_log2 = warps_log2_for(p.tokens, most);
+    const int64_t blocks = ((p.tokens << a.warps_log2) + 7) / 8;
     FCK_REQUIRE(blocks < (1ll << 31), FLASHCK_ERR_UNSUPPORTED, "FmhaRotary: too many tokens");
     if (p.dtype == FLASHCK_DTYPE_BFLOAT16) FCK_CUDA(launch_type<__nv_bfloat16>(a, (unsigned)blocks, stream));
     else FCK_CUDA(launch_type<__half>(a, (unsigned)blocks, stream));
