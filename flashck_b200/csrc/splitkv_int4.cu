@@ -248,8 +248,10 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             sequences += __popc(__ballot_sync(0xffffffffu, n > 0));
             mx = max(mx, __reduce_max_sync(0xffffffffu, n));
         }
-        // (only where a piece has many tiles anyway: it must not pass over a sequence without having a tile of it)
-        const int extra = !per_sequence && run / 4 >= kBegin * (int)gridDim.x ? kBegin : 0;
+        // (where the CTAs have kBegin units each and more; a piece, which has to have a tile of a sequence that it cuts, would else be longer than the
+        // share of a CTA.  Below: one sequence of 3000 keys 18.5 -> 22.5 us.  Above: 256 of 10-200 keys, 6.4 units a CTA, 47 -> 41, 16 of 500-8000,
+        // 16 a CTA, 41 -> 39.)
+        const int extra = !per_sequence && run / kBegin >= (int)gridDim.x ? kBegin : 0;
         if (extra) {
             __syncwarp();
             int before = 0;  // sequences with tiles
