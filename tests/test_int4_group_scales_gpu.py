@@ -9,20 +9,24 @@ pytestmark = pytest.mark.gpu
 
 
 def _bound(q, kc, kp, vc, vp, scale, mask):
-    """(o, its bound, lse, its bound) as ref.attend has them, but what a weight loses below a half's normal numbers counts by the scales of the
-    channel's own group: 8 n 2^-24 of the largest p s there."""
-    o, lse, bound, lse_bound = ref.attend(q, kc, kp, vc, vp, scale, mask)
+    """(o, its bound, lse, its bound) as ref.attend has them, but for what a weight loses below a half's normal numbers, which counts by the scales of
+    the channel's own group: 8 n 2^-24 of the largest p s there.  (Summed up anew: a bound of all groups does not go back to a small one's.)"""
+    o, lse, _, lse_bound = ref.attend(q, kc, kp, vc, vp, scale, mask)
     n, hq, d = kc.shape[0], q.shape[1], q.shape[2]
-    per = hq // kc.shape[1]
+    per, bound = hq // kc.shape[1], torch.zeros_like(o)
     k = ref.values(kc, kp)
-    vs = vp[..., 0].double().repeat_interleave(d // vp.shape[-2], -1)
+    ks, vs, kl, vl = (p[..., i].double().repeat_interleave(d // p.shape[-2], -1) for i in (0, 1) for p in (kp, vp))
     seen = ref.visible(q.shape[0], n, mask, q.device)
     for h in range(hq):
-        x = torch.where(seen, q[:, h].double() @ k[:, h // per].T * scale, -torch.inf)
+        kh = h // per
+        x = torch.where(seen, q[:, h].double() @ k[:, kh].T * scale, -torch.inf)
         any_ = seen.any(-1)
         p = torch.where(any_[:, None], torch.exp(x - torch.where(any_, torch.logsumexp(x, -1), 0)[:, None]), 0)
-        top = (p[:, :, None] * vs[None, :, h // per]).amax(1)
-        bound[:, h] += 8 * n * 2.0 ** -24 * (top - top.amax(-1, keepdim=True))
+        size = (q[:, h].double().abs() @ (kl[:, kh].abs() + 15 * ks[:, kh]).T * abs(scale)).masked_fill(~seen, 0).amax(-1)
+        e = 2.0 ** -20 * (size + 1) + 2.0 ** -22 * torch.where(seen, x, 0).abs().amax(-1)
+        top = (p[:, :, None] * vs[None, :, kh]).amax(1)
+        bound[:, h] = ref.half_step(q.dtype) * o[:, h].abs() * 1.01 + 2.0 ** -11 * (p @ (8 * vs[:, kh])) + 8 * n * 2.0 ** -24 * top + \
+            (3 * e[:, None] + 2.0 ** -18) * (p @ (vl[:, kh].abs() + 15 * vs[:, kh]))
     return o, lse, bound, lse_bound
 
 
