@@ -7,8 +7,8 @@
 //
 // A job is one token's keys, values and queries (queries that are not the new tokens are jobs of their own); 1 to 8 warps share it.  What bounds
 // the append of a decode step (32 tokens: 7 us) is a chain of memory round trips -- sequence starts, lengths, pages, angles -- and what bounds a
-// long one its traffic and the issue slots about equally: 43178 tokens of 32 / 8 heads with the held values returned, 1.12 GB, 203 us, floor 174 at
-// 6.46 TB/s.  Reading 48855 tokens of 8 heads back, 253 MB: 44 us, floor 39.
+// long one its traffic and the issue slots about equally: 43178 tokens of 32 / 8 heads with the held values returned, 1.12 GB, 197-203 us, floor 172 at
+// 6.54 TB/s.  Reading 48855 tokens of 8 heads back, 253 MB: 44 us, floor 39.
 #include <algorithm>
 #include <type_traits>
 

@@ -1,7 +1,8 @@
 // Rotation of queries and keys by the positions of their tokens, along one or several axes (int4.cuh has the arithmetic).
 //
 // Bound by its traffic: each row read and written once.  A warp turns a token (a few warps, where tokens are few); a lane keeps the cosines
-// and sines of its 16 channels for all heads.  16384 tokens of 32 + 8 heads of 128: 57 us, floor 52 at 6.46 TB/s (the copy rate).
+// and sines of its 16 channels for all heads.  16384 tokens of 32 + 8 heads of 128: 53 us among other calls, floor 51 at 6.54 TB/s (the copy rate).
+// Widths whose 16-channel pieces do not divide a warp go channel by channel: heads of 96 174 us, floor 39.
 #include <algorithm>
 #include <type_traits>
 

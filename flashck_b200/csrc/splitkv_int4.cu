@@ -29,9 +29,10 @@
 // beginning kBegin units.
 //
 // What bounds it (B200, bf16, hdim 128, 8 kv heads): the floor is the cache's bytes in HBM, 136 a token and head with one group.  64 sequences of
-// 1-32k keys under 32 heads: 198 us and 5 for the merge, floor 173 at 6.46 TB/s; with the arithmetic left out of a copy the loads alone take 192.
-// About 380 instructions a warp and 32 keys, at 0.62 a cycle and scheduler, are what the rest is.  4 x 524288 keys under 64 heads with two groups:
-// 545-558 us, floor 374: eight rows and two groups have more sums than registers, and 40 loads and stores of spilled ones per 32 keys.
+// 1-32k keys under 32 heads: 202-204 us and 5 for the merge, floor 171 at 6.54 TB/s; with the arithmetic left out of a copy the loads alone take
+// 178-181, with the codes' loads left out the arithmetic 193-195: about 380 instructions a warp and 32 keys, at 0.6 a cycle and scheduler.  4 x 524288
+// keys under 64 heads with two groups: 540-545 us, floor 370: eight rows and two groups have more sums than registers, and 30 loads and stores of
+// spilled ones per 32 keys.
 #include <algorithm>
 #include <type_traits>
 

@@ -181,9 +181,10 @@ def fmha_fwd_splitkv_int4(q: torch.Tensor, k_cache: torch.Tensor, k_params: torc
 
     As :func:`fmha_fwd_splitkv`: q ``[b, sq, hq, d]``, or packed ``[total_q, hq, d]`` with ``cu_seqlens_q``; a cache of :func:`int4_cache`,
     paged (pages of a multiple of 16 tokens) with ``block_table`` int32 ``[b, pages_per_seq]``, or contiguous; ``seqlen_k`` int32 ``[b]``,
-    the new tokens among them.  Keys and values count as exactly ``lo + scale * code``.  Any number of query rows is taken, but the cache is
-    read once per 16 rows of a kv head (``sq * hq / hkv``): a chunk of a prompt goes through :func:`fmha_read_kv_int4` and
-    :func:`fmha_fwd_var_len`.
+    the new tokens among them.  Keys and values count as exactly ``lo + scale * code``; the softmax's weights are rounded to 11 bits on their way to
+    the values (of P times scale; sums are 32-bit), and of a query row what is below 2^-34 of its largest magnitude is dropped.  Any number of query
+    rows is taken, but the cache is read once per 16 rows of a kv head (``sq * hq / hkv``): a chunk of a prompt goes through
+    :func:`fmha_read_kv_int4` and :func:`fmha_fwd_var_len`.  There are no ALiBi slopes.
 
     Returns o like q (and LSE fp32 ``[b, hq, sq]`` / ``[hq, total_q]``); packed rows that belong to no sequence hold nothing of meaning."""
     native = _f._native()
