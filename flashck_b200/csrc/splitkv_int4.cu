@@ -18,8 +18,9 @@
 // Halves have no range for arbitrary Q and scales.  A row of Q is scaled by a power of two.  The weights p s are kept in range by the row's
 // reference R (p' = exp2(x - R)): it follows the largest x + log2 s seen, moves when a weight passes 2^13, and then everything the row
 // has summed is rescaled.  Moves are rare, and what decides one is a maximum over packed halves and a vote, without a shuffle.
-// Of several groups each follows its own largest x + log2 s, by a power of two (its lift) that its weights are multiplied by on top: with R
-// alone a group whose scales are 2^-20 of another's would keep 9 of its weights' 11 bits, and none at 2^-30.
+// Each group of channels follows its own largest x + log2 s, by a power of two (its lift) that its weights are multiplied by on top: with R
+// alone a group whose scales are 2^-20 of another's would keep 9 of its weights' 11 bits, and none at 2^-30; and R keeps p' within 2^-96 and 2^60, which
+// scales outside 2^-60 and 2^100 need more than.
 //
 // A CTA per SM: four producer warps and 16 consumer warps.  A stage is 256 (head, token) pairs -- 32 tokens of 8 heads, 256 of one -- of K and V
 // codes, by TMA (boxes of up to 256 tokens of a page, rows of 128 bytes, swizzled: a warp's reads meet no bank twice), and their scales, by 4- to
@@ -50,8 +51,8 @@ constexpr int kMeetWarps = 4;  // warps that hand their sums over at a time
 // of 1-32k keys and 64 / 8 heads 165 -> 159; 3 and 10 gave about the same.
 constexpr int kBegin = 6;
 constexpr uint32_t kCode = 0x000f000fu;
-// Least lift of a group, as a power of two.  (Below it the largest weights are 2^-2 and more, and a half's numbers are normal down to 2^-14; groups whose
-// scales are of a kind, the usual ones, then take no lift at all.)
+// Least lift of a group, as a power of two, up or down.  (Below it the largest weights are within 2^-2 and 2^10, and a half's numbers are normal down to
+// 2^-14; groups whose scales are of a kind, the usual ones, then take no lift at all.)
 constexpr float kLeastLift = 6.f;
 constexpr float kNoKey = -1e30f;  // (any score is so far above it that the reference moves)
 
@@ -176,7 +177,7 @@ struct Stage {
 constexpr int kConsumers = 16, kThreads = (kConsumers + 4) * 32, kLaunch = 65536 / kThreads / 8 * 8, kProducerRegs = 32, kConsumerRegs = 112;
 static_assert((kConsumers * kConsumerRegs + 4 * kProducerRegs) * 32 <= kThreads * kLaunch, "an increase would wait for good");
 
-// What one warp has summed over its keys (weights w = p' s, of several groups times the group's lift, a power of two in shared memory), for the lane's E rows: 2t and 2t + 1 of 8 (E = 2, t = lane % 4), or t of 4 (E = 1; what belongs to odd
+// What one warp has summed over its keys (weights w = p' s times the group's lift, a power of two in shared memory), for the lane's E rows: 2t and 2t + 1 of 8 (E = 2, t = lane % 4), or t of 4 (E = 1; what belongs to odd
 // columns then stays zero).
 template <int D, int NG, int E>
 struct Sums {
@@ -735,15 +736,12 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                                 z.l[e] *= f;
 #pragma unroll
                                 for (int k = 0; k < NG; ++k) {
-                                    float fo = f;  // for sums of weights
-                                    if constexpr (NG > 1) {
-                                        // weights up to 2^4 in each group, and no more against what the group has summed than the new reference takes off
-                                        const int was = lifted ? (int)(__float_as_uint(lifts[k * 4 * E + e]) >> 23) : 127;
-                                        const float most = floorf(fminf((float)(was - 127) + (ref - z.ref[e]), 4.f - (jk[k] - ref)));
-                                        const int is = most < kLeastLift ? 127 : 127 + (int)fminf(most, 100.f);
-                                        lift[k][e] = __uint_as_float((uint32_t)is << 23);
-                                        fo *= __uint_as_float((uint32_t)max(0, 127 + is - was) << 23);
-                                    }
+                                    // weights up to 2^4 in each group, and no more against what the group has summed than the new reference takes off
+                                    const int was = lifted ? (int)(__float_as_uint(lifts[k * 4 * E + e]) >> 23) : 127;
+                                    const float most = floorf(fminf((float)(was - 127) + (ref - z.ref[e]), 4.f - (jk[k] - ref)));
+                                    const int is = fabsf(most) < kLeastLift ? 127 : 127 + (int)fminf(fmaxf(most, -100.f), 100.f);
+                                    lift[k][e] = __uint_as_float((uint32_t)is << 23);
+                                    const float fo = f * __uint_as_float((uint32_t)max(0, min(254, 127 + is - was)) << 23);  // for sums of weights
                                     z.mid[k][e] *= f;
                                     z.ones[k][e] *= fo;
 #pragma unroll
@@ -758,18 +756,16 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
                                 for (int i = 0; i < 4; ++i) x[i][e] -= ref;
                             }
-                            if constexpr (NG > 1) {
-                                bool any = false;
-                                __syncwarp();  // (8 lanes have a row: all have read what it was lifted by)
+                            bool any = false;
+                            __syncwarp();  // (8 lanes have a row: all have read what it was lifted by)
 #pragma unroll
-                                for (int k = 0; k < NG; ++k)
+                            for (int k = 0; k < NG; ++k)
 #pragma unroll
-                                    for (int e = 0; e < E; ++e) {
-                                        lifts[k * 4 * E + e] = lift[k][e];
-                                        any |= lift[k][e] != 1.f;
-                                    }
-                                lifted = __any_sync(0xffffffffu, any);
-                            }
+                                for (int e = 0; e < E; ++e) {
+                                    lifts[k * 4 * E + e] = lift[k][e];
+                                    any |= lift[k][e] != 1.f;
+                                }
+                            lifted = __any_sync(0xffffffffu, any);
                         }
                         // ---- weights ----
                         float sum[E];
@@ -888,7 +884,7 @@ splitkv_int4_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
                 for (int c = 0; c < GR; ++c) {
                     const float add = rest[c / PER], even0 = z.o[c][0][e], even2 = z.o[c][0][2 + e];
                     // 2^24 and 2^20 over the group's lift
-                    const float whole = NG == 1 || !lifted ? 16777216.f : __uint_as_float((278u << 23) - __float_as_uint(lifts[(c / PER) * 4 * E + e]));
+                    const float whole = !lifted ? 16777216.f : __uint_as_float((278u << 23) - __float_as_uint(lifts[(c / PER) * 4 * E + e]));
                     const float byte = whole * 0.0625f;
                     o[e][c] = make_float4(fmaf(whole, even0, add), fmaf(byte, z.o[c][1][e] - even0, add), fmaf(whole, even2, add),
                                           fmaf(byte, z.o[c][1][2 + e] - even2, add));
@@ -986,7 +982,7 @@ int launch(const SplitKVInt4Params& p, Int4Dev dev, cudaStream_t stream) {
     dev.chunk_log2 = 4;
     while (2 * chunk <= toks && (!c.block_table || c.page % (2 * chunk) == 0)) { chunk *= 2; ++dev.chunk_log2; }
     const size_t meet = (size_t)kMeetWarps * E * ((D / 32) * 32 * 16 + 32);
-    const size_t lifts = NG > 1 ? (size_t)kConsumers * NG * 4 * E * sizeof(float) : 0;
+    const size_t lifts = (size_t)kConsumers * NG * 4 * E * sizeof(float);
     const size_t fixed = 1024 + meet + lifts + (size_t)(2 * c.batch + 6) * sizeof(int);
     const size_t room = 227 * 1024;
     FCK_REQUIRE(fixed + 2 * (St::kBytes + 16) <= room, FLASHCK_ERR_UNSUPPORTED, "FmhaFwdSplitKVInt4: batch %lld leaves no room for two stages",
