@@ -139,7 +139,7 @@ template <typename T>
 __device__ __forceinline__ uint32_t quantise(const Vec8<T>& x, uint32_t both, T& scale_t, T& lo_t) {
     lo_t = reinterpret_cast<const T*>(&both)[0];
     const float lo = Elem<T>::to_f32(lo_t), hi = -Elem<T>::to_f32(reinterpret_cast<const T*>(&both)[1]);
-    // A quotient is rounded correctly by a product with the reciprocal, and once more with its exact remainder.
+    // A quotient is rounded correctly by a product with the reciprocal, and once more with its exact remainder (Markstein's correction).
     const float range = hi - lo;
     constexpr float kFifteenth = 1.f / 15.f;
     float step = range * kFifteenth;
